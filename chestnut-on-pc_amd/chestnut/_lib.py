@@ -69,6 +69,15 @@ _SIGS = {
                              c_int, c_int, c_void_p, c_void_p]),
     'ck_attention': (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     'ck_layernorm': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p]),
+    'ck_rope': (c_int, [c_void_p] * 4 + [c_int] * 4 + [c_long] * 4 + [c_int, c_int, c_float, c_int, c_void_p]),
+    'ck_cache_write': (c_int, [c_void_p] * 7 + [c_int] * 5 + [c_long] * 4 + [c_int, c_int, c_void_p]),
+    'ck_cache_read': (c_int, [c_void_p] * 5 + [c_int, c_void_p] + [c_int] * 6 + [c_void_p, c_void_p, c_int, c_int,
+                                                                                 c_void_p]),
+    'ck_attention_workspace': (c_int, [c_int, c_int, c_long, c_int, c_int, c_int, P(c_size_t)]),
+    'ck_attention_varlen': (c_int, [c_void_p] * 6 + [c_int] * 6 + [c_long] * 8 + [c_int, c_int, c_float, c_void_p,
+                                                                                  c_size_t, c_void_p]),
+    'ck_attention_paged': (c_int, [c_void_p] * 7 + [c_int, c_void_p, c_void_p] + [c_int] * 7 + [c_long] * 4 +
+                           [c_int, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p]),
 }
 
 

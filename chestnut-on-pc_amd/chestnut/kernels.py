@@ -11,6 +11,7 @@ alignment again.  Shapes are checked before the device, so the checks run
 """
 import ctypes
 import functools
+import math
 
 import torch
 
@@ -280,3 +281,281 @@ def warp_nv12(frame, big_frame, tfm, big_tfm, cam_w, cam_h, stride, y_height, mo
                              cam_h, stride, y_height, model_w, model_h, 1 if division == 'rcp' else 0, out.data_ptr(),
                              _raw_stream(dev)))
     return out
+
+
+# ------------------------------------------------------------ the token cache --
+# K and V rows of past tokens in pages k_pages, v_pages [n_pages, n_kv, page, head_dim] (page a
+# power of two, 16 to 1024): f16, bf16, or float8_e4m3fn with k_scale, v_scale [n_pages, n_kv, page]
+# of float8_e8m0fnu, a power of two a row.  A slot is page index * page + place.
+#
+# Index tensors are int32 on the device; their values are not checked here (that would wait for
+# the device).  Whatever they hold, nothing outside the tensors of a call is read or written.
+
+_F16, _BF16, _E4M3, _E8M0 = torch.float16, torch.bfloat16, torch.float8_e4m3fn, torch.float8_e8m0fnu
+_DTYPE = {_F16: 1, _BF16: 4, _E4M3: 5}   # the codes of include/chestnut.h
+
+
+def _rows(t, dtype, name, shape, unit=8, write=False):
+    """Strides of tokens and heads of rows [tokens, heads, head_dim]; the
+    elements of a head are contiguous, and every row starts at a multiple of
+    `unit` elements."""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f'{name} must be a torch tensor')
+    if t.dtype is not dtype:
+        raise ValueError(f'{name} must be {dtype}, got {t.dtype}')
+    if t.shape != shape:
+        raise ValueError(f'{name} must have shape {tuple(shape)}, got {tuple(t.shape)}')
+    s0, s1, s2 = t.stride()
+    T, H, hd = shape
+    if s2 != 1 and hd > 1:
+        raise ValueError(f'{name} must be contiguous in its last dimension')
+    s0 = s0 if T > 1 else 0
+    s1 = s1 if H > 1 else 0
+    if s0 % unit or s1 % unit or t.data_ptr() % (2 * unit):
+        raise ValueError(f'{name} must have rows that start at multiples of {2 * unit} bytes')
+    if write and ((T > 1 and s0 < hd) or (H > 1 and s1 < hd)):
+        raise ValueError(f'{name} must not overlap itself')
+    return s0, s1
+
+
+def _int32(t, name, shape):
+    """A contiguous int32 tensor; None entries of shape are free."""
+    _check(t, torch.int32, name, shape)
+
+
+def _on_device(*named):
+    """The current device, on which every present tensor must be (the first one always is)."""
+    dev = named[0][0].get_device()
+    for t, name in named:
+        if t is not None and (t.get_device() != dev or dev < 0):
+            if not t.is_cuda:
+                raise ValueError(f'{name} must be a CUDA tensor')
+            dev = -2   # not where the others are
+            break
+    if dev != _device():
+        raise ValueError('; '.join(f'{name} is on {t.device}' for t, name in named if t is not None) +
+                         f', not the current device cuda:{_device()}')
+    return dev
+
+
+def _cache(k_pages, v_pages, k_scale, v_scale):
+    """The checks of a cache; its shape (n_pages, n_kv, page, head_dim)."""
+    if not isinstance(k_pages, torch.Tensor) or k_pages.dim() != 4:
+        raise ValueError('k_pages must be [n_pages, n_kv, page, head_dim]')
+    if k_pages.dtype not in _DTYPE:
+        raise ValueError(f'k_pages must be float16, bfloat16 or float8_e4m3fn, got {k_pages.dtype}')
+    n, kv, page, hd = shape = k_pages.shape
+    if page < 16 or page > 1024 or page & (page - 1):
+        raise ValueError(f'the page size must be a power of two from 16 to 1024, got {page}')
+    if n < 1 or kv < 1:
+        raise ValueError('k_pages must hold a page and a head')
+    _check(k_pages, k_pages.dtype, 'k_pages')
+    _check(v_pages, k_pages.dtype, 'v_pages', shape)
+    if k_pages.dtype is _E4M3:
+        if k_scale is None or v_scale is None:
+            raise ValueError('an e4m3 cache needs k_scale and v_scale')
+        _check(k_scale, _E8M0, 'k_scale', (n, kv, page))
+        _check(v_scale, _E8M0, 'v_scale', (n, kv, page))
+    elif k_scale is not None or v_scale is not None:
+        raise ValueError('k_scale and v_scale belong to an e4m3 cache')
+    return shape
+
+
+def rope_frequencies(rot, base=10000.0, method='none', factor=1.0, context=None, slow=1.0, fast=32.0, device='cuda'):
+    """(inv_freq f64 [rot/2], scale) for `rope`: the inverse frequencies
+    base^(-2i/rot) of the pairs of the first `rot` elements of a head, fitted
+    to a context `factor` times as long as the one trained on:
+      'none'    as they are;
+      'linear'  positions divided by factor (Chen et al. 2023);
+      'base'    base * factor^(rot/(rot-2)), which stretches the slowest pair by
+                factor and leaves the fastest;
+      'parts'   pairs that turn fewer than `slow` times within `context`
+                positions (the trained length) divided by factor, those that turn
+                more than `fast` times left, linear in the turns between, and
+                scale 0.1 ln(factor) + 1 (YaRN, Peng et al. 2023)."""
+    if not isinstance(rot, int) or rot < 2 or rot % 2:
+        raise ValueError('rot must be an even number of elements')
+    if method not in ('none', 'linear', 'base', 'parts'):
+        raise ValueError("method must be 'none', 'linear', 'base' or 'parts'")
+    if not base > 1.0 or not factor >= 1.0:
+        raise ValueError('base must be above 1 and factor at least 1')
+    if method == 'base':
+        if rot < 4:
+            raise ValueError("method 'base' needs rot of at least 4")
+        base = base * factor ** (rot / (rot - 2.0))
+    f = torch.pow(torch.tensor(float(base), dtype=torch.float64), -torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+    scale = 1.0
+    if method == 'linear':
+        f = f / factor
+    elif method == 'parts':
+        if not context or context < 1 or not 0 < slow < fast:
+            raise ValueError("method 'parts' needs the trained context and 0 < slow < fast")
+        keep = ((context * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0.0, 1.0)
+        f = f * keep + f / factor * (1.0 - keep)
+        scale = 0.1 * math.log(factor) + 1.0
+    return f.to(device), scale
+
+
+def rope(x, positions, inv_freq, interleaved=False, scale=1.0, inverse=False, out=None):
+    """Rotary positions: the first 2 * len(inv_freq) elements of every head of x
+    [T, heads, head_dim] (f16 or bf16; token and head strides are free) turned
+    by positions[t] * inv_freq[i], pairs (i, i + rot/2) or, interleaved, (2i,
+    2i+1), times scale; the rest is copied.  positions int32 [T], inv_freq f64.
+    out: x itself (in place) or rows that do not overlap it."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 3 or x.dtype not in (_F16, _BF16):
+        raise ValueError('x must be float16 or bfloat16 [T, heads, head_dim]')
+    T, H, hd = x.shape
+    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dim() != 1:
+        raise ValueError('inv_freq must be float64 [rot/2]')
+    rot = 2 * inv_freq.shape[0]
+    _check(inv_freq, torch.float64, 'inv_freq')
+    if rot < 2 or rot > hd:
+        raise ValueError(f'inv_freq must have 1 to head_dim / 2 = {hd // 2} entries, got {rot // 2}')
+    if H < 1 or hd > 512 or H > 1024 or H * hd > 65536:
+        raise ValueError('rope takes head_dim up to 512, heads up to 1024 and 65536 elements a token')
+    _int32(positions, 'positions', (T,))
+    st, sh = _rows(x, x.dtype, 'x', x.shape, 1, out is x)
+    if out is None:
+        ot, oh = H * hd, hd
+    else:
+        ot, oh = (st, sh) if out is x else _rows(out, x.dtype, 'out', x.shape, 1, True)
+    dev = _on_device((x, 'x'), (positions, 'positions'), (inv_freq, 'inv_freq'), (out, 'out'))
+    y = out if out is not None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    check(lib().ck_rope(x.data_ptr(), y.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), T, H, hd, rot, st, sh,
+                        ot, oh, _DTYPE[x.dtype], 1 if interleaved else 0, scale, 1 if inverse else 0, _raw_stream(dev)))
+    return y
+
+
+def cache_write(k, v, k_pages, v_pages, slots, k_scale=None, v_scale=None):
+    """Rows k and v [T, n_kv, head_dim] (token and head strides are free) to
+    slots [T] of the cache; negative slots are left out, the others must
+    differ.  The cache has the rows' type, or is e4m3: every row is then scaled
+    by the least power of two that fits it and rounded to nearest even."""
+    n, kv, page, hd = _cache(k_pages, v_pages, k_scale, v_scale)
+    if not isinstance(k, torch.Tensor) or k.dim() != 3 or k.dtype not in (_F16, _BF16):
+        raise ValueError('k must be float16 or bfloat16 [T, n_kv, head_dim]')
+    if k_pages.dtype not in (k.dtype, _E4M3):
+        raise ValueError(f'the cache must be {k.dtype} or float8_e4m3fn, got {k_pages.dtype}')
+    T = k.shape[0]
+    kt, kh = _rows(k, k.dtype, 'k', (T, kv, hd))
+    vt, vh = _rows(v, k.dtype, 'v', (T, kv, hd))
+    _int32(slots, 'slots', (T,))
+    dev = _on_device((k, 'k'), (v, 'v'), (k_pages, 'k_pages'), (v_pages, 'v_pages'), (slots, 'slots'),
+                     (k_scale, 'k_scale'), (v_scale, 'v_scale'))
+    check(lib().ck_cache_write(k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale),
+                               _ptr(v_scale), slots.data_ptr(), T, n, kv, page, hd, kt, kh, vt, vh, _DTYPE[k.dtype],
+                               _DTYPE[k_pages.dtype], _raw_stream(dev)))
+
+
+def cache_read(k_pages, v_pages, block_table, cu_seqlens, tokens, k_scale=None, v_scale=None, dtype=None, k_out=None,
+               v_out=None):
+    """(k, v) [tokens, n_kv, head_dim]: the first cu_seqlens[b+1] - cu_seqlens[b]
+    places of every sequence b, whose pages are block_table[b] (int32 [B,
+    width]), at rows cu_seqlens[b]...  dtype: float16 or bfloat16 for an e4m3
+    cache, else the cache's own.  Rows behind the last sequence are not written."""
+    n, kv, page, hd = _cache(k_pages, v_pages, k_scale, v_scale)
+    if dtype is None:
+        dtype = k_out.dtype if k_out is not None else k_pages.dtype
+    if dtype not in (_F16, _BF16) or k_pages.dtype not in (dtype, _E4M3):
+        raise ValueError(f'dtype must be float16 or bfloat16, and that of the cache ({k_pages.dtype}) unless it is e4m3')
+    if not isinstance(tokens, int) or tokens < 0:
+        raise ValueError('tokens must be the number of rows')
+    _int32(block_table, 'block_table', (None, None))
+    B, width = block_table.shape
+    _int32(cu_seqlens, 'cu_seqlens', (B + 1,))
+    for t, name in ((k_out, 'k_out'), (v_out, 'v_out')):
+        if t is not None:
+            _check(t, dtype, name, (tokens, kv, hd))
+    dev = _on_device((k_pages, 'k_pages'), (v_pages, 'v_pages'), (block_table, 'block_table'),
+                     (cu_seqlens, 'cu_seqlens'), (k_scale, 'k_scale'), (v_scale, 'v_scale'), (k_out, 'k_out'),
+                     (v_out, 'v_out'))
+    k, v = (t if t is not None else torch.empty((tokens, kv, hd), dtype=dtype, device=k_pages.device)
+            for t in (k_out, v_out))
+    check(lib().ck_cache_read(k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale),
+                              block_table.data_ptr(), width, cu_seqlens.data_ptr(), B, tokens, n, kv, page, hd,
+                              k.data_ptr(), v.data_ptr(), _DTYPE[dtype], _DTYPE[k_pages.dtype], _raw_stream(dev)))
+    return k, v
+
+
+def _queries(q, cu_q, kv, hd, out, scale):
+    """The checks of packed queries [T, heads, head_dim] over kv K/V heads of hd:
+    (T, heads, B, q strides, out strides, scale)."""
+    if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in (_F16, _BF16):
+        raise ValueError('q must be float16 or bfloat16 [T, heads, head_dim]')
+    T, H, d = q.shape
+    if d not in (64, 128) or hd != d:
+        raise ValueError(f'head_dim must be 64 or 128 for q and the keys alike, got {d} and {hd}')
+    if kv < 1 or H < 1 or H % kv or H > 1024:
+        raise ValueError(f'the query heads ({H}, up to 1024) must be a multiple of the K/V heads ({kv})')
+    _int32(cu_q, 'cu_q', (None,))
+    if cu_q.shape[0] < 1:
+        raise ValueError('cu_q must hold B + 1 offsets')
+    qs = _rows(q, q.dtype, 'q', q.shape)
+    os = (H * d, d) if out is None else _rows(out, q.dtype, 'out', q.shape, 4, True)
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError('scale must be positive and finite')
+    return T, H, cu_q.shape[0] - 1, qs, os, scale
+
+
+def _attention_workspace(ws, B, T, keys, H, kv, hd, device):
+    """The workspace of an attention call: the caller's if it is large enough."""
+    nb = ctypes.c_size_t()
+    check(lib().ck_attention_workspace(B, T, keys, H, kv, hd, ctypes.byref(nb)))
+    ws = _workspace(ws, nb.value, device)
+    return _ptr(ws), nb.value
+
+
+def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None, workspace=None):
+    """Attention of packed sequences: q [Tq, heads, head_dim] over k, v [Tk, n_kv,
+    head_dim] (f16 or bf16; token and head strides are free), sequence b at rows
+    cu_q[b] .. cu_q[b+1] of q and cu_k[b] .. cu_k[b+1] of k and v (int32 [B+1];
+    cu_k None: the same).  causal: query i of n over m keys sees the keys
+    j <= i + m - n; else all.  heads a multiple of n_kv, head_dim 64 or 128,
+    scale 1/sqrt(head_dim) unless given.  A query without a key gets zeros; rows
+    behind the last sequence are not written."""
+    if not isinstance(k, torch.Tensor) or k.dim() != 3:
+        raise ValueError('k must be [Tk, n_kv, head_dim]')
+    Tk, kv, hd = k.shape
+    T, H, B, (qt, qh), (ot, oh), scale = _queries(q, cu_q, kv, hd, out, scale)
+    kt, kh = _rows(k, q.dtype, 'k', k.shape)
+    vt, vh = _rows(v, q.dtype, 'v', k.shape)
+    if cu_k is None:
+        if Tk != T:
+            raise ValueError(f'k must have the {T} rows of q where cu_k is not given, got {Tk}')
+        cu_k = cu_q
+    else:
+        _int32(cu_k, 'cu_k', (B + 1,))
+    dev = _on_device((q, 'q'), (k, 'k'), (v, 'v'), (cu_q, 'cu_q'), (cu_k, 'cu_k'), (out, 'out'))
+    o = out if out is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ws, nb = _attention_workspace(workspace, B, T, Tk, H, kv, hd, q.device)
+    check(lib().ck_attention_varlen(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu_q.data_ptr(),
+                                    cu_k.data_ptr(), B, T, Tk, H, kv, hd, qt, qh, kt, kh, vt, vh, ot, oh,
+                                    _DTYPE[q.dtype], 1 if causal else 0, scale, ws, nb, _raw_stream(dev)))
+    return o
+
+
+def attention_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, k_scale=None, v_scale=None, causal=True,
+                    scale=None, out=None, workspace=None):
+    """Attention of new tokens over a paged cache that holds their own K and V
+    rows already: q [Tq, heads, head_dim], sequence b at rows cu_q[b] ..
+    cu_q[b+1] (int32 [B+1]), its kv_lens[b] keys (int32 [B]) at places 0.. of the
+    pages block_table[b] (int32 [B, width]); the queries are the last of them
+    (causal: query i of n sees the keys j <= i + kv_lens[b] - n; else all).  The
+    cache has q's type or is e4m3.  Otherwise as attention_varlen."""
+    n, kv, page, hd = _cache(k_pages, v_pages, k_scale, v_scale)
+    T, H, B, (qt, qh), (ot, oh), scale = _queries(q, cu_q, kv, hd, out, scale)
+    if k_pages.dtype not in (q.dtype, _E4M3):
+        raise ValueError(f'the cache must be {q.dtype} or float8_e4m3fn, got {k_pages.dtype}')
+    _int32(kv_lens, 'kv_lens', (B,))
+    _int32(block_table, 'block_table', (B, None))
+    width = block_table.shape[1]
+    dev = _on_device((q, 'q'), (k_pages, 'k_pages'), (v_pages, 'v_pages'), (block_table, 'block_table'), (cu_q, 'cu_q'),
+                     (kv_lens, 'kv_lens'), (k_scale, 'k_scale'), (v_scale, 'v_scale'), (out, 'out'))
+    o = out if out is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ws, nb = _attention_workspace(workspace, B, T, width * page, H, kv, hd, q.device)
+    check(lib().ck_attention_paged(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale),
+                                   o.data_ptr(), block_table.data_ptr(), width, cu_q.data_ptr(), kv_lens.data_ptr(), B,
+                                   T, H, n, kv, page, hd, qt, qh, ot, oh, _DTYPE[q.dtype], _DTYPE[k_pages.dtype],
+                                   1 if causal else 0, scale, ws, nb, _raw_stream(dev)))
+    return o

@@ -427,4 +427,101 @@ int ck_layernorm(const float* x, const float* g, const float* b, void* out, int 
   CK_API_END
 }
 
+int ck_rope(const void* x, void* out, const int32_t* positions, const double* inv_freq, int T, int n_heads,
+            int head_dim, int rot, long x_st, long x_sh, long o_st, long o_sh, int dtype, int interleaved, float scale,
+            int inverse, void* stream) {
+  CK_API_BEGIN
+  launch_rope(x, out, positions, inv_freq, T, n_heads, head_dim, rot, x_st, x_sh, o_st, o_sh, dtype, interleaved != 0,
+              scale, inverse != 0, as_stream(stream));
+  CK_API_END
+}
+
+static PagedCache paged_cache(const void* k, const void* v, const void* k_scale, const void* v_scale, int n_pages,
+                              int n_kv, int page, int head_dim, int cache_dtype) {
+  PagedCache c;
+  c.k = const_cast<void*>(k);
+  c.v = const_cast<void*>(v);
+  c.k_scale = static_cast<uint8_t*>(const_cast<void*>(k_scale));
+  c.v_scale = static_cast<uint8_t*>(const_cast<void*>(v_scale));
+  c.n_pages = n_pages;
+  c.n_kv = n_kv;
+  c.page = page;
+  c.head_dim = head_dim;
+  c.dtype = cache_dtype;
+  return c;
+}
+
+int ck_cache_write(const void* k, const void* v, void* k_pages, void* v_pages, void* k_scale, void* v_scale,
+                   const int32_t* slots, int T, int n_pages, int n_kv, int page, int head_dim, long k_st, long k_sh,
+                   long v_st, long v_sh, int dtype, int cache_dtype, void* stream) {
+  CK_API_BEGIN
+  launch_cache_write(k, v, paged_cache(k_pages, v_pages, k_scale, v_scale, n_pages, n_kv, page, head_dim, cache_dtype),
+                     slots, T, k_st, k_sh, v_st, v_sh, dtype, as_stream(stream));
+  CK_API_END
+}
+
+int ck_cache_read(const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale,
+                  const int32_t* block_table, int table_width, const int32_t* cu_seqlens, int B, int tokens,
+                  int n_pages, int n_kv, int page, int head_dim, void* k, void* v, int dtype, int cache_dtype,
+                  void* stream) {
+  CK_API_BEGIN
+  launch_cache_read(paged_cache(k_pages, v_pages, k_scale, v_scale, n_pages, n_kv, page, head_dim, cache_dtype),
+                    block_table, table_width, cu_seqlens, B, tokens, k, v, dtype, as_stream(stream));
+  CK_API_END
+}
+
+static AttendQuery attend_query(const void* q, void* out, const int32_t* cu_q, int B, int Tq, int n_heads,
+                                int head_dim, long q_st, long q_sh, long o_st, long o_sh, int dtype, int causal,
+                                float scale, void* workspace, size_t ws_bytes) {
+  AttendQuery a;
+  a.q = q;
+  a.out = out;
+  a.cu_q = cu_q;
+  a.B = B;
+  a.T = Tq;
+  a.n_heads = n_heads;
+  a.head_dim = head_dim;
+  a.q_st = q_st;
+  a.q_sh = q_sh;
+  a.o_st = o_st;
+  a.o_sh = o_sh;
+  a.dtype = dtype;
+  a.causal = causal != 0;
+  a.scale = scale;
+  a.ws = static_cast<float*>(workspace);
+  a.ws_floats = ws_bytes / sizeof(float);
+  return a;
+}
+
+int ck_attention_workspace(int B, int Tq, long max_keys, int n_heads, int n_kv, int head_dim, size_t* ws_bytes) {
+  CK_API_BEGIN
+  CK_REQUIRE(ws_bytes, "ck_attention_workspace: null argument");
+  *ws_bytes = attention_workspace(B, Tq, max_keys, n_heads, n_kv, head_dim) * sizeof(float);
+  CK_API_END
+}
+
+int ck_attention_varlen(const void* q, const void* k, const void* v, void* out, const int32_t* cu_q,
+                        const int32_t* cu_k, int B, int Tq, int Tk, int n_heads, int n_kv, int head_dim, long q_st,
+                        long q_sh, long k_st, long k_sh, long v_st, long v_sh, long o_st, long o_sh, int dtype,
+                        int causal, float scale, void* workspace, size_t ws_bytes, void* stream) {
+  CK_API_BEGIN
+  launch_attention_varlen(attend_query(q, out, cu_q, B, Tq, n_heads, head_dim, q_st, q_sh, o_st, o_sh, dtype, causal,
+                                       scale, workspace, ws_bytes),
+                          k, v, k_st, k_sh, v_st, v_sh, cu_k, Tk, n_kv, as_stream(stream));
+  CK_API_END
+}
+
+int ck_attention_paged(const void* q, const void* k_pages, const void* v_pages, const void* k_scale,
+                       const void* v_scale, void* out, const int32_t* block_table, int table_width,
+                       const int32_t* cu_q, const int32_t* kv_lens, int B, int Tq, int n_heads, int n_pages, int n_kv,
+                       int page, int head_dim, long q_st, long q_sh, long o_st, long o_sh, int dtype, int cache_dtype,
+                       int causal, float scale, void* workspace, size_t ws_bytes, void* stream) {
+  CK_API_BEGIN
+  launch_attention_paged(attend_query(q, out, cu_q, B, Tq, n_heads, head_dim, q_st, q_sh, o_st, o_sh, dtype, causal,
+                                      scale, workspace, ws_bytes),
+                         paged_cache(k_pages, v_pages, k_scale, v_scale, n_pages, n_kv, page, head_dim, cache_dtype),
+                         block_table, table_width, kv_lens, as_stream(stream));
+  CK_API_END
+}
+
 }  // extern "C"

@@ -111,6 +111,54 @@ int attention_oproj_tiles(int T, int n_heads, int head_dim);
 void launch_attention_oproj(const half_t* qk, const half_t* vt, const half_t* wo, float* opart, int T, int n_heads,
                             int head_dim, hipStream_t s);
 
+// ---- the token cache: rotary positions, paged K/V rows, attention over them ----
+// Element types: DT_F16, DT_BF16, DT_E4M3 (elem16.h), the codes of include/chestnut.h.
+// Index tensors (positions, slots, tables, lengths) are device data that the host does not
+// see: whatever they hold, no kernel reads or writes outside the tensors it is given.
+//
+// out = x with the first rot elements of every head turned (rope.hip); strides in elements.
+void launch_rope(const void* x, void* out, const int* positions, const double* inv_freq, int T, int H, int hd, int rot,
+                 long xst, long xsh, long ost, long osh, int dtype, bool interleaved, float scale, bool inverse,
+                 hipStream_t s);
+// K and V pages [n_pages][n_kv][page][head_dim]; e4m3: scales [n_pages][n_kv][page], a
+// row's power of two as its biased exponent.
+struct PagedCache {
+  void *k = nullptr, *v = nullptr;
+  uint8_t *k_scale = nullptr, *v_scale = nullptr;
+  int n_pages = 0, n_kv = 0, page = 0, head_dim = 0, dtype = 0;
+};
+void check_pages(const char* what, const PagedCache& c);   // throws
+int page_shift(int page);                                  // log2 of a power of two
+// Row t of k and v ([T][n_kv][hd], element strides) to slot slots[t] = page * size + place; a
+// slot outside the cache (a negative one) is not written.
+void launch_cache_write(const void* k, const void* v, const PagedCache& c, const int* slots, int T, long kst, long ksh,
+                        long vst, long vsh, int dtype, hipStream_t s);
+// The first cu[b+1] - cu[b] places of every sequence b (its pages: table[b][...]) to rows
+// cu[b].. of k and v [tokens][n_kv][hd]; rows that belong to no sequence are left as they are.
+void launch_cache_read(const PagedCache& c, const int* table, int table_w, const int* cu, int B, int tokens, void* k,
+                       void* v, int dtype, hipStream_t s);
+// Packed queries: sequence b's are rows cu_q[b] .. cu_q[b+1] of q [T][n_heads][head_dim]
+// (element strides); rows of out that belong to no sequence are left as they are.
+struct AttendQuery {
+  const void* q = nullptr;
+  void* out = nullptr;
+  long q_st = 0, q_sh = 0, o_st = 0, o_sh = 0;
+  const int* cu_q = nullptr;   // [B + 1]
+  int B = 0, T = 0, n_heads = 0, head_dim = 0, dtype = 0;
+  bool causal = true;
+  float scale = 0.f;
+  float* ws = nullptr;         // attention_workspace floats
+  size_t ws_floats = 0;
+};
+// Workspace of a call over sequences of up to max_keys keys (0: none needed).
+size_t attention_workspace(int B, int Tq, long max_keys, int n_heads, int n_kv, int head_dim);
+// K/V rows contiguous, sequence b's at rows cu_k[b] .. cu_k[b+1] of k and v [Tk][n_kv][head_dim].
+void launch_attention_varlen(const AttendQuery& a, const void* k, const void* v, long kst, long ksh, long vst, long vsh,
+                             const int* cu_k, int Tk, int n_kv, hipStream_t s);
+// K/V rows in a paged cache, kv_lens[b] of them (the queries' own are the last).
+void launch_attention_paged(const AttendQuery& a, const PagedCache& c, const int* table, int table_w, const int* kv_lens,
+                            hipStream_t s);
+
 // ---- normalisation / small elementwise ---------------------------------------
 void launch_layernorm(const float* x, const float* g, const float* b, void* out, bool out_f16, int rows,
                       int d, float eps, hipStream_t s);

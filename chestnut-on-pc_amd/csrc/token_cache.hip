@@ -1,0 +1,252 @@
+// Writing and reading a paged cache of K and V rows.
+//
+// A cache is `n_pages` pages of [Hkv][page][hd] elements, K and V apart: the rows of one
+// head on one page lie together, which is what attention reads in one go.  The elements
+// are the model's (f16, bf16) or e4m3 with one scale a row, a power of two kept as its
+// biased exponent: the least 2^e with amax <= 448 * 2^e.  A power of two makes the
+// scaling and its undoing exact, so the one rounding is the one to e4m3 (nearest even);
+// a float format gains nothing from a finer scale but the last bits of its range.
+//
+// Bound by memory: every row is read and written once.
+#include "common.h"
+#include "elem16.h"
+#include "kernels.h"
+
+namespace ck {
+namespace {
+
+struct WriteParams {
+  const void *k, *v;
+  void *kp, *vp;
+  uint8_t *ks, *vs;
+  const int* slots;
+  long kst, ksh, vst, vsh;
+  int T, Hkv, hd, page_shift;
+  long n_slots;
+  unsigned rows;   // T * Hkv
+};
+
+// Rows in the cache: slot's page, head h, place.
+__device__ __forceinline__ long cache_row(long page, int h, int place, int Hkv, int page_shift) {
+  return ((page * Hkv + h) << page_shift) + place;
+}
+
+// LPR lanes a row, 8 elements each (lanes behind hd / 8 idle).
+template <typename T, bool Q, int LPR>
+__global__ __launch_bounds__(256) void cache_write_kernel(const WriteParams p) {
+  constexpr int RPB = 256 / LPR;
+  const int c = threadIdx.x % LPR;
+  const unsigned r = blockIdx.x * RPB + threadIdx.x / LPR;
+  const bool isv = blockIdx.y;
+  if (r >= p.rows) return;
+  const unsigned t = r / (unsigned)p.Hkv, h = r - t * p.Hkv;
+  const int slot = p.slots[t];
+  if (slot < 0 || slot >= p.n_slots) return;
+  const T* src = static_cast<const T*>(isv ? p.v : p.k) + t * (isv ? p.vst : p.kst) + h * (isv ? p.vsh : p.ksh);
+  const long row = cache_row(slot >> p.page_shift, h, slot & ((1 << p.page_shift) - 1), p.Hkv, p.page_shift);
+  typedef typename Elem<T>::v8 v8;
+  const bool in = c * 8 < p.hd;
+  v8 x{};
+  if (in) x = *reinterpret_cast<const v8*>(src + c * 8);
+  if constexpr (!Q) {
+    if (in) *reinterpret_cast<v8*>(static_cast<T*>(isv ? p.vp : p.kp) + row * p.hd + c * 8) = x;
+  } else {
+    // values that four significant bits would carry past the type's range are held at its top; NaN stays
+    float f[8], amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      f[j] = (float)x[j];
+      f[j] = f[j] > Elem<T>::top ? Elem<T>::top : f[j] < -Elem<T>::top ? -Elem<T>::top : f[j];
+      amax = fmaxf(amax, fabsf(f[j]));
+    }
+#pragma unroll
+    for (int o = LPR / 2; o; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+    const unsigned bits = __builtin_bit_cast(unsigned, amax);
+    const int e = max(1, (int)(bits >> 23) - 8 + ((bits & 0x7FFFFF) > 0x600000 ? 1 : 0));
+    const float inv = __builtin_bit_cast(float, (unsigned)(254 - e) << 23);
+    int lo = 0, hi = 0;
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0] * inv, f[1] * inv, lo, false);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[2] * inv, f[3] * inv, lo, true);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[4] * inv, f[5] * inv, hi, false);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[6] * inv, f[7] * inv, hi, true);
+    if (in) *reinterpret_cast<u32x2_t*>(static_cast<uint8_t*>(isv ? p.vp : p.kp) + row * p.hd + c * 8) =
+        u32x2_t{(unsigned)lo, (unsigned)hi};
+    if (c == 0) (isv ? p.vs : p.ks)[row] = (uint8_t)e;
+  }
+}
+
+struct ReadParams {
+  const void *kp, *vp;
+  const uint8_t *ks, *vs;
+  void *k, *v;
+  const int *table, *cu;
+  int B, table_w, tokens, Hkv, hd, page_shift, n_pages;
+};
+
+constexpr int READ_TOK = 16;   // tokens per workgroup
+
+// Token t's sequence: the last b with cu[b] <= t (cu[0] is taken as 0); -1 behind the last sequence.
+__device__ __forceinline__ int sequence_of(const int* cu, int B, int t) {
+  if (t >= cu[B]) return -1;
+  int lo = 0, hi = B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (cu[mid] <= t) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+template <typename T, bool Q>
+__global__ __launch_bounds__(256) void cache_read_kernel(const ReadParams p) {
+  __shared__ long base[READ_TOK];   // page * Hkv * page size + place; -1: no such token
+  const int t0 = blockIdx.x * READ_TOK;
+  const bool isv = blockIdx.y;
+  if (threadIdx.x < READ_TOK) {
+    const int t = t0 + threadIdx.x;
+    long at = -1;
+    if (t < p.tokens) {
+      const int b = sequence_of(p.cu, p.B, t);
+      if (b >= 0) {
+        const int i = t - p.cu[b];
+        const int pi = i >> p.page_shift;
+        if (i >= 0 && pi < p.table_w) {
+          const long page = min(max(p.table[(long)b * p.table_w + pi], 0), p.n_pages - 1);
+          at = cache_row(page, 0, i & ((1 << p.page_shift) - 1), p.Hkv, p.page_shift);
+        }
+      }
+    }
+    base[threadIdx.x] = at;
+  }
+  __syncthreads();
+  typedef typename Elem<T>::v8 v8;
+  const int ch = p.hd / 8, per_tok = ch * p.Hkv;
+  for (int i = threadIdx.x; i < READ_TOK * per_tok; i += 256) {
+    const int t = i / per_tok, r = i - t * per_tok, h = r / ch, c = r - h * ch;
+    if (base[t] < 0) continue;
+    const long row = base[t] + ((long)h << p.page_shift);
+    v8 y;
+    if constexpr (!Q) {
+      y = *reinterpret_cast<const v8*>(static_cast<const T*>(isv ? p.vp : p.kp) + row * p.hd + c * 8);
+    } else {
+      const u32x2_t w = *reinterpret_cast<const u32x2_t*>(static_cast<const uint8_t*>(isv ? p.vp : p.kp) + row * p.hd + c * 8);
+      const float s = __builtin_bit_cast(float, (unsigned)(isv ? p.vs : p.ks)[row] << 23);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[j], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[j], true);
+        y[4 * j] = (T)(a[0] * s);
+        y[4 * j + 1] = (T)(a[1] * s);
+        y[4 * j + 2] = (T)(b[0] * s);
+        y[4 * j + 3] = (T)(b[1] * s);
+      }
+    }
+    *reinterpret_cast<v8*>(static_cast<T*>(isv ? p.v : p.k) + ((long)(t0 + t) * p.Hkv + h) * p.hd + c * 8) = y;
+  }
+}
+
+template <typename T, bool Q>
+void write_t(const WriteParams& p, hipStream_t s) {
+  const int lpr = p.hd <= 64 ? 8 : p.hd <= 128 ? 16 : 32;
+  const dim3 grid(ceil_div(p.rows, 256 / lpr), 2), block(256);
+  if (lpr == 8) CK_LAUNCH((cache_write_kernel<T, Q, 8>), grid, block, 0, s, p);
+  else if (lpr == 16) CK_LAUNCH((cache_write_kernel<T, Q, 16>), grid, block, 0, s, p);
+  else CK_LAUNCH((cache_write_kernel<T, Q, 32>), grid, block, 0, s, p);
+}
+
+}  // namespace
+
+int page_shift(int page) {
+  int s = 0;
+  while ((1 << s) < page) ++s;
+  return s;
+}
+
+void check_pages(const char* what, const PagedCache& c) {
+  const std::string w(what);
+  CK_REQUIRE(c.k && c.v, w + ": null cache");
+  CK_REQUIRE(c.dtype == DT_F16 || c.dtype == DT_BF16 || c.dtype == DT_E4M3, w + ": the cache must be f16, bf16 or e4m3");
+  CK_REQUIRE(c.n_pages > 0 && c.n_kv > 0 && c.n_kv <= 1024, w + ": pages and K/V heads (up to 1024) must be positive");
+  CK_REQUIRE(c.page >= 16 && c.page <= 1024 && (c.page & (c.page - 1)) == 0,
+             w + ": page size must be a power of two from 16 to 1024");
+  CK_REQUIRE((long)c.n_pages * c.page < (1L << 31), w + ": the cache must have under 2^31 slots");
+  CK_REQUIRE(c.head_dim > 0 && c.head_dim % 8 == 0 && c.head_dim <= 256, w + ": head_dim must be a multiple of 8 up to 256");
+  CK_REQUIRE(c.dtype != DT_E4M3 || (c.k_scale && c.v_scale), w + ": an e4m3 cache needs its scales");
+  CK_REQUIRE(((reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) & 15) == 0,
+             w + ": pages must be 16-byte aligned");
+}
+
+void launch_cache_write(const void* k, const void* v, const PagedCache& c, const int* slots, int T, long kst, long ksh,
+                        long vst, long vsh, int dtype, hipStream_t s) {
+  CK_REQUIRE(dtype == DT_F16 || dtype == DT_BF16, "cache_write: rows must be f16 or bf16");
+  check_pages("cache_write", c);
+  CK_REQUIRE(c.dtype == dtype || c.dtype == DT_E4M3, "cache_write: the cache must be of the rows' type or e4m3");
+  CK_REQUIRE(T >= 0 && (long)T * c.n_kv < (1L << 31), "cache_write: under 2^31 rows");
+  if (T == 0) return;
+  CK_REQUIRE(k && v && slots, "cache_write: null pointer");
+  CK_REQUIRE(((kst | ksh | vst | vsh) & 7) == 0 && ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0,
+             "cache_write: rows must be 16-byte aligned");
+  WriteParams p{};
+  p.k = k;
+  p.v = v;
+  p.kp = c.k;
+  p.vp = c.v;
+  p.ks = c.k_scale;
+  p.vs = c.v_scale;
+  p.slots = slots;
+  p.kst = kst;
+  p.ksh = ksh;
+  p.vst = vst;
+  p.vsh = vsh;
+  p.T = T;
+  p.Hkv = c.n_kv;
+  p.hd = c.head_dim;
+  p.page_shift = page_shift(c.page);
+  p.n_slots = (long)c.n_pages * c.page;
+  p.rows = (unsigned)T * c.n_kv;
+  if (dtype == DT_F16) {
+    if (c.dtype == DT_E4M3) write_t<half_t, true>(p, s);
+    else write_t<half_t, false>(p, s);
+  } else {
+    if (c.dtype == DT_E4M3) write_t<bf16_t, true>(p, s);
+    else write_t<bf16_t, false>(p, s);
+  }
+  CK_LAUNCHED("cache_write");
+}
+
+void launch_cache_read(const PagedCache& c, const int* table, int table_w, const int* cu, int B, int tokens, void* k,
+                       void* v, int dtype, hipStream_t s) {
+  CK_REQUIRE(dtype == DT_F16 || dtype == DT_BF16, "cache_read: rows must be f16 or bf16");
+  check_pages("cache_read", c);
+  CK_REQUIRE(c.dtype == dtype || c.dtype == DT_E4M3, "cache_read: the cache must be of the rows' type or e4m3");
+  CK_REQUIRE(tokens >= 0 && B >= 0 && table_w >= 0 && (long)tokens * c.n_kv < (1L << 31), "cache_read: bad sizes");
+  if (tokens == 0 || B == 0 || table_w == 0) return;
+  CK_REQUIRE(table && cu && k && v, "cache_read: null pointer");
+  CK_REQUIRE(((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0, "cache_read: rows must be 16-byte aligned");
+  ReadParams p{};
+  p.kp = c.k;
+  p.vp = c.v;
+  p.ks = c.k_scale;
+  p.vs = c.v_scale;
+  p.k = k;
+  p.v = v;
+  p.table = table;
+  p.cu = cu;
+  p.B = B;
+  p.table_w = table_w;
+  p.tokens = tokens;
+  p.Hkv = c.n_kv;
+  p.hd = c.head_dim;
+  p.page_shift = page_shift(c.page);
+  p.n_pages = c.n_pages;
+  const dim3 grid(ceil_div(tokens, READ_TOK), 2), block(256);
+  if (dtype == DT_F16) {
+    if (c.dtype == DT_E4M3) CK_LAUNCH((cache_read_kernel<half_t, true>), grid, block, 0, s, p);
+    else CK_LAUNCH((cache_read_kernel<half_t, false>), grid, block, 0, s, p);
+  } else {
+    if (c.dtype == DT_E4M3) CK_LAUNCH((cache_read_kernel<bf16_t, true>), grid, block, 0, s, p);
+    else CK_LAUNCH((cache_read_kernel<bf16_t, false>), grid, block, 0, s, p);
+  }
+  CK_LAUNCHED("cache_read");
+}
+
+}  // namespace ck

@@ -296,6 +296,84 @@ int ck_attention(const void* qk, const void* vt, void* out, int T, int n_heads, 
 int ck_layernorm(const float* x, const float* g, const float* b, void* out, int out_f16, int rows, int d, float eps,
                  void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* The token cache: rotary positions, a paged cache of K/V rows, attention   */
+/* of new tokens over it and of whole packed sequences.  The reference has   */
+/* no counterpart: its temporal memory is one pooled vector a frame          */
+/* (compile_modeld.py:149-163), and its attention stays inside a frame.      */
+/* ------------------------------------------------------------------------ */
+
+/* Element types of the functions below: 1 = f16, 4 = bf16, 5 = e4m3 (cache
+ * pages only).  Rows are [tokens][heads][head_dim] with element strides of
+ * tokens (_st) and heads (_sh), the elements of a head contiguous.
+ *
+ * Index arrays (positions, slots, block tables, lengths) are device memory
+ * and cannot be checked on the host: what they hold decides results only,
+ * never whether an access stays inside the arrays given (a page index
+ * outside the cache reads one inside it, a slot outside it is not written).
+ * Packed sequences: sequence b is rows cu[b] .. cu[b+1]; rows that belong to
+ * no sequence are not written. */
+
+/* out = x with the first `rot` elements of every head turned by the angles
+ * a_i = positions[t] * inv_freq[i], i < rot / 2 (64-bit product, reduced to
+ * one turn): y0 = scale (x0 cos a - x1 sin a), y1 = scale (x1 cos a +
+ * x0 sin a) for the pairs (i, i + rot/2), or (2i, 2i+1) where interleaved;
+ * inverse: by -a.  Elements behind rot are copied.  out may be x (same
+ * strides) but not overlap it otherwise.  rot even, <= head_dim <= 512. */
+int ck_rope(const void* x, void* out, const int32_t* positions, const double* inv_freq, int T, int n_heads,
+            int head_dim, int rot, long x_st, long x_sh, long o_st, long o_sh, int dtype, int interleaved, float scale,
+            int inverse, void* stream);
+
+/* A cache: k_pages, v_pages [n_pages][n_kv][page][head_dim], 16-byte
+ * aligned; page a power of two from 16 to 1024, head_dim a multiple of 8 up
+ * to 256, n_pages * page < 2^31.  cache_dtype e4m3: k_scale, v_scale
+ * [n_pages][n_kv][page] hold each row's scale 2^(byte - 127); a value is
+ * code * scale.  Other cache types: the scales are NULL.
+ *
+ * ck_cache_write: row t of k and v to slot slots[t] = page index * page +
+ * place; negative slots are not written, slots must differ.  e4m3: the scale
+ * is the least power of two with max |row| <= 448 scale, codes are rounded to
+ * nearest even; infinities and values above 61440 (f16) are held as the
+ * largest that reads back finite, NaN stays NaN.
+ * Rows 16-byte aligned (strides multiples of 8). */
+int ck_cache_write(const void* k, const void* v, void* k_pages, void* v_pages, void* k_scale, void* v_scale,
+                   const int32_t* slots, int T, int n_pages, int n_kv, int page, int head_dim, long k_st, long k_sh,
+                   long v_st, long v_sh, int dtype, int cache_dtype, void* stream);
+
+/* The first cu[b+1] - cu[b] places of each sequence (pages block_table[b][..],
+ * int32 [B][table_width]) to rows cu[b].. of k and v [tokens][n_kv][head_dim]
+ * (contiguous, dtype f16 or bf16; the cache's own type unless that is e4m3). */
+int ck_cache_read(const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale,
+                  const int32_t* block_table, int table_width, const int32_t* cu_seqlens, int B, int tokens,
+                  int n_pages, int n_kv, int page, int head_dim, void* k, void* v, int dtype, int cache_dtype,
+                  void* stream);
+
+/* Workspace of the attention calls below, in bytes (0: none).  max_keys: the
+ * most keys a sequence can have (Tk, or table_width * page). */
+int ck_attention_workspace(int B, int Tq, long max_keys, int n_heads, int n_kv, int head_dim, size_t* ws_bytes);
+
+/* out[i] = sum_j softmax_j(scale q_i . k_j) v_j over packed sequences:
+ * queries cu_q[b] .. cu_q[b+1] of sequence b over keys cu_k[b] .. cu_k[b+1];
+ * causal: query i of n over m keys sees keys j <= i + m - n, else all.  A
+ * query that sees none gets zeros; what a query does not see (infinities and
+ * NaN included) does not reach it.  Query head h reads K/V head
+ * h / (n_heads / n_kv).  head_dim 64 or 128, scale > 0, f16 or bf16;
+ * q, k, v rows 16-byte aligned, out rows 8-byte aligned. */
+int ck_attention_varlen(const void* q, const void* k, const void* v, void* out, const int32_t* cu_q,
+                        const int32_t* cu_k, int B, int Tq, int Tk, int n_heads, int n_kv, int head_dim, long q_st,
+                        long q_sh, long k_st, long k_sh, long v_st, long v_sh, long o_st, long o_sh, int dtype,
+                        int causal, float scale, void* workspace, size_t ws_bytes, void* stream);
+
+/* The same over a paged cache: sequence b has kv_lens[b] keys, at places
+ * 0 .. of its pages block_table[b][..]; its queries are the last of them.
+ * The workspace belongs to this call until it has run: calls that may
+ * overlap, and graphs that may, need one each. */
+int ck_attention_paged(const void* q, const void* k_pages, const void* v_pages, const void* k_scale,
+                       const void* v_scale, void* out, const int32_t* block_table, int table_width,
+                       const int32_t* cu_q, const int32_t* kv_lens, int B, int Tq, int n_heads, int n_pages, int n_kv,
+                       int page, int head_dim, long q_st, long q_sh, long o_st, long o_sh, int dtype, int cache_dtype,
+                       int causal, float scale, void* workspace, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,421 @@
+"""Rotary positions, the paged cache and attention over packed sequences and pages on the
+GPU, against oracle.token_cache in 64 bits.
+
+Tolerances.  u = eps / 2 of the element type is the relative error of one rounding.
+rope: angles are exact to 2^-45 turns, cos and sin to 2^-22 each; two products and a sum
+in f32, one rounding to the type.
+cache: bit-exact codes and scales; a value read back is one rounding of code * scale.
+attention: the output is rounded once (u |o|) and each softmax weight once (u a weight, so
+u times A = the same sum with |v|); f16 weights below the smallest normal round to its
+subnormals (2^-25 each, n of them at most, each times |v| < 6, against a row sum of at least
+1); a score is a chain of hd f32 sums ((hd + 4) 2^-24 of its sum
+of magnitudes, twice: numerator and denominator); exp2, the rescalings and the sums add
+less than 2^-17."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import token_cache as O
+
+pytestmark = pytest.mark.gpu
+DT = {'f16': torch.float16, 'bf16': torch.bfloat16}
+TOP = {'f16': 61440.0, 'bf16': 1.875 * 2.0 ** 127}
+
+
+def u(dt):
+    return torch.finfo(DT[dt]).eps / 2
+
+
+def f64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def rows(seed, T, H, hd, dt, scale=1.0):
+    """Values of the type, exact in f64, on the device."""
+    x = np.random.default_rng(seed).standard_normal((T, H, hd)) * scale
+    return torch.from_numpy(x).to(DT[dt]).cuda()
+
+
+def i32(v):
+    return torch.tensor(np.asarray(v, np.int32).reshape(-1) if np.ndim(v) < 2 else np.asarray(v, np.int32)).cuda()
+
+
+def cu(lens):
+    return i32(np.concatenate([[0], np.cumsum(lens)]))
+
+
+def near(out, ref, mag, most, n, hd, dt, what=''):
+    out = f64(out)
+    tiny = 6 * n * 2.0 ** -25 if dt == 'f16' else 0.0
+    tol = u(dt) * (np.abs(ref) + mag) * (1 + 2.0 ** -6) + (2 * (hd + 4) * 2.0 ** -24 * most + 2.0 ** -17) * mag + tiny
+    bad = ~(np.abs(out - ref) <= tol)
+    assert not bad.any(), f'{what}: {bad.sum()} of {bad.size}, worst {np.nanmax(np.abs(out - ref) - tol)}, first {np.argwhere(bad)[0]}'
+
+
+# ---------------------------------------------------------------------- rope --
+@pytest.mark.parametrize('T,H,hd,rot', [(1, 1, 64, 64), (3, 5, 128, 64), (17, 20, 128, 128), (700, 3, 64, 16),
+                                        (9, 2, 80, 24), (5, 3, 33, 10), (2, 1, 2, 2), (33, 4, 256, 256)])
+@pytest.mark.parametrize('inter', [False, True])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+def test_rope(gpu, T, H, hd, rot, inter, dt):
+    from chestnut import kernels as K
+    x = rows(T + hd, T, H, hd, dt)
+    pos = np.random.default_rng(1).integers(0, 1 << 20, T)
+    pos[0] = 0 if T > 1 else 999999
+    f, s = K.rope_frequencies(rot, base=5e5, method='parts', factor=8.0, context=8192)
+    ref = O.rope(f64(x), pos, f64(f), inter, s)
+    mag = np.abs(f64(x)).max() * 2 * s
+    out = K.rope(x, i32(pos), f, interleaved=inter, scale=s)
+    assert np.all(np.abs(f64(out) - ref) <= u(dt) * np.abs(ref) * (1 + 2.0 ** -6) + 2.0 ** -20 * mag + 2.0 ** -25)
+    assert torch.equal(out[..., rot:], x[..., rot:])
+    back = K.rope(out, i32(pos), f, interleaved=inter, scale=1 / s, inverse=True)
+    assert np.all(np.abs(f64(back) - f64(x)) <= 4 * u(dt) * mag)
+    y = x.clone()
+    assert K.rope(y, i32(pos), f, interleaved=inter, scale=s, out=y) is y and torch.equal(y, out)
+
+
+@pytest.mark.parametrize('off', [0, 1, 8])
+def test_rope_strided_views(gpu, off):
+    from chestnut import kernels as K
+    T, H, hd = 6, 3, 64
+    qkv = rows(2, T, 9, hd + 16, 'f16')
+    x = qkv[:, 2:2 + H, off:off + hd]
+    buf = torch.full((T, 5, 100), 7.0, dtype=torch.float16, device='cuda')
+    f, _ = K.rope_frequencies(32)
+    want = K.rope(x.contiguous(), i32(np.arange(T)), f)
+    got = K.rope(x, i32(np.arange(T)), f, out=buf[:, 1:1 + H, 8:8 + hd])
+    assert torch.equal(got, want) and torch.equal(buf[:, 1:1 + H, 8:8 + hd], want)
+    buf[:, 1:1 + H, 8:8 + hd] = 7.0
+    assert (buf == 7.0).all()
+
+
+# --------------------------------------------------------------------- cache --
+def pages_of(n, kv, page, hd, dt, cache):
+    if cache != 'e4m3':
+        return [torch.full((n, kv, page, hd), 3.0, dtype=DT[dt], device='cuda') for _ in 'kv'] + [None, None]
+    return ([torch.full((n, kv, page, hd), 0x5A, dtype=torch.uint8, device='cuda').view(torch.float8_e4m3fn) for _ in 'kv'] +
+            [torch.full((n, kv, page), 99, dtype=torch.uint8, device='cuda').view(torch.float8_e8m0fnu) for _ in 'kv'])
+
+
+@pytest.mark.parametrize('T,kv,hd,page', [(1, 1, 128, 16), (7, 3, 64, 32), (100, 8, 128, 64), (33, 2, 40, 16), (20, 1, 256, 1024),
+                                          (5, 5, 8, 16)])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('quant', [False, True])
+def test_cache_write_and_read_back(gpu, T, kv, hd, page, dt, quant):
+    from chestnut import kernels as K
+    rng = np.random.default_rng(T + hd)
+    k, v = rows(3, T, 2 * kv, hd, dt, 5.0)[:, :kv], rows(4, T, kv, hd, dt, 1e-3)
+    v[0, 0] = 0
+    v[0, 0, hd // 2] = 448 * 2.0 ** -9          # the scale's border: held, and the next value up
+    if T > 1:
+        v[1, 0] = v[1, 0] * 0
+        v[1, 0, 0] = torch.nextafter(torch.tensor(448 * 2.0 ** -9, dtype=DT[dt]), torch.tensor(9e9, dtype=DT[dt]))
+        k[1, 0] = torch.linspace(-500, 500, hd).to(DT[dt]).cuda()
+    if T > 3:
+        k[2, 0], k[3, 0] = 0, 0
+        k[3, 0, 0], k[3, 0, 1], k[3, 0, 2] = float('inf'), float('-inf'), float('nan')
+    n = -(-T // page) + 2
+    slots = rng.permutation(n * page)[:T]
+    keep = np.ones(T, bool)
+    if T > 5:
+        slots[4], keep[4] = -1, False
+        slots[5], keep[5] = n * page, False     # outside the cache: not written
+    kp, vp, ks, vs = pages_of(n, kv, page, hd, dt, 'e4m3' if quant else dt)
+    K.cache_write(k, v, kp, vp, i32(slots), k_scale=ks, v_scale=vs)
+    for x, p, s in ((k, kp, ks), (v, vp, vs)):
+        if quant:
+            codes, byte = O.quantise(f64(x), TOP[dt])
+            wantp, wants = np.full(p.shape, 0x5A, np.uint8), np.full(s.shape, 99, np.uint8)
+            for t in np.nonzero(keep)[0]:
+                wantp[slots[t] // page, :, slots[t] % page] = codes[t]
+                wants[slots[t] // page, :, slots[t] % page] = byte[t]
+            got = p.view(torch.uint8).cpu().numpy()
+            nan = (wantp & 127) == 127
+            assert np.array_equal(got[~nan], wantp[~nan]) and np.all((got[nan] & 127) == 127)
+            assert np.array_equal(s.view(torch.uint8).cpu().numpy(), wants)
+        else:
+            want = torch.full(p.shape, 3.0, dtype=DT[dt])
+            for t in np.nonzero(keep)[0]:
+                want[slots[t] // page, :, slots[t] % page] = x[t].cpu()
+            assert torch.equal(p.cpu().view(torch.int16), want.view(torch.int16))
+
+
+@pytest.mark.parametrize('lens,kv,hd,page', [([1], 1, 64, 16), ([0, 33, 0, 5, 64], 3, 128, 32), ([700, 16], 2, 72, 16),
+                                             ([1] * 150, 1, 64, 16)])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('quant', [False, True])
+def test_cache_read(gpu, lens, kv, hd, page, dt, quant):
+    from chestnut import kernels as K
+    table, n = tables(lens, page, 7)
+    kp, vp, ks, vs = filled(n, kv, page, hd, dt, 'e4m3' if quant else dt, 9)
+    T = sum(lens) + 3
+    ko = torch.full((T, kv, hd), 5.0, dtype=DT[dt], device='cuda')
+    k, v = K.cache_read(kp, vp, i32(table), cu(lens), T, k_scale=ks, v_scale=vs, dtype=DT[dt], k_out=ko)
+    assert k is ko and (k[T - 3:] == 5.0).all()
+    for got, p, s in ((k, kp, ks), (v, vp, vs)):
+        want = np.concatenate([gathered(p, s, table[b], m, page) for b, m in enumerate(lens)])
+        assert torch.equal(got[:T - 3].cpu(), torch.from_numpy(want).to(DT[dt]))
+
+
+def tables(lens, page, seed):
+    """Shuffled pages; entries behind a sequence's last page point nowhere."""
+    need = [-(-m // page) for m in lens]
+    perm = np.random.default_rng(seed).permutation(sum(need) + 1)
+    t = np.full((len(lens), max(need + [0]) + 2), -123456, np.int64)
+    t[:, -1] = 2 ** 31 - 1
+    at = 0
+    for b, m in enumerate(need):
+        t[b, :m] = perm[at:at + m]
+        at += m
+    return t, sum(need) + 1
+
+
+def filled(n, kv, page, hd, dt, cache, seed):
+    """Pages full of normal values; every place that holds none is NaN (quantised: code 0x7F)."""
+    r = np.random.default_rng(seed)
+    out = []
+    for _ in 'kv':
+        x = r.standard_normal((n, kv, page, hd))
+        if cache == 'e4m3':
+            c, b = O.quantise(x, TOP[dt])
+            out.append((torch.from_numpy(c).cuda().view(torch.float8_e4m3fn), torch.from_numpy(b).cuda().view(torch.float8_e8m0fnu)))
+        else:
+            out.append((torch.from_numpy(x).to(DT[dt]).cuda(), None))
+    return out[0][0], out[1][0], out[0][1], out[1][1]
+
+
+def gathered(p, s, row, m, page):
+    """The first m places of a sequence, [m, kv, hd] f64."""
+    x = f64(p) if s is None else O.values(p.view(torch.uint8).cpu().numpy(), s.view(torch.uint8).cpu().numpy())
+    return x[row[:-(-m // page)]].transpose(0, 2, 1, 3).reshape(-1, x.shape[1], x.shape[3])[:m]
+
+
+# ----------------------------------------------------------------- attention --
+VARLEN = [([1], None), ([64], None), ([33, 1, 0, 257], None), ([127, 129, 128], None), ([700], None), ([5, 3], [900, 65]),
+          ([40, 7, 9], [8, 0, 9]), ([1] * 70, None), ([1, 1, 1], [1, 4000, 130])]
+
+
+@pytest.mark.parametrize('lens,klens', VARLEN, ids=lambda x: str(x)[:20])
+@pytest.mark.parametrize('H,kv,hd', [(2, 2, 64), (5, 1, 128), (8, 2, 128)])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('causal', [True, False])
+def test_attention_varlen(gpu, lens, klens, H, kv, hd, dt, causal):
+    from chestnut import kernels as K
+    T, kl = sum(lens), klens or lens
+    qkv = rows(T, T, H + 2, hd, dt)
+    kvb = rows(T + 1, sum(kl), 2 * kv + 1, hd, dt)
+    q, k, v = qkv[:, 1:1 + H], kvb[:, :kv], kvb[:, kv:2 * kv]
+    out = torch.full((T + 2, H, hd), 9.0, dtype=DT[dt], device='cuda')
+    qq = torch.cat((q, q[:1], q[:1])) if T else q
+    got = K.attention_varlen(qq, k, v, cu(lens), cu(kl), causal=causal, out=out)
+    assert got is out and (out[T:] == 9.0).all()
+    a = b = 0
+    for n, m in zip(lens, kl):
+        ref, mag, most = O.attention(f64(q[a:a + n]), f64(k[b:b + m]), f64(v[b:b + m]), causal)
+        near(out[a:a + n], ref, mag, most, m, hd, dt, f'{n} over {m}')
+        a, b = a + n, b + m
+
+
+@pytest.mark.parametrize('qlens,klens', [([1], [1]), ([1, 1, 1], [63, 64, 1025]), ([64], [64]), ([5, 0, 100], [5, 20, 333]),
+                                         ([130, 1, 31], [700, 900, 17]), ([1] * 9, [100 * i for i in range(9)]), ([1], [5000])])
+@pytest.mark.parametrize('H,kv,hd,page', [(4, 4, 64, 16), (8, 2, 128, 32), (7, 1, 128, 256)])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('quant', [False, True])
+@pytest.mark.parametrize('causal', [True, False])
+def test_attention_paged(gpu, qlens, klens, H, kv, hd, page, dt, quant, causal):
+    from chestnut import kernels as K
+    table, n = tables(klens, page, 5)
+    kp, vp, ks, vs = filled(n, kv, page, hd, dt, 'e4m3' if quant else dt, 6)
+    q = rows(8, sum(qlens), H, hd, dt)
+    out = K.attention_paged(q, kp, vp, i32(table), cu(qlens), i32(klens), k_scale=ks, v_scale=vs, causal=causal)
+    a = 0
+    for b, (x, m) in enumerate(zip(qlens, klens)):
+        k, v = gathered(kp, ks, table[b], m, page), gathered(vp, vs, table[b], m, page)
+        ref, mag, most = O.attention(f64(q[a:a + x]), k, v, causal)
+        near(out[a:a + x], ref, mag, most, m, hd, dt, f'{x} over {m}')
+        a += x
+
+
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('hd', [64, 128])
+@pytest.mark.parametrize('paged', [False, True])
+@pytest.mark.parametrize('n,m', [(200, 200), (40, 170), (3, 64), (1, 66)])
+def test_what_a_row_does_not_see_does_not_reach_it(gpu, dt, hd, paged, n, m):
+    """NaN and infinities in K and V of later tokens, and in the places behind the last key."""
+    from chestnut import kernels as K
+    H, kv, page = 4, 2, 64
+    q, k, v = rows(1, n, H, hd, dt), rows(2, m, kv, hd, dt), rows(3, m, kv, hd, dt)
+    first = m - n                     # the first query's own place
+    for j, x in ((first + (n + 1) // 2, float('nan')), (first + (3 * n) // 4, float('inf')), (m - 1, float('-inf'))):
+        if first < j < m:
+            v[j, :, j % hd] = x
+            k[j, :, 3] = x
+    if paged:
+        need = -(-m // page)
+        kp, vp = (torch.full((need, page, kv, hd), float('nan'), dtype=DT[dt], device='cuda') for _ in 'kv')
+        kp.view(-1, kv, hd)[:m], vp.view(-1, kv, hd)[:m] = k, v
+        kp, vp = (t.permute(0, 2, 1, 3).contiguous() for t in (kp, vp))
+        out = K.attention_paged(q, kp, vp, i32([list(range(need))]), cu([n]), i32([m]))
+    else:
+        big = torch.full((m + 70, 2 * kv, hd), float('nan'), dtype=DT[dt], device='cuda')
+        big[:m, :kv], big[:m, kv:] = k, v
+        out = K.attention_varlen(q, big[:, :kv], big[:, kv:], cu([n]), cu([m]))
+    clean = min([j for j in range(first, m) if not torch.isfinite(k[j]).all()] + [m]) - first
+    ref, mag, most = O.attention(f64(q[:clean]), f64(k[:first + clean]), f64(v[:first + clean]))
+    near(out[:clean], ref, mag, most, m, hd, dt)
+    assert clean > 0 and not torch.isfinite(out[clean:]).all(-1).any() or clean == n
+
+
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+def test_infinite_values_of_v_reach_the_rows_that_see_them(gpu, dt):
+    from chestnut import kernels as K
+    n, hd = 150, 64
+    q, k, v = rows(1, n, 2, hd, dt), rows(2, n, 2, hd, dt), rows(3, n, 2, hd, dt)
+    v[70, 0, 5], v[100, 0, 5], v[90, 1, 7] = float('inf'), float('-inf'), float('-inf')
+    out = f64(K.attention_varlen(q, k, v, cu([n])))
+    ref, _, _ = O.attention(f64(q), f64(k), f64(v))
+    assert np.array_equal(np.isfinite(out), np.isfinite(ref))
+    assert np.array_equal(out[70:100, 0, 5], np.full(30, np.inf)) and np.all(out[90:, 1, 7] == -np.inf)
+    assert np.isnan(out[100:, 0, 5]).all()
+
+
+@pytest.mark.parametrize('hd', [64, 128])
+def test_one_key_rules_each_row(gpu, hd):
+    """Row t's output is V's row (37 t + 5) mod (t + 1): the order of keys and features."""
+    from chestnut import kernels as K
+    n = 300
+    at = (37 * np.arange(n) + 5) % (np.arange(n) + 1)
+    k = rows(1, n, 1, hd, 'f16')
+    k = k / k.float().norm(dim=-1, keepdim=True).half()
+    q = (k[torch.from_numpy(at).cuda()].float() * 400).half()
+    v = rows(2, n, 1, hd, 'f16')
+    out = K.attention_varlen(q, k, v, cu([n]), scale=1.0)
+    assert torch.equal(out[:, 0].cpu(), v[:, 0].cpu()[torch.from_numpy(at)])
+
+
+def test_index_values_outside_the_tensors_stay_inside(gpu):
+    """Lengths, offsets and pages that point outside: the call ends, nothing outside is written,
+    and well-formed sequences of the same call are right."""
+    from chestnut import kernels as K
+    H, kv, hd, page = 2, 1, 64, 16
+    kp, vp, _, _ = filled(3, kv, page, hd, 'f16', 'f16', 1)
+    q = rows(1, 4, H, hd, 'f16')
+    guard = torch.full((6, H, hd), 4.0, dtype=torch.float16, device='cuda')
+    K.attention_paged(q, kp, vp, i32([[0, 1], [-7, 99], [2, 0]]), i32([0, 1, 3, 900]), i32([20, 1000000, -5]), out=guard[1:5])
+    assert (guard[0] == 4.0).all() and (guard[5] == 4.0).all()
+    ref, mag, most = O.attention(f64(q[:1]), gathered(kp, None, np.array([0, 1]), 20, page), gathered(vp, None, np.array([0, 1]), 20, page))
+    near(guard[1:2], ref, mag, most, 20, hd, 'f16')
+    k, v = K.cache_read(kp, vp, i32([[0, -1], [50, 1]]), i32([0, 17, 40]), 30)
+    assert torch.equal(k[:16], kp[0].permute(1, 0, 2)) and k.shape == (30, kv, hd)
+    K.cache_read(kp, vp, i32([[0, -1], [50, 1]]), i32([5, -3, 10 ** 9]), 30)
+
+
+def test_empty_calls(gpu):
+    from chestnut import kernels as K
+    kp, vp, _, _ = filled(1, 1, 16, 64, 'f16', 'f16', 1)
+    e = torch.empty(0, 2, 64, dtype=torch.float16, device='cuda')
+    assert K.attention_varlen(e, e[:, :1], e[:, :1], cu([0])).shape == (0, 2, 64)
+    assert K.attention_paged(e, kp, vp, torch.empty(0, 1, dtype=torch.int32, device='cuda'), i32([0]), i32([])).shape == (0, 2, 64)
+    assert K.rope(e, i32([]), K.rope_frequencies(64)[0]).shape == (0, 2, 64)
+    K.cache_write(e[:, :1], e[:, :1], kp, vp, i32([]))
+    assert K.cache_read(kp, vp, torch.empty(0, 0, dtype=torch.int32, device='cuda'), i32([0]), 0)[0].shape == (0, 1, 64)
+    out = K.attention_paged(rows(1, 2, 2, 64, 'f16'), kp, vp, torch.empty(1, 0, dtype=torch.int32, device='cuda'), i32([0, 2]), i32([7]))
+    assert (out == 0).all()
+
+
+# ------------------------------------------------------- a run of them together --
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('quant', [False, True])
+def test_prompt_then_tokens_through_the_cache(gpu, dt, quant):
+    """Two streams: a prompt as one packed call, its rows kept in the cache, then a chunk and single
+    tokens over the cache.  Without quantisation every step equals attention over the whole sequence."""
+    from chestnut import kernels as K
+    H, kv, hd, page = 4, 2, 64, 16
+    prompt, steps = [37, 90], [20, 1, 1]
+    total = [p + sum(steps) for p in prompt]
+    f, s = K.rope_frequencies(hd, method='linear', factor=4.0)
+    stream = [rows(10 + b, t, H + 2 * kv, hd, dt) for b, t in enumerate(total)]
+    need = [-(-t // page) for t in total]
+    table = np.zeros((2, max(need)), int)
+    table[0, :need[0]] = np.arange(need[0])[::-1]
+    table[1, :need[1]] = need[0] + np.arange(need[1])
+    kp, vp, ks, vs = pages_of(sum(need), kv, page, hd, dt, 'e4m3' if quant else dt)
+    done, outs = [0, 0], [[], []]
+    for lens in [prompt] + [[x, x] for x in steps]:
+        x = torch.cat([stream[b][done[b]:done[b] + lens[b]] for b in range(2)])
+        pos = np.concatenate([np.arange(done[b], done[b] + lens[b]) for b in range(2)])
+        slots = np.concatenate([table[b][np.arange(done[b], done[b] + lens[b]) // page] * page +
+                                np.arange(done[b], done[b] + lens[b]) % page for b in range(2)])
+        x[:, :H + kv] = K.rope(x[:, :H + kv], i32(pos), f, scale=s)
+        K.cache_write(x[:, H:H + kv], x[:, H + kv:], kp, vp, i32(slots), k_scale=ks, v_scale=vs)
+        done = [d + n for d, n in zip(done, lens)]
+        if lens is prompt and not quant:
+            o = K.attention_varlen(x[:, :H], x[:, H:H + kv], x[:, H + kv:], cu(lens))
+        else:
+            o = K.attention_paged(x[:, :H], kp, vp, i32(table), cu(lens), i32(done), k_scale=ks, v_scale=vs)
+        outs[0].append(o[:lens[0]])
+        outs[1].append(o[lens[0]:])
+    k, v = K.cache_read(kp, vp, i32(table), cu(total), sum(total), k_scale=ks, v_scale=vs, dtype=DT[dt])
+    at = 0
+    for b, t in enumerate(total):
+        x = stream[b]
+        q = f64(K.rope(x[:, :H], i32(np.arange(t)), f, scale=s))
+        ref, mag, most = O.attention(q, f64(k[at:at + t]), f64(v[at:at + t]))
+        near(torch.cat(outs[b]), ref, mag, most, t, hd, dt)
+        if not quant:
+            assert torch.equal(k[at:at + t], K.rope(x[:, H:H + kv], i32(np.arange(t)), f, scale=s))
+            assert torch.equal(v[at:at + t], x[:, H + kv:])
+        at += t
+
+
+def test_a_captured_step_replays(gpu):
+    """One graph of a decoding step (rotate, write, attend) replayed over moving positions,
+    slots and lengths, with eager work between the replays."""
+    from chestnut import kernels as K
+    H, kv, hd, page, B = 8, 2, 128, 32, 3
+    f, _ = K.rope_frequencies(hd)
+    kp, vp, ks, vs = filled(60, kv, page, hd, 'bf16', 'e4m3', 3)
+    table = i32(np.random.default_rng(0).permutation(60).reshape(B, 20))
+    x = rows(1, B, H + 2 * kv, hd, 'bf16')
+    pos, slots, lens, cq = i32([0] * B), i32([-1] * B), i32([1] * B), cu([1] * B)
+
+    def step(kp, vp, ks, vs):
+        y = K.rope(x[:, :H + kv], pos, f)
+        K.cache_write(y[:, H:], x[:, H + kv:], kp, vp, slots, k_scale=ks, v_scale=vs)
+        return K.attention_paged(y[:, :H], kp, vp, table, cq, lens, k_scale=ks, v_scale=vs)
+
+    other = [t.clone() for t in (kp, vp)] + [t.view(torch.uint8).clone().view(torch.float8_e8m0fnu) for t in (ks, vs)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*other)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(kp, vp, ks, vs)
+    t = table.cpu().numpy()
+    for n in (1, 31, 32, 33, 500, 640, 7):
+        place = np.array([n, max(1, n // 2), max(1, n - 1)]) - 1
+        pos.copy_(i32(place))
+        lens.copy_(i32(place + 1))
+        slots.copy_(i32(t[np.arange(B), place // page] * page + place % page))
+        x.copy_(rows(n, B, H + 2 * kv, hd, 'bf16'))
+        want = step(*other)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), n
+        assert torch.equal(kp.view(torch.uint8), other[0].view(torch.uint8))
+
+
+def test_on_another_stream(gpu):
+    from chestnut import kernels as K
+    q, k, v = rows(1, 300, 4, 64, 'f16'), rows(2, 300, 2, 64, 'f16'), rows(3, 300, 2, 64, 'f16')
+    want = K.attention_varlen(q, k, v, cu([100, 200]))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    c = cu([100, 200])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        got = K.attention_varlen(q, k, v, c)
+    s.synchronize()
+    assert torch.equal(got, want)

@@ -1,0 +1,204 @@
+"""The token cache's operators without a GPU: what the entry points refuse, the frequencies
+of rope, and the 64-bit oracle against torch and against itself."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from chestnut import _lib
+from chestnut import kernels as K
+from oracle import token_cache as O
+
+f16, bf16, f32, i32 = torch.float16, torch.bfloat16, torch.float32, torch.int32
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def z(*shape, dtype=f16):
+    return torch.zeros(*shape, dtype=torch.uint8).view(dtype) if dtype in (E4M3, E8M0) else torch.zeros(*shape, dtype=dtype)
+
+
+def cache(n=3, kv=2, page=16, hd=64, dtype=f16):
+    return z(n, kv, page, hd, dtype=dtype), z(n, kv, page, hd, dtype=dtype)
+
+
+def paged(q=None, kp=None, vp=None, table=None, cu=None, lens=None, **kw):
+    a, b = cache()
+    return K.attention_paged(z(4, 4, 64) if q is None else q, a if kp is None else kp, b if vp is None else vp,
+                             z(2, 3, dtype=i32) if table is None else table, z(3, dtype=i32) if cu is None else cu,
+                             z(2, dtype=i32) if lens is None else lens, **kw)
+
+
+def varlen(q=None, k=None, v=None, cu=None, **kw):
+    return K.attention_varlen(z(4, 4, 64) if q is None else q, z(4, 2, 64) if k is None else k,
+                              z(4, 2, 64) if v is None else v, z(3, dtype=i32) if cu is None else cu, **kw)
+
+
+F = torch.ones(16, dtype=torch.float64)
+S = dict(k_scale=z(3, 2, 16, dtype=E8M0), v_scale=z(3, 2, 16, dtype=E8M0))
+REFUSED = [
+    ('rope x type', lambda: K.rope(z(4, 2, 64, dtype=f32), z(4, dtype=i32), F), 'x must be float16 or bfloat16'),
+    ('rope x rank', lambda: K.rope(z(4, 64), z(4, dtype=i32), F), 'x must be'),
+    ('rope positions type', lambda: K.rope(z(4, 2, 64), z(4, dtype=torch.int64), F), 'positions must be torch.int32'),
+    ('rope positions length', lambda: K.rope(z(4, 2, 64), z(5, dtype=i32), F), 'positions must have shape'),
+    ('rope inv_freq type', lambda: K.rope(z(4, 2, 64), z(4, dtype=i32), F.float()), 'inv_freq must be torch.float64'),
+    ('rope inv_freq too long', lambda: K.rope(z(4, 2, 24), z(4, dtype=i32), F), 'inv_freq must have 1 to'),
+    ('rope inv_freq empty', lambda: K.rope(z(4, 2, 24), z(4, dtype=i32), F[:0]), 'inv_freq must have 1 to'),
+    ('rope last stride', lambda: K.rope(z(4, 64, 2).transpose(1, 2), z(4, dtype=i32), F), 'contiguous in its last'),
+    ('rope out type', lambda: K.rope(z(4, 2, 64), z(4, dtype=i32), F, out=z(4, 2, 64, dtype=bf16)), 'out must be torch.float16'),
+    ('rope out overlaps itself', lambda: K.rope(z(4, 2, 64), z(4, dtype=i32), F, out=z(1, 2, 64).expand(4, 2, 64)),
+     'must not overlap itself'),
+    ('rope in place on an expanded x', lambda: (lambda x: K.rope(x, z(4, dtype=i32), F, out=x))(z(1, 2, 64).expand(4, 2, 64)),
+     'must not overlap itself'),
+    ('rope head_dim', lambda: K.rope(z(1, 1, 514), z(1, dtype=i32), F), 'head_dim up to 512'),
+    ('write cache rank', lambda: K.cache_write(z(4, 2, 64), z(4, 2, 64), z(3, 16, 64), z(3, 16, 64), z(4, dtype=i32)), 'k_pages must be'),
+    ('write page size', lambda: K.cache_write(z(4, 2, 64), z(4, 2, 64), *cache(page=24), z(4, dtype=i32)), 'power of two'),
+    ('write page too small', lambda: K.cache_write(z(4, 2, 64), z(4, 2, 64), *cache(page=8), z(4, dtype=i32)), 'power of two'),
+    ('write rows type', lambda: K.cache_write(z(4, 2, 64, dtype=bf16), z(4, 2, 64, dtype=bf16), *cache(), z(4, dtype=i32)),
+     'cache must be torch.bfloat16 or'),
+    ('write v type', lambda: K.cache_write(z(4, 2, 64), z(4, 2, 64, dtype=bf16), *cache(), z(4, dtype=i32)), 'v must be torch.float16'),
+    ('write heads', lambda: K.cache_write(z(4, 3, 64), z(4, 3, 64), *cache(), z(4, dtype=i32)), 'k must have shape'),
+    ('write slots', lambda: K.cache_write(z(4, 2, 64), z(4, 2, 64), *cache(), z(3, dtype=i32)), 'slots must have shape'),
+    ('write row alignment', lambda: K.cache_write(z(4, 2, 68)[:, :, 2:66], z(4, 2, 64), *cache(), z(4, dtype=i32)), 'multiples of 16 bytes'),
+    ('write e4m3 without scales', lambda: K.cache_write(z(4, 2, 64), z(4, 2, 64), *cache(dtype=E4M3), z(4, dtype=i32)), 'needs k_scale'),
+    ('write scales of f16', lambda: K.cache_write(z(4, 2, 64), z(4, 2, 64), *cache(), z(4, dtype=i32), **S), 'belong to an e4m3'),
+    ('write scale shape', lambda: K.cache_write(z(4, 2, 64), z(4, 2, 64), *cache(dtype=E4M3), z(4, dtype=i32),
+                                                k_scale=z(3, 2, 8, dtype=E8M0), v_scale=S['v_scale']), 'k_scale must have shape'),
+    ('write scale type', lambda: K.cache_write(z(4, 2, 64), z(4, 2, 64), *cache(dtype=E4M3), z(4, dtype=i32),
+                                               k_scale=z(3, 2, 16, dtype=torch.uint8), v_scale=S['v_scale']), 'k_scale must be'),
+    ('read dtype', lambda: K.cache_read(*cache(), z(2, 3, dtype=i32), z(3, dtype=i32), 4, dtype=bf16), 'dtype must be'),
+    ('read e4m3 without a dtype', lambda: K.cache_read(*cache(dtype=E4M3), z(2, 3, dtype=i32), z(3, dtype=i32), 4, **S), 'dtype must be'),
+    ('read cu', lambda: K.cache_read(*cache(), z(2, 3, dtype=i32), z(2, dtype=i32), 4), 'cu_seqlens must have shape'),
+    ('read tokens', lambda: K.cache_read(*cache(), z(2, 3, dtype=i32), z(3, dtype=i32), -1), 'tokens must be'),
+    ('read out', lambda: K.cache_read(*cache(), z(2, 3, dtype=i32), z(3, dtype=i32), 4, k_out=z(5, 2, 64)), 'k_out must have shape'),
+    ('varlen head_dim', lambda: varlen(z(4, 4, 96), z(4, 2, 96), z(4, 2, 96)), 'head_dim must be 64 or 128'),
+    ('varlen heads', lambda: varlen(z(4, 3, 64)), 'multiple of the K/V heads'),
+    ('varlen types', lambda: varlen(k=z(4, 2, 64, dtype=bf16)), 'k must be torch.float16'),
+    ('varlen f32', lambda: varlen(z(4, 4, 64, dtype=f32)), 'q must be float16 or bfloat16'),
+    ('varlen k rows', lambda: varlen(k=z(5, 2, 64), v=z(5, 2, 64)), 'k must have the 4 rows'),
+    ('varlen v rows', lambda: varlen(v=z(5, 2, 64)), 'v must have shape'),
+    ('varlen cu_k', lambda: varlen(cu_k=z(4, dtype=i32)), 'cu_k must have shape'),
+    ('varlen cu type', lambda: varlen(cu=z(3, dtype=torch.int64)), 'cu_q must be torch.int32'),
+    ('varlen cu empty', lambda: varlen(cu=z(0, dtype=i32)), 'B \\+ 1 offsets'),
+    ('varlen scale', lambda: varlen(scale=0.0), 'scale must be positive'),
+    ('varlen nan scale', lambda: varlen(scale=math.nan), 'scale must be positive'),
+    ('varlen out', lambda: varlen(out=z(4, 4, 65)[:, :, :64]), 'multiples of 8 bytes'),
+    ('varlen q alignment', lambda: varlen(z(4, 4, 72)[:, :, 1:65]), 'multiples of 16 bytes'),
+    ('varlen out overlaps itself', lambda: varlen(out=z(1, 4, 64).expand(4, 4, 64)), 'must not overlap itself'),
+    ('paged cache type', lambda: paged(z(4, 4, 64, dtype=bf16)), 'cache must be torch.bfloat16 or'),
+    ('paged head_dim', lambda: paged(z(4, 4, 128)), 'head_dim must be 64 or 128 for q and the keys alike'),
+    ('paged table rows', lambda: paged(table=z(3, 3, dtype=i32)), 'block_table must have shape'),
+    ('paged table type', lambda: paged(table=z(2, 3, dtype=torch.int64)), 'block_table must be torch.int32'),
+    ('paged lens', lambda: paged(lens=z(3, dtype=i32)), 'kv_lens must have shape'),
+    ('paged table strided', lambda: paged(table=z(2, 6, dtype=i32)[:, ::2]), 'block_table must be contiguous'),
+    ('paged cpu tensors', paged, 'must be a CUDA tensor'),
+    ('varlen cpu tensors', varlen, 'must be a CUDA tensor'),
+    ('rope cpu tensors', lambda: K.rope(z(4, 2, 64), z(4, dtype=i32), F), 'must be a CUDA tensor'),
+    ('write cpu tensors', lambda: K.cache_write(z(4, 2, 64), z(4, 2, 64), *cache(), z(4, dtype=i32)), 'must be a CUDA tensor'),
+    ('read cpu tensors', lambda: K.cache_read(*cache(), z(2, 3, dtype=i32), z(3, dtype=i32), 4), 'must be a CUDA tensor'),
+]
+
+
+@pytest.mark.parametrize('name,fn,msg', REFUSED, ids=[r[0] for r in REFUSED])
+def test_refused_with_value_error(name, fn, msg):
+    with pytest.raises(ValueError, match=msg):
+        fn()
+
+
+# The native entry points check again what reaches them as plain numbers (no call below launches).
+X = ctypes.c_void_p(1 << 20)      # an aligned address that nothing reads
+
+
+def attn(T=4, H=4, n=3, kv=2, page=16, hd=64, dtype=1, cdtype=1, scale=0.1, q=X, ks=None, width=3, st=256):
+    return ('ck_attention_paged', q, X, X, ks, ks, X, X, width, X, X, 2, T, H, n, kv, page, hd, st, hd, st, hd, dtype, cdtype, 1,
+            scale, None, 0, None)
+
+
+NATIVE = [
+    ('rope rot', ('ck_rope', X, X, X, X, 4, 2, 64, 7, 128, 64, 128, 64, 1, 0, 1.0, 0, None), 'must be even'),
+    ('rope dtype', ('ck_rope', X, X, X, X, 4, 2, 64, 64, 128, 64, 128, 64, 0, 0, 1.0, 0, None), 'f16 or bf16'),
+    ('rope null', ('ck_rope', None, X, X, X, 4, 2, 64, 64, 128, 64, 128, 64, 1, 0, 1.0, 0, None), 'null pointer'),
+    ('rope in place', ('ck_rope', X, X, X, X, 4, 2, 64, 64, 128, 64, 256, 64, 1, 0, 1.0, 0, None), 'in place'),
+    ('write page', ('ck_cache_write', X, X, X, X, None, None, X, 4, 3, 2, 24, 64, 128, 64, 128, 64, 1, 1, None), 'power of two'),
+    ('write type', ('ck_cache_write', X, X, X, X, None, None, X, 4, 3, 2, 16, 64, 128, 64, 128, 64, 1, 4, None), "rows' type or e4m3"),
+    ('write scales', ('ck_cache_write', X, X, X, X, None, None, X, 4, 3, 2, 16, 64, 128, 64, 128, 64, 1, 5, None), 'needs its scales'),
+    ('write stride', ('ck_cache_write', X, X, X, X, None, None, X, 4, 3, 2, 16, 64, 130, 64, 128, 64, 1, 1, None), '16-byte aligned'),
+    ('write slots', ('ck_cache_write', X, X, X, X, None, None, X, 4, 1 << 28, 2, 16, 64, 128, 64, 128, 64, 1, 1, None), '2\\^31 slots'),
+    ('read null', ('ck_cache_read', X, X, None, None, None, 3, X, 2, 4, 3, 2, 16, 64, X, X, 1, 1, None), 'null pointer'),
+    ('paged heads', attn(H=3), 'multiple of the K/V heads'),
+    ('paged head_dim', attn(hd=96), 'head_dim must be 64 or 128'),
+    ('paged dtype', attn(dtype=0), 'q must be f16 or bf16|of q'),
+    ('paged cache dtype', attn(cdtype=4), "q's type or e4m3"),
+    ('paged scales', attn(cdtype=5), 'needs its scales'),
+    ('paged scale', attn(scale=-1.0), 'positive and finite'),
+    ('paged null', attn(q=None), 'null pointer'),
+    ('paged stride', attn(st=250), 'aligned'),
+]
+
+
+@pytest.mark.parametrize('name,args,msg', NATIVE, ids=[r[0] for r in NATIVE])
+def test_native_checks(name, args, msg):
+    with pytest.raises(RuntimeError, match=msg):
+        _lib.call(*args)
+
+
+def test_frequencies():
+    f, s = K.rope_frequencies(8, base=100.0, device='cpu')
+    assert s == 1.0 and f.dtype is torch.float64 and np.allclose(f, [100.0 ** (-i / 4) for i in range(4)], rtol=1e-15)
+    g, s = K.rope_frequencies(8, base=100.0, method='linear', factor=4.0, device='cpu')
+    assert s == 1.0 and torch.equal(g, f / 4)
+    g, _ = K.rope_frequencies(8, base=100.0, method='base', factor=4.0, device='cpu')
+    assert g[0] == 1.0 and math.isclose(g[-1], f[-1] / 4, rel_tol=1e-14)
+    g, s = K.rope_frequencies(128, method='parts', factor=8.0, context=4096, device='cpu')
+    f, _ = K.rope_frequencies(128, device='cpu')
+    turns = 4096 * f / (2 * math.pi)
+    assert torch.equal(g[turns >= 32], f[turns >= 32]) and torch.equal(g[turns <= 1], f[turns <= 1] / 8)
+    mid = (turns > 1) & (turns < 32)
+    assert mid.any() and (g[mid] < f[mid]).all() and (g[mid] > f[mid] / 8).all() and math.isclose(s, 0.1 * math.log(8) + 1)
+    for bad in (dict(rot=7), dict(rot=0), dict(rot=8, method='x'), dict(rot=8, factor=0.5), dict(rot=2, method='base'),
+                dict(rot=8, method='parts', factor=2.0), dict(rot=8, base=1.0)):
+        with pytest.raises(ValueError):
+            K.rope_frequencies(device='cpu', **bad)
+
+
+def test_oracle_codes_are_the_formats():
+    v = O.e4m3_values()
+    t = torch.arange(256, dtype=torch.uint8).view(E4M3).double().numpy()
+    assert np.array_equal(v[~np.isnan(v)], t[~np.isnan(t)]) and np.array_equal(np.isnan(v), np.isnan(t))
+    x = np.concatenate([np.random.default_rng(0).standard_normal(5000) * 100, v[~np.isnan(v)], (v[:126] + v[1:127]) / 2,
+                        np.arange(-40, 40) * 2.0 ** -11]).clip(-448, 448).astype(np.float32)
+    assert np.array_equal(O.e4m3_codes(x.astype(np.float64)), torch.from_numpy(x).to(E4M3).view(torch.uint8).numpy())
+
+
+def test_oracle_rows_hold_half_a_step():
+    x = np.random.default_rng(1).standard_normal((50, 64)) * np.logspace(-4, 4, 50)[:, None]
+    c, b = O.quantise(x, 61440.0)
+    y, s = O.values(c, b), 2.0 ** (b.astype(float) - 127)
+    assert np.all(np.abs(x) <= 448 * s[:, None]) and np.all(np.abs(x).max(-1) > 224 * s)
+    assert np.all(np.abs(y - x) <= np.maximum(2.0 ** -4 * np.abs(x), 2.0 ** -10 * s[:, None]))
+
+
+@pytest.mark.parametrize('n,m,causal', [(5, 5, True), (3, 9, True), (6, 2, True), (4, 7, False), (2, 0, True)])
+def test_oracle_attention_is_the_masked_softmax(n, m, causal):
+    r = np.random.default_rng(n + m)
+    q, k, v = r.standard_normal((n, 4, 8)), r.standard_normal((m, 2, 8)), r.standard_normal((m, 2, 8))
+    out, mag, _ = O.attention(q, k, v, causal)
+    for i in range(n):
+        for h in range(4):
+            js = [j for j in range(m) if not causal or j <= i + m - n]
+            w = np.array([math.exp(q[i, h] @ k[j, h // 2] / math.sqrt(8)) for j in js])
+            want = sum((x * v[j, h // 2] for x, j in zip(w / w.sum(), js)), np.zeros(8)) if js else np.zeros(8)
+            assert np.allclose(out[i, h], want, atol=1e-12) and np.all(mag[i, h] >= np.abs(want) - 1e-12)
+
+
+def test_oracle_rope_turns_and_turns_back():
+    x = np.random.default_rng(2).standard_normal((4, 2, 12))
+    f = np.array([1.0, 0.1, 0.01])
+    for inter in (False, True):
+        y = O.rope(x, [0, 1, 5, 1000], f, inter, 2.0)
+        assert np.allclose(y[0, :, :6], 2 * x[0, :, :6]) and np.array_equal(y[..., 6:], x[..., 6:])
+        assert np.allclose(O.rope(y, [0, 1, 5, 1000], f, inter, 0.5, True), x)
+        i, j = (0, 1) if inter else (0, 3)
+        z = (x[2, 1, i] + 1j * x[2, 1, j]) * np.exp(5j) * 2
+        assert np.allclose([y[2, 1, i], y[2, 1, j]], [z.real, z.imag])
