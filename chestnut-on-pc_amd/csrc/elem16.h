@@ -31,6 +31,9 @@ struct Elem<half_t> {
   static __device__ __forceinline__ float16_t mfma32(v8 a, v8 b, float16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
+  static __device__ __forceinline__ float add2(v2 a, float c) {   // c + a[0] + a[1]
+    return __builtin_amdgcn_fdot2(a, v2{(half_t)1.0f, (half_t)1.0f}, c, false);
+  }
 };
 template <>
 struct Elem<bf16_t> {
@@ -41,6 +44,9 @@ struct Elem<bf16_t> {
   static constexpr unsigned EXP = 0x7F807F80u, LOW = 0x00800080u;
   static __device__ __forceinline__ float16_t mfma32(v8 a, v8 b, float16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float add2(v2 a, float c) {
+    return __builtin_amdgcn_fdot2_f32_bf16(a, v2{(bf16_t)1.0f, (bf16_t)1.0f}, c, false);
   }
 };
 

@@ -305,6 +305,12 @@ def test_index_values_outside_the_tensors_stay_inside(gpu):
     assert (guard[0] == 4.0).all() and (guard[5] == 4.0).all()
     ref, mag, most = O.attention(f64(q[:1]), gathered(kp, None, np.array([0, 1]), 20, page), gathered(vp, None, np.array([0, 1]), 20, page))
     near(guard[1:2], ref, mag, most, 20, hd, 'f16')
+    # offsets that do not ascend name more rows than there are
+    kp2, vp2, _, _ = filled(200, kv, page, hd, 'f16', 'f16', 2)
+    buf = torch.full((42, H, hd), 4.0, dtype=torch.float16, device='cuda')
+    K.attention_paged(rows(2, 40, H, hd, 'f16'), kp2, vp2, i32([list(range(200))] * 5), i32([0, 40, 0, 40, 0, 40]),
+                      i32([3000] * 5), out=buf[1:41])
+    assert (buf[0] == 4.0).all() and (buf[41] == 4.0).all()
     k, v = K.cache_read(kp, vp, i32([[0, -1], [50, 1]]), i32([0, 17, 40]), 30)
     assert torch.equal(k[:16], kp[0].permute(1, 0, 2)) and k.shape == (30, kv, hd)
     K.cache_read(kp, vp, i32([[0, -1], [50, 1]]), i32([5, -3, 10 ** 9]), 30)
