@@ -204,6 +204,28 @@ struct Stage {
       }
     }
   }
+  // load() straight into LDS, as store() would leave it: a wave's 64 pieces of 16 bytes land side by
+  // side, so each lane fetches the chunk that belongs in its place
+  __device__ __forceinline__ void dma(const AttendParams& p, const Item& it, int hk, int key0, int tid, int wave, T* kt, T* vt) const {
+    typedef const __attribute__((address_space(1))) void* src_t;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int row = i * RPL + tid / CPR, pos = tid % CPR, key = min(key0 + row, it.s.nk - 1);
+      const int ck = (k_at<HD>(row, pos) >> 3) % CPR, cv = (v_at<HD>(row, pos) >> 3) % CPR;
+      const T *kb, *vb;
+      if constexpr (KV == KV_ROWS) {
+        kb = static_cast<const T*>(p.k) + (long)(it.s.k0 + key) * p.k_st + (long)hk * p.k_sh;
+        vb = static_cast<const T*>(p.v) + (long)(it.s.k0 + key) * p.v_st + (long)hk * p.v_sh;
+      } else {
+        const long pg = min(max(page[i], 0), p.n_pages - 1);
+        const long at = ((pg * p.Hkv + hk) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
+        kb = static_cast<const T*>(p.k) + at * HD;
+        vb = static_cast<const T*>(p.v) + at * HD;
+      }
+      __builtin_amdgcn_global_load_lds((src_t)(kb + ck * 8), (lds_ptr_t)(kt + (i * NT + wave * 64) * 8), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((src_t)(vb + cv * 8), (lds_ptr_t)(vt + (i * NT + wave * 64) * 8), 16, 0, 0);
+    }
+  }
   static __device__ __forceinline__ v8 values(unsigned lo, unsigned hi, float s) {
     v2 a, b, c, d;
     if constexpr (std::is_same_v<T, half_t>) {
@@ -219,35 +241,23 @@ struct Stage {
     }
     return v8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
   }
-  static __device__ __forceinline__ unsigned odd(v8 x) {
-    const u32x4_t u = __builtin_bit_cast(u32x4_t, x);
-    return ((u[0] & Elem<T>::EXP) + Elem<T>::LOW) | ((u[1] & Elem<T>::EXP) + Elem<T>::LOW) |
-           ((u[2] & Elem<T>::EXP) + Elem<T>::LOW) | ((u[3] & Elem<T>::EXP) + Elem<T>::LOW);
-  }
-  // look: whether to look for infinities and NaN in V; true if this thread's part has one
-  __device__ __forceinline__ bool store(T* kt, T* vt, int tid, bool look) const {
-    unsigned acc = 0;
+  __device__ __forceinline__ void store(T* kt, T* vt, int tid) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int key = i * RPL + tid / CPR, c = tid % CPR;
       if constexpr (KV != KV_E4M3) {
-        const v8 x = __builtin_bit_cast(v8, v[i]);
         *reinterpret_cast<raw*>(kt + k_at<HD>(key, c)) = k[i];
-        *reinterpret_cast<v8*>(vt + v_at<HD>(key, c)) = x;
-        if (look) acc |= odd(x);
+        *reinterpret_cast<raw*>(vt + v_at<HD>(key, c)) = v[i];
       } else {
         const float fk = __builtin_bit_cast(float, ks[i] << 23), fv = __builtin_bit_cast(float, vs[i] << 23);
 #pragma unroll
         for (int j = 0; j < EPL / 8; ++j) {
           const int cc = c * (EPL / 8) + j;
-          const v8 x = values(v[i][2 * j], v[i][2 * j + 1], fv);
           *reinterpret_cast<v8*>(kt + k_at<HD>(key, cc)) = values(k[i][2 * j], k[i][2 * j + 1], fk);
-          *reinterpret_cast<v8*>(vt + v_at<HD>(key, cc)) = x;
-          if (look) acc |= odd(x);
+          *reinterpret_cast<v8*>(vt + v_at<HD>(key, cc)) = values(v[i][2 * j], v[i][2 * j + 1], fv);
         }
       }
     }
-    return acc & 0x80008000u;
   }
 };
 
@@ -297,6 +307,11 @@ struct Rows {
     for (int ct = 0; ct < CT; ++ct) o[ct] = float16_t{};
     m = -INFINITY;
     l = 0.f;
+  }
+
+  __device__ __forceinline__ void arrived() {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
   }
 
   // NB blocks of 32 keys from key0 on, in LDS.  part: some row may not see all of them.
@@ -379,8 +394,8 @@ struct Rows {
         float add = bad[0][d] < lim ? INFINITY : 0.f;
         add += bad[1][d] < lim ? -INFINITY : 0.f;
         add += bad[2][d] < lim ? NAN : 0.f;
+        asm volatile("" : "+v"(add)::"memory");   // one element at a time: a rare path, and no registers for it
         o[ct][i] += add;
-        __builtin_amdgcn_sched_barrier(0);
       }
   }
   __device__ __forceinline__ float sum() const { return l + __shfl_xor(l, 32); }
@@ -398,6 +413,19 @@ struct Rows {
       }
   }
 };
+
+// Whether this thread's part of a tile in LDS holds an infinity or a NaN.
+template <typename T, int TILE, int NT>
+__device__ __forceinline__ bool any_odd(const T* vt, int tid) {
+  unsigned acc = 0;
+#pragma unroll
+  for (int i = 0; i < TILE / 8 / NT; ++i) {
+    const u32x4_t u = reinterpret_cast<const u32x4_t*>(vt)[i * NT + tid];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc |= (u[j] & Elem<T>::EXP) + Elem<T>::LOW;
+  }
+  return acc & 0x80008000u;
+}
 
 // Takes infinities and NaN out of a V tile in LDS: zero in their places, the first key of
 // each kind and feature in bad.  For the rows that do not see them (0 * inf is not 0).
@@ -423,18 +451,19 @@ __device__ __forceinline__ float2_t* part_ml(const AttendParams& p, long row) {
 }
 
 // ---- many rows: NW waves of 32 rows over the same keys -----------------------------------
+// Tiles of 64 keys in two buffers: the next one is under way (f16, bf16: straight to LDS;
+// e4m3: through registers, where it is turned into values) while this one is used.
 template <typename T, int HD, int KV, int NW>
-__global__ __launch_bounds__(64 * NW) void attend_tile_kernel(const AttendParams p) {
+__global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendParams p) {
   constexpr int BM = 32 * NW, TILE = AT_KEYS * HD, NT = 64 * NW;
-  __shared__ __attribute__((aligned(16))) T kt[2][TILE], vt[2][TILE];
-  __shared__ int bad[3][HD], odd[2];
+  constexpr bool DMA = KV != KV_E4M3;
+  __shared__ __attribute__((aligned(1024))) T kt[2][TILE], vt[2][TILE];
+  __shared__ int bad[3][HD], odd;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hk = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv;
   Item it;
   if (!find_item<KV, BM, false>(p, index, it)) return;
   const int tile = tiles_of<KV, BM>(it.s, p.G) - 1 - it.tile;   // the longest first
-  Rows<T, HD> r;
-  r.begin(p, it, hk, tile * BM + wave * 32 + (lane & 31), lane);
   // the keys of the tile's first and last rows, and of this chunk
   const int klo = keys_of(p, it.s, tile * BM / p.G);
   const int khi = keys_of(p, it.s, min(it.s.nq - 1, (tile * BM + BM - 1) / p.G));
@@ -442,37 +471,47 @@ __global__ __launch_bounds__(64 * NW) void attend_tile_kernel(const AttendParams
   const int kend = it.nch > 1 ? min(khi, kbeg + it.c * AT_KEYS) : khi;
 
   Stage<T, HD, KV, AT_KEYS, NT> st;
-  if (tid < 2) odd[tid] = 0;
+  if (tid == 0) odd = 0;
   if (kbeg < kend) {
     st.pages(p, it, kbeg, wave);
-    st.load(p, it, hk, kbeg, tid);
+    if constexpr (DMA) st.dma(p, it, hk, kbeg, tid, wave, kt[0], vt[0]);
+    else st.load(p, it, hk, kbeg, tid);
     st.pages(p, it, kbeg + AT_KEYS, wave);
-    __syncthreads();
-    if (st.store(kt[0], vt[0], tid, kbeg + AT_KEYS > klo)) odd[0] = 1;
   }
+  Rows<T, HD> r;
+  r.begin(p, it, hk, tile * BM + wave * 32 + (lane & 31), lane);
+  // Q has arrived before the loop, whose waits would otherwise count its loads every time
+  r.arrived();
+  if (!DMA && kbeg < kend) st.store(kt[0], vt[0], tid);
   for (int key0 = kbeg, cur = 0; key0 < kend; key0 += AT_KEYS, cur ^= 1) {
     const bool more = key0 + AT_KEYS < kend;
+    __syncthreads();   // this tile is there, and the other buffer is free
     if (more) {
-      st.load(p, it, hk, key0 + AT_KEYS, tid);
+      if constexpr (DMA) st.dma(p, it, hk, key0 + AT_KEYS, tid, wave, kt[cur ^ 1], vt[cur ^ 1]);
+      else st.load(p, it, hk, key0 + AT_KEYS, tid);
       st.pages(p, it, key0 + 2 * AT_KEYS, wave);
     }
-    __syncthreads();
-    // a tile that some row sees in part: an infinity or NaN of V must not reach that row
+    // A tile that some row sees in part: an infinity or NaN of V must not reach that row.
     const bool part = key0 + AT_KEYS > klo;
-    const bool fix = part && odd[cur];
-    if (fix) {
-      for (int i = tid; i < 3 * HD; i += NT) (&bad[0][0])[i] = 0x7FFFFFFF;
+    bool fix = false;
+    if (part) {
+      if (any_odd<T, TILE, NT>(vt[cur], tid)) odd = 1;
       __syncthreads();
-      take_out_odd<T, HD, AT_KEYS, NT>(vt[cur], bad, key0, tid);
-      __syncthreads();
+      fix = odd;
+      if (fix) {
+        for (int i = tid; i < 3 * HD; i += NT) (&bad[0][0])[i] = 0x7FFFFFFF;
+        __syncthreads();
+        take_out_odd<T, HD, AT_KEYS, NT>(vt[cur], bad, key0, tid);
+        __syncthreads();
+      }
     }
     r.template step<2>(kt[cur], vt[cur], key0, part, p.scale_log2e, lane);
     if (fix) {
       r.add_odd(bad, lane);
       __syncthreads();
-      if (tid == 0) odd[cur] = 0;
+      if (tid == 0) odd = 0;
     }
-    if (more && st.store(kt[cur ^ 1], vt[cur ^ 1], tid, key0 + 2 * AT_KEYS > klo)) odd[cur ^ 1] = 1;
+    if (!DMA && more) st.store(kt[cur ^ 1], vt[cur ^ 1], tid);
   }
 
   if (it.nch == 1) {
@@ -514,6 +553,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attend_few_kernel(const Att
   const int kbeg = it.nch > 1 ? it.chunk * it.c * AT_KEYS : 0;
   const int kend = it.nch > 1 ? min(khi, kbeg + it.c * AT_KEYS) : khi;
 
+  r.arrived();
   Stage<T, HD, KV, KEYS, 64> st;
   T* const kt = lds[wave];
   T* const vt = kt + TILE;
@@ -526,12 +566,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attend_few_kernel(const Att
   for (; key0 < kend; key0 += NW * KEYS) {
     const bool part = key0 + KEYS > klo;
     wave_order();
-    const bool fix = __any(st.store(kt, vt, lane, part));
+    st.store(kt, vt, lane);
     if (key0 + NW * KEYS < kend) {
       st.load(p, it, hk, key0 + NW * KEYS, lane);
       st.pages(p, it, key0 + 2 * NW * KEYS, 0);
     }
     wave_order();
+    const bool fix = part && __any(any_odd<T, TILE, 64>(vt, lane));
     if (fix) {
       for (int i = lane; i < 3 * HD; i += 64) (&bad[wave][0][0])[i] = 0x7FFFFFFF;
       wave_order();
