@@ -158,10 +158,9 @@ __device__ __forceinline__ int v_at(int key, int c) {
   return HD == 128 ? key * HD + ((c ^ ((key & 3) << 2)) << 3) : key * HD + ((c ^ ((key & 2) << 1)) << 3);
 }
 
-// KEYS rows of K and V on their way through the registers of NT threads: load() sends for
-// them, store() leaves them (e4m3: as values of T) in LDS.  Places behind the last key
-// repeat it.  A wave's rows of one load lie in one group of 16, so on one page.
-template <typename T, int HD, int KV, int KEYS, int NT>
+// KEYS rows of K or V on their way to LDS by NT threads.  Places behind the last key repeat
+// it.  A wave's rows of one load lie in one group of 16, so on one page.
+template <typename T, int HD, int KV, int KEYS, int NT, bool V>
 struct Stage {
   typedef typename Elem<T>::v2 v2;
   typedef typename Elem<T>::v8 v8;
@@ -170,10 +169,11 @@ struct Stage {
   static constexpr int BPL = KV == KV_E4M3 ? EPL : 16;                         // bytes per load
   typedef std::conditional_t<BPL == 16, u32x4_t, u32x2_t> raw;
   static_assert(N * NT == KEYS * CPR && (RPL >= 16 || 16 % RPL == 0), "tile");
-  raw k[N], v[N];
-  unsigned ks[N], vs[N];
+  raw x[N];
+  unsigned scale[N];
   int page[N];
 
+  static __device__ __forceinline__ int at(int key, int c) { return V ? v_at<HD>(key, c) : k_at<HD>(key, c); }
   // the pages of the keys from key0 on
   __device__ __forceinline__ void pages(const AttendParams& p, const Item& it, int key0, int wave) {
     if constexpr (KV != KV_ROWS) {
@@ -184,47 +184,66 @@ struct Stage {
       }
     }
   }
-  __device__ __forceinline__ void load(const AttendParams& p, const Item& it, int hk, int key0, int tid) {
+  // Load i brings the rows from first(key0, i) on to a wave: their place in the cache (or among
+  // the packed rows) is the same for all lanes but for lane_row() rows of `pitch` bytes.
+  static __device__ __forceinline__ int lane_row(int lane) { return lane / CPR; }
+  static __device__ __forceinline__ int first(int key0, int i, int wave) { return key0 + i * RPL + wave * (64 / CPR); }
+  __device__ __forceinline__ long row_of(const AttendParams& p, const Item& it, int hk, int key, int i) const {
+    if constexpr (KV == KV_ROWS) return it.s.k0 + key;
+    const long pg = min(max(__builtin_amdgcn_readfirstlane(page[i]), 0), p.n_pages - 1);
+    return ((pg * p.Hkv + hk) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
+  }
+  static __device__ __forceinline__ const char* base(const AttendParams& p, int hk) {
+    const char* b = static_cast<const char*>(V ? p.v : p.k);
+    if constexpr (KV == KV_ROWS) b += (long)hk * (V ? p.v_sh : p.k_sh) * 2;
+    return b;
+  }
+  static __device__ __forceinline__ long pitch(const AttendParams& p) {
+    if constexpr (KV == KV_ROWS) return (V ? p.v_st : p.k_st) * 2;
+    return HD / EPL * BPL;
+  }
+  // bytes from a load's first row to the lane's piece (for good: begin() once)
+  unsigned lane_off;
+  int piece;
+  __device__ __forceinline__ void begin(const AttendParams& p, int lane, int wave, bool swizzled) {
+    // straight to LDS a wave's 64 pieces of 16 bytes land side by side, so each lane fetches the
+    // chunk that belongs in its place
+    piece = swizzled ? (at(first(0, 0, wave) + lane_row(lane), lane % CPR) >> 3) % CPR * 16 : lane % CPR * BPL;
+    lane_off = lane_row(lane) * (unsigned)pitch(p) + piece;
+    asm volatile("" : "+v"(lane_off));
+  }
+  // f(i, address of the lane's piece, its row's number) for every load
+  template <typename F>
+  __device__ __forceinline__ void rows(const AttendParams& p, const Item& it, int hk, int key0, int lane, int wave, F f) const {
+    if (key0 + KEYS <= it.s.nk) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int key = min(key0 + i * RPL + tid / CPR, it.s.nk - 1), c = tid % CPR;
-      if constexpr (KV == KV_ROWS) {
-        k[i] = *reinterpret_cast<const raw*>(static_cast<const T*>(p.k) + (long)(it.s.k0 + key) * p.k_st + (long)hk * p.k_sh + c * 8);
-        v[i] = *reinterpret_cast<const raw*>(static_cast<const T*>(p.v) + (long)(it.s.k0 + key) * p.v_st + (long)hk * p.v_sh + c * 8);
-      } else {
-        const long pg = min(max(page[i], 0), p.n_pages - 1);
-        const long at = ((pg * p.Hkv + hk) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
-        const long off = at * (HD / EPL * BPL) + c * BPL;
-        k[i] = *reinterpret_cast<const raw*>(static_cast<const char*>(p.k) + off);
-        v[i] = *reinterpret_cast<const raw*>(static_cast<const char*>(p.v) + off);
-        if constexpr (KV == KV_E4M3) {
-          ks[i] = p.ks[at];
-          vs[i] = p.vs[at];
-        }
+      for (int i = 0; i < N; ++i) {
+        const long row = row_of(p, it, hk, first(key0, i, wave), i);
+        const char* b = base(p, hk) + row * pitch(p);
+        f(i, b + lane_off, row + lane_row(lane));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const long row = row_of(p, it, hk, min(first(key0, i, wave) + lane_row(lane), it.s.nk - 1), i);
+        f(i, base(p, hk) + row * pitch(p) + piece, row);
       }
     }
   }
-  // load() straight into LDS, as store() would leave it: a wave's 64 pieces of 16 bytes land side by
-  // side, so each lane fetches the chunk that belongs in its place
-  __device__ __forceinline__ void dma(const AttendParams& p, const Item& it, int hk, int key0, int tid, int wave, T* kt, T* vt) const {
+  // sends for the rows; store() leaves them (e4m3: as values of T) in LDS
+  __device__ __forceinline__ void load(const AttendParams& p, const Item& it, int hk, int key0, int lane, int wave) {
+    rows(p, it, hk, key0, lane, wave, [&](int i, const char* at, long row) {
+      x[i] = *reinterpret_cast<const raw*>(at);
+      if constexpr (KV == KV_E4M3) scale[i] = (V ? p.vs : p.ks)[row];
+    });
+  }
+  // load() straight into LDS, as store() would leave it
+  __device__ __forceinline__ void dma(const AttendParams& p, const Item& it, int hk, int key0, int lane, int wave, T* t) const {
     typedef const __attribute__((address_space(1))) void* src_t;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int row = i * RPL + tid / CPR, pos = tid % CPR, key = min(key0 + row, it.s.nk - 1);
-      const int ck = (k_at<HD>(row, pos) >> 3) % CPR, cv = (v_at<HD>(row, pos) >> 3) % CPR;
-      const T *kb, *vb;
-      if constexpr (KV == KV_ROWS) {
-        kb = static_cast<const T*>(p.k) + (long)(it.s.k0 + key) * p.k_st + (long)hk * p.k_sh;
-        vb = static_cast<const T*>(p.v) + (long)(it.s.k0 + key) * p.v_st + (long)hk * p.v_sh;
-      } else {
-        const long pg = min(max(page[i], 0), p.n_pages - 1);
-        const long at = ((pg * p.Hkv + hk) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
-        kb = static_cast<const T*>(p.k) + at * HD;
-        vb = static_cast<const T*>(p.v) + at * HD;
-      }
-      __builtin_amdgcn_global_load_lds((src_t)(kb + ck * 8), (lds_ptr_t)(kt + (i * NT + wave * 64) * 8), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((src_t)(vb + cv * 8), (lds_ptr_t)(vt + (i * NT + wave * 64) * 8), 16, 0, 0);
-    }
+    static_assert(RPL % 16 == 0, "the chunk of a lane is that of every load");
+    rows(p, it, hk, key0, lane, wave, [&](int i, const char* from, long) {
+      __builtin_amdgcn_global_load_lds((src_t)from, (lds_ptr_t)(t + (i * NT + wave * 64) * 8), 16, 0, 0);
+    });
   }
   static __device__ __forceinline__ v8 values(unsigned lo, unsigned hi, float s) {
     v2 a, b, c, d;
@@ -241,21 +260,17 @@ struct Stage {
     }
     return v8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
   }
-  __device__ __forceinline__ void store(T* kt, T* vt, int tid) const {
+  __device__ __forceinline__ void store(T* t, int tid) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int key = i * RPL + tid / CPR, c = tid % CPR;
       if constexpr (KV != KV_E4M3) {
-        *reinterpret_cast<raw*>(kt + k_at<HD>(key, c)) = k[i];
-        *reinterpret_cast<raw*>(vt + v_at<HD>(key, c)) = v[i];
+        *reinterpret_cast<raw*>(t + at(key, c)) = x[i];
       } else {
-        const float fk = __builtin_bit_cast(float, ks[i] << 23), fv = __builtin_bit_cast(float, vs[i] << 23);
+        const float f = __builtin_bit_cast(float, scale[i] << 23);
 #pragma unroll
-        for (int j = 0; j < EPL / 8; ++j) {
-          const int cc = c * (EPL / 8) + j;
-          *reinterpret_cast<v8*>(kt + k_at<HD>(key, cc)) = values(k[i][2 * j], k[i][2 * j + 1], fk);
-          *reinterpret_cast<v8*>(vt + v_at<HD>(key, cc)) = values(v[i][2 * j], v[i][2 * j + 1], fv);
-        }
+        for (int j = 0; j < EPL / 8; ++j)
+          *reinterpret_cast<v8*>(t + at(key, c * (EPL / 8) + j)) = values(x[i][2 * j], x[i][2 * j + 1], f);
       }
     }
   }
@@ -314,36 +329,41 @@ struct Rows {
     for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
   }
 
-  // NB blocks of 32 keys from key0 on, in LDS.  part: some row may not see all of them.
+  // S^T of NB blocks of 32 keys in LDS
   template <int NB>
-  __device__ __forceinline__ void step(const T* kt, const T* vt, int key0, bool part, float c, int lane) {
-    const int half = lane >> 5, r32 = lane & 31;
-    float16_t s[NB];
+  __device__ __forceinline__ void scores(float16_t (&s)[NB], const T* kt, int lane) const {
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) {
       s[kb] = float16_t{};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const v8 kf = *reinterpret_cast<const v8*>(kt + k_at<HD>(kb * 32 + r32, ks * 2 + half));
+        const v8 kf = *reinterpret_cast<const v8*>(kt + k_at<HD>(kb * 32 + (lane & 31), ks * 2 + (lane >> 5)));
         s[kb] = Elem<T>::mfma32(kf, qf[ks], s[kb]);
       }
     }
-    if (part) {
-      const int left = lim - key0 - 4 * half;
+  }
+  // nothing of the keys from key0 on that the row does not see
+  template <int NB>
+  __device__ __forceinline__ void mask(float16_t (&s)[NB], int key0, int lane) const {
+    const int left = lim - key0 - 4 * (lane >> 5);
 #pragma unroll
-      for (int kb = 0; kb < NB; ++kb)
+    for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (kb * 32 + 8 * (i >> 2) + (i & 3) >= left) s[kb][i] = -INFINITY;
-    }
+      for (int i = 0; i < 16; ++i)
+        if (kb * 32 + 8 * (i >> 2) + (i & 3) >= left) s[kb][i] = -INFINITY;
+  }
+  template <int NB>
+  static __device__ __forceinline__ float top(const float16_t (&s)[NB]) {
     float mx = s[0][0];
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
-    mx = half_max(mx);
-    // The maximum that the exponents are taken from may lag behind the true one by 2^8: O and l
-    // are rescaled only when some row's has moved further, so hardly ever after the first tiles.
+    return half_max(mx);
+  }
+  // The maximum that the exponents are taken from may lag behind the true one by 2^8: O and l
+  // are rescaled only when some row's has moved further, so hardly ever after the first tiles.
+  __device__ __forceinline__ void raise(float mx, float c) {
     if (__any((mx - m) * c > 8.0f || (m == -INFINITY && mx > -INFINITY))) {
       const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
       m = mn;
@@ -351,50 +371,134 @@ struct Rows {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) o[ct] *= f;
     }
-    const float mc = m == -INFINITY ? 0.f : m * c;
-    v8 pf[2 * NB];
+  }
+  // the weights, rounded, as the product takes them; the sum is that of the rounded ones, so
+  // their rounding cancels where few keys rule
+  __device__ __forceinline__ float origin(float c) const { return m == -INFINITY ? 0.f : m * c; }
+  template <int NB>
+  __device__ __forceinline__ void weigh(v8 (&pf)[2 * NB], const float16_t (&s)[NB], int pair, float c, float mc) {
+    const int kb = pair >> 3, i = (pair & 7) * 2;
+    const v2 u = pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], c, -mc)),
+                          __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i + 1], c, -mc)));
+    l = Elem<T>::add2(u, l);
+    pf[pair >> 2][i & 7] = u[0];
+    pf[pair >> 2][(i & 7) + 1] = u[1];
+  }
+  template <int NB>
+  __device__ __forceinline__ void weights(v8 (&pf)[2 * NB], const float16_t (&s)[NB], float c) {
+    const float mc = origin(c);
 #pragma unroll
-    for (int kb = 0; kb < NB; ++kb)
+    for (int pair = 0; pair < 8 * NB; ++pair) weigh<NB>(pf, s, pair, c, mc);
+  }
+  // V^T's operands of 16 keys, transposed on their way from LDS.  va: values_at(); OFF: the
+  // keys' bytes from there.  In asm with its own wait: the compiler holds the builtin back
+  // until every load to LDS that is under way has landed, which is the whole next tile.
+  static __device__ __forceinline__ void values_at(unsigned (&va)[CT], const T* vt, int lane) {
+    const int key = 4 * (lane >> 5) + ((lane >> 2) & 3), d = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], c, -mc));
-        const float d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i + 1], c, -mc));
-        // the sum is that of the rounded weights, so their rounding cancels where few keys rule
-        const v2 u = pack2<T>(a, d);
-        l = Elem<T>::add2(u, l);
-        pf[kb * 2 + (i >> 3)][i & 7] = u[0];
-        pf[kb * 2 + (i >> 3)][(i & 7) + 1] = u[1];
-      }
-    // O^T += V^T P^T
-    const int va = 4 * half + ((lane >> 2) & 3), vd = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    for (int ct = 0; ct < CT; ++ct)
+      va[ct] = (unsigned)(uintptr_t)(lds_ptr_t)(const_cast<T*>(vt) + v_at<HD>(key, (ct * 32 + d) >> 3) + (d & 7));
+  }
+  template <int OFF>
+  static __device__ __forceinline__ void read_values(v8 (&vf)[CT], const unsigned (&va)[CT]) {
+    u32x2_t x[2 * CT];
+    if constexpr (CT == 4) {
+      asm volatile(
+          "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
+          "ds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+          "ds_read_b64_tr_b16 %2, %9 offset:%12\n\t"
+          "ds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+          "ds_read_b64_tr_b16 %4, %10 offset:%12\n\t"
+          "ds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+          "ds_read_b64_tr_b16 %6, %11 offset:%12\n\t"
+          "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
+          : "v"(va[0]), "v"(va[1]), "v"(va[CT - 2]), "v"(va[CT - 1]), "n"(OFF), "n"(OFF + 8 * HD * 2));
+    } else {
+      asm volatile(
+          "ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
+          "ds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+          "ds_read_b64_tr_b16 %2, %5 offset:%6\n\t"
+          "ds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
+          : "v"(va[0]), "v"(va[1]), "n"(OFF), "n"(OFF + 8 * HD * 2));
+    }
 #pragma unroll
-    for (int kk = 0; kk < 2 * NB; ++kk)
+    for (int ct = 0; ct < CT; ++ct)
+      vf[ct] = __builtin_bit_cast(v8, u32x4_t{x[2 * ct][0], x[2 * ct][1], x[2 * ct + 1][0], x[2 * ct + 1][1]});
+  }
+  // O^T += V^T P^T
+  template <int NB, int OFF, int KK = 0>
+  __device__ __forceinline__ void values(const unsigned (&va)[CT], const v8 (&pf)[2 * NB]) {
+    if constexpr (KK < 2 * NB) {
+      v8 vf[CT];
+      read_values<OFF + KK * 16 * HD * 2>(vf, va);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) o[ct] = Elem<T>::mfma32(vf[ct], pf[KK], o[ct]);
+      values<NB, OFF, KK + 1>(va, pf);
+    }
+  }
+  // One step of the pipeline: n = K Q^T of the next tile beside the weights of s, then
+  // O^T += V^T P^T beside the next tile's maximum, which is returned.  The order is pinned: a
+  // wave issues in order, and MFMAs on end leave the vector unit idle.
+  template <int VOFF>
+  __device__ __forceinline__ float step(float16_t (&n)[2], const float16_t (&s)[2], const T* kt, const unsigned (&va)[CT],
+                                        float c, int lane) {
+    constexpr int NK = 2 * KS, AHEAD = 4, PPM = 16 / NK;
+    const float mc = origin(c);
+    auto key = [&](int i) {
+      return *reinterpret_cast<const v8*>(kt + k_at<HD>((i / KS) * 32 + (lane & 31), (i % KS) * 2 + (lane >> 5)));
+    };
+    v8 kf[AHEAD], pf[4], vf[2][CT];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) kf[i] = key(i);
+    n[0] = float16_t{};
+    n[1] = float16_t{};
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      n[i / KS] = Elem<T>::mfma32(kf[i % AHEAD], qf[i % KS], n[i / KS]);
+      if (i + AHEAD < NK) kf[i % AHEAD] = key(i + AHEAD);
+#pragma unroll
+      for (int j = 0; j < PPM; ++j) weigh<2>(pf, s, i * PPM + j, c, mc);
+      if (i == NK - 2) read_values<VOFF>(vf[0], va);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    float mx = -INFINITY;
+    auto pv = [&](auto KK) {
+      constexpr int kk = decltype(KK)::value;
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        v8 vf;
+        o[ct] = Elem<T>::mfma32(vf[kk & 1][ct], pf[kk], o[ct]);
+        // the next tile's scores: 8 of them here, those of the second block last
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = kk * 16 + e * 8 + va, d = ct * 32 + vd;
-          typedef short s16x4 __attribute__((ext_vector_type(4)));
-          const v4 x = __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                  (__attribute__((address_space(3))) s16x4*)(vt + v_at<HD>(key, d >> 3) + (d & 7))));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) vf[e * 4 + j] = x[j];
-        }
-        o[ct] = Elem<T>::mfma32(vf, pf[kk], o[ct]);
+        for (int i = 0; i < 8 / CT; ++i) mx = fmaxf(mx, n[kk >> 1][(kk & 1) * 8 + ct * (8 / CT) + i]);
+        if (ct == CT / 2 - 1 && kk < 3) read_values<VOFF + (kk < 3 ? kk + 1 : 3) * 16 * HD * 2>(vf[(kk + 1) & 1], va);
+        __builtin_amdgcn_sched_barrier(0);
       }
+    };
+    pv(std::integral_constant<int, 0>{});
+    pv(std::integral_constant<int, 1>{});
+    pv(std::integral_constant<int, 2>{});
+    pv(std::integral_constant<int, 3>{});
+    return half_max(mx);
   }
   // bad[k][d]: the first key whose V is +inf, -inf or NaN (k = 0, 1, 2) in feature d
   __device__ __forceinline__ void add_odd(const int (*bad)[HD], int lane) {
+    typedef const __attribute__((address_space(3))) int* lds_int_t;
+    unsigned at = (unsigned)(uintptr_t)(lds_int_t)&bad[0][4 * (lane >> 5)];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int d = ct * 32 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-        float add = bad[0][d] < lim ? INFINITY : 0.f;
-        add += bad[1][d] < lim ? -INFINITY : 0.f;
-        add += bad[2][d] < lim ? NAN : 0.f;
-        asm volatile("" : "+v"(add)::"memory");   // one element at a time: a rare path, and no registers for it
+        asm volatile("" : "+v"(at)::"memory");   // one element at a time: a rare path, and no registers for it
+        const lds_int_t k = (lds_int_t)(uintptr_t)at + ct * 32 + 8 * (i >> 2) + (i & 3);
+        float add = k[0] < lim ? INFINITY : 0.f;
+        add += k[HD] < lim ? -INFINITY : 0.f;
+        add += k[2 * HD] < lim ? NAN : 0.f;
+        asm volatile("" : "+v"(add)::"memory");
         o[ct][i] += add;
       }
   }
@@ -451,14 +555,24 @@ __device__ __forceinline__ float2_t* part_ml(const AttendParams& p, long row) {
 }
 
 // ---- many rows: NW waves of 32 rows over the same keys -----------------------------------
-// Tiles of 64 keys in two buffers: the next one is under way (f16, bf16: straight to LDS;
-// e4m3: through registers, where it is turned into values) while this one is used.
+// Tiles of 64 keys.  A wave computes the scores of one tile while it turns those of the tile
+// before into weights, so that the matrix cores and the vector unit work at the same time:
+//   step j:  S(j+1) = K(j+1) Q^T  beside  P(j) = 2^(S(j) - m);
+//            O += V(j)^T P(j)     beside  max S(j+1).
+// K is therefore one tile ahead of V; both have two buffers in LDS, and what step j+1 needs
+// (K(j+2), V(j+1)) is under way meanwhile (f16, bf16: straight to LDS; e4m3: through
+// registers, where it is turned into values).
 template <typename T, int HD, int KV, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendParams p) {
   constexpr int BM = 32 * NW, TILE = AT_KEYS * HD, NT = 64 * NW;
   constexpr bool DMA = KV != KV_E4M3;
-  __shared__ __attribute__((aligned(1024))) T kt[2][TILE], vt[2][TILE];
-  __shared__ int bad[3][HD], odd;
+  // one array: with several, the compiler holds every read of one back until all loads to the
+  // others have landed
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE * 2 + 3 * HD * 4 + 16];
+  auto kt = [&](int buf) { return reinterpret_cast<T*>(lds) + buf * TILE; };
+  auto vt = [&](int buf) { return reinterpret_cast<T*>(lds) + (2 + buf) * TILE; };
+  int (*const bad)[HD] = reinterpret_cast<int (*)[HD]>(lds + 4 * TILE * 2);
+  int& odd = *reinterpret_cast<int*>(lds + 4 * TILE * 2 + 3 * HD * 4);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hk = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv;
   Item it;
@@ -470,48 +584,107 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
   const int kbeg = it.nch > 1 ? it.chunk * it.c * AT_KEYS : 0;
   const int kend = it.nch > 1 ? min(khi, kbeg + it.c * AT_KEYS) : khi;
 
-  Stage<T, HD, KV, AT_KEYS, NT> st;
-  if (tid == 0) odd = 0;
-  if (kbeg < kend) {
-    st.pages(p, it, kbeg, wave);
-    if constexpr (DMA) st.dma(p, it, hk, kbeg, tid, wave, kt[0], vt[0]);
-    else st.load(p, it, hk, kbeg, tid);
-    st.pages(p, it, kbeg + AT_KEYS, wave);
-  }
+  Stage<T, HD, KV, AT_KEYS, NT, false> ks;
+  Stage<T, HD, KV, AT_KEYS, NT, true> vs;
+  auto send = [&](auto& st, int key0, T* t) {
+    if constexpr (DMA) st.dma(p, it, hk, key0, lane, wave, t);
+    else st.load(p, it, hk, key0, lane, wave);
+  };
+  ks.begin(p, lane, wave, DMA);
+  vs.begin(p, lane, wave, DMA);
   Rows<T, HD> r;
-  r.begin(p, it, hk, tile * BM + wave * 32 + (lane & 31), lane);
-  // Q has arrived before the loop, whose waits would otherwise count its loads every time
-  r.arrived();
-  if (!DMA && kbeg < kend) st.store(kt[0], vt[0], tid);
-  for (int key0 = kbeg, cur = 0; key0 < kend; key0 += AT_KEYS, cur ^= 1) {
-    const bool more = key0 + AT_KEYS < kend;
-    __syncthreads();   // this tile is there, and the other buffer is free
-    if (more) {
-      if constexpr (DMA) st.dma(p, it, hk, key0 + AT_KEYS, tid, wave, kt[cur ^ 1], vt[cur ^ 1]);
-      else st.load(p, it, hk, key0 + AT_KEYS, tid);
-      st.pages(p, it, key0 + 2 * AT_KEYS, wave);
+  unsigned va[Rows<T, HD>::CT];
+  r.values_at(va, vt(0), lane);
+  const float c = p.scale_log2e;
+  if (tid == 0) odd = 0;
+  float16_t sa[2], sb[2];
+  if (kbeg < kend) {
+    ks.pages(p, it, kbeg, wave);
+    vs.pages(p, it, kbeg, wave);
+    send(ks, kbeg, kt(0));
+    send(vs, kbeg, vt(0));
+    r.begin(p, it, hk, tile * BM + wave * 32 + (lane & 31), lane);
+    if constexpr (!DMA) {
+      ks.store(kt(0), tid);
+      vs.store(vt(0), tid);
     }
+    ks.pages(p, it, kbeg + AT_KEYS, wave);
+    vs.pages(p, it, kbeg + AT_KEYS, wave);
+    send(ks, kbeg + AT_KEYS, kt(1));
+    if constexpr (!DMA) ks.store(kt(1), tid);
+    ks.pages(p, it, kbeg + 2 * AT_KEYS, wave);
+    r.arrived();
+    wait_vm_lgkm0<0>();
+    lds_barrier();
+    r.template scores<2>(sa, kt(0), lane);
+  } else {
+    r.begin(p, it, hk, tile * BM + wave * 32 + (lane & 31), lane);
+  }
+  // what step j sends for, once K(j+1) and V(j) are there and K(j)'s and V(j-1)'s buffers are free
+  auto next = [&](int key0, int cur) {
+    wait_vm_lgkm0<0>();
+    lds_barrier();
+    send(vs, key0 + AT_KEYS, vt(cur ^ 1));
+    vs.pages(p, it, key0 + 2 * AT_KEYS, wave);
+    send(ks, key0 + 2 * AT_KEYS, kt(cur));
+    ks.pages(p, it, key0 + 3 * AT_KEYS, wave);
+  };
+  auto keep = [&](int cur) {
+    if constexpr (!DMA) {
+      vs.store(vt(cur ^ 1), tid);
+      ks.store(kt(cur), tid);
+    }
+  };
+  int key0 = kbeg;
+  // two steps at a time while every row sees all of this tile and of the two after it
+  const int kfull = min(klo, kend) - 3 * AT_KEYS;
+  if (key0 <= kfull) {
+    float mx = r.template top<2>(sa);
+    auto step = [&](float16_t (&s)[2], float16_t (&n)[2], int at, auto CUR) {
+      constexpr int cur = decltype(CUR)::value;
+      next(at, cur);
+      r.raise(mx, c);
+      mx = r.template step<cur * TILE * 2>(n, s, kt(cur ^ 1), va, c, lane);
+      keep(cur);
+    };
+    for (; key0 <= kfull; key0 += 2 * AT_KEYS) {
+      step(sa, sb, key0, std::integral_constant<int, 0>{});
+      step(sb, sa, key0 + AT_KEYS, std::integral_constant<int, 1>{});
+    }
+  }
+  // the rest one by one
+  for (int cur = 0; key0 < kend; key0 += AT_KEYS, cur ^= 1) {
+    next(key0, cur);
     // A tile that some row sees in part: an infinity or NaN of V must not reach that row.
-    const bool part = key0 + AT_KEYS > klo;
     bool fix = false;
-    if (part) {
-      if (any_odd<T, TILE, NT>(vt[cur], tid)) odd = 1;
+    if (key0 + AT_KEYS > klo) {
+      r.template mask<2>(sa, key0, lane);
+      if (any_odd<T, TILE, NT>(vt(cur), tid)) odd = 1;
       __syncthreads();
       fix = odd;
       if (fix) {
         for (int i = tid; i < 3 * HD; i += NT) (&bad[0][0])[i] = 0x7FFFFFFF;
         __syncthreads();
-        take_out_odd<T, HD, AT_KEYS, NT>(vt[cur], bad, key0, tid);
+        take_out_odd<T, HD, AT_KEYS, NT>(vt(cur), bad, key0, tid);
         __syncthreads();
       }
     }
-    r.template step<2>(kt[cur], vt[cur], key0, part, p.scale_log2e, lane);
+    r.raise(r.template top<2>(sa), c);
+    typename Elem<T>::v8 pf[4];
+    r.template weights<2>(pf, sa, c);
+    unsigned vc[Rows<T, HD>::CT];
+#pragma unroll
+    for (int ct = 0; ct < Rows<T, HD>::CT; ++ct) vc[ct] = va[ct] + cur * TILE * 2;
+    r.template values<2, 0>(vc, pf);
     if (fix) {
       r.add_odd(bad, lane);
       __syncthreads();
       if (tid == 0) odd = 0;
     }
-    if (!DMA && more) st.store(kt[cur ^ 1], vt[cur ^ 1], tid);
+    if (key0 + AT_KEYS < kend) {
+      r.template scores<2>(sa, kt(cur ^ 1), lane);
+      keep(cur);
+    }
   }
 
   if (it.nch == 1) {
@@ -554,23 +727,32 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attend_few_kernel(const Att
   const int kend = it.nch > 1 ? min(khi, kbeg + it.c * AT_KEYS) : khi;
 
   r.arrived();
-  Stage<T, HD, KV, KEYS, 64> st;
+  Stage<T, HD, KV, KEYS, 64, false> ks;
+  Stage<T, HD, KV, KEYS, 64, true> vs;
   T* const kt = lds[wave];
   T* const vt = kt + TILE;
+  ks.begin(p, lane, 0, false);
+  vs.begin(p, lane, 0, false);
+  unsigned va[Rows<T, HD>::CT];
+  r.values_at(va, vt, lane);
   int key0 = kbeg + wave * KEYS;
+  auto load = [&](int key) {
+    ks.load(p, it, hk, key, lane, 0);
+    vs.load(p, it, hk, key, lane, 0);
+    ks.pages(p, it, key + NW * KEYS, 0);
+    vs.pages(p, it, key + NW * KEYS, 0);
+  };
   if (key0 < kend) {
-    st.pages(p, it, key0, 0);
-    st.load(p, it, hk, key0, lane);
-    st.pages(p, it, key0 + NW * KEYS, 0);
+    ks.pages(p, it, key0, 0);
+    vs.pages(p, it, key0, 0);
+    load(key0);
   }
   for (; key0 < kend; key0 += NW * KEYS) {
     const bool part = key0 + KEYS > klo;
     wave_order();
-    st.store(kt, vt, lane);
-    if (key0 + NW * KEYS < kend) {
-      st.load(p, it, hk, key0 + NW * KEYS, lane);
-      st.pages(p, it, key0 + 2 * NW * KEYS, 0);
-    }
+    ks.store(kt, lane);
+    vs.store(vt, lane);
+    if (key0 + NW * KEYS < kend) load(key0 + NW * KEYS);
     wave_order();
     const bool fix = part && __any(any_odd<T, TILE, 64>(vt, lane));
     if (fix) {
@@ -579,7 +761,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attend_few_kernel(const Att
       take_out_odd<T, HD, KEYS, 64>(vt, bad[wave], key0, lane);
       wave_order();
     }
-    r.template step<1>(kt, vt, key0, part, p.scale_log2e, lane);
+    float16_t s[1];
+    typename Elem<T>::v8 pf[2];
+    r.template scores<1>(s, kt, lane);
+    if (part) r.template mask<1>(s, key0, lane);
+    r.raise(r.template top<1>(s), p.scale_log2e);
+    r.template weights<1>(pf, s, p.scale_log2e);
+    r.template values<1, 0>(va, pf);
     if (fix) r.add_odd(bad[wave], lane);
   }
 
