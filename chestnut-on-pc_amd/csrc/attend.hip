@@ -133,6 +133,9 @@ __device__ __forceinline__ bool find_item(const AttendParams& p, int index, Item
       it.s.nq = __builtin_amdgcn_readlane(s.nq, w);
       it.s.k0 = __builtin_amdgcn_readlane(s.k0, w);
       it.s.nk = __builtin_amdgcn_readlane(s.nk, w);
+      // the compiler does not see that these are the same for all lanes
+      for (int* x : {&it.b, &it.tile, &it.chunk, &it.nch, &it.c, &it.base, &it.s.q0, &it.s.nq, &it.s.k0, &it.s.nk})
+        *x = __builtin_amdgcn_readfirstlane(*x);
       return true;
     }
     index -= __builtin_amdgcn_readlane(su, 63);
@@ -219,8 +222,9 @@ struct Stage {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const long row = row_of(p, it, hk, first(key0, i, wave), i);
-        const char* b = base(p, hk) + row * pitch(p);
-        f(i, b + lane_off, row + lane_row(lane));
+        uintptr_t b = (uintptr_t)(base(p, hk) + row * pitch(p));
+        asm("" : "+s"(b));   // in scalar registers: the same address in vector ones costs four multiplications
+        f(i, (const char*)b + lane_off, row + lane_row(lane));
       }
     } else {
 #pragma unroll
