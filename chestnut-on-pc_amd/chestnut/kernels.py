@@ -553,7 +553,7 @@ def attention_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, k_scale=Non
     dev = _on_device((q, 'q'), (k_pages, 'k_pages'), (v_pages, 'v_pages'), (block_table, 'block_table'), (cu_q, 'cu_q'),
                      (kv_lens, 'kv_lens'), (k_scale, 'k_scale'), (v_scale, 'v_scale'), (out, 'out'))
     o = out if out is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ws, nb = _attention_workspace(workspace, B, T, width * page, H, kv, hd, q.device)
+    ws, nb = _attention_workspace(workspace, B, T, B * width * page, H, kv, hd, q.device)
     check(lib().ck_attention_paged(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale),
                                    o.data_ptr(), block_table.data_ptr(), width, cu_q.data_ptr(), kv_lens.data_ptr(), B,
                                    T, H, n, kv, page, hd, qt, qh, ot, oh, _DTYPE[q.dtype], _DTYPE[k_pages.dtype],

@@ -80,49 +80,82 @@ __device__ __forceinline__ int tiles_of(const Seq& s, int G) {
 }
 __device__ __forceinline__ int blocks_of(int keys) { return (keys + AT_KEYS - 1) / AT_KEYS; }
 
+// Sum over lanes 0..l, in lane l (DPP: six steps without LDS).
+template <typename N>
+__device__ __forceinline__ N lanes_scan(N v) {
+  auto shifted = [](N x, auto CTRL, auto ROWS) {
+    return __builtin_bit_cast(N, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(CTRL)::value,
+                                                             decltype(ROWS)::value, 0xF, false));
+  };
+  using std::integral_constant;
+  v += shifted(v, integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{});   // row_shr:1, 2, 4, 8
+  v += shifted(v, integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{});
+  v += shifted(v, integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{});
+  v += shifted(v, integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{});
+  v += shifted(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});   // row_bcast:15, 31
+  v += shifted(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});
+  return v;
+}
+__device__ __forceinline__ int lane63(int v) { return __builtin_amdgcn_readlane(v, 63); }
+
 // index counts items, or tiles where TILES.  False: there are not so many.
 template <int KV, int BM, bool TILES>
 __device__ __forceinline__ bool find_item(const AttendParams& p, int index, Item& it) {
   const int lane = threadIdx.x & 63;
-  int c = 1 << 30;
-  if (p.target) {
-    long work = 0;
-    int tiles = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64)
-      if (b0 + lane < p.B) {
-        const Seq s = sequence<KV>(p, b0 + lane);
-        const int n = tiles_of<KV, BM>(s, p.G);
-        tiles += n;
-        work += (long)n * blocks_of(s.nk);
-      }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      tiles += __shfl_xor(tiles, o);
-      work += __shfl_xor(work, o);
-    }
-    // each tile adds up to one item that is not full
-    const int full = max(p.target - tiles, (p.target + 1) >> 1);
-    c = max(p.min_blocks, (int)min((work + full - 1) / full, 1L << 30));
-  }
-  int base = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    int tiles = 0, nch = 1;
-    Seq s{};
+  // the first 64 sequences, one a lane
+  Seq s{};
+  int tiles = 0, blocks = 0;
+  auto get = [&](int b0) {
+    s = Seq{};
+    tiles = blocks = 0;
     if (b0 + lane < p.B) {
       s = sequence<KV>(p, b0 + lane);
       tiles = tiles_of<KV, BM>(s, p.G);
-      nch = max(1, (blocks_of(s.nk) + c - 1) / c);
+      blocks = blocks_of(s.nk);
     }
-    int items = tiles * nch, units = TILES ? tiles : items, su = units, si = items;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(su, o), z = __shfl_up(si, o);
-      if (lane >= o) su += y, si += z;
+  };
+  get(0);
+  int c = 1 << 30;
+  if (p.target) {
+    float work = readlane_f32(lanes_scan((float)tiles * (float)blocks), 63);
+    int all = lane63(lanes_scan(tiles));
+    for (int b0 = 64; b0 < p.B; b0 += 64) {
+      get(b0);
+      work += readlane_f32(lanes_scan((float)tiles * (float)blocks), 63);
+      all += lane63(lanes_scan(tiles));
     }
+    // each tile adds up to one item that is not full
+    const int full = max(p.target - all, (p.target + 1) >> 1);
+    if (work < 16777216.f) {   // a whole number
+      const int w = (int)work;
+      c = max(p.min_blocks, (w + full - 1) / full);
+      if (p.B <= 4) {
+        // few sequences: lane i counts the items that chunks of c0 + i blocks make, and the
+        // shortest chunk that does not make too many is taken
+        const int c0 = max(p.min_blocks, (w + p.target - 1) / p.target), ci = c0 + lane;
+        int items = 0;
+        for (int b = 0; b < p.B; ++b) {
+          const int nb = __builtin_amdgcn_readlane(blocks, b), nt = __builtin_amdgcn_readlane(tiles, b);
+          items += nt * max(1, (nb + ci - 1) / ci);
+        }
+        const unsigned long long fits = __ballot(items <= p.target);
+        if (fits) c = min(c, c0 + __ffsll(fits) - 1);
+      }
+    } else {
+      c = max(p.min_blocks, (int)fminf(work / (float)full * 1.0001f, 1e9f) + 1);
+    }
+    c = __builtin_amdgcn_readfirstlane(c);
+    if (p.B > 64) get(0);
+  }
+  int base = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    if (b0) get(b0);
+    const int nch = max(1, (blocks + c - 1) / c), items = tiles * nch;
+    const int si = lanes_scan(items), su = TILES ? lanes_scan(tiles) : si;
     const unsigned long long m = __ballot(su > index);
     if (m) {
       const int w = __ffsll(m) - 1;
-      const int local = __builtin_amdgcn_readlane(index - (su - units), w);
+      const int local = __builtin_amdgcn_readlane(index - (su - (TILES ? tiles : items)), w);
       it.b = b0 + w;
       it.nch = __builtin_amdgcn_readlane(nch, w);
       it.tile = TILES ? local : local / it.nch;
@@ -138,8 +171,8 @@ __device__ __forceinline__ bool find_item(const AttendParams& p, int index, Item
         *x = __builtin_amdgcn_readfirstlane(*x);
       return true;
     }
-    index -= __builtin_amdgcn_readlane(su, 63);
-    base += __builtin_amdgcn_readlane(si, 63);
+    index -= lane63(su);
+    base += lane63(si);
   }
   return false;
 }
@@ -205,47 +238,64 @@ struct Stage {
     if constexpr (KV == KV_ROWS) return (V ? p.v_st : p.k_st) * 2;
     return HD / EPL * BPL;
   }
-  // bytes from a load's first row to the lane's piece (for good: begin() once)
+  // bytes from a load's first row to the lane's piece, and of the piece within its row; KV_ROWS:
+  // the first row of the next tile, which is `ahead` keys after this one, and bytes between loads
   unsigned lane_off;
   int piece;
-  __device__ __forceinline__ void begin(const AttendParams& p, int lane, int wave, bool swizzled) {
+  uintptr_t next;
+  long between, ahead;
+  __device__ __forceinline__ void begin(const AttendParams& p, const Item& it, int hk, int key0, int keys_ahead, int lane,
+                                        int wave, bool swizzled) {
     // straight to LDS a wave's 64 pieces of 16 bytes land side by side, so each lane fetches the
     // chunk that belongs in its place
     piece = swizzled ? (at(first(0, 0, wave) + lane_row(lane), lane % CPR) >> 3) % CPR * 16 : lane % CPR * BPL;
     lane_off = lane_row(lane) * (unsigned)pitch(p) + piece;
     asm volatile("" : "+v"(lane_off));
+    if constexpr (KV == KV_ROWS) {
+      next = (uintptr_t)base(p, hk) + (it.s.k0 + first(key0, 0, wave)) * pitch(p);
+      between = RPL * pitch(p);
+      ahead = keys_ahead * pitch(p);
+    }
   }
-  // f(i, address of the lane's piece, its row's number) for every load
+  // f(i, address of the lane's piece, its row's number) for every load of the next tile
   template <typename F>
-  __device__ __forceinline__ void rows(const AttendParams& p, const Item& it, int hk, int key0, int lane, int wave, F f) const {
+  __device__ __forceinline__ void rows(const AttendParams& p, const Item& it, int hk, int key0, int lane, int wave, F f) {
+    typedef const __attribute__((address_space(1))) char* glob_t;
     if (key0 + KEYS <= it.s.nk) {
+      uintptr_t a = next;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const long row = row_of(p, it, hk, first(key0, i, wave), i);
-        uintptr_t b = (uintptr_t)(base(p, hk) + row * pitch(p));
-        asm("" : "+s"(b));   // in scalar registers: the same address in vector ones costs four multiplications
-        f(i, (const char*)b + lane_off, row + lane_row(lane));
+        long row = 0;
+        if constexpr (KV != KV_ROWS) {
+          row = row_of(p, it, hk, first(key0, i, wave), i);
+          a = (uintptr_t)(base(p, hk) + row * pitch(p));
+        }
+        // in scalar registers: the same address in vector ones costs four multiplications
+        const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)a), hi = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
+        f(i, (glob_t)(((uintptr_t)hi << 32) | lo) + lane_off, row + lane_row(lane));
+        if constexpr (KV == KV_ROWS) a += between;
       }
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const long row = row_of(p, it, hk, min(first(key0, i, wave) + lane_row(lane), it.s.nk - 1), i);
-        f(i, base(p, hk) + row * pitch(p) + piece, row);
+        f(i, (glob_t)(base(p, hk) + row * pitch(p) + piece), row);
       }
     }
+    if constexpr (KV == KV_ROWS) next += ahead;
   }
   // sends for the rows; store() leaves them (e4m3: as values of T) in LDS
   __device__ __forceinline__ void load(const AttendParams& p, const Item& it, int hk, int key0, int lane, int wave) {
-    rows(p, it, hk, key0, lane, wave, [&](int i, const char* at, long row) {
-      x[i] = *reinterpret_cast<const raw*>(at);
+    rows(p, it, hk, key0, lane, wave, [&](int i, auto at, long row) {
+      x[i] = *(const __attribute__((address_space(1))) raw*)at;
       if constexpr (KV == KV_E4M3) scale[i] = (V ? p.vs : p.ks)[row];
     });
   }
   // load() straight into LDS, as store() would leave it
-  __device__ __forceinline__ void dma(const AttendParams& p, const Item& it, int hk, int key0, int lane, int wave, T* t) const {
+  __device__ __forceinline__ void dma(const AttendParams& p, const Item& it, int hk, int key0, int lane, int wave, T* t) {
     typedef const __attribute__((address_space(1))) void* src_t;
     static_assert(RPL % 16 == 0, "the chunk of a lane is that of every load");
-    rows(p, it, hk, key0, lane, wave, [&](int i, const char* from, long) {
+    rows(p, it, hk, key0, lane, wave, [&](int i, auto from, long) {
       __builtin_amdgcn_global_load_lds((src_t)from, (lds_ptr_t)(t + (i * NT + wave * 64) * 8), 16, 0, 0);
     });
   }
@@ -594,8 +644,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
     if constexpr (DMA) st.dma(p, it, hk, key0, lane, wave, t);
     else st.load(p, it, hk, key0, lane, wave);
   };
-  ks.begin(p, lane, wave, DMA);
-  vs.begin(p, lane, wave, DMA);
+  ks.begin(p, it, hk, kbeg, AT_KEYS, lane, wave, DMA);
+  vs.begin(p, it, hk, kbeg, AT_KEYS, lane, wave, DMA);
   Rows<T, HD> r;
   unsigned va[Rows<T, HD>::CT];
   r.values_at(va, vt(0), lane);
@@ -735,11 +785,11 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attend_few_kernel(const Att
   Stage<T, HD, KV, KEYS, 64, true> vs;
   T* const kt = lds[wave];
   T* const vt = kt + TILE;
-  ks.begin(p, lane, 0, false);
-  vs.begin(p, lane, 0, false);
+  int key0 = kbeg + wave * KEYS;
+  ks.begin(p, it, hk, key0, NW * KEYS, lane, 0, false);
+  vs.begin(p, it, hk, key0, NW * KEYS, lane, 0, false);
   unsigned va[Rows<T, HD>::CT];
   r.values_at(va, vt, lane);
-  int key0 = kbeg + wave * KEYS;
   auto load = [&](int key) {
     ks.load(p, it, hk, key, lane, 0);
     vs.load(p, it, hk, key, lane, 0);
@@ -882,16 +932,17 @@ struct Plan {
   int bm, target, min_blocks;
   long tiles, items;   // at most
 };
-Plan plan_of(int B, int Tq, long max_keys, int n_heads, int n_kv) {
+// keys: the most that the sequences can have, all together
+Plan plan_of(int B, int Tq, long keys, int n_heads, int n_kv) {
   Plan pl{};
   const int G = n_heads / n_kv;
   const long rows = (long)Tq * G;
-  pl.bm = rows <= 32L * B ? 32 : 128;
+  pl.bm = rows <= 32L * B ? 32 : (rows / 256 + B) * n_kv >= 512 ? 256 : 128;
   pl.tiles = rows / pl.bm + B;       // sum of ceil(rows_b / bm) is at most this
-  const long slots = 512;            // workgroups that run at once, two a CU
-  const long blocks = (max_keys + AT_KEYS - 1) / AT_KEYS;
+  const long slots = pl.bm == 256 ? 256 : 512;   // workgroups that run at once: one a CU, or two
   pl.min_blocks = pl.bm == 32 ? 2 : 4;
-  if (blocks > pl.min_blocks && (pl.bm == 32 || pl.tiles * n_kv < 2 * slots)) pl.target = (int)std::max(1L, slots / n_kv);
+  const bool many = pl.bm != 32 && pl.tiles * n_kv >= 2 * slots;
+  if (!many && keys / B > 2 * pl.min_blocks * AT_KEYS) pl.target = (int)std::max(1L, slots / n_kv);
   pl.items = pl.tiles + pl.target;
   return pl;
 }
@@ -900,11 +951,13 @@ template <typename T, int HD, int KV>
 void launch_kv(const AttendParams& p, const Plan& pl, hipStream_t s) {
   const dim3 grid((unsigned)(pl.items * p.Hkv));
   if (pl.bm == 32) CK_LAUNCH((attend_few_kernel<T, HD, KV>), grid, dim3(64 * FEW_WAVES), 0, s, p);
-  else CK_LAUNCH((attend_tile_kernel<T, HD, KV, 4>), grid, dim3(256), 0, s, p);
+  else if (pl.bm == 128) CK_LAUNCH((attend_tile_kernel<T, HD, KV, 4>), grid, dim3(256), 0, s, p);
+  else CK_LAUNCH((attend_tile_kernel<T, HD, KV, 8>), grid, dim3(512), 0, s, p);
   if (!pl.target) return;
   const unsigned tiles = (unsigned)(pl.tiles * p.Hkv);
   if (pl.bm == 32) CK_LAUNCH((attend_join_kernel<T, HD, KV, 32>), dim3(tiles, 32), dim3(256), 0, s, p);
-  else CK_LAUNCH((attend_join_kernel<T, HD, KV, 128>), dim3(tiles, 128 / (1024 / HD)), dim3(256), 0, s, p);
+  else if (pl.bm == 128) CK_LAUNCH((attend_join_kernel<T, HD, KV, 128>), dim3(tiles, 128 / (1024 / HD)), dim3(256), 0, s, p);
+  else CK_LAUNCH((attend_join_kernel<T, HD, KV, 256>), dim3(tiles, 256 / (1024 / HD)), dim3(256), 0, s, p);
 }
 template <typename T, int HD>
 void launch_hd(const AttendParams& p, int kv, const Plan& pl, hipStream_t s) {
@@ -913,7 +966,7 @@ void launch_hd(const AttendParams& p, int kv, const Plan& pl, hipStream_t s) {
   else launch_kv<T, HD, KV_E4M3>(p, pl, s);
 }
 
-void launch_attend(const char* what, AttendParams& p, const AttendQuery& a, int kv, long max_keys, hipStream_t s) {
+void launch_attend(const char* what, AttendParams& p, const AttendQuery& a, int kv, long keys, hipStream_t s) {
   const std::string w(what);
   CK_REQUIRE(a.dtype == DT_F16 || a.dtype == DT_BF16, w + ": q must be f16 or bf16");
   CK_REQUIRE(a.head_dim == 64 || a.head_dim == 128, w + ": head_dim must be 64 or 128");
@@ -938,10 +991,10 @@ void launch_attend(const char* what, AttendParams& p, const AttendQuery& a, int 
   p.G = a.n_heads / p.Hkv;
   p.causal = a.causal;
   p.scale_log2e = a.scale * AT_LOG2E;
-  const Plan pl = plan_of(a.B, a.T, max_keys, a.n_heads, p.Hkv);
+  const Plan pl = plan_of(a.B, a.T, keys, a.n_heads, p.Hkv);
   CK_REQUIRE(pl.items * p.Hkv < (1L << 31), w + ": too many rows");
   if (pl.target) {
-    const size_t need = attention_workspace(a.B, a.T, max_keys, a.n_heads, p.Hkv, a.head_dim);
+    const size_t need = attention_workspace(a.B, a.T, keys, a.n_heads, p.Hkv, a.head_dim);
     CK_REQUIRE(a.ws && a.ws_floats >= need, w + ": workspace too small (ck_attention_workspace)");
     CK_REQUIRE((reinterpret_cast<uintptr_t>(a.ws) & 15) == 0, w + ": workspace must be 16-byte aligned");
   }
@@ -962,11 +1015,11 @@ void launch_attend(const char* what, AttendParams& p, const AttendQuery& a, int 
 
 }  // namespace
 
-size_t attention_workspace(int B, int Tq, long max_keys, int n_heads, int n_kv, int head_dim) {
-  CK_REQUIRE(B >= 0 && Tq >= 0 && max_keys >= 0 && n_kv > 0 && n_heads > 0 && n_heads % n_kv == 0 && head_dim > 0,
+size_t attention_workspace(int B, int Tq, long keys, int n_heads, int n_kv, int head_dim) {
+  CK_REQUIRE(B >= 0 && Tq >= 0 && keys >= 0 && n_kv > 0 && n_heads > 0 && n_heads % n_kv == 0 && head_dim > 0,
              "attention_workspace: bad sizes");
   if (B == 0 || Tq == 0) return 0;
-  const Plan pl = plan_of(B, Tq, max_keys, n_heads, n_kv);
+  const Plan pl = plan_of(B, Tq, keys, n_heads, n_kv);
   return pl.target ? (size_t)pl.items * n_kv * pl.bm * (head_dim + 2) : 0;
 }
 
@@ -1007,7 +1060,7 @@ void launch_attention_paged(const AttendQuery& a, const PagedCache& c, const int
   p.page_shift = page_shift(c.page);
   p.n_pages = c.n_pages;
   launch_attend("attention_paged", p, a, c.dtype == DT_E4M3 ? KV_E4M3 : KV_PAGES,
-                (long)table_w * c.page, s);
+                (long)a.B * table_w * c.page, s);
 }
 
 }  // namespace ck

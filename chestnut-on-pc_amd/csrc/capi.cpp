@@ -493,10 +493,10 @@ static AttendQuery attend_query(const void* q, void* out, const int32_t* cu_q, i
   return a;
 }
 
-int ck_attention_workspace(int B, int Tq, long max_keys, int n_heads, int n_kv, int head_dim, size_t* ws_bytes) {
+int ck_attention_workspace(int B, int Tq, long keys, int n_heads, int n_kv, int head_dim, size_t* ws_bytes) {
   CK_API_BEGIN
   CK_REQUIRE(ws_bytes, "ck_attention_workspace: null argument");
-  *ws_bytes = attention_workspace(B, Tq, max_keys, n_heads, n_kv, head_dim) * sizeof(float);
+  *ws_bytes = attention_workspace(B, Tq, keys, n_heads, n_kv, head_dim) * sizeof(float);
   CK_API_END
 }
 

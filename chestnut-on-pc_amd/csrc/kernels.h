@@ -150,8 +150,8 @@ struct AttendQuery {
   float* ws = nullptr;         // attention_workspace floats
   size_t ws_floats = 0;
 };
-// Workspace of a call over sequences of up to max_keys keys (0: none needed).
-size_t attention_workspace(int B, int Tq, long max_keys, int n_heads, int n_kv, int head_dim);
+// Workspace of a call, in floats (0: none needed); keys: the most that its sequences can have, all together.
+size_t attention_workspace(int B, int Tq, long keys, int n_heads, int n_kv, int head_dim);
 // K/V rows contiguous, sequence b's at rows cu_k[b] .. cu_k[b+1] of k and v [Tk][n_kv][head_dim].
 void launch_attention_varlen(const AttendQuery& a, const void* k, const void* v, long kst, long ksh, long vst, long vsh,
                              const int* cu_k, int Tk, int n_kv, hipStream_t s);

@@ -348,9 +348,9 @@ int ck_cache_read(const void* k_pages, const void* v_pages, const void* k_scale,
                   int n_pages, int n_kv, int page, int head_dim, void* k, void* v, int dtype, int cache_dtype,
                   void* stream);
 
-/* Workspace of the attention calls below, in bytes (0: none).  max_keys: the
- * most keys a sequence can have (Tk, or table_width * page). */
-int ck_attention_workspace(int B, int Tq, long max_keys, int n_heads, int n_kv, int head_dim, size_t* ws_bytes);
+/* Workspace of the attention calls below, in bytes (0: none).  keys: the most
+ * that their sequences can have, all together (Tk, or B * table_width * page). */
+int ck_attention_workspace(int B, int Tq, long keys, int n_heads, int n_kv, int head_dim, size_t* ws_bytes);
 
 /* out[i] = sum_j softmax_j(scale q_i . k_j) v_j over packed sequences:
  * queries cu_q[b] .. cu_q[b+1] of sequence b over keys cu_k[b] .. cu_k[b+1];
