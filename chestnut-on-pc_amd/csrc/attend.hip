@@ -207,26 +207,22 @@ struct Stage {
   static_assert(N * NT == KEYS * CPR && (RPL >= 16 || 16 % RPL == 0), "tile");
   raw x[N];
   unsigned scale[N];
-  int page[N];
+  // lane l: the page of group l (of 16 keys) of the window of 1024 keys that is read, and of the next
+  int page, later, window;
 
   static __device__ __forceinline__ int at(int key, int c) { return V ? v_at<HD>(key, c) : k_at<HD>(key, c); }
-  // the pages of the keys from key0 on
-  __device__ __forceinline__ void pages(const AttendParams& p, const Item& it, int key0, int wave) {
-    if constexpr (KV != KV_ROWS) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int key = min(key0 + ((i * RPL + wave * (64 / CPR)) & ~15), it.s.nk - 1);
-        page[i] = p.table[(long)it.b * p.table_w + (key >> p.page_shift)];
-      }
-    }
+  __device__ __forceinline__ int pages(const AttendParams& p, const Item& it, int w, int lane) const {
+    const int key = min(w * 1024 + lane * 16, it.s.nk - 1);
+    return p.table[(long)it.b * p.table_w + (key >> p.page_shift)];
   }
   // Load i brings the rows from first(key0, i) on to a wave: their place in the cache (or among
   // the packed rows) is the same for all lanes but for lane_row() rows of `pitch` bytes.
   static __device__ __forceinline__ int lane_row(int lane) { return lane / CPR; }
   static __device__ __forceinline__ int first(int key0, int i, int wave) { return key0 + i * RPL + wave * (64 / CPR); }
-  __device__ __forceinline__ long row_of(const AttendParams& p, const Item& it, int hk, int key, int i) const {
+  // place of a key; of: the load's first row, whose group of 16 it is in (or the last key's)
+  __device__ __forceinline__ long row_of(const AttendParams& p, const Item& it, int hk, int key, int of) const {
     if constexpr (KV == KV_ROWS) return it.s.k0 + key;
-    const long pg = min(max(__builtin_amdgcn_readfirstlane(page[i]), 0), p.n_pages - 1);
+    const long pg = min(max(__builtin_amdgcn_readlane(page, (of >> 4) & 63), 0), p.n_pages - 1);
     return ((pg * p.Hkv + hk) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
   }
   static __device__ __forceinline__ const char* base(const AttendParams& p, int hk) {
@@ -255,19 +251,29 @@ struct Stage {
       next = (uintptr_t)base(p, hk) + (it.s.k0 + first(key0, 0, wave)) * pitch(p);
       between = RPL * pitch(p);
       ahead = keys_ahead * pitch(p);
+    } else {
+      window = key0 >> 10;
+      page = pages(p, it, window, lane);
+      later = pages(p, it, window + 1, lane);
     }
   }
   // f(i, address of the lane's piece, its row's number) for every load of the next tile
   template <typename F>
   __device__ __forceinline__ void rows(const AttendParams& p, const Item& it, int hk, int key0, int lane, int wave, F f) {
     typedef const __attribute__((address_space(1))) char* glob_t;
+    if constexpr (KV != KV_ROWS)
+      if (key0 >> 10 != window) {
+        window = key0 >> 10;
+        page = later;
+        later = pages(p, it, window + 1, lane);
+      }
     if (key0 + KEYS <= it.s.nk) {
       uintptr_t a = next;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         long row = 0;
         if constexpr (KV != KV_ROWS) {
-          row = row_of(p, it, hk, first(key0, i, wave), i);
+          row = row_of(p, it, hk, first(key0, i, wave), first(key0, i, wave));
           a = (uintptr_t)(base(p, hk) + row * pitch(p));
         }
         // in scalar registers: the same address in vector ones costs four multiplications
@@ -278,7 +284,7 @@ struct Stage {
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const long row = row_of(p, it, hk, min(first(key0, i, wave) + lane_row(lane), it.s.nk - 1), i);
+        const long row = row_of(p, it, hk, min(first(key0, i, wave) + lane_row(lane), it.s.nk - 1), first(key0, i, wave));
         f(i, (glob_t)(base(p, hk) + row * pitch(p) + piece), row);
       }
     }
@@ -329,6 +335,16 @@ struct Stage {
     }
   }
 };
+
+// f(integral_constant<int, 0>) ... f(integral_constant<int, N - 1>)
+template <typename F, int... I>
+__device__ __forceinline__ void each_of(F& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F& f) {
+  each_of(f, std::make_integer_sequence<int, N>{});
+}
 
 // LDS accesses of one wave complete in order; this keeps the compiler to that order.
 __device__ __forceinline__ void wave_order() {
@@ -483,6 +499,15 @@ struct Rows {
     for (int ct = 0; ct < CT; ++ct)
       vf[ct] = __builtin_bit_cast(v8, u32x4_t{x[2 * ct][0], x[2 * ct][1], x[2 * ct + 1][0], x[2 * ct + 1][1]});
   }
+  // The same of one block of 32 features by the builtin, for tiles that come through registers.
+  template <int OFF>
+  static __device__ __forceinline__ v8 read_value(unsigned va) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4* at_t;
+    const v4 a = __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_t)(uintptr_t)(va + OFF)));
+    const v4 b = __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_t)(uintptr_t)(va + OFF + 8 * HD * 2)));
+    return v8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  }
   // O^T += V^T P^T
   template <int NB, int OFF, int KK = 0>
   __device__ __forceinline__ void values(const unsigned (&va)[CT], const v8 (&pf)[2 * NB]) {
@@ -497,46 +522,49 @@ struct Rows {
   // One step of the pipeline: n = K Q^T of the next tile beside the weights of s, then
   // O^T += V^T P^T beside the next tile's maximum, which is returned.  The order is pinned: a
   // wave issues in order, and MFMAs on end leave the vector unit idle.
-  template <int VOFF>
+  template <int VOFF, bool ASM>
   __device__ __forceinline__ float step(float16_t (&n)[2], const float16_t (&s)[2], const T* kt, const unsigned (&va)[CT],
                                         float c, int lane) {
-    constexpr int NK = 2 * KS, AHEAD = 4, PPM = 16 / NK;
+    constexpr int NK = 2 * KS, AHEAD = ASM ? 4 : 2, PPM = 16 / NK;
     const float mc = origin(c);
     auto key = [&](int i) {
       return *reinterpret_cast<const v8*>(kt + k_at<HD>((i / KS) * 32 + (lane & 31), (i % KS) * 2 + (lane >> 5)));
     };
-    v8 kf[AHEAD], pf[4], vf[2][CT];
+    constexpr int VR = ASM ? 2 * CT : 3;   // V fragments held
+    v8 kf[AHEAD], pf[4], vf[VR];
+    auto value = [&](auto I) {   // fragment I = kk * CT + ct
+      constexpr int i = decltype(I)::value;
+      if constexpr (!ASM && i < 4 * CT) vf[i % VR] = read_value<VOFF + (i / CT) * 16 * HD * 2>(va[i % CT]);
+    };
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) kf[i] = key(i);
     n[0] = float16_t{};
     n[1] = float16_t{};
     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int i = 0; i < NK; ++i) {
+    auto qk = [&](auto I) {
+      constexpr int i = decltype(I)::value;
       n[i / KS] = Elem<T>::mfma32(kf[i % AHEAD], qf[i % KS], n[i / KS]);
-      if (i + AHEAD < NK) kf[i % AHEAD] = key(i + AHEAD);
+      if constexpr (i + AHEAD < NK) kf[i % AHEAD] = key(i + AHEAD);
+      if constexpr (!ASM && i >= NK - VR) value(std::integral_constant<int, i - (NK - VR)>{});
 #pragma unroll
       for (int j = 0; j < PPM; ++j) weigh<2>(pf, s, i * PPM + j, c, mc);
-      if (i == NK - 2) read_values<VOFF>(vf[0], va);
+      if constexpr (ASM && i == NK - 2) read_values<VOFF>(*reinterpret_cast<v8 (*)[CT]>(&vf[0]), va);
       __builtin_amdgcn_sched_barrier(0);
-    }
-    float mx = -INFINITY;
-    auto pv = [&](auto KK) {
-      constexpr int kk = decltype(KK)::value;
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        o[ct] = Elem<T>::mfma32(vf[kk & 1][ct], pf[kk], o[ct]);
-        // the next tile's scores: 8 of them here, those of the second block last
-#pragma unroll
-        for (int i = 0; i < 8 / CT; ++i) mx = fmaxf(mx, n[kk >> 1][(kk & 1) * 8 + ct * (8 / CT) + i]);
-        if (ct == CT / 2 - 1 && kk < 3) read_values<VOFF + (kk < 3 ? kk + 1 : 3) * 16 * HD * 2>(vf[(kk + 1) & 1], va);
-        __builtin_amdgcn_sched_barrier(0);
-      }
     };
-    pv(std::integral_constant<int, 0>{});
-    pv(std::integral_constant<int, 1>{});
-    pv(std::integral_constant<int, 2>{});
-    pv(std::integral_constant<int, 3>{});
+    each<NK>(qk);
+    float mx = -INFINITY;
+    auto pv = [&](auto I) {
+      constexpr int i = decltype(I)::value, kk = i / CT, ct = i % CT;
+      o[ct] = Elem<T>::mfma32(vf[i % VR], pf[kk], o[ct]);
+      value(std::integral_constant<int, i + VR>{});
+      // the next tile's scores: 8 of them here, those of the second block last
+#pragma unroll
+      for (int j = 0; j < 8 / CT; ++j) mx = fmaxf(mx, n[kk >> 1][(kk & 1) * 8 + ct * (8 / CT) + j]);
+      if constexpr (ASM && ct == CT / 2 - 1 && kk < 3)
+        read_values<VOFF + (kk < 3 ? kk + 1 : 3) * 16 * HD * 2>(*reinterpret_cast<v8 (*)[CT]>(&vf[((kk + 1) & 1) * CT]), va);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    each<4 * CT>(pv);
     return half_max(mx);
   }
   // bad[k][d]: the first key whose V is +inf, -inf or NaN (k = 0, 1, 2) in feature d
@@ -613,20 +641,21 @@ __device__ __forceinline__ float2_t* part_ml(const AttendParams& p, long row) {
 // before into weights, so that the matrix cores and the vector unit work at the same time:
 //   step j:  S(j+1) = K(j+1) Q^T  beside  P(j) = 2^(S(j) - m);
 //            O += V(j)^T P(j)     beside  max S(j+1).
-// K is therefore one tile ahead of V; both have two buffers in LDS, and what step j+1 needs
-// (K(j+2), V(j+1)) is under way meanwhile (f16, bf16: straight to LDS; e4m3: through
-// registers, where it is turned into values).
-template <typename T, int HD, int KV, int NW>
+// K is therefore one tile ahead of V.  Both have S buffers in LDS; step j sends for V(j+S-1)
+// and K(j+S) (f16, bf16: straight to LDS; e4m3: through registers, where it is turned into
+// values, with two buffers).
+template <typename T, int HD, int KV, int NW, int S>
 __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendParams p) {
   constexpr int BM = 32 * NW, TILE = AT_KEYS * HD, NT = 64 * NW;
   constexpr bool DMA = KV != KV_E4M3;
+  static_assert(DMA || S == 2, "through registers one tile at a time");
   // one array: with several, the compiler holds every read of one back until all loads to the
   // others have landed
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE * 2 + 3 * HD * 4 + 16];
+  __shared__ __attribute__((aligned(1024))) char lds[2 * S * TILE * 2 + 3 * HD * 4 + 16];
   auto kt = [&](int buf) { return reinterpret_cast<T*>(lds) + buf * TILE; };
-  auto vt = [&](int buf) { return reinterpret_cast<T*>(lds) + (2 + buf) * TILE; };
-  int (*const bad)[HD] = reinterpret_cast<int (*)[HD]>(lds + 4 * TILE * 2);
-  int& odd = *reinterpret_cast<int*>(lds + 4 * TILE * 2 + 3 * HD * 4);
+  auto vt = [&](int buf) { return reinterpret_cast<T*>(lds) + (S + buf) * TILE; };
+  int (*const bad)[HD] = reinterpret_cast<int (*)[HD]>(lds + 2 * S * TILE * 2);
+  int& odd = *reinterpret_cast<int*>(lds + 2 * S * TILE * 2 + 3 * HD * 4);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hk = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv;
   Item it;
@@ -640,12 +669,16 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
 
   Stage<T, HD, KV, AT_KEYS, NT, false> ks;
   Stage<T, HD, KV, AT_KEYS, NT, true> vs;
+  constexpr int LOADS = 2 * decltype(ks)::N;   // of a step, K and V
   auto send = [&](auto& st, int key0, T* t) {
     if constexpr (DMA) st.dma(p, it, hk, key0, lane, wave, t);
     else st.load(p, it, hk, key0, lane, wave);
   };
-  ks.begin(p, it, hk, kbeg, AT_KEYS, lane, wave, DMA);
-  vs.begin(p, it, hk, kbeg, AT_KEYS, lane, wave, DMA);
+  // all but the loads of the last S - 2 steps have landed, here and (barrier) in the other waves
+  auto landed = [&] {
+    wait_vm_lgkm0<DMA ? (S - 2) * LOADS : 0>();
+    lds_barrier();
+  };
   Rows<T, HD> r;
   unsigned va[Rows<T, HD>::CT];
   r.values_at(va, vt(0), lane);
@@ -653,35 +686,31 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
   if (tid == 0) odd = 0;
   float16_t sa[2], sb[2];
   if (kbeg < kend) {
-    ks.pages(p, it, kbeg, wave);
-    vs.pages(p, it, kbeg, wave);
-    send(ks, kbeg, kt(0));
-    send(vs, kbeg, vt(0));
+    ks.begin(p, it, hk, kbeg, AT_KEYS, lane, wave, DMA);
+    vs.begin(p, it, hk, kbeg, AT_KEYS, lane, wave, DMA);
     r.begin(p, it, hk, tile * BM + wave * 32 + (lane & 31), lane);
-    if constexpr (!DMA) {
-      ks.store(kt(0), tid);
-      vs.store(vt(0), tid);
-    }
-    ks.pages(p, it, kbeg + AT_KEYS, wave);
-    vs.pages(p, it, kbeg + AT_KEYS, wave);
+    r.arrived();   // before the loads to LDS, so that no later wait counts Q's loads
+    send(ks, kbeg, kt(0));
+    if constexpr (!DMA) ks.store(kt(0), tid);
+    send(vs, kbeg, vt(0));
+    if constexpr (!DMA) vs.store(vt(0), tid);
     send(ks, kbeg + AT_KEYS, kt(1));
     if constexpr (!DMA) ks.store(kt(1), tid);
-    ks.pages(p, it, kbeg + 2 * AT_KEYS, wave);
-    r.arrived();
-    wait_vm_lgkm0<0>();
-    lds_barrier();
+#pragma unroll
+    for (int j = 1; j < S - 1; ++j) {
+      send(vs, kbeg + j * AT_KEYS, vt(j));
+      send(ks, kbeg + (j + 1) * AT_KEYS, kt(j + 1));
+    }
+    landed();
     r.template scores<2>(sa, kt(0), lane);
   } else {
     r.begin(p, it, hk, tile * BM + wave * 32 + (lane & 31), lane);
   }
-  // what step j sends for, once K(j+1) and V(j) are there and K(j)'s and V(j-1)'s buffers are free
+  // step j begins: K(j+1) and V(j) are there, K(j)'s and V(j-1)'s buffers free
   auto next = [&](int key0, int cur) {
-    wait_vm_lgkm0<0>();
-    lds_barrier();
-    send(vs, key0 + AT_KEYS, vt(cur ^ 1));
-    vs.pages(p, it, key0 + 2 * AT_KEYS, wave);
-    send(ks, key0 + 2 * AT_KEYS, kt(cur));
-    ks.pages(p, it, key0 + 3 * AT_KEYS, wave);
+    landed();
+    send(vs, key0 + (S - 1) * AT_KEYS, vt((cur + S - 1) % S));
+    send(ks, key0 + S * AT_KEYS, kt(cur));
   };
   auto keep = [&](int cur) {
     if constexpr (!DMA) {
@@ -689,25 +718,37 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
       ks.store(kt(cur), tid);
     }
   };
-  int key0 = kbeg;
-  // two steps at a time while every row sees all of this tile and of the two after it
-  const int kfull = min(klo, kend) - 3 * AT_KEYS;
+  int key0 = kbeg, cur = 0;
+  // while every row sees all of this tile and of the next one
+  const int kfull = min(klo, kend) - 2 * AT_KEYS;
   if (key0 <= kfull) {
     float mx = r.template top<2>(sa);
-    auto step = [&](float16_t (&s)[2], float16_t (&n)[2], int at, auto CUR) {
-      constexpr int cur = decltype(CUR)::value;
-      next(at, cur);
+    auto step = [&](float16_t (&s)[2], float16_t (&n)[2], auto CUR) {
+      constexpr int cu = decltype(CUR)::value;
+      next(key0, cu);
       r.raise(mx, c);
-      mx = r.template step<cur * TILE * 2>(n, s, kt(cur ^ 1), va, c, lane);
-      keep(cur);
+      mx = r.template step<cu * TILE * 2, DMA>(n, s, kt((cu + 1) % S), va, c, lane);
+      keep(cu);
+      key0 += AT_KEYS;
+      cur = (cu + 1) % S;
+      return key0 <= kfull;
     };
-    for (; key0 <= kfull; key0 += 2 * AT_KEYS) {
-      step(sa, sb, key0, std::integral_constant<int, 0>{});
-      step(sb, sa, key0 + AT_KEYS, std::integral_constant<int, 1>{});
+    using std::integral_constant;
+    for (;;) {
+      if (!step(sa, sb, integral_constant<int, 0>{})) break;
+      if (!step(sb, sa, integral_constant<int, 1>{})) break;
+      if constexpr (S == 4) {
+        if (!step(sa, sb, integral_constant<int, 2>{})) break;
+        if (!step(sb, sa, integral_constant<int, 3>{})) break;
+      }
+    }
+    if (cur & 1) {
+      sa[0] = sb[0];
+      sa[1] = sb[1];
     }
   }
   // the rest one by one
-  for (int cur = 0; key0 < kend; key0 += AT_KEYS, cur ^= 1) {
+  for (; key0 < kend; key0 += AT_KEYS, cur = (cur + 1) % S) {
     next(key0, cur);
     // A tile that some row sees in part: an infinity or NaN of V must not reach that row.
     bool fix = false;
@@ -736,10 +777,11 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
       if (tid == 0) odd = 0;
     }
     if (key0 + AT_KEYS < kend) {
-      r.template scores<2>(sa, kt(cur ^ 1), lane);
+      r.template scores<2>(sa, kt((cur + 1) % S), lane);
       keep(cur);
     }
   }
+  wait_vm_lgkm0<0>();   // the loads past the last tile land before this workgroup's LDS is another's
 
   if (it.nch == 1) {
     r.finish(p, it, hk, lane);
@@ -786,21 +828,17 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attend_few_kernel(const Att
   T* const kt = lds[wave];
   T* const vt = kt + TILE;
   int key0 = kbeg + wave * KEYS;
-  ks.begin(p, it, hk, key0, NW * KEYS, lane, 0, false);
-  vs.begin(p, it, hk, key0, NW * KEYS, lane, 0, false);
+  if (key0 < kend) {
+    ks.begin(p, it, hk, key0, NW * KEYS, lane, 0, false);
+    vs.begin(p, it, hk, key0, NW * KEYS, lane, 0, false);
+  }
   unsigned va[Rows<T, HD>::CT];
   r.values_at(va, vt, lane);
   auto load = [&](int key) {
     ks.load(p, it, hk, key, lane, 0);
     vs.load(p, it, hk, key, lane, 0);
-    ks.pages(p, it, key + NW * KEYS, 0);
-    vs.pages(p, it, key + NW * KEYS, 0);
   };
-  if (key0 < kend) {
-    ks.pages(p, it, key0, 0);
-    vs.pages(p, it, key0, 0);
-    load(key0);
-  }
+  if (key0 < kend) load(key0);
   for (; key0 < kend; key0 += NW * KEYS) {
     const bool part = key0 + KEYS > klo;
     wave_order();
@@ -951,8 +989,8 @@ template <typename T, int HD, int KV>
 void launch_kv(const AttendParams& p, const Plan& pl, hipStream_t s) {
   const dim3 grid((unsigned)(pl.items * p.Hkv));
   if (pl.bm == 32) CK_LAUNCH((attend_few_kernel<T, HD, KV>), grid, dim3(64 * FEW_WAVES), 0, s, p);
-  else if (pl.bm == 128) CK_LAUNCH((attend_tile_kernel<T, HD, KV, 4>), grid, dim3(256), 0, s, p);
-  else CK_LAUNCH((attend_tile_kernel<T, HD, KV, 8>), grid, dim3(512), 0, s, p);
+  else if (pl.bm == 128) CK_LAUNCH((attend_tile_kernel<T, HD, KV, 4, 2>), grid, dim3(256), 0, s, p);
+  else CK_LAUNCH((attend_tile_kernel<T, HD, KV, 8, 2>), grid, dim3(512), 0, s, p);
   if (!pl.target) return;
   const unsigned tiles = (unsigned)(pl.tiles * p.Hkv);
   if (pl.bm == 32) CK_LAUNCH((attend_join_kernel<T, HD, KV, 32>), dim3(tiles, 32), dim3(256), 0, s, p);
