@@ -641,21 +641,20 @@ __device__ __forceinline__ float2_t* part_ml(const AttendParams& p, long row) {
 // before into weights, so that the matrix cores and the vector unit work at the same time:
 //   step j:  S(j+1) = K(j+1) Q^T  beside  P(j) = 2^(S(j) - m);
 //            O += V(j)^T P(j)     beside  max S(j+1).
-// K is therefore one tile ahead of V.  Both have S buffers in LDS; step j sends for V(j+S-1)
-// and K(j+S) (f16, bf16: straight to LDS; e4m3: through registers, where it is turned into
-// values, with two buffers).
-template <typename T, int HD, int KV, int NW, int S>
+// K is therefore one tile ahead of V.  Both have two buffers in LDS; step j sends for V(j+1)
+// and K(j+2) (f16, bf16: straight to LDS; e4m3: through registers, where it is turned into
+// values).
+template <typename T, int HD, int KV, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendParams p) {
   constexpr int BM = 32 * NW, TILE = AT_KEYS * HD, NT = 64 * NW;
   constexpr bool DMA = KV != KV_E4M3;
-  static_assert(DMA || S == 2, "through registers one tile at a time");
   // one array: with several, the compiler holds every read of one back until all loads to the
   // others have landed
-  __shared__ __attribute__((aligned(1024))) char lds[2 * S * TILE * 2 + 3 * HD * 4 + 16];
+  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE * 2 + 3 * HD * 4 + 16];
   auto kt = [&](int buf) { return reinterpret_cast<T*>(lds) + buf * TILE; };
-  auto vt = [&](int buf) { return reinterpret_cast<T*>(lds) + (S + buf) * TILE; };
-  int (*const bad)[HD] = reinterpret_cast<int (*)[HD]>(lds + 2 * S * TILE * 2);
-  int& odd = *reinterpret_cast<int*>(lds + 2 * S * TILE * 2 + 3 * HD * 4);
+  auto vt = [&](int buf) { return reinterpret_cast<T*>(lds) + (2 + buf) * TILE; };
+  int (*const bad)[HD] = reinterpret_cast<int (*)[HD]>(lds + 4 * TILE * 2);
+  int& odd = *reinterpret_cast<int*>(lds + 4 * TILE * 2 + 3 * HD * 4);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hk = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv;
   Item it;
@@ -669,14 +668,13 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
 
   Stage<T, HD, KV, AT_KEYS, NT, false> ks;
   Stage<T, HD, KV, AT_KEYS, NT, true> vs;
-  constexpr int LOADS = 2 * decltype(ks)::N;   // of a step, K and V
   auto send = [&](auto& st, int key0, T* t) {
     if constexpr (DMA) st.dma(p, it, hk, key0, lane, wave, t);
     else st.load(p, it, hk, key0, lane, wave);
   };
-  // all but the loads of the last S - 2 steps have landed, here and (barrier) in the other waves
+  // what was sent for has landed, here and (barrier) in the other waves
   auto landed = [&] {
-    wait_vm_lgkm0<DMA ? (S - 2) * LOADS : 0>();
+    wait_vm_lgkm0<0>();
     lds_barrier();
   };
   Rows<T, HD> r;
@@ -696,11 +694,6 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
     if constexpr (!DMA) vs.store(vt(0), tid);
     send(ks, kbeg + AT_KEYS, kt(1));
     if constexpr (!DMA) ks.store(kt(1), tid);
-#pragma unroll
-    for (int j = 1; j < S - 1; ++j) {
-      send(vs, kbeg + j * AT_KEYS, vt(j));
-      send(ks, kbeg + (j + 1) * AT_KEYS, kt(j + 1));
-    }
     landed();
     r.template scores<2>(sa, kt(0), lane);
   } else {
@@ -709,8 +702,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
   // step j begins: K(j+1) and V(j) are there, K(j)'s and V(j-1)'s buffers free
   auto next = [&](int key0, int cur) {
     landed();
-    send(vs, key0 + (S - 1) * AT_KEYS, vt((cur + S - 1) % S));
-    send(ks, key0 + S * AT_KEYS, kt(cur));
+    send(vs, key0 + AT_KEYS, vt(cur ^ 1));
+    send(ks, key0 + 2 * AT_KEYS, kt(cur));
   };
   auto keep = [&](int cur) {
     if constexpr (!DMA) {
@@ -727,28 +720,23 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
       constexpr int cu = decltype(CUR)::value;
       next(key0, cu);
       r.raise(mx, c);
-      mx = r.template step<cu * TILE * 2, DMA>(n, s, kt((cu + 1) % S), va, c, lane);
+      mx = r.template step<cu * TILE * 2, DMA>(n, s, kt(cu ^ 1), va, c, lane);
       keep(cu);
       key0 += AT_KEYS;
-      cur = (cu + 1) % S;
-      return key0 <= kfull;
     };
-    using std::integral_constant;
-    for (;;) {
-      if (!step(sa, sb, integral_constant<int, 0>{})) break;
-      if (!step(sb, sa, integral_constant<int, 1>{})) break;
-      if constexpr (S == 4) {
-        if (!step(sa, sb, integral_constant<int, 2>{})) break;
-        if (!step(sb, sa, integral_constant<int, 3>{})) break;
-      }
+    while (key0 + AT_KEYS <= kfull) {
+      step(sa, sb, std::integral_constant<int, 0>{});
+      step(sb, sa, std::integral_constant<int, 1>{});
     }
-    if (cur & 1) {
+    if (key0 <= kfull) {
+      step(sa, sb, std::integral_constant<int, 0>{});
+      cur = 1;
       sa[0] = sb[0];
       sa[1] = sb[1];
     }
   }
   // the rest one by one
-  for (; key0 < kend; key0 += AT_KEYS, cur = (cur + 1) % S) {
+  for (; key0 < kend; key0 += AT_KEYS, cur ^= 1) {
     next(key0, cur);
     // A tile that some row sees in part: an infinity or NaN of V must not reach that row.
     bool fix = false;
@@ -777,7 +765,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
       if (tid == 0) odd = 0;
     }
     if (key0 + AT_KEYS < kend) {
-      r.template scores<2>(sa, kt((cur + 1) % S), lane);
+      r.template scores<2>(sa, kt(cur ^ 1), lane);
       keep(cur);
     }
   }
@@ -989,8 +977,8 @@ template <typename T, int HD, int KV>
 void launch_kv(const AttendParams& p, const Plan& pl, hipStream_t s) {
   const dim3 grid((unsigned)(pl.items * p.Hkv));
   if (pl.bm == 32) CK_LAUNCH((attend_few_kernel<T, HD, KV>), grid, dim3(64 * FEW_WAVES), 0, s, p);
-  else if (pl.bm == 128) CK_LAUNCH((attend_tile_kernel<T, HD, KV, 4, 2>), grid, dim3(256), 0, s, p);
-  else CK_LAUNCH((attend_tile_kernel<T, HD, KV, 8, 2>), grid, dim3(512), 0, s, p);
+  else if (pl.bm == 128) CK_LAUNCH((attend_tile_kernel<T, HD, KV, 4>), grid, dim3(256), 0, s, p);
+  else CK_LAUNCH((attend_tile_kernel<T, HD, KV, 8>), grid, dim3(512), 0, s, p);
   if (!pl.target) return;
   const unsigned tiles = (unsigned)(pl.tiles * p.Hkv);
   if (pl.bm == 32) CK_LAUNCH((attend_join_kernel<T, HD, KV, 32>), dim3(tiles, 32), dim3(256), 0, s, p);
