@@ -309,31 +309,38 @@ def _rows(t, dtype, name, shape, unit=8, write=False):
     T, H, hd = shape
     if s2 != 1 and hd > 1:
         raise ValueError(f'{name} must be contiguous in its last dimension')
-    s0 = s0 if T > 1 else 0
-    s1 = s1 if H > 1 else 0
-    if s0 % unit or s1 % unit or t.data_ptr() % (2 * unit):
+    if T <= 1:
+        s0 = 0
+    if H <= 1:
+        s1 = 0
+    if (s0 | s1) % unit or t.data_ptr() % (2 * unit):
         raise ValueError(f'{name} must have rows that start at multiples of {2 * unit} bytes')
+    if s0 >= 1 << 24:
+        raise ValueError(f'{name} must have under 2^24 elements from one token to the next')
     if write and ((T > 1 and s0 < hd) or (H > 1 and s1 < hd)):
         raise ValueError(f'{name} must not overlap itself')
     return s0, s1
 
 
-def _int32(t, name, shape):
-    """A contiguous int32 tensor; None entries of shape are free."""
-    _check(t, torch.int32, name, shape)
+def _is(t, dtype, name, shape):
+    """_check, at a fraction of its time where all is well."""
+    if type(t) is not torch.Tensor or t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        _check(t, dtype, name, shape)
 
 
-def _on_device(*named):
+def _on_device(names, *tensors):
     """The current device, on which every present tensor must be (the first one always is)."""
-    dev = named[0][0].get_device()
-    for t, name in named:
-        if t is not None and (t.get_device() != dev or dev < 0):
-            if not t.is_cuda:
-                raise ValueError(f'{name} must be a CUDA tensor')
-            dev = -2   # not where the others are
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            dev = -2
             break
-    if dev != _device():
-        raise ValueError('; '.join(f'{name} is on {t.device}' for t, name in named if t is not None) +
+    if dev < 0 or dev != _device():
+        present = [(t, n) for t, n in zip(tensors, names.split()) if t is not None]
+        for t, n in present:
+            if not t.is_cuda:
+                raise ValueError(f'{n} must be a CUDA tensor')
+        raise ValueError('; '.join(f'{n} is on {t.device}' for t, n in present) +
                          f', not the current device cuda:{_device()}')
     return dev
 
@@ -342,20 +349,21 @@ def _cache(k_pages, v_pages, k_scale, v_scale):
     """The checks of a cache; its shape (n_pages, n_kv, page, head_dim)."""
     if not isinstance(k_pages, torch.Tensor) or k_pages.dim() != 4:
         raise ValueError('k_pages must be [n_pages, n_kv, page, head_dim]')
-    if k_pages.dtype not in _DTYPE:
-        raise ValueError(f'k_pages must be float16, bfloat16 or float8_e4m3fn, got {k_pages.dtype}')
+    dtype = k_pages.dtype
+    if dtype not in _DTYPE:
+        raise ValueError(f'k_pages must be float16, bfloat16 or float8_e4m3fn, got {dtype}')
     n, kv, page, hd = shape = k_pages.shape
     if page < 16 or page > 1024 or page & (page - 1):
         raise ValueError(f'the page size must be a power of two from 16 to 1024, got {page}')
     if n < 1 or kv < 1:
         raise ValueError('k_pages must hold a page and a head')
-    _check(k_pages, k_pages.dtype, 'k_pages')
-    _check(v_pages, k_pages.dtype, 'v_pages', shape)
-    if k_pages.dtype is _E4M3:
+    _is(k_pages, dtype, 'k_pages', shape)
+    _is(v_pages, dtype, 'v_pages', shape)
+    if dtype is _E4M3:
         if k_scale is None or v_scale is None:
             raise ValueError('an e4m3 cache needs k_scale and v_scale')
-        _check(k_scale, _E8M0, 'k_scale', (n, kv, page))
-        _check(v_scale, _E8M0, 'v_scale', (n, kv, page))
+        _is(k_scale, _E8M0, 'k_scale', shape[:3])
+        _is(v_scale, _E8M0, 'v_scale', shape[:3])
     elif k_scale is not None or v_scale is not None:
         raise ValueError('k_scale and v_scale belong to an e4m3 cache')
     return shape
@@ -413,13 +421,13 @@ def rope(x, positions, inv_freq, interleaved=False, scale=1.0, inverse=False, ou
         raise ValueError(f'inv_freq must have 1 to head_dim / 2 = {hd // 2} entries, got {rot // 2}')
     if H < 1 or hd > 512 or H > 1024 or H * hd > 65536:
         raise ValueError('rope takes head_dim up to 512, heads up to 1024 and 65536 elements a token')
-    _int32(positions, 'positions', (T,))
+    _is(positions, torch.int32, 'positions', (T,))
     st, sh = _rows(x, x.dtype, 'x', x.shape, 1, out is x)
     if out is None:
         ot, oh = H * hd, hd
     else:
         ot, oh = (st, sh) if out is x else _rows(out, x.dtype, 'out', x.shape, 1, True)
-    dev = _on_device((x, 'x'), (positions, 'positions'), (inv_freq, 'inv_freq'), (out, 'out'))
+    dev = _on_device('x positions inv_freq out', x, positions, inv_freq, out)
     y = out if out is not None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
     check(lib().ck_rope(x.data_ptr(), y.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), T, H, hd, rot, st, sh,
                         ot, oh, _DTYPE[x.dtype], 1 if interleaved else 0, scale, 1 if inverse else 0, _raw_stream(dev)))
@@ -439,9 +447,8 @@ def cache_write(k, v, k_pages, v_pages, slots, k_scale=None, v_scale=None):
     T = k.shape[0]
     kt, kh = _rows(k, k.dtype, 'k', (T, kv, hd))
     vt, vh = _rows(v, k.dtype, 'v', (T, kv, hd))
-    _int32(slots, 'slots', (T,))
-    dev = _on_device((k, 'k'), (v, 'v'), (k_pages, 'k_pages'), (v_pages, 'v_pages'), (slots, 'slots'),
-                     (k_scale, 'k_scale'), (v_scale, 'v_scale'))
+    _is(slots, torch.int32, 'slots', (T,))
+    dev = _on_device('k v k_pages v_pages slots k_scale v_scale', k, v, k_pages, v_pages, slots, k_scale, v_scale)
     check(lib().ck_cache_write(k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale),
                                _ptr(v_scale), slots.data_ptr(), T, n, kv, page, hd, kt, kh, vt, vh, _DTYPE[k.dtype],
                                _DTYPE[k_pages.dtype], _raw_stream(dev)))
@@ -460,15 +467,14 @@ def cache_read(k_pages, v_pages, block_table, cu_seqlens, tokens, k_scale=None, 
         raise ValueError(f'dtype must be float16 or bfloat16, and that of the cache ({k_pages.dtype}) unless it is e4m3')
     if not isinstance(tokens, int) or tokens < 0:
         raise ValueError('tokens must be the number of rows')
-    _int32(block_table, 'block_table', (None, None))
+    _check(block_table, torch.int32, 'block_table', (None, None))
     B, width = block_table.shape
-    _int32(cu_seqlens, 'cu_seqlens', (B + 1,))
+    _is(cu_seqlens, torch.int32, 'cu_seqlens', (B + 1,))
     for t, name in ((k_out, 'k_out'), (v_out, 'v_out')):
         if t is not None:
             _check(t, dtype, name, (tokens, kv, hd))
-    dev = _on_device((k_pages, 'k_pages'), (v_pages, 'v_pages'), (block_table, 'block_table'),
-                     (cu_seqlens, 'cu_seqlens'), (k_scale, 'k_scale'), (v_scale, 'v_scale'), (k_out, 'k_out'),
-                     (v_out, 'v_out'))
+    dev = _on_device('k_pages v_pages block_table cu_seqlens k_scale v_scale k_out v_out', k_pages, v_pages,
+                     block_table, cu_seqlens, k_scale, v_scale, k_out, v_out)
     k, v = (t if t is not None else torch.empty((tokens, kv, hd), dtype=dtype, device=k_pages.device)
             for t in (k_out, v_out))
     check(lib().ck_cache_read(k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale),
@@ -487,7 +493,8 @@ def _queries(q, cu_q, kv, hd, out, scale):
         raise ValueError(f'head_dim must be 64 or 128 for q and the keys alike, got {d} and {hd}')
     if kv < 1 or H < 1 or H % kv or H > 1024:
         raise ValueError(f'the query heads ({H}, up to 1024) must be a multiple of the K/V heads ({kv})')
-    _int32(cu_q, 'cu_q', (None,))
+    if type(cu_q) is not torch.Tensor or cu_q.dtype is not torch.int32 or cu_q.dim() != 1 or not cu_q.is_contiguous():
+        _check(cu_q, torch.int32, 'cu_q', (None,))
     if cu_q.shape[0] < 1:
         raise ValueError('cu_q must hold B + 1 offsets')
     qs = _rows(q, q.dtype, 'q', q.shape)
@@ -498,12 +505,11 @@ def _queries(q, cu_q, kv, hd, out, scale):
     return T, H, cu_q.shape[0] - 1, qs, os, scale
 
 
-def _attention_workspace(ws, B, T, keys, H, kv, hd, device):
-    """The workspace of an attention call: the caller's if it is large enough."""
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(B, T, keys, H, kv, hd):
     nb = ctypes.c_size_t()
     check(lib().ck_attention_workspace(B, T, keys, H, kv, hd, ctypes.byref(nb)))
-    ws = _workspace(ws, nb.value, device)
-    return _ptr(ws), nb.value
+    return nb.value
 
 
 def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None, workspace=None):
@@ -525,13 +531,14 @@ def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None
             raise ValueError(f'k must have the {T} rows of q where cu_k is not given, got {Tk}')
         cu_k = cu_q
     else:
-        _int32(cu_k, 'cu_k', (B + 1,))
-    dev = _on_device((q, 'q'), (k, 'k'), (v, 'v'), (cu_q, 'cu_q'), (cu_k, 'cu_k'), (out, 'out'))
+        _is(cu_k, torch.int32, 'cu_k', (B + 1,))
+    dev = _on_device('q k v cu_q cu_k out', q, k, v, cu_q, cu_k, out)
     o = out if out is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ws, nb = _attention_workspace(workspace, B, T, Tk, H, kv, hd, q.device)
+    nb = _workspace_bytes(B, T, Tk, H, kv, hd)
+    ws = _workspace(workspace, nb, q.device)
     check(lib().ck_attention_varlen(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu_q.data_ptr(),
                                     cu_k.data_ptr(), B, T, Tk, H, kv, hd, qt, qh, kt, kh, vt, vh, ot, oh,
-                                    _DTYPE[q.dtype], 1 if causal else 0, scale, ws, nb, _raw_stream(dev)))
+                                    _DTYPE[q.dtype], 1 if causal else 0, scale, _ptr(ws), nb, _raw_stream(dev)))
     return o
 
 
@@ -547,15 +554,18 @@ def attention_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, k_scale=Non
     T, H, B, (qt, qh), (ot, oh), scale = _queries(q, cu_q, kv, hd, out, scale)
     if k_pages.dtype not in (q.dtype, _E4M3):
         raise ValueError(f'the cache must be {q.dtype} or float8_e4m3fn, got {k_pages.dtype}')
-    _int32(kv_lens, 'kv_lens', (B,))
-    _int32(block_table, 'block_table', (B, None))
+    _is(kv_lens, torch.int32, 'kv_lens', (B,))
+    if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
+        raise ValueError('block_table must be int32 [B, width]')
     width = block_table.shape[1]
-    dev = _on_device((q, 'q'), (k_pages, 'k_pages'), (v_pages, 'v_pages'), (block_table, 'block_table'), (cu_q, 'cu_q'),
-                     (kv_lens, 'kv_lens'), (k_scale, 'k_scale'), (v_scale, 'v_scale'), (out, 'out'))
+    _is(block_table, torch.int32, 'block_table', (B, width))
+    dev = _on_device('q k_pages v_pages block_table cu_q kv_lens k_scale v_scale out', q, k_pages, v_pages, block_table,
+                     cu_q, kv_lens, k_scale, v_scale, out)
     o = out if out is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ws, nb = _attention_workspace(workspace, B, T, B * width * page, H, kv, hd, q.device)
+    nb = _workspace_bytes(B, T, B * width * page, H, kv, hd)
+    ws = _workspace(workspace, nb, q.device)
     check(lib().ck_attention_paged(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale),
                                    o.data_ptr(), block_table.data_ptr(), width, cu_q.data_ptr(), kv_lens.data_ptr(), B,
                                    T, H, n, kv, page, hd, qt, qh, ot, oh, _DTYPE[q.dtype], _DTYPE[k_pages.dtype],
-                                   1 if causal else 0, scale, ws, nb, _raw_stream(dev)))
+                                   1 if causal else 0, scale, _ptr(ws), nb, _raw_stream(dev)))
     return o

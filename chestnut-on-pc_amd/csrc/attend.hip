@@ -196,7 +196,8 @@ __device__ __forceinline__ int v_at(int key, int c) {
 
 // KEYS rows of K or V on their way to LDS by NT threads.  Places behind the last key repeat
 // it.  A wave's rows of one load lie in one group of 16, so on one page.
-template <typename T, int HD, int KV, int KEYS, int NT, bool V>
+// ONCE: this workgroup alone reads them, past the caches.
+template <typename T, int HD, int KV, int KEYS, int NT, bool V, bool ONCE = false>
 struct Stage {
   typedef typename Elem<T>::v2 v2;
   typedef typename Elem<T>::v8 v8;
@@ -293,7 +294,8 @@ struct Stage {
   // sends for the rows; store() leaves them (e4m3: as values of T) in LDS
   __device__ __forceinline__ void load(const AttendParams& p, const Item& it, int hk, int key0, int lane, int wave) {
     rows(p, it, hk, key0, lane, wave, [&](int i, auto at, long row) {
-      x[i] = *(const __attribute__((address_space(1))) raw*)at;
+      const auto from = (const __attribute__((address_space(1))) raw*)at;
+      x[i] = ONCE ? __builtin_nontemporal_load(from) : *from;
       if constexpr (KV == KV_E4M3) scale[i] = (V ? p.vs : p.ks)[row];
     });
   }
@@ -811,8 +813,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attend_few_kernel(const Att
   const int kend = it.nch > 1 ? min(khi, kbeg + it.c * AT_KEYS) : khi;
 
   r.arrived();
-  Stage<T, HD, KV, KEYS, 64, false> ks;
-  Stage<T, HD, KV, KEYS, 64, true> vs;
+  Stage<T, HD, KV, KEYS, 64, false, true> ks;
+  Stage<T, HD, KV, KEYS, 64, true, true> vs;
   T* const kt = lds[wave];
   T* const vt = kt + TILE;
   int key0 = kbeg + wave * KEYS;
@@ -1002,6 +1004,8 @@ void launch_attend(const char* what, AttendParams& p, const AttendQuery& a, int 
   CK_REQUIRE(a.scale > 0.f && a.scale < INFINITY, w + ": scale must be positive and finite");
   if (a.T == 0 || a.B == 0) return;
   CK_REQUIRE(a.q && a.out && a.cu_q && p.kv, w + ": null pointer");
+  // a lane's bytes from its wave's first row are counted in 32 bits
+  CK_REQUIRE(p.k_st < (1L << 24) && p.v_st < (1L << 24) && p.k_st >= 0 && p.v_st >= 0, w + ": token strides must be under 2^24");
   CK_REQUIRE(((a.q_st | a.q_sh) & 7) == 0 && ((a.o_st | a.o_sh) & 3) == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 &&
                  (reinterpret_cast<uintptr_t>(a.out) & 7) == 0,
              w + ": q rows must be 16-byte and out rows 8-byte aligned");

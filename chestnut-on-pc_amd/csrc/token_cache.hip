@@ -31,47 +31,69 @@ __device__ __forceinline__ long cache_row(long page, int h, int place, int Hkv, 
   return ((page * Hkv + h) << page_shift) + place;
 }
 
-// LPR lanes a row, 8 elements each (lanes behind hd / 8 idle).
-template <typename T, bool Q, int LPR>
+// The maximum over the LPR lanes (a power of two) of a row, in each of them.
+template <int LPR>
+__device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, dpp_mov<DPP_QUAD_1032>(v));
+  v = fmaxf(v, dpp_mov<DPP_QUAD_2301>(v));
+  if (LPR > 4) v = fmaxf(v, dpp_mov<DPP_ROW_HALF_MIRROR>(v));
+  if (LPR > 8) v = fmaxf(v, dpp_mov<DPP_ROW_MIRROR>(v));
+  if (LPR > 16) v = fmaxf(v, __shfl_xor(v, 16));
+  return v;
+}
+
+// LPR lanes a row (those behind its end idle), E elements each, K and V of a row together:
+// four 16-byte loads a thread are under way at once.
+template <typename T, bool Q, int E, int LPR>
 __global__ __launch_bounds__(256) void cache_write_kernel(const WriteParams p) {
-  constexpr int RPB = 256 / LPR;
+  typedef typename Elem<T>::v8 v8;
   const int c = threadIdx.x % LPR;
-  const unsigned r = blockIdx.x * RPB + threadIdx.x / LPR;
-  const bool isv = blockIdx.y;
+  const unsigned r = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
   if (r >= p.rows) return;
   const unsigned t = r / (unsigned)p.Hkv, h = r - t * p.Hkv;
+  const bool in = c * E < p.hd;
+  v8 x[2][E / 8];
+#pragma unroll
+  for (int v = 0; v < 2; ++v) {
+    const T* src = static_cast<const T*>(v ? p.v : p.k) + t * (v ? p.vst : p.kst) + h * (v ? p.vsh : p.ksh) + c * E;
+#pragma unroll
+    for (int i = 0; i < E / 8; ++i) {
+      x[v][i] = v8{};
+      if (in) x[v][i] = __builtin_nontemporal_load(reinterpret_cast<const v8*>(src) + i);
+    }
+  }
   const int slot = p.slots[t];
   if (slot < 0 || slot >= p.n_slots) return;
-  const T* src = static_cast<const T*>(isv ? p.v : p.k) + t * (isv ? p.vst : p.kst) + h * (isv ? p.vsh : p.ksh);
   const long row = cache_row(slot >> p.page_shift, h, slot & ((1 << p.page_shift) - 1), p.Hkv, p.page_shift);
-  typedef typename Elem<T>::v8 v8;
-  const bool in = c * 8 < p.hd;
-  v8 x{};
-  if (in) x = *reinterpret_cast<const v8*>(src + c * 8);
-  if constexpr (!Q) {
-    if (in) *reinterpret_cast<v8*>(static_cast<T*>(isv ? p.vp : p.kp) + row * p.hd + c * 8) = x;
-  } else {
-    // values that four significant bits would carry past the type's range are held at its top; NaN stays
-    float f[8], amax = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      f[j] = (float)x[j];
-      f[j] = f[j] > Elem<T>::top ? Elem<T>::top : f[j] < -Elem<T>::top ? -Elem<T>::top : f[j];
-      amax = fmaxf(amax, fabsf(f[j]));
+  for (int v = 0; v < 2; ++v) {
+    void* const dst = v ? p.vp : p.kp;
+    if constexpr (!Q) {
+#pragma unroll
+      for (int i = 0; i < E / 8; ++i)
+        if (in) *(reinterpret_cast<v8*>(static_cast<T*>(dst) + row * p.hd + c * E) + i) = x[v][i];
+    } else {
+      // values that four significant bits would carry past the type's range are held at its top; NaN stays
+      float f[E], amax = 0.f;
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        f[j] = (float)x[v][j / 8][j % 8];
+        f[j] = f[j] > Elem<T>::top ? Elem<T>::top : f[j] < -Elem<T>::top ? -Elem<T>::top : f[j];
+        amax = fmaxf(amax, fabsf(f[j]));
+      }
+      const unsigned bits = __builtin_bit_cast(unsigned, row_max<LPR>(amax));
+      const int e = max(1, (int)(bits >> 23) - 8 + ((bits & 0x7FFFFF) > 0x600000 ? 1 : 0));
+      const float inv = __builtin_bit_cast(float, (unsigned)(254 - e) << 23);
+      typedef unsigned codes __attribute__((ext_vector_type(E / 4)));
+      codes w;
+#pragma unroll
+      for (int j = 0; j < E; j += 4) {
+        const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[j] * inv, f[j + 1] * inv, 0, false);
+        w[j / 4] = __builtin_amdgcn_cvt_pk_fp8_f32(f[j + 2] * inv, f[j + 3] * inv, lo, true);
+      }
+      if (in) *reinterpret_cast<codes*>(static_cast<uint8_t*>(dst) + row * p.hd + c * E) = w;
+      if (c == 0) (v ? p.vs : p.ks)[row] = (uint8_t)e;
     }
-#pragma unroll
-    for (int o = LPR / 2; o; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-    const unsigned bits = __builtin_bit_cast(unsigned, amax);
-    const int e = max(1, (int)(bits >> 23) - 8 + ((bits & 0x7FFFFF) > 0x600000 ? 1 : 0));
-    const float inv = __builtin_bit_cast(float, (unsigned)(254 - e) << 23);
-    int lo = 0, hi = 0;
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0] * inv, f[1] * inv, lo, false);
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[2] * inv, f[3] * inv, lo, true);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[4] * inv, f[5] * inv, hi, false);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[6] * inv, f[7] * inv, hi, true);
-    if (in) *reinterpret_cast<u32x2_t*>(static_cast<uint8_t*>(isv ? p.vp : p.kp) + row * p.hd + c * 8) =
-        u32x2_t{(unsigned)lo, (unsigned)hi};
-    if (c == 0) (isv ? p.vs : p.ks)[row] = (uint8_t)e;
   }
 }
 
@@ -146,11 +168,11 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const ReadParams p) {
 
 template <typename T, bool Q>
 void write_t(const WriteParams& p, hipStream_t s) {
-  const int lpr = p.hd <= 64 ? 8 : p.hd <= 128 ? 16 : 32;
-  const dim3 grid(ceil_div(p.rows, 256 / lpr), 2), block(256);
-  if (lpr == 8) CK_LAUNCH((cache_write_kernel<T, Q, 8>), grid, block, 0, s, p);
-  else if (lpr == 16) CK_LAUNCH((cache_write_kernel<T, Q, 16>), grid, block, 0, s, p);
-  else CK_LAUNCH((cache_write_kernel<T, Q, 32>), grid, block, 0, s, p);
+  auto go = [&](auto kernel, int lpr) { CK_LAUNCH(kernel, dim3(ceil_div(p.rows, 256 / lpr)), dim3(256), 0, s, p); };
+  if (p.hd % 16) go(cache_write_kernel<T, Q, 8, 32>, 32);
+  else if (p.hd <= 64) go(cache_write_kernel<T, Q, 16, 4>, 4);
+  else if (p.hd <= 128) go(cache_write_kernel<T, Q, 16, 8>, 8);
+  else go(cache_write_kernel<T, Q, 16, 16>, 16);
 }
 
 }  // namespace

@@ -46,10 +46,8 @@ def quantise(x, top):
     rounding to four significant bits leaves finite in x's type; larger ones are held at it."""
     x = np.clip(np.asarray(x, np.float64), -top, top)
     amax = np.nanmax(np.where(np.isnan(x), 0, np.abs(x)), -1)
-    byte = np.full(amax.shape, 1)
-    nz = amax > 0
-    byte[nz] = np.maximum(1, np.array([math.ceil(math.log2(a / 448)) if a / 448 != 2.0 ** math.floor(math.log2(a / 448))
-                                       else math.floor(math.log2(a / 448)) for a in amax[nz]]) + 127)
+    m, e = np.frexp(amax / 448)                # amax / 448 = m 2^e, m in [0.5, 1)
+    byte = np.maximum(1, np.where(amax > 0, e - (m == 0.5) + 127, 1))
     return e4m3_codes(x * 2.0 ** (127.0 - byte)[..., None]), byte.astype(np.uint8)
 
 

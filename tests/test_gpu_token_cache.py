@@ -236,6 +236,61 @@ def test_attention_paged(gpu, qlens, klens, H, kv, hd, page, dt, quant, causal):
         a += x
 
 
+def attention_on_gpu(q, k, v, causal):
+    """oracle.attention's three results for long sequences of finite values: f64 on the device."""
+    q, k, v = q.double(), k.double(), v.double()
+    (n, H, hd), (m, kv, _) = q.shape, k.shape
+    out, mag, most = torch.zeros_like(q), torch.zeros_like(q), 0.0
+    see = torch.arange(m, device='cuda')[None] <= torch.arange(n, device='cuda')[:, None] + (m - n if causal else m)
+    for h in range(H):
+        g = h // (H // kv)
+        p = torch.softmax((q[:, h] @ k[:, g].T / hd ** 0.5).masked_fill(~see, -float('inf')), -1)
+        out[:, h], mag[:, h] = p @ v[:, g], p @ v[:, g].abs()
+        most = max(most, (q[:, h].norm(dim=-1).max() * k[:, g].norm(dim=-1).max() / hd ** 0.5).item())
+    return f64(out), f64(mag), most
+
+
+@pytest.mark.parametrize('lens,H,kv,hd', [([4500, 300, 1111], 8, 2, 128), ([3000], 4, 4, 64), ([2500, 2049, 64], 32, 8, 64),
+                                          ([4200], 32, 8, 128)])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('causal', [True, False])
+def test_long_prompts(gpu, lens, H, kv, hd, dt, causal):
+    """Many tiles a row: every buffer of the pipeline many times over, and both tile heights."""
+    from chestnut import kernels as K
+    q, k, v = rows(1, sum(lens), H, hd, dt), rows(2, sum(lens), kv, hd, dt), rows(3, sum(lens), kv, hd, dt)
+    out = K.attention_varlen(q, k, v, cu(lens), causal=causal)
+    assert torch.equal(out, K.attention_varlen(q, k, v, cu(lens), causal=causal))
+    a = 0
+    for n in lens:
+        near(out[a:a + n], *attention_on_gpu(q[a:a + n], k[a:a + n], v[a:a + n], causal), n, hd, dt, str(n))
+        a += n
+
+
+@pytest.mark.parametrize('qlens,klens,H,kv,hd,page', [([512], [5000], 2, 2, 128, 64), ([1, 300, 2, 77], [3000, 2500, 6000, 77], 8, 2, 128, 32),
+                                                      ([1] * 12, [300 * i + 1 for i in range(12)], 16, 2, 64, 256),
+                                                      ([1] * 130, [7 * i for i in range(130)], 4, 2, 128, 16),
+                                                      ([800, 900], [3000, 900], 4, 4, 64, 128)])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('quant', [False, True])
+@pytest.mark.parametrize('causal', [True, False])
+def test_long_histories(gpu, qlens, klens, H, kv, hd, page, dt, quant, causal):
+    """Keys split over workgroups: chunks, more sequences than lanes, ragged lengths."""
+    from chestnut import kernels as K
+    table, n = tables(klens, page, 5)
+    kp, vp, ks, vs = filled(n, kv, page, hd, dt, 'e4m3' if quant else dt, 6)
+    q = rows(8, sum(qlens), H, hd, dt)
+    out = K.attention_paged(q, kp, vp, i32(table), cu(qlens), i32(klens), k_scale=ks, v_scale=vs, causal=causal)
+    assert torch.equal(out, K.attention_paged(q, kp, vp, i32(table), cu(qlens), i32(klens), k_scale=ks, v_scale=vs, causal=causal))
+    a = 0
+    for b, (x, m) in enumerate(zip(qlens, klens)):
+        if m:
+            k, v = (torch.from_numpy(gathered(p, s, table[b], m, page)).cuda() for p, s in ((kp, ks), (vp, vs)))
+            near(out[a:a + x], *attention_on_gpu(q[a:a + x], k, v, causal), m, hd, dt, f'{x} over {m}')
+        else:
+            assert (out[a:a + x] == 0).all()
+        a += x
+
+
 @pytest.mark.parametrize('dt', ['f16', 'bf16'])
 @pytest.mark.parametrize('hd', [64, 128])
 @pytest.mark.parametrize('paged', [False, True])

@@ -92,6 +92,9 @@ REFUSED = [
     ('paged table type', lambda: paged(table=z(2, 3, dtype=torch.int64)), 'block_table must be torch.int32'),
     ('paged lens', lambda: paged(lens=z(3, dtype=i32)), 'kv_lens must have shape'),
     ('paged table strided', lambda: paged(table=z(2, 6, dtype=i32)[:, ::2]), 'block_table must be contiguous'),
+    ('varlen token stride', lambda: varlen(k=torch.empty_strided((4, 2, 64), (1 << 24, 64, 1), dtype=f16, device='meta')),
+     'under 2\\^24 elements'),
+    ('paged table rank', lambda: paged(table=z(6, dtype=i32)), 'block_table must be int32'),
     ('paged cpu tensors', paged, 'must be a CUDA tensor'),
     ('varlen cpu tensors', varlen, 'must be a CUDA tensor'),
     ('rope cpu tensors', lambda: K.rope(z(4, 2, 64), z(4, dtype=i32), F), 'must be a CUDA tensor'),
