@@ -967,7 +967,9 @@ Plan plan_of(int B, int Tq, long keys, int n_heads, int n_kv) {
   const long rows = (long)Tq * G;
   pl.bm = rows <= 32L * B ? 32 : (rows / 256 + B) * n_kv >= 512 ? 256 : 128;
   pl.tiles = rows / pl.bm + B;       // sum of ceil(rows_b / bm) is at most this
-  const long slots = pl.bm == 256 ? 256 : 512;   // workgroups that run at once: one a CU, or two
+  // items to aim at: workgroups that run at once, one a CU or two; of few rows twice as many, as
+  // their chunks come out uneven (32 ragged histories 127 -> 122 us; three times as many 125)
+  const long slots = pl.bm == 256 ? 256 : pl.bm == 128 ? 512 : 1024;
   pl.min_blocks = pl.bm == 32 ? 2 : 4;
   const bool many = pl.bm != 32 && pl.tiles * n_kv >= 2 * slots;
   if (!many && keys / B > 2 * pl.min_blocks * AT_KEYS) pl.target = (int)std::max(1L, slots / n_kv);

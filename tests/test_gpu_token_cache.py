@@ -186,8 +186,12 @@ def filled(n, kv, page, hd, dt, cache, seed):
 
 def gathered(p, s, row, m, page):
     """The first m places of a sequence, [m, kv, hd] f64."""
-    x = f64(p) if s is None else O.values(p.view(torch.uint8).cpu().numpy(), s.view(torch.uint8).cpu().numpy())
-    return x[row[:-(-m // page)]].transpose(0, 2, 1, 3).reshape(-1, x.shape[1], x.shape[3])[:m]
+    row = torch.from_numpy(np.ascontiguousarray(row[:-(-m // page)])).cuda()
+    if s is None:
+        x = f64(p[row])
+    else:
+        x = O.values(p.view(torch.uint8)[row].cpu().numpy(), s.view(torch.uint8)[row].cpu().numpy())
+    return x.transpose(0, 2, 1, 3).reshape(-1, x.shape[1], x.shape[3])[:m]
 
 
 # ----------------------------------------------------------------- attention --
