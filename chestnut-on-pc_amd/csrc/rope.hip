@@ -31,7 +31,9 @@ struct RopeParams {
 };
 
 // V: pairs per item.  8 where rows and strides are whole 16-byte chunks and rot a multiple of 16, else 1.
-template <typename T, int V>
+// NT: written past the caches, for an output that the L2s do not hold (8 x 4 MiB): 12288 tokens of
+// 20 heads of 128, 126 MB in all, 29.6 -> 23.7 us (loads past them too: 32.9).
+template <typename T, int V, bool NT>
 __global__ __launch_bounds__(256) void rope_kernel(const RopeParams p) {
   __shared__ float2_t cs[ROPE_LDS];
   const int t0 = blockIdx.x * p.tpw, nt = min(p.tpw, p.T - t0), half = p.rot >> 1;
@@ -47,6 +49,10 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeParams p) {
   const T* x = static_cast<const T*>(p.x);
   T* out = static_cast<T*>(p.out);
   typedef T vec __attribute__((ext_vector_type(V)));
+  auto put = [](T* to, vec v) {
+    if (NT) __builtin_nontemporal_store(v, reinterpret_cast<vec*>(to));
+    else *reinterpret_cast<vec*>(to) = v;
+  };
   for (unsigned i = threadIdx.x; i < nt * p.per_tok; i += 256) {
     const unsigned t = div_by(i, p.m_tok), r = i - t * p.per_tok, h = div_by(r, p.m_head);
     const int e = (int)(r - h * p.per_head) * V;   // first pair of the item; elements 2e.. behind rot
@@ -58,8 +64,9 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeParams p) {
         yr[2 * e] = xr[2 * e];
         if (2 * e + 1 < p.hd) yr[2 * e + 1] = xr[2 * e + 1];
       } else {
-        *reinterpret_cast<vec*>(yr + 2 * e) = *reinterpret_cast<const vec*>(xr + 2 * e);
-        *reinterpret_cast<vec*>(yr + 2 * e + V) = *reinterpret_cast<const vec*>(xr + 2 * e + V);
+        const vec v0 = *reinterpret_cast<const vec*>(xr + 2 * e), v1 = *reinterpret_cast<const vec*>(xr + 2 * e + V);
+        put(yr + 2 * e, v0);
+        put(yr + 2 * e + V, v1);
       }
       continue;
     }
@@ -86,8 +93,8 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeParams p) {
         y1[j] = (T)(a1 * u[0] + a0 * u[1]);
       }
     }
-    *reinterpret_cast<vec*>(yr + a) = y0;
-    *reinterpret_cast<vec*>(yr + b) = y1;
+    put(yr + a, y0);
+    put(yr + b, y1);
   }
 }
 
@@ -131,13 +138,10 @@ void launch_rope(const void* x, void* out, const int* positions, const double* i
   tpw = std::max(1, std::min(tpw, ROPE_LDS / (rot / 2)));
   p.tpw = tpw;
   const dim3 grid(ceil_div(T, tpw)), block(256);
-  if (dtype == DT_F16) {
-    if (wide) CK_LAUNCH((rope_kernel<half_t, 8>), grid, block, 0, s, p);
-    else CK_LAUNCH((rope_kernel<half_t, 1>), grid, block, 0, s, p);
-  } else {
-    if (wide) CK_LAUNCH((rope_kernel<bf16_t, 8>), grid, block, 0, s, p);
-    else CK_LAUNCH((rope_kernel<bf16_t, 1>), grid, block, 0, s, p);
-  }
+  const bool large = (long)T * H * hd * 2 > (32L << 20);
+  auto go = [&](auto kernel) { CK_LAUNCH(kernel, grid, block, 0, s, p); };
+  if (dtype == DT_F16) !wide ? go(rope_kernel<half_t, 1, false>) : large ? go(rope_kernel<half_t, 8, true>) : go(rope_kernel<half_t, 8, false>);
+  else !wide ? go(rope_kernel<bf16_t, 1, false>) : large ? go(rope_kernel<bf16_t, 8, true>) : go(rope_kernel<bf16_t, 8, false>);
   CK_LAUNCHED("rope");
 }
 
