@@ -303,10 +303,10 @@ def _rows(t, dtype, name, shape, unit=8, write=False):
         raise ValueError(f'{name} must be a torch tensor')
     if t.dtype is not dtype:
         raise ValueError(f'{name} must be {dtype}, got {t.dtype}')
-    if t.shape != shape:
-        raise ValueError(f'{name} must have shape {tuple(shape)}, got {tuple(t.shape)}')
-    s0, s1, s2 = t.stride()
     T, H, hd = shape
+    if t.shape != shape:
+        raise ValueError(f'{name} must have shape {(T, H, hd)}, got {tuple(t.shape)}')
+    s0, s1, s2 = t.stride()
     if s2 != 1 and hd > 1:
         raise ValueError(f'{name} must be contiguous in its last dimension')
     if T <= 1:
@@ -345,28 +345,47 @@ def _on_device(names, *tensors):
     return dev
 
 
-def _cache(k_pages, v_pages, k_scale, v_scale):
-    """The checks of a cache; its shape (n_pages, n_kv, page, head_dim)."""
+def _cache_each(k_pages, v_pages, k_scale, v_scale):
+    """The checks of _cache one by one, with the message of the first that fails."""
     if not isinstance(k_pages, torch.Tensor) or k_pages.dim() != 4:
         raise ValueError('k_pages must be [n_pages, n_kv, page, head_dim]')
     dtype = k_pages.dtype
     if dtype not in _DTYPE:
         raise ValueError(f'k_pages must be float16, bfloat16 or float8_e4m3fn, got {dtype}')
-    n, kv, page, hd = shape = k_pages.shape
+    n, kv, page, hd = k_pages.shape
     if page < 16 or page > 1024 or page & (page - 1):
         raise ValueError(f'the page size must be a power of two from 16 to 1024, got {page}')
     if n < 1 or kv < 1:
         raise ValueError('k_pages must hold a page and a head')
-    _is(k_pages, dtype, 'k_pages', shape)
-    _is(v_pages, dtype, 'v_pages', shape)
+    _check(k_pages, dtype, 'k_pages')
+    _check(v_pages, dtype, 'v_pages', (n, kv, page, hd))
     if dtype is _E4M3:
         if k_scale is None or v_scale is None:
             raise ValueError('an e4m3 cache needs k_scale and v_scale')
-        _is(k_scale, _E8M0, 'k_scale', shape[:3])
-        _is(v_scale, _E8M0, 'v_scale', shape[:3])
+        _check(k_scale, _E8M0, 'k_scale', (n, kv, page))
+        _check(v_scale, _E8M0, 'v_scale', (n, kv, page))
     elif k_scale is not None or v_scale is not None:
         raise ValueError('k_scale and v_scale belong to an e4m3 cache')
-    return shape
+
+
+def _cache(k_pages, v_pages, k_scale, v_scale):
+    """The checks of a cache; its shape (n_pages, n_kv, page, head_dim)."""
+    T = torch.Tensor
+    if type(k_pages) is T and type(v_pages) is T:
+        dtype, shape = k_pages.dtype, k_pages.shape
+        if len(shape) == 4 and v_pages.dtype is dtype and v_pages.shape == shape:
+            n, kv, page, _ = shape
+            if 16 <= page <= 1024 and not page & (page - 1) and n and kv and k_pages.is_contiguous() and \
+                    v_pages.is_contiguous():
+                if dtype is _E4M3:
+                    if type(k_scale) is T and type(v_scale) is T and k_scale.dtype is v_scale.dtype is _E8M0 and \
+                            k_scale.shape == v_scale.shape == shape[:3] and k_scale.is_contiguous() and \
+                            v_scale.is_contiguous():
+                        return shape
+                elif dtype in _DTYPE and k_scale is None and v_scale is None:
+                    return shape
+    _cache_each(k_pages, v_pages, k_scale, v_scale)
+    return k_pages.shape
 
 
 def rope_frequencies(rot, base=10000.0, method='none', factor=1.0, context=None, slow=1.0, fast=32.0, device='cuda'):

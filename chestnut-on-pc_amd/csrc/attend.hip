@@ -919,14 +919,34 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const AttendParams p) 
   float4_t a = {0.f, 0.f, 0.f, 0.f};
   if (in) {
     const long row = ((long)it.base * p.Hkv + hk) * BM + q;
-    for (int n = cg; n < it.nch; n += CG) {
-      const float2_t x = *part_ml<HD>(p, row + (long)n * p.Hkv * BM);
-      if (x[0] == -INFINITY) continue;   // saw no key, has no O
-      const float4_t y = *reinterpret_cast<const float4_t*>(part_o<HD>(p, row + (long)n * p.Hkv * BM) + c * 4);
-      const float m = fmaxf(M, x[0]), f = __builtin_amdgcn_exp2f(M - m), h = __builtin_amdgcn_exp2f(x[0] - m);
+    // four at a time, their loads together
+    constexpr int AT = 4;
+    for (int n0 = cg; n0 < it.nch; n0 += AT * CG) {
+      float2_t x[AT];
+      float4_t y[AT];
+#pragma unroll
+      for (int i = 0; i < AT; ++i) {
+        const long at = row + (long)min(n0 + i * CG, it.nch - 1) * p.Hkv * BM;
+        x[i] = *part_ml<HD>(p, at);
+        y[i] = *reinterpret_cast<const float4_t*>(part_o<HD>(p, at) + c * 4);
+      }
+      float m = M;
+#pragma unroll
+      for (int i = 0; i < AT; ++i) {
+        if (n0 + i * CG >= it.nch) x[i][0] = -INFINITY;
+        m = fmaxf(m, x[i][0]);
+      }
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - m);
       M = m;
-      sum = sum * f + x[1] * h;
-      a = a * f + y * h;
+      sum *= f;
+      a *= f;
+#pragma unroll
+      for (int i = 0; i < AT; ++i) {
+        if (x[i][0] == -INFINITY) continue;   // saw no key, has no O
+        const float h = __builtin_amdgcn_exp2f(x[i][0] - m);
+        sum += x[i][1] * h;
+        a += y[i] * h;
+      }
     }
   }
   if constexpr (CG > 1) {
