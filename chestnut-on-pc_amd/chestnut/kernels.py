@@ -286,7 +286,8 @@ def warp_nv12(frame, big_frame, tfm, big_tfm, cam_w, cam_h, stride, y_height, mo
 # ------------------------------------------------------------ the token cache --
 # K and V rows of past tokens in pages k_pages, v_pages [n_pages, n_kv, page, head_dim] (page a
 # power of two, 16 to 1024): f16, bf16, or float8_e4m3fn with k_scale, v_scale [n_pages, n_kv, page]
-# of float8_e8m0fnu, a power of two a row.  A slot is page index * page + place.
+# of float8_e8m0fnu, a power of two a row (cache_write leaves 2^-126 to 2^120; 2^-127 reads as 0).
+# A slot is page index * page + place.
 #
 # Index tensors are int32 on the device; their values are not checked here (that would wait for
 # the device).  Whatever they hold, nothing outside the tensors of a call is read or written.
@@ -315,8 +316,6 @@ def _rows(t, dtype, name, shape, unit=8, write=False):
         s1 = 0
     if (s0 | s1) % unit or t.data_ptr() % (2 * unit):
         raise ValueError(f'{name} must have rows that start at multiples of {2 * unit} bytes')
-    if s0 >= 1 << 24:
-        raise ValueError(f'{name} must have under 2^24 elements from one token to the next')
     if write and ((T > 1 and s0 < hd) or (H > 1 and s1 < hd)):
         raise ValueError(f'{name} must not overlap itself')
     return s0, s1
@@ -545,6 +544,8 @@ def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None
     T, H, B, (qt, qh), (ot, oh), scale = _queries(q, cu_q, kv, hd, out, scale)
     kt, kh = _rows(k, q.dtype, 'k', k.shape)
     vt, vh = _rows(v, q.dtype, 'v', k.shape)
+    if kt >= 1 << 24 or vt >= 1 << 24:
+        raise ValueError('k and v must have under 2^24 elements from one token to the next')
     if cu_k is None:
         if Tk != T:
             raise ValueError(f'k must have the {T} rows of q where cu_k is not given, got {Tk}')
@@ -577,6 +578,8 @@ def attention_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, k_scale=Non
     if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
         raise ValueError('block_table must be int32 [B, width]')
     width = block_table.shape[1]
+    if width * page > 1 << 30:
+        raise ValueError('block_table must name at most 2^30 places of a sequence')
     _is(block_table, torch.int32, 'block_table', (B, width))
     dev = _on_device('q k_pages v_pages block_table cu_q kv_lens k_scale v_scale out', q, k_pages, v_pages, block_table,
                      cu_q, kv_lens, k_scale, v_scale, out)

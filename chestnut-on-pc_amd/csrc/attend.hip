@@ -1078,7 +1078,7 @@ size_t attention_workspace(int B, int Tq, long keys, int n_heads, int n_kv, int 
 void launch_attention_varlen(const AttendQuery& a, const void* k, const void* v, long kst, long ksh, long vst, long vsh,
                              const int* cu_k, int Tk, int n_kv, hipStream_t s) {
   AttendParams p{};
-  CK_REQUIRE(Tk >= 0 && n_kv > 0, "attention_varlen: bad sizes");
+  CK_REQUIRE(Tk >= 0 && Tk <= (1 << 30) && n_kv > 0, "attention_varlen: bad sizes");
   CK_REQUIRE(a.T == 0 || Tk == 0 || (k && v), "attention_varlen: null pointer");
   CK_REQUIRE(((kst | ksh | vst | vsh) & 7) == 0 && ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0,
              "attention_varlen: k and v rows must be 16-byte aligned");
@@ -1100,6 +1100,7 @@ void launch_attention_paged(const AttendQuery& a, const PagedCache& c, const int
   CK_REQUIRE(c.dtype == a.dtype || c.dtype == DT_E4M3, "attention_paged: the cache must be of q's type or e4m3");
   CK_REQUIRE(c.head_dim == a.head_dim, "attention_paged: the cache's head_dim must be q's");
   CK_REQUIRE(table_w >= 0 && (table || !table_w || !a.B || !a.T), "attention_paged: null block table");
+  CK_REQUIRE((long)table_w * c.page <= (1L << 30), "attention_paged: at most 2^30 places a sequence");
   AttendParams p{};
   p.k = c.k;
   p.v = c.v;

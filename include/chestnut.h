@@ -327,8 +327,8 @@ int ck_rope(const void* x, void* out, const int32_t* positions, const double* in
 /* A cache: k_pages, v_pages [n_pages][n_kv][page][head_dim], 16-byte
  * aligned; page a power of two from 16 to 1024, head_dim a multiple of 8 up
  * to 256, n_pages * page < 2^31.  cache_dtype e4m3: k_scale, v_scale
- * [n_pages][n_kv][page] hold each row's scale 2^(byte - 127); a value is
- * code * scale.  Other cache types: the scales are NULL.
+ * [n_pages][n_kv][page] hold each row's scale 2^(byte - 127), byte 1 to 254;
+ * a value is code * scale.  Other cache types: the scales are NULL.
  *
  * ck_cache_write: row t of k and v to slot slots[t] = page index * page +
  * place; negative slots are not written, slots must differ.  e4m3: the scale
@@ -358,16 +358,16 @@ int ck_attention_workspace(int B, int Tq, long keys, int n_heads, int n_kv, int 
  * query that sees none gets zeros; what a query does not see (infinities and
  * NaN included) does not reach it.  Query head h reads K/V head
  * h / (n_heads / n_kv).  head_dim 64 or 128, scale > 0, f16 or bf16;
- * q, k, v rows 16-byte aligned, out rows 8-byte aligned. */
+ * q, k, v rows 16-byte aligned, out rows 8-byte aligned; k_st, v_st < 2^24,
+ * at most 2^30 keys.  The workspace belongs to the call until it has run:
+ * calls that may overlap, and graphs that may, need one each. */
 int ck_attention_varlen(const void* q, const void* k, const void* v, void* out, const int32_t* cu_q,
                         const int32_t* cu_k, int B, int Tq, int Tk, int n_heads, int n_kv, int head_dim, long q_st,
                         long q_sh, long k_st, long k_sh, long v_st, long v_sh, long o_st, long o_sh, int dtype,
                         int causal, float scale, void* workspace, size_t ws_bytes, void* stream);
 
 /* The same over a paged cache: sequence b has kv_lens[b] keys, at places
- * 0 .. of its pages block_table[b][..]; its queries are the last of them.
- * The workspace belongs to this call until it has run: calls that may
- * overlap, and graphs that may, need one each. */
+ * 0 .. of its pages block_table[b][..]; its queries are the last of them. */
 int ck_attention_paged(const void* q, const void* k_pages, const void* v_pages, const void* k_scale,
                        const void* v_scale, void* out, const int32_t* block_table, int table_width,
                        const int32_t* cu_q, const int32_t* kv_lens, int B, int Tq, int n_heads, int n_pages, int n_kv,

@@ -326,6 +326,26 @@ def test_what_a_row_does_not_see_does_not_reach_it(gpu, dt, hd, paged, n, m):
 
 
 @pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('n,m', [(200, 200), (40, 1170), (3, 64)])
+def test_nan_codes_that_a_row_does_not_see_do_not_reach_it(gpu, dt, n, m):
+    from chestnut import kernels as K
+    H, kv, hd, page = 4, 2, 128, 32
+    table, total = tables([m], page, 3)
+    kp, vp, ks, vs = filled(total, kv, page, hd, dt, 'e4m3', 4)
+    k, v = gathered(kp, ks, table[0], m, page), gathered(vp, vs, table[0], m, page)
+    first, bad = m - n, m - n // 2          # the first query's own place, and of the first NaN
+    for j in list(range(bad, m)) + list(range(m, -(-m // page) * page)):
+        vp.view(torch.uint8)[table[0][j // page], :, j % page, j % hd] = 0x7F
+        kp.view(torch.uint8)[table[0][j // page], :, j % page, 5] = 0xFF
+    q = rows(1, n, H, hd, dt)
+    out = K.attention_paged(q, kp, vp, i32(table), cu([n]), i32([m]), k_scale=ks, v_scale=vs)
+    clean = bad - first
+    ref, mag, most = O.attention(f64(q[:clean]), k[:bad], v[:bad])
+    near(out[:clean], ref, mag, most, m, hd, dt)
+    assert not torch.isfinite(out[clean:]).all(-1).any()
+
+
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
 def test_infinite_values_of_v_reach_the_rows_that_see_them(gpu, dt):
     from chestnut import kernels as K
     n, hd = 150, 64
@@ -470,6 +490,51 @@ def test_a_captured_step_replays(gpu):
         torch.cuda.synchronize()
         assert torch.equal(out, want), n
         assert torch.equal(kp.view(torch.uint8), other[0].view(torch.uint8))
+
+
+def test_two_streams_at_once(gpu):
+    """Split calls on two streams, each with its own workspace, and a workspace that the caller keeps."""
+    from chestnut import kernels as K
+    H, kv, hd, page = 8, 2, 128, 32
+    sets = []
+    for i in range(2):
+        table, n = tables([3000, 900], page, i)
+        c = filled(n, kv, page, hd, 'f16', 'e4m3', i)
+        sets.append((rows(i, 60, H, hd, 'f16'), c, i32(table), cu([1, 59]), i32([3000, 900])))
+    run = lambda s, ws=None: K.attention_paged(s[0], s[1][0], s[1][1], s[2], s[3], s[4], k_scale=s[1][2], v_scale=s[1][3], workspace=ws)
+    want = [run(s) for s in sets]
+    kept = [torch.full((1 << 22,), float('nan'), device='cuda') for _ in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(run(sets[i], kept[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+def test_long_cache_offsets_pass_32_bits(gpu):
+    """A cache of over 2^32 elements: a sequence on its last pages, written, read back and attended."""
+    from chestnut import kernels as K
+    kv, hd, page, n = 8, 128, 1024, 4200                 # 4.4e9 elements of one byte, K and V
+    kp, vp = (torch.zeros(n, kv, page, hd, dtype=torch.uint8, device='cuda').view(torch.float8_e4m3fn) for _ in 'kv')
+    ks, vs = (torch.full((n, kv, page), 127, dtype=torch.uint8, device='cuda').view(torch.float8_e8m0fnu) for _ in 'kv')
+    m = 1500
+    table = np.array([[n - 1, n - 3]])
+    k, v, q = rows(1, m, kv, hd, 'f16'), rows(2, m, kv, hd, 'f16'), rows(3, 70, kv, hd, 'f16')
+    place = np.arange(m)
+    K.cache_write(k, v, kp, vp, i32(table[0][place // page] * page + place % page), k_scale=ks, v_scale=vs)
+    gk, gv = K.cache_read(kp, vp, i32(table), cu([m]), m, k_scale=ks, v_scale=vs, dtype=torch.float16)
+    for x, g in ((k, gk), (v, gv)):
+        assert np.array_equal(f64(g), O.values(*O.quantise(f64(x), TOP['f16'])))
+    for rows_of in (q, q[:1]):                           # many rows, few rows
+        x = rows_of.shape[0]
+        out = K.attention_paged(rows_of, kp, vp, i32(table), cu([x]), i32([m]), k_scale=ks, v_scale=vs)
+        ref, mag, most = O.attention(f64(rows_of), f64(gk), f64(gv))
+        near(out, ref, mag, most, m, hd, 'f16')
 
 
 def test_on_another_stream(gpu):

@@ -94,6 +94,7 @@ REFUSED = [
     ('paged table strided', lambda: paged(table=z(2, 6, dtype=i32)[:, ::2]), 'block_table must be contiguous'),
     ('varlen token stride', lambda: varlen(k=torch.empty_strided((4, 2, 64), (1 << 24, 64, 1), dtype=f16, device='meta')),
      'under 2\\^24 elements'),
+    ('paged table width', lambda: paged(table=torch.empty(2, (1 << 26) + 1, dtype=i32, device='meta')), 'at most 2\\^30 places'),
     ('paged table rank', lambda: paged(table=z(6, dtype=i32)), 'block_table must be int32'),
     ('paged cpu tensors', paged, 'must be a CUDA tensor'),
     ('varlen cpu tensors', varlen, 'must be a CUDA tensor'),
@@ -137,6 +138,7 @@ NATIVE = [
     ('paged scale', attn(scale=-1.0), 'positive and finite'),
     ('paged null', attn(q=None), 'null pointer'),
     ('paged stride', attn(st=250), 'aligned'),
+    ('paged width', attn(width=(1 << 26) + 1), 'at most 2\\^30 places'),
 ]
 
 
