@@ -129,14 +129,16 @@ __device__ __forceinline__ bool find_item(const AttendParams& p, int index, Item
     if (work < 16777216.f) {   // a whole number
       const int w = (int)work;
       c = max(p.min_blocks, (w + full - 1) / full);
-      if (p.B <= 4) {
-        // few sequences: lane i counts the items that chunks of c0 + i blocks make, and the
-        // shortest chunk that does not make too many is taken
+      if (p.B <= 16) {
+        // few sequences: lane i counts the items that chunks of c0 + i blocks make, and the shortest
+        // chunk that does not make too many is taken (eight chunks and tokens, 80 -> 76 us)
         const int c0 = max(p.min_blocks, (w + p.target - 1) / p.target), ci = c0 + lane;
+        const float inv = __builtin_amdgcn_rcpf((float)ci);
         int items = 0;
         for (int b = 0; b < p.B; ++b) {
           const int nb = __builtin_amdgcn_readlane(blocks, b), nt = __builtin_amdgcn_readlane(tiles, b);
-          items += nt * max(1, (nb + ci - 1) / ci);
+          const int q = (int)((float)nb * inv + 0.5f);   // nb / ci to the nearest: the ceiling is it or the next
+          items += nt * max(1, q + (q * ci < nb ? 1 : 0));
         }
         const unsigned long long fits = __ballot(items <= p.target);
         if (fits) c = min(c, c0 + __ffsll(fits) - 1);
