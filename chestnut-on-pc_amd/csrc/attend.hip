@@ -691,14 +691,16 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
     ks.begin(p, it, hk, kbeg, AT_KEYS, lane, wave, DMA);
     vs.begin(p, it, hk, kbeg, AT_KEYS, lane, wave, DMA);
     r.begin(p, it, hk, tile * BM + wave * 32 + (lane & 31), lane);
-    r.arrived();   // before the loads to LDS, so that no later wait counts Q's loads
     send(ks, kbeg, kt(0));
-    if constexpr (!DMA) ks.store(kt(0), tid);
     send(vs, kbeg, vt(0));
-    if constexpr (!DMA) vs.store(vt(0), tid);
+    if constexpr (!DMA) ks.store(kt(0), tid);
     send(ks, kbeg + AT_KEYS, kt(1));
-    if constexpr (!DMA) ks.store(kt(1), tid);
+    if constexpr (!DMA) {
+      vs.store(vt(0), tid);
+      ks.store(kt(1), tid);
+    }
     landed();
+    r.arrived();   // so that no wait in the loop counts Q's loads
     r.template scores<2>(sa, kt(0), lane);
   } else {
     r.begin(p, it, hk, tile * BM + wave * 32 + (lane & 31), lane);
