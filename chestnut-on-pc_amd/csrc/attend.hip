@@ -447,8 +447,8 @@ struct Rows {
     }
   }
   // the weights, rounded, as the product takes them; the sum is that of the rounded ones, so
-  // their rounding cancels where few keys rule
-  __device__ __forceinline__ float origin(float c) const { return m == -INFINITY ? 0.f : m * c; }
+  // their rounding cancels where few keys rule.  All are 2^LIFT times what they would be from m.
+  __device__ __forceinline__ float origin(float c) const { return m == -INFINITY ? 0.f : __builtin_fmaf(m, c, -Elem<T>::LIFT); }
   template <int NB>
   __device__ __forceinline__ void weigh(v8 (&pf)[2 * NB], const float16_t (&s)[NB], int pair, float c, float mc) {
     const int kb = pair >> 3, i = (pair & 7) * 2;
@@ -913,7 +913,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const AttendParams p) 
   const int hk = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv;
   Item it;
   // (offsets that do not ascend may name more rows than there are: what has no item has no sums)
-  if (!find_item<KV, BM, true>(p, index, it) || it.nch == 1 || it.base + it.nch > p.items) return;
+  if (!find_item<KV, BM, true>(p, index, it) || it.nch == 1 || it.base < 0 || it.base + it.nch > p.items) return;
   const int c = threadIdx.x % LPR, cg = CG > 1 ? threadIdx.x / LPR : 0;
   const int q = blockIdx.y * RP + (CG > 1 ? 0 : threadIdx.x / LPR);
   const int tile = BM == 32 ? it.tile : tiles_of<KV, BM>(it.s, p.G) - 1 - it.tile;
@@ -1048,7 +1048,8 @@ void launch_attend(const char* what, AttendParams& p, const AttendQuery& a, int 
   p.causal = a.causal;
   p.scale_log2e = a.scale * AT_LOG2E;
   const Plan pl = plan_of(a.B, a.T, keys, a.n_heads, p.Hkv);
-  CK_REQUIRE(pl.items * p.Hkv < (1L << 31), w + ": too many rows");
+  // (a launch has under 2^32 threads)
+  CK_REQUIRE(pl.items * p.Hkv < (1L << 32) / std::max(256, 2 * pl.bm), w + ": too many sequences and rows for one launch");
   if (pl.target) {
     const size_t need = attention_workspace(a.B, a.T, keys, a.n_heads, p.Hkv, a.head_dim);
     CK_REQUIRE(a.ws && a.ws_floats >= need, w + ": workspace too small (ck_attention_workspace)");

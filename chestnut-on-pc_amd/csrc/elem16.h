@@ -28,6 +28,9 @@ struct Elem<half_t> {
   // exponent field of two packed values, and its lowest bit: (u & EXP) + LOW has a
   // half's top bit set where that half is an infinity or a NaN
   static constexpr unsigned EXP = 0x7C007C00u, LOW = 0x04000400u;
+  // softmax weights, up to 2^8 before this, are kept 2^LIFT times as large: the type's top is not
+  // far, its bottom is (many keys at 2^-25 of the strongest one's weight still count)
+  static constexpr float LIFT = 7.0f;
   static __device__ __forceinline__ float16_t mfma32(v8 a, v8 b, float16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -42,6 +45,7 @@ struct Elem<bf16_t> {
   typedef bf16x8_t v8;
   static constexpr float top = 3.19014718988379809496913694467282698e38f;   // 1.875 * 2^127
   static constexpr unsigned EXP = 0x7F807F80u, LOW = 0x00800080u;
+  static constexpr float LIFT = 0.0f;
   static __device__ __forceinline__ float16_t mfma32(v8 a, v8 b, float16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }

@@ -138,6 +138,7 @@ void launch_rope(const void* x, void* out, const int* positions, const double* i
   tpw = std::max(1, std::min(tpw, ROPE_LDS / (rot / 2)));
   p.tpw = tpw;
   const dim3 grid(ceil_div(T, tpw)), block(256);
+  CK_REQUIRE(grid.x < (1u << 24), "rope: too many tokens for one launch");   // of under 2^32 threads
   const bool large = (long)T * H * hd * 2 > (32L << 20);
   auto go = [&](auto kernel) { CK_LAUNCH(kernel, grid, block, 0, s, p); };
   if (dtype == DT_F16) !wide ? go(rope_kernel<half_t, 1, false>) : large ? go(rope_kernel<half_t, 8, true>) : go(rope_kernel<half_t, 8, false>);

@@ -219,7 +219,8 @@ void launch_cache_write(const void* k, const void* v, const PagedCache& c, const
   CK_REQUIRE(dtype == DT_F16 || dtype == DT_BF16, "cache_write: rows must be f16 or bf16");
   check_pages("cache_write", c);
   CK_REQUIRE(c.dtype == dtype || c.dtype == DT_E4M3, "cache_write: the cache must be of the rows' type or e4m3");
-  CK_REQUIRE(T >= 0 && (long)T * c.n_kv < (1L << 31), "cache_write: under 2^31 rows");
+  // (a launch has under 2^32 threads, of which a row takes up to 32)
+  CK_REQUIRE(T >= 0 && (long)T * c.n_kv < (1L << 27), "cache_write: under 2^27 rows");
   if (T == 0) return;
   CK_REQUIRE(k && v && slots, "cache_write: null pointer");
   CK_REQUIRE(((kst | ksh | vst | vsh) & 7) == 0 && ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0,
@@ -257,7 +258,8 @@ void launch_cache_read(const PagedCache& c, const int* table, int table_w, const
   CK_REQUIRE(dtype == DT_F16 || dtype == DT_BF16, "cache_read: rows must be f16 or bf16");
   check_pages("cache_read", c);
   CK_REQUIRE(c.dtype == dtype || c.dtype == DT_E4M3, "cache_read: the cache must be of the rows' type or e4m3");
-  CK_REQUIRE(tokens >= 0 && B >= 0 && table_w >= 0 && (long)tokens * c.n_kv < (1L << 31), "cache_read: bad sizes");
+  CK_REQUIRE(tokens >= 0 && B >= 0 && table_w >= 0 && tokens < (1 << 28) && (long)tokens * c.n_kv < (1L << 31),
+             "cache_read: under 2^28 tokens and 2^31 rows");
   if (tokens == 0 || B == 0 || table_w == 0) return;
   CK_REQUIRE(table && cu && k && v, "cache_read: null pointer");
   CK_REQUIRE(((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0, "cache_read: rows must be 16-byte aligned");

@@ -319,7 +319,8 @@ int ck_layernorm(const float* x, const float* g, const float* b, void* out, int 
  * one turn): y0 = scale (x0 cos a - x1 sin a), y1 = scale (x1 cos a +
  * x0 sin a) for the pairs (i, i + rot/2), or (2i, 2i+1) where interleaved;
  * inverse: by -a.  Elements behind rot are copied.  out may be x (same
- * strides) but not overlap it otherwise.  rot even, <= head_dim <= 512. */
+ * strides) but not overlap it otherwise.  rot even, <= head_dim <= 512;
+ * n_heads <= 1024, n_heads * head_dim <= 65536. */
 int ck_rope(const void* x, void* out, const int32_t* positions, const double* inv_freq, int T, int n_heads,
             int head_dim, int rot, long x_st, long x_sh, long o_st, long o_sh, int dtype, int interleaved, float scale,
             int inverse, void* stream);
@@ -335,14 +336,15 @@ int ck_rope(const void* x, void* out, const int32_t* positions, const double* in
  * is the least power of two with max |row| <= 448 scale, codes are rounded to
  * nearest even; infinities and values above 61440 (f16) are held as the
  * largest that reads back finite, NaN stays NaN.
- * Rows 16-byte aligned (strides multiples of 8). */
+ * Rows 16-byte aligned (strides multiples of 8), T * n_kv < 2^27. */
 int ck_cache_write(const void* k, const void* v, void* k_pages, void* v_pages, void* k_scale, void* v_scale,
                    const int32_t* slots, int T, int n_pages, int n_kv, int page, int head_dim, long k_st, long k_sh,
                    long v_st, long v_sh, int dtype, int cache_dtype, void* stream);
 
 /* The first cu[b+1] - cu[b] places of each sequence (pages block_table[b][..],
  * int32 [B][table_width]) to rows cu[b].. of k and v [tokens][n_kv][head_dim]
- * (contiguous, dtype f16 or bf16; the cache's own type unless that is e4m3). */
+ * (contiguous, dtype f16 or bf16; the cache's own type unless that is e4m3),
+ * tokens < 2^28. */
 int ck_cache_read(const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale,
                   const int32_t* block_table, int table_width, const int32_t* cu_seqlens, int B, int tokens,
                   int n_pages, int n_kv, int page, int head_dim, void* k, void* v, int dtype, int cache_dtype,
@@ -359,7 +361,8 @@ int ck_attention_workspace(int B, int Tq, long keys, int n_heads, int n_kv, int 
  * NaN included) does not reach it.  Query head h reads K/V head
  * h / (n_heads / n_kv).  head_dim 64 or 128, scale > 0, f16 or bf16;
  * q, k, v rows 16-byte aligned, out rows 8-byte aligned; k_st, v_st < 2^24,
- * at most 2^30 keys.  The workspace belongs to the call until it has run:
+ * at most 2^30 keys a sequence, B < 2^20, Tq * n_heads < 2^31 and fewer than
+ * 2^24 workgroups (B * n_kv at least).  The workspace belongs to the call until it has run:
  * calls that may overlap, and graphs that may, need one each. */
 int ck_attention_varlen(const void* q, const void* k, const void* v, void* out, const int32_t* cu_q,
                         const int32_t* cu_k, int B, int Tq, int Tk, int n_heads, int n_kv, int head_dim, long q_st,

@@ -6,9 +6,9 @@ rope: angles are exact to 2^-45 turns, cos and sin to 2^-22 each; two products a
 in f32, one rounding to the type.
 cache: bit-exact codes and scales; a value read back is one rounding of code * scale.
 attention: the output is rounded once (u |o|) and each softmax weight once (u a weight, so
-u times A = the same sum with |v|); f16 weights below the smallest normal round to its
-subnormals (2^-25 each, n of them at most, each times |v| < 6, against a row sum of at least
-1); a score is a chain of hd f32 sums ((hd + 4) 2^-24 of its sum
+u times A = the same sum with |v|); f16 weights are kept 2^7 times as large, and those below the
+smallest normal round to its subnormals (2^-32 of the strongest each, n of them at most, each
+times |v| < 6, against a row sum of at least 1); a score is a chain of hd f32 sums ((hd + 4) 2^-24 of its sum
 of magnitudes, twice: numerator and denominator); exp2, the rescalings and the sums add
 less than 2^-17."""
 import numpy as np
@@ -46,7 +46,7 @@ def cu(lens):
 
 def near(out, ref, mag, most, n, hd, dt, what=''):
     out = f64(out)
-    tiny = 6 * n * 2.0 ** -25 if dt == 'f16' else 0.0
+    tiny = 6 * n * 2.0 ** -32 if dt == 'f16' else 0.0
     tol = u(dt) * (np.abs(ref) + mag) * (1 + 2.0 ** -6) + (2 * (hd + 4) * 2.0 ** -24 * most + 2.0 ** -17) * mag + tiny
     bad = ~(np.abs(out - ref) <= tol)
     assert not bad.any(), f'{what}: {bad.sum()} of {bad.size}, worst {np.nanmax(np.abs(out - ref) - tol)}, first {np.argwhere(bad)[0]}'
@@ -370,6 +370,27 @@ def test_one_key_rules_each_row(gpu, hd):
     v = rows(2, n, 1, hd, 'f16')
     out = K.attention_varlen(q, k, v, cu([n]), scale=1.0)
     assert torch.equal(out[:, 0].cpu(), v[:, 0].cpu()[torch.from_numpy(at)])
+
+
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('T', [1, 300])
+@pytest.mark.parametrize('last', [False, True])
+def test_many_weak_keys_beside_a_strong_one(gpu, dt, T, last):
+    """One key of score 17 and v = 0 beside 60000 of score 0 and v = 1: each of those weighs 2^-24.5
+    of it, less than f16 can tell from 1 or 0.  Output 60000 e^-17 / (1 + 60000 e^-17): u of a
+    weight and of the output, f16's subnormals 2^-32 each, and 2^-17 for the exponentials and sums."""
+    from chestnut import kernels as K
+    n = 60001
+    q, k, v = (torch.zeros(m, 1, 64, dtype=DT[dt], device='cuda') for m in (T, n, n))
+    q[..., 0] = 8.0
+    k[n - 1 if last else 0, 0, 0] = 17.0
+    v[...] = 1.0
+    v[n - 1 if last else 0] = 0.0
+    out = f64(K.attention_varlen(q, k, v, cu([T]), cu([n]), causal=False, scale=0.125))
+    w = (n - 1) * np.exp(-17.0)
+    ref = w / (1 + w)
+    tol = ref * (2 * u(dt) * (1 + 2.0 ** -6) + 2.0 ** -17) + ((n - 1) * 2.0 ** -32 if dt == 'f16' else 0.0)
+    assert np.abs(out - ref).max() <= tol
 
 
 def test_index_values_outside_the_tensors_stay_inside(gpu):

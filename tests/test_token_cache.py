@@ -114,8 +114,8 @@ def test_refused_with_value_error(name, fn, msg):
 X = ctypes.c_void_p(1 << 20)      # an aligned address that nothing reads
 
 
-def attn(T=4, H=4, n=3, kv=2, page=16, hd=64, dtype=1, cdtype=1, scale=0.1, q=X, ks=None, width=3, st=256):
-    return ('ck_attention_paged', q, X, X, ks, ks, X, X, width, X, X, 2, T, H, n, kv, page, hd, st, hd, st, hd, dtype, cdtype, 1,
+def attn(T=4, H=4, n=3, kv=2, page=16, hd=64, dtype=1, cdtype=1, scale=0.1, q=X, ks=None, width=3, st=256, B=2):
+    return ('ck_attention_paged', q, X, X, ks, ks, X, X, width, X, X, B, T, H, n, kv, page, hd, st, hd, st, hd, dtype, cdtype, 1,
             scale, None, 0, None)
 
 
@@ -138,6 +138,11 @@ NATIVE = [
     ('paged scale', attn(scale=-1.0), 'positive and finite'),
     ('paged null', attn(q=None), 'null pointer'),
     ('paged stride', attn(st=250), 'aligned'),
+    # a launch has under 2^32 threads
+    ('rope tokens', ('ck_rope', X, X, X, X, 1 << 28, 1, 512, 510, 513, 512, 513, 512, 1, 0, 1.0, 0, None), 'too many tokens'),
+    ('write rows', ('ck_cache_write', X, X, X, X, None, None, X, 1 << 26, 3, 2, 16, 64, 0, 64, 0, 64, 1, 1, None), '2\\^27 rows'),
+    ('read tokens', ('ck_cache_read', X, X, None, None, X, 3, X, 2, 1 << 28, 3, 1, 16, 8, X, X, 1, 1, None), '2\\^28 tokens'),
+    ('paged sequences', attn(T=1 << 19, B=1 << 19, H=32, kv=32), 'too many sequences'),
     ('paged width', attn(width=(1 << 26) + 1), 'at most 2\\^30 places'),
 ]
 
