@@ -7,13 +7,20 @@
 //
 // Rows.  The queries of the G heads that share a K/V head are the rows of one product:
 // row r of a sequence is query r / G of head g = r % G, so that K and V pass once for all
-// of them.  A wave owns 32 rows, a workgroup 128, over tiles of 64 keys in LDS:
+// of them.  A wave owns 32 rows:
 //   S^T = K Q^T (v_mfma 32x32x16, A = 32 keys, B = 32 rows): lane l holds row l % 32 and
 //     the keys 8 (i / 4) + 4 (l / 32) + i % 4, i < 16, of a block of 32;
 //   the softmax needs the other half of the wave for its maximum and sum only;
 //   O^T = V^T P^T: the lane's own exponentials, rounded to the element type, are the B operand
 //     as they stand; V^T's operand takes its keys in the same order through transposed LDS reads.
-// The running maximum and sum and O are f32.
+// The running maximum and sum and O are f32; the weights and the output are rounded to the
+// element type, the weights because the matrix product takes them so.
+//
+// Three kernels (their figures stand at each):
+//   attend_tile_kernel  128 or 256 rows, tiles of 64 keys in LDS: prompts and chunks of one;
+//                       bound by the matrix cores beside the vector unit's exponentials;
+//   attend_few_kernel   32 rows, the keys over four waves: tokens one by one; bound by memory;
+//   attend_join_kernel  joins the parts of rows whose keys were split over workgroups.
 #include <algorithm>
 #include <type_traits>
 
@@ -69,6 +76,10 @@ __device__ __forceinline__ Seq sequence(const AttendParams& p, int b) {
 // about `target` items of equal length per K/V head fill the card whatever the lengths are:
 // every workgroup adds up the lengths (64 sequences a step) and finds its own item.  The
 // items of a tile with one chunk write the output, the others partial sums, item by item.
+// The lengths are the device's, so a captured call follows them, and no launch, counter or
+// copy to the host stands before the first load.  Dividing all blocks of keys exactly, with
+// several pieces a workgroup, measured no faster for single tokens and 80 -> 115 us for mixed
+// chunks (the loop over pieces costs the tile loop its registers).
 struct Item {
   int b, tile, chunk, nch, c, base;   // base: the tile's first item
   Seq s;
@@ -648,6 +659,15 @@ __device__ __forceinline__ float2_t* part_ml(const AttendParams& p, long row) {
 // K is therefore one tile ahead of V.  Both have two buffers in LDS; step j sends for V(j+1)
 // and K(j+2) (f16, bf16: straight to LDS; e4m3: through registers, where it is turned into
 // values).
+// 256 rows (two waves a SIMD, one workgroup a CU): prompts of 9001, 5120 and 2263 tokens, 16
+// heads on 4 of 128, bf16, 441 us = 1.04 PFLOP/s, where a product of 8192^3 reaches 1.55; 128
+// rows 508.  Without its loads it takes 392 (less than 471 at the time), without barrier and LDS
+// reads too 369, without the softmax as well 316 = the matrix cores at the clock their power
+// leaves: what bounds it is those two side by side.  Slower were the compiler's own order (sched
+// groups 517-535 against 508), rings of four tiles (467 against 455) and f16 tiles by way of
+// registers (466).  128 rows with the keys split: 512 tokens on 12800 keys, 16 heads of 128,
+// f16, 71 us and 8 to join them, 690 TFLOP/s in all; from an e4m3 cache, eight sequences of 1 to
+// 511 tokens, 75 us = 545.  Short prompts (40 of 1 to 239 tokens, 8 heads of 64) 12.3 us.
 template <typename T, int HD, int KV, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendParams p) {
   constexpr int BM = 32 * NW, TILE = AT_KEYS * HD, NT = 64 * NW;
@@ -796,7 +816,11 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
 
 // ---- few rows: 32 of them, the keys over the waves ----------------------------------------
 // Every wave streams its own blocks of 32 keys (w, w + 4, ...) through LDS of its own; nothing
-// waits for another wave until the end, where the waves' sums are joined.
+// waits for another wave until the end, where the waves' sums are joined.  Bound by memory: the
+// rows come past the caches, K and V of the next step under way during this one's products (two
+// steps ahead: spills, 151 us against 124).  32 tokens on 1025 to 32701 keys, 16 heads on 4 of
+// 128, e4m3: 117 us = 5.5 TB/s, where plain reads of this kind reach 7.1 and the card's copy 4.9;
+// one token on 6144 keys, 8 heads of 64, f16: 6.6 us.
 constexpr int FEW_WAVES = 4;
 
 template <typename T, int HD, int KV>
@@ -904,7 +928,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attend_few_kernel(const Att
 }
 
 // ---- the chunks of a tile joined ----------------------------------------------------------
-// HD / 4 lanes a row, RP rows and CG groups of chunks a workgroup of 256.
+// HD / 4 lanes a row, RP rows and CG groups of chunks a workgroup of 256.  Its work is small (4
+// to 11 us); a launch of its own, as the last workgroup of a tile doing it needs counters that
+// are zero at the start and stay so where a call is cut short or two replays overlap.
 template <typename T, int HD, int KV, int BM>
 __global__ __launch_bounds__(256) void attend_join_kernel(const AttendParams p) {
   constexpr int LPR = HD / 4, CG = BM == 32 ? 256 / LPR : 1, RP = 256 / LPR / CG;
@@ -989,12 +1015,18 @@ Plan plan_of(int B, int Tq, long keys, int n_heads, int n_kv) {
   Plan pl{};
   const int G = n_heads / n_kv;
   const long rows = (long)Tq * G;
+  // 32 rows where a sequence has that many on average: bound by the keys, not by the rows.
+  // 256 rows where they fill the 256 CUs at least twice without splitting keys (prompt of 16384
+  // tokens, 441 us against 508 with 128); with fewer, tiles of 256 with their keys split take
+  // 80 us against 82 (512 tokens on 12800 keys) and 81 against 77 (eight mixed chunks).
   pl.bm = rows <= 32L * B ? 32 : (rows / 256 + B) * n_kv >= 512 ? 256 : 128;
   pl.tiles = rows / pl.bm + B;       // sum of ceil(rows_b / bm) is at most this
-  // items to aim at: workgroups that run at once, one a CU or two; of few rows twice as many, as
-  // their chunks come out uneven (32 ragged histories 127 -> 122 us; three times as many 125)
+  // items to aim at: workgroups that run at once, one a CU or two (tiles of 128, three, four, six
+  // a CU in place of two: 512 tokens on 12800 keys 99, 104, 119 for 86 us); of few rows twice as
+  // many, as their chunks come out uneven (32 ragged histories 127 -> 122 us; three times 125)
   const long slots = pl.bm == 256 ? 256 : pl.bm == 128 ? 512 : 1024;
   pl.min_blocks = pl.bm == 32 ? 2 : 4;
+  // keys stay whole where the tiles fill the card twice, or there are too few keys to gain from it
   const bool many = pl.bm != 32 && pl.tiles * n_kv >= 2 * slots;
   if (!many && keys / B > 2 * pl.min_blocks * AT_KEYS) pl.target = (int)std::max(1L, slots / n_kv);
   pl.items = pl.tiles + pl.target;

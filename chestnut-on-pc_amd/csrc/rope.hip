@@ -32,7 +32,8 @@ struct RopeParams {
 
 // V: pairs per item.  8 where rows and strides are whole 16-byte chunks and rot a multiple of 16, else 1.
 // NT: written past the caches, for an output that the L2s do not hold (8 x 4 MiB): 12288 tokens of
-// 20 heads of 128, 126 MB in all, 29.6 -> 23.7 us (loads past them too: 32.9).
+// 20 heads of 128, 126 MB in all, 29.6 -> 23.3 us = 5.4 TB/s (loads past
+// them too: 32.9).  4 tokens of 8 heads of 64: 2.4 us, a launch.
 template <typename T, int V, bool NT>
 __global__ __launch_bounds__(256) void rope_kernel(const RopeParams p) {
   __shared__ float2_t cs[ROPE_LDS];
