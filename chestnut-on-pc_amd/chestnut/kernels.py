@@ -316,7 +316,9 @@ def _rows(t, dtype, name, shape, unit=8, write=False):
         s1 = 0
     if (s0 | s1) % unit or t.data_ptr() % (2 * unit):
         raise ValueError(f'{name} must have rows that start at multiples of {2 * unit} bytes')
-    if write and ((T > 1 and s0 < hd) or (H > 1 and s1 < hd)):
+    # written rows: token by token or head by head, each behind the end of the last
+    if write and T > 0 and ((H > 1 and s1 < hd) or (T > 1 and s0 < (H - 1) * s1 + hd)) and \
+            ((T > 1 and s0 < hd) or (H > 1 and s1 < (T - 1) * s0 + hd)):
         raise ValueError(f'{name} must not overlap itself')
     return s0, s1
 
@@ -524,9 +526,12 @@ def _queries(q, cu_q, kv, hd, out, scale):
 
 
 @functools.lru_cache(maxsize=256)
-def _workspace_bytes(B, T, keys, H, kv, hd):
+def attention_workspace(B, Tq, keys, n_heads, n_kv, head_dim):
+    """Bytes of workspace (0: none) of attention_varlen (keys = Tk) and
+    attention_paged (keys = B * table width * page) for B sequences of Tq
+    queries in all."""
     nb = ctypes.c_size_t()
-    check(lib().ck_attention_workspace(B, T, keys, H, kv, hd, ctypes.byref(nb)))
+    check(lib().ck_attention_workspace(B, Tq, keys, n_heads, n_kv, head_dim, ctypes.byref(nb)))
     return nb.value
 
 
@@ -537,7 +542,10 @@ def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None
     cu_k None: the same).  causal: query i of n over m keys sees the keys
     j <= i + m - n; else all.  heads a multiple of n_kv, head_dim 64 or 128,
     scale 1/sqrt(head_dim) unless given.  A query without a key gets zeros; rows
-    behind the last sequence are not written."""
+    behind the last sequence are not written.  out must not overlap k or v.
+    workspace: a buffer to keep, of at least attention_workspace bytes (else a new
+    one is made); one for each call that may run beside another, and for each
+    captured graph."""
     if not isinstance(k, torch.Tensor) or k.dim() != 3:
         raise ValueError('k must be [Tk, n_kv, head_dim]')
     Tk, kv, hd = k.shape
@@ -554,7 +562,7 @@ def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None
         _is(cu_k, torch.int32, 'cu_k', (B + 1,))
     dev = _on_device('q k v cu_q cu_k out', q, k, v, cu_q, cu_k, out)
     o = out if out is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    nb = _workspace_bytes(B, T, Tk, H, kv, hd)
+    nb = attention_workspace(B, T, Tk, H, kv, hd)
     ws = _workspace(workspace, nb, q.device)
     check(lib().ck_attention_varlen(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu_q.data_ptr(),
                                     cu_k.data_ptr(), B, T, Tk, H, kv, hd, qt, qh, kt, kh, vt, vh, ot, oh,
@@ -584,7 +592,7 @@ def attention_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, k_scale=Non
     dev = _on_device('q k_pages v_pages block_table cu_q kv_lens k_scale v_scale out', q, k_pages, v_pages, block_table,
                      cu_q, kv_lens, k_scale, v_scale, out)
     o = out if out is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    nb = _workspace_bytes(B, T, B * width * page, H, kv, hd)
+    nb = attention_workspace(B, T, B * width * page, H, kv, hd)
     ws = _workspace(workspace, nb, q.device)
     check(lib().ck_attention_paged(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale),
                                    o.data_ptr(), block_table.data_ptr(), width, cu_q.data_ptr(), kv_lens.data_ptr(), B,

@@ -1026,7 +1026,9 @@ Plan plan_of(int B, int Tq, long keys, int n_heads, int n_kv) {
   // many, as their chunks come out uneven (32 ragged histories 127 -> 122 us; three times 125)
   const long slots = pl.bm == 256 ? 256 : pl.bm == 128 ? 512 : 1024;
   pl.min_blocks = pl.bm == 32 ? 2 : 4;
-  // keys stay whole where the tiles fill the card twice, or there are too few keys to gain from it
+  // keys stay whole where the tiles fill the card twice, or the sequences have too few to pay for
+  // the second launch (prompts of 548, 652 and less, 128 features, split 31 us, whole 20; one of
+  // 1031 with two short ones 20 and 26, but the host knows the average only)
   const bool many = pl.bm != 32 && pl.tiles * n_kv >= 2 * slots;
   if (!many && keys / B > 2 * pl.min_blocks * AT_KEYS) pl.target = (int)std::max(1L, slots / n_kv);
   pl.items = pl.tiles + pl.target;

@@ -86,6 +86,11 @@ REFUSED = [
     ('varlen out', lambda: varlen(out=z(4, 4, 65)[:, :, :64]), 'multiples of 8 bytes'),
     ('varlen q alignment', lambda: varlen(z(4, 4, 72)[:, :, 1:65]), 'multiples of 16 bytes'),
     ('varlen out overlaps itself', lambda: varlen(out=z(1, 4, 64).expand(4, 4, 64)), 'must not overlap itself'),
+    ('rope out token 1 is head 1 of token 0', lambda: K.rope(z(4, 2, 64), z(4, dtype=i32), F, out=z(320).as_strided((4, 2, 64), (64, 64, 1))),
+     'must not overlap itself'),
+    ('varlen out heads in each other', lambda: varlen(out=z(1024).as_strided((4, 4, 64), (128, 64, 1))), 'must not overlap itself'),
+    ('varlen out head by head', lambda: varlen(out=z(4, 4, 64).transpose(0, 1)), 'must be a CUDA tensor'),
+    ('varlen out in wider rows', lambda: varlen(out=z(4, 6, 72)[:, 1:5, :64]), 'must be a CUDA tensor'),
     ('paged cache type', lambda: paged(z(4, 4, 64, dtype=bf16)), 'cache must be torch.bfloat16 or'),
     ('paged head_dim', lambda: paged(z(4, 4, 128)), 'head_dim must be 64 or 128 for q and the keys alike'),
     ('paged table rows', lambda: paged(table=z(3, 3, dtype=i32)), 'block_table must have shape'),
@@ -212,3 +217,12 @@ def test_oracle_rope_turns_and_turns_back():
         i, j = (0, 1) if inter else (0, 3)
         z = (x[2, 1, i] + 1j * x[2, 1, j]) * np.exp(5j) * 2
         assert np.allclose([y[2, 1, i], y[2, 1, j]], [z.real, z.imag])
+
+
+def test_attention_workspace():
+    assert K.attention_workspace(0, 0, 0, 8, 8, 64) == K.attention_workspace(40, 4000, 4000, 8, 8, 64) == 0
+    one = K.attention_workspace(1, 1, 6144, 8, 8, 64)
+    assert one % 16 == 0 and one >= 8 * 32 * (64 + 2) * 4 * 2     # two parts of a tile of 32 rows a head at least
+    for bad in ((1, 1, 64, 8, 3, 64), (-1, 1, 64, 8, 8, 64), (1, 1, -64, 8, 8, 64)):
+        with pytest.raises(RuntimeError, match='bad sizes'):
+            K.attention_workspace(*bad)
