@@ -270,6 +270,30 @@ def test_long_prompts(gpu, lens, H, kv, hd, dt, causal):
         a += n
 
 
+@pytest.mark.parametrize('qlens,klens,H,kv,hd', [([2417, 2], [2417, 2], 16, 4, 128), ([5800], [5800], 1, 1, 64), ([1300], [1300], 1, 1, 128),
+                                                 ([700, 33, 1500], [4000, 20, 1500], 3, 1, 64), ([200], [9000], 2, 1, 128),
+                                                 ([601] * 9 + [40, 0, 1] * 3, [601] * 5 + [1777] * 4 + [2900, 5, 63] * 3, 6, 2, 64)])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+def test_causal_prompts_with_their_keys_split(gpu, qlens, klens, H, kv, hd, dt):
+    """Tiles of one sequence with different numbers of chunks; nothing behind the workspace is written."""
+    from chestnut import kernels as K
+    q, k, v = rows(1, sum(qlens), H, hd, dt), rows(2, sum(klens), kv, hd, dt), rows(3, sum(klens), kv, hd, dt)
+    nf = K.attention_workspace(len(qlens), sum(qlens), sum(klens), H, kv, hd) // 4
+    assert nf > 0
+    ws = torch.full((nf + 4096,), 7.0, device='cuda')
+    out = K.attention_varlen(q, k, v, cu(qlens), cu(klens), workspace=ws)
+    assert (ws[nf:] == 7.0).all()
+    ws[:nf] = float('nan')
+    assert torch.equal(out, K.attention_varlen(q, k, v, cu(qlens), cu(klens), workspace=ws))
+    a = c = 0
+    for n, m in zip(qlens, klens):
+        e = max(0, n - m)
+        assert (out[a:a + e] == 0).all()
+        if n > e:
+            near(out[a + e:a + n], *attention_on_gpu(q[a + e:a + n], k[c:c + m], v[c:c + m], True), m, hd, dt, f'{n} over {m}')
+        a, c = a + n, c + m
+
+
 @pytest.mark.parametrize('qlens,klens,H,kv,hd,page', [([512], [5000], 2, 2, 128, 64), ([1, 300, 2, 77], [3000, 2500, 6000, 77], 8, 2, 128, 32),
                                                       ([1] * 12, [300 * i + 1 for i in range(12)], 16, 2, 64, 256),
                                                       ([1] * 130, [7 * i for i in range(130)], 4, 2, 128, 16),
