@@ -207,7 +207,7 @@ __device__ __forceinline__ int k_at(int key, int c) {
 }
 template <int HD>
 __device__ __forceinline__ int v_at(int key, int c) {
-  return HD == 128 ? key * HD + ((c ^ ((key & 3) << 2)) << 3) : key * HD + ((c ^ ((key & 2) << 1)) << 3);
+  return key * HD + ((c ^ (HD == 128 ? (key & 3) << 2 : (key & 2) << 1) ^ ((key >> 1) & 2)) << 3);
 }
 
 // KEYS rows of K or V on their way to LDS by NT threads.  Places behind the last key repeat
@@ -380,13 +380,21 @@ __device__ __forceinline__ float half_max(float v) {
   return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
 }
 
+// The maximum of lanes l and l ^ 16, in both.
+__device__ __forceinline__ float quarter_max(float v) {
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  const auto x = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const unsigned a = x[0], b = x[1];
+  return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+
 // ---- 32 rows of a wave ------------------------------------------------------------------
 template <typename T, int HD>
 struct Rows {
   typedef typename Elem<T>::v2 v2;
   typedef typename Elem<T>::v4 v4;
   typedef typename Elem<T>::v8 v8;
-  static constexpr int KS = HD / 16, CT = HD / 32;
+  static constexpr int BM = 32, KS = HD / 16, CT = HD / 32, VA = CT;
   v8 qf[KS];
   float16_t o[CT];
   float m, l;         // running maximum of the raw scores; this half's part of the sum
@@ -602,7 +610,26 @@ struct Rows {
         o[ct][i] += add;
       }
   }
+  // the 32 keys from key0 on, of a wave by itself; part: some row does not see all of them
+  __device__ __forceinline__ void step(const T* kt, const unsigned (&va)[VA], bool part, int key0, float c, int lane) {
+    float16_t s[1];
+    v8 pf[2];
+    scores<1>(s, kt, lane);
+    if (part) mask<1>(s, key0, lane);
+    raise(top<1>(s), c);
+    weights<1>(pf, s, c);
+    values<1, 0>(va, pf);
+  }
   __device__ __forceinline__ float sum() const { return l + __shfl_xor(l, 32); }
+  // f(chunk, values) for every four features of the row in this lane
+  template <typename F>
+  __device__ __forceinline__ void chunks(int lane, F f) const {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        f(ct * 8 + (i >> 1) + (lane >> 5), float4_t{o[ct][i], o[ct][i + 1], o[ct][i + 2], o[ct][i + 3]});
+  }
   // the output rows, O / l
   __device__ __forceinline__ void finish(const AttendParams& p, const Item& it, int hk, int lane) const {
     const float t = sum(), r = t == 0.f ? 0.f : 1.0f / t;
@@ -615,6 +642,121 @@ struct Rows {
         const v2 a = pack2<T>(o[ct][i] * r, o[ct][i + 1] * r), b = pack2<T>(o[ct][i + 2] * r, o[ct][i + 3] * r);
         *reinterpret_cast<v4*>(out + ct * 32 + 2 * i) = v4{a[0], a[1], b[0], b[1]};
       }
+  }
+};
+
+// ---- 16 rows of a wave ------------------------------------------------------------------
+// The same with 16x16x32 products, where 32 rows would stand half empty: half the registers.  Lane
+// l holds row l % 16, of a block of 16 keys those 4 (l / 16) + i, i < 4; two blocks make the second
+// product's operand.  Steps of 32 keys.
+template <typename T, int HD>
+struct Rows16 {
+  typedef typename Elem<T>::v2 v2;
+  typedef typename Elem<T>::v4 v4;
+  typedef typename Elem<T>::v8 v8;
+  static constexpr int BM = 16, KS = HD / 32, CT = HD / 16, VA = HD / 32;
+  v8 qf[KS];
+  float4_t o[CT];
+  float m, l;
+  int lim;
+
+  __device__ __forceinline__ void begin(const AttendParams& p, const Item& it, int hk, int row, int lane) {
+    const int tok = row / p.G, g = row - tok * p.G;
+    const bool valid = tok < it.s.nq;
+    lim = valid ? keys_of(p, it.s, tok) : 0;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = v8{};
+    if (valid) {
+      const T* q = static_cast<const T*>(p.q) + (long)(it.s.q0 + tok) * p.q_st + (long)(hk * p.G + g) * p.q_sh;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const v8*>(q + ks * 32 + (lane >> 4) * 8);
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) o[ct] = float4_t{};
+    m = -INFINITY;
+    l = 0.f;
+  }
+  __device__ __forceinline__ void arrived() {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
+  }
+  static __device__ __forceinline__ void values_at(unsigned (&va)[VA], const T* vt, int lane) {
+    const int key = 4 * (lane >> 4) + ((lane >> 2) & 3), d = 4 * (lane & 3);
+#pragma unroll
+    for (int i = 0; i < VA; ++i)
+      va[i] = (unsigned)(uintptr_t)(lds_ptr_t)(const_cast<T*>(vt) + v_at<HD>(key, (i * 32 + d) >> 3) + (d & 7));
+  }
+  // the 32 keys from key0 on; part: some row does not see all of them
+  __device__ __forceinline__ void step(const T* kt, const unsigned (&va)[VA], bool part, int key0, float c, int lane) {
+    float4_t s[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      s[kb] = float4_t{};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        s[kb] = Elem<T>::mfma16(*reinterpret_cast<const v8*>(kt + k_at<HD>(kb * 16 + (lane & 15), ks * 4 + (lane >> 4))), qf[ks], s[kb]);
+    }
+    if (part) {
+      const int left = lim - key0 - 4 * (lane >> 4);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (kb * 16 + i >= left) s[kb][i] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i >> 2][i & 3]);
+    mx = half_max(quarter_max(mx));
+    if (__any((mx - m) * c > 8.0f || (m == -INFINITY && mx > -INFINITY))) {   // as Rows::raise
+      const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) o[ct] *= f;
+    }
+    const float mc = m == -INFINITY ? 0.f : __builtin_fmaf(m, c, -Elem<T>::LIFT);
+    v8 pf;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const v2 u = pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][i & 3], c, -mc)),
+                            __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 2][(i & 3) + 1], c, -mc)));
+      l = Elem<T>::add2(u, l);
+      pf[i] = u[0];
+      pf[i + 1] = u[1];
+    }
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4* at_t;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const unsigned at = va[ct >> 1] ^ ((ct & 1) * 32);   // 16-byte chunk c and c ^ 2
+      const v4 a = __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_t)(uintptr_t)at));
+      const v4 b = __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_t)(uintptr_t)(at + 16 * HD * 2)));
+      o[ct] = Elem<T>::mfma16(v8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}, pf, o[ct]);
+    }
+  }
+  // as Rows::add_odd
+  __device__ __forceinline__ void add_odd(const int (*bad)[HD], int lane) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int* k = &bad[0][ct * 16 + 4 * (lane >> 4) + i];
+        float add = k[0] < lim ? INFINITY : 0.f;
+        add += k[HD] < lim ? -INFINITY : 0.f;
+        add += k[2 * HD] < lim ? NAN : 0.f;
+        o[ct][i] += add;
+      }
+  }
+  __device__ __forceinline__ float sum() const {
+    const float t = l + __shfl_xor(l, 16);
+    return t + __shfl_xor(t, 32);
+  }
+  // f(chunk, values) for every four features of the row in this lane
+  template <typename F>
+  __device__ __forceinline__ void chunks(int lane, F f) const {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) f(ct * 4 + (lane >> 4), o[ct]);
   }
 };
 
@@ -826,18 +968,18 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
 // one token on 6144 keys, 8 heads of 64, f16: 6.6 us.
 constexpr int FEW_WAVES = 4;
 
-template <typename T, int HD, int KV>
+template <typename T, int HD, int KV, typename R>
 __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attend_few_kernel(const AttendParams p) {
-  constexpr int BM = 32, KEYS = 32, TILE = KEYS * HD, NW = FEW_WAVES;
-  __shared__ __attribute__((aligned(16))) T lds[NW][2 * TILE];   // at the end: O f32 [NW][32][HD]
+  constexpr int BM = R::BM, KEYS = 32, TILE = KEYS * HD, NW = FEW_WAVES;
+  __shared__ __attribute__((aligned(1024))) T lds[NW][2 * TILE];   // at the end: O f32 [NW][32][HD]
   __shared__ float2_t ml[NW][BM];
   __shared__ int bad[NW][3][HD];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hk = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv;
   Item it;
   if (!find_item<KV, BM, false>(p, index, it)) return;
-  Rows<T, HD> r;
-  r.begin(p, it, hk, it.tile * BM + (lane & 31), lane);
+  R r;
+  r.begin(p, it, hk, it.tile * BM + lane % BM, lane);
   const int klo = keys_of(p, it.s, it.tile * BM / p.G);
   const int khi = keys_of(p, it.s, min(it.s.nq - 1, (it.tile * BM + BM - 1) / p.G));
   const int kbeg = it.nch > 1 ? it.chunk * it.c * AT_KEYS : 0;
@@ -853,7 +995,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attend_few_kernel(const Att
     ks.begin(p, it, hk, key0, NW * KEYS, lane, 0, false);
     vs.begin(p, it, hk, key0, NW * KEYS, lane, 0, false);
   }
-  unsigned va[Rows<T, HD>::CT];
+  unsigned va[R::VA];
   r.values_at(va, vt, lane);
   auto load = [&](int key) {
     ks.load(p, it, hk, key, lane, 0);
@@ -874,13 +1016,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attend_few_kernel(const Att
       take_out_odd<T, HD, KEYS, 64>(vt, bad[wave], key0, lane);
       wave_order();
     }
-    float16_t s[1];
-    typename Elem<T>::v8 pf[2];
-    r.template scores<1>(s, kt, lane);
-    if (part) r.template mask<1>(s, key0, lane);
-    r.raise(r.template top<1>(s), p.scale_log2e);
-    r.template weights<1>(pf, s, p.scale_log2e);
-    r.template values<1, 0>(va, pf);
+    r.step(kt, va, part, key0, p.scale_log2e, lane);
     if (fix) r.add_odd(bad[wave], lane);
   }
 
@@ -889,16 +1025,11 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attend_few_kernel(const Att
   const int rows = min(BM, it.s.nq * p.G - it.tile * BM);
   float* const ob = reinterpret_cast<float*>(&lds[0][0]);
   const float t = r.sum();
-  if (lane < 32) ml[wave][lane] = float2_t{r.m * p.scale_log2e, t};
-  if ((lane & 31) < rows) {
+  if (lane < BM) ml[wave][lane] = float2_t{r.m * p.scale_log2e, t};
+  if (lane % BM < rows) {
     // 16-byte chunk c of row q at c ^ (q & 7): 8 rows of a chunk in 8 different places
-    float* o = ob + (wave * BM + (lane & 31)) * HD;
-#pragma unroll
-    for (int ct = 0; ct < HD / 32; ++ct)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        *reinterpret_cast<float4_t*>(o + (((ct * 8 + (i >> 1) + (lane >> 5)) ^ (lane & 7)) << 2)) =
-            float4_t{r.o[ct][i], r.o[ct][i + 1], r.o[ct][i + 2], r.o[ct][i + 3]};
+    float* o = ob + (wave * BM + lane % BM) * HD;
+    r.chunks(lane, [&](int c, float4_t x) { *reinterpret_cast<float4_t*>(o + ((c ^ (lane & 7)) << 2)) = x; });
   }
   __syncthreads();
   for (int i = tid; i < rows * (HD / 4); i += 64 * NW) {
@@ -936,7 +1067,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attend_few_kernel(const Att
 // are zero at the start and stay so where a call is cut short or two replays overlap.
 template <typename T, int HD, int KV, int BM>
 __global__ __launch_bounds__(256) void attend_join_kernel(const AttendParams p) {
-  constexpr int LPR = HD / 4, CG = BM == 32 ? 256 / LPR : 1, RP = 256 / LPR / CG;
+  constexpr int LPR = HD / 4, CG = BM <= 32 ? 256 / LPR : 1, RP = 256 / LPR / CG;
   __shared__ float4_t so[CG][LPR];
   __shared__ float2_t sm[CG];
   const int hk = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv;
@@ -945,7 +1076,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const AttendParams p) 
   if (!find_item<KV, BM, true>(p, index, it) || it.nch == 1 || it.base < 0 || it.base + it.nch > p.items) return;
   const int c = threadIdx.x % LPR, cg = CG > 1 ? threadIdx.x / LPR : 0;
   const int q = blockIdx.y * RP + (CG > 1 ? 0 : threadIdx.x / LPR);
-  const int tile = BM == 32 ? it.tile : tiles_of<KV, BM>(it.s, p.G) - 1 - it.tile;
+  const int tile = BM <= 32 ? it.tile : tiles_of<KV, BM>(it.s, p.G) - 1 - it.tile;
   const bool in = (long)tile * BM + q < (long)it.s.nq * p.G;
   if (CG > 1 && !in) return;
   float M = -INFINITY, sum = 0.f;
@@ -1022,17 +1153,17 @@ Plan plan_of(int B, int Tq, long keys, int n_heads, int n_kv) {
   // 256 rows where they fill the 256 CUs at least twice without splitting keys (prompt of 16384
   // tokens, 441 us against 508 with 128); with fewer, tiles of 256 with their keys split take
   // 80 us against 82 (512 tokens on 12800 keys) and 81 against 77 (eight mixed chunks).
-  pl.bm = rows <= 32L * B ? 32 : (rows / 256 + B) * n_kv >= 512 ? 256 : 128;
+  pl.bm = rows <= 16L * B ? 16 : rows <= 32L * B ? 32 : (rows / 256 + B) * n_kv >= 512 ? 256 : 128;
   pl.tiles = rows / pl.bm + B;       // sum of ceil(rows_b / bm) is at most this
   // items to aim at: workgroups that run at once, one a CU or two (tiles of 128, three, four, six
   // a CU in place of two: 512 tokens on 12800 keys 99, 104, 119 for 86 us); of few rows twice as
   // many, as their chunks come out uneven (32 ragged histories 127 -> 122 us; three times 125)
   const long slots = pl.bm == 256 ? 256 : pl.bm == 128 ? 512 : 1024;
-  pl.min_blocks = pl.bm == 32 ? 2 : 4;
+  pl.min_blocks = pl.bm <= 32 ? 2 : 4;
   // keys stay whole where the tiles fill the card twice, or the sequences have too few to pay for
   // the second launch (prompts of 548, 652 and less, 128 features, split 31 us, whole 20; one of
   // 1031 with two short ones 20 and 26, but the host knows the average only)
-  const bool many = pl.bm != 32 && pl.tiles * n_kv >= 2 * slots;
+  const bool many = pl.bm > 32 && pl.tiles * n_kv >= 2 * slots;
   if (!many && keys / B > 2 * pl.min_blocks * AT_KEYS) pl.target = (int)std::max(1L, slots / n_kv);
   pl.items = pl.tiles + pl.target;
   return pl;
@@ -1041,12 +1172,14 @@ Plan plan_of(int B, int Tq, long keys, int n_heads, int n_kv) {
 template <typename T, int HD, int KV>
 void launch_kv(const AttendParams& p, const Plan& pl, hipStream_t s) {
   const dim3 grid((unsigned)(pl.items * p.Hkv));
-  if (pl.bm == 32) CK_LAUNCH((attend_few_kernel<T, HD, KV>), grid, dim3(64 * FEW_WAVES), 0, s, p);
+  if (pl.bm == 16) CK_LAUNCH((attend_few_kernel<T, HD, KV, Rows16<T, HD>>), grid, dim3(64 * FEW_WAVES), 0, s, p);
+  else if (pl.bm == 32) CK_LAUNCH((attend_few_kernel<T, HD, KV, Rows<T, HD>>), grid, dim3(64 * FEW_WAVES), 0, s, p);
   else if (pl.bm == 128) CK_LAUNCH((attend_tile_kernel<T, HD, KV, 4>), grid, dim3(256), 0, s, p);
   else CK_LAUNCH((attend_tile_kernel<T, HD, KV, 8>), grid, dim3(512), 0, s, p);
   if (!pl.target) return;
   const unsigned tiles = (unsigned)(pl.tiles * p.Hkv);
-  if (pl.bm == 32) CK_LAUNCH((attend_join_kernel<T, HD, KV, 32>), dim3(tiles, 32), dim3(256), 0, s, p);
+  if (pl.bm == 16) CK_LAUNCH((attend_join_kernel<T, HD, KV, 16>), dim3(tiles, 16), dim3(256), 0, s, p);
+  else if (pl.bm == 32) CK_LAUNCH((attend_join_kernel<T, HD, KV, 32>), dim3(tiles, 32), dim3(256), 0, s, p);
   else if (pl.bm == 128) CK_LAUNCH((attend_join_kernel<T, HD, KV, 128>), dim3(tiles, 128 / (1024 / HD)), dim3(256), 0, s, p);
   else CK_LAUNCH((attend_join_kernel<T, HD, KV, 256>), dim3(tiles, 256 / (1024 / HD)), dim3(256), 0, s, p);
 }

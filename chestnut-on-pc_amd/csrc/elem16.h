@@ -1,5 +1,5 @@
 // The 16-bit element types of the token-cache kernels (f16 and bf16): vector types,
-// conversions, the 32x32x16 matrix product, and the division by a launch constant.
+// conversions, the matrix products, and the division by a launch constant.
 #pragma once
 
 #include "common.h"
@@ -34,6 +34,9 @@ struct Elem<half_t> {
   static __device__ __forceinline__ float16_t mfma32(v8 a, v8 b, float16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
+  static __device__ __forceinline__ float4_t mfma16(v8 a, v8 b, float4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
   static __device__ __forceinline__ float add2(v2 a, float c) {   // c + a[0] + a[1]
     return __builtin_amdgcn_fdot2(a, v2{(half_t)1.0f, (half_t)1.0f}, c, false);
   }
@@ -48,6 +51,9 @@ struct Elem<bf16_t> {
   static constexpr float LIFT = 0.0f;
   static __device__ __forceinline__ float16_t mfma32(v8 a, v8 b, float16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float4_t mfma16(v8 a, v8 b, float4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
   static __device__ __forceinline__ float add2(v2 a, float c) {
     return __builtin_amdgcn_fdot2_f32_bf16(a, v2{(bf16_t)1.0f, (bf16_t)1.0f}, c, false);
