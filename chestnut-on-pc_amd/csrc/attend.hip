@@ -19,7 +19,7 @@
 // Three kernels (their figures stand at each):
 //   attend_tile_kernel  128 or 256 rows, tiles of 64 keys in LDS: prompts and chunks of one;
 //                       bound by the matrix cores beside the vector unit's exponentials;
-//   attend_few_kernel   32 rows, the keys over four waves: tokens one by one; bound by memory;
+//   attend_few_kernel   16 or 32 rows, the keys over four waves: tokens one by one; bound by memory;
 //   attend_join_kernel  joins the parts of rows whose keys were split over workgroups.
 #include <algorithm>
 #include <type_traits>
@@ -610,12 +610,15 @@ struct Rows {
         o[ct][i] += add;
       }
   }
-  // the 32 keys from key0 on, of a wave by itself; part: some row does not see all of them
-  __device__ __forceinline__ void step(const T* kt, const unsigned (&va)[VA], bool part, int key0, float c, int lane) {
-    float16_t s[1];
-    v8 pf[2];
+  // For a wave by itself: S^T of the 32 keys from key0 on; part: some row does not see all of them
+  typedef float16_t scores_t[1];
+  __device__ __forceinline__ void look(scores_t& s, const T* kt, bool part, int key0, int lane) const {
     scores<1>(s, kt, lane);
     if (part) mask<1>(s, key0, lane);
+  }
+  // and O^T += V^T P^T of them
+  __device__ __forceinline__ void take(const scores_t& s, const unsigned (&va)[VA], float c, int lane) {
+    v8 pf[2];
     raise(top<1>(s), c);
     weights<1>(pf, s, c);
     values<1, 0>(va, pf);
@@ -686,9 +689,9 @@ struct Rows16 {
     for (int i = 0; i < VA; ++i)
       va[i] = (unsigned)(uintptr_t)(lds_ptr_t)(const_cast<T*>(vt) + v_at<HD>(key, (i * 32 + d) >> 3) + (d & 7));
   }
-  // the 32 keys from key0 on; part: some row does not see all of them
-  __device__ __forceinline__ void step(const T* kt, const unsigned (&va)[VA], bool part, int key0, float c, int lane) {
-    float4_t s[2];
+  typedef float4_t scores_t[2];
+  // S^T of the 32 keys from key0 on; part: some row does not see all of them
+  __device__ __forceinline__ void look(scores_t& s, const T* kt, bool part, int key0, int lane) const {
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       s[kb] = float4_t{};
@@ -704,6 +707,9 @@ struct Rows16 {
         for (int i = 0; i < 4; ++i)
           if (kb * 16 + i >= left) s[kb][i] = -INFINITY;
     }
+  }
+  // O^T += V^T P^T of them
+  __device__ __forceinline__ void take(const scores_t& s, const unsigned (&va)[VA], float c, int lane) {
     float mx = s[0][0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i >> 2][i & 3]);
@@ -959,19 +965,27 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
       *reinterpret_cast<float4_t*>(o + ct * 32 + 2 * i) = float4_t{r.o[ct][i], r.o[ct][i + 1], r.o[ct][i + 2], r.o[ct][i + 3]};
 }
 
-// ---- few rows: 32 of them, the keys over the waves ----------------------------------------
+// ---- few rows: 16 or 32 of them, the keys over the waves -----------------------------------
 // Every wave streams its own blocks of 32 keys (w, w + 4, ...) through LDS of its own; nothing
 // waits for another wave until the end, where the waves' sums are joined.  Bound by memory: the
-// rows come past the caches, K and V of the next step under way during this one's products (two
-// steps ahead: spills, 151 us against 124).  32 tokens on 1025 to 32701 keys, 16 heads on 4 of
-// 128, e4m3: 117 us = 5.5 TB/s, where plain reads of this kind reach 7.1 and the card's copy 4.9;
-// one token on 6144 keys, 8 heads of 64, f16: 6.6 us.
+// rows come past the caches, K and V of the next step under way during this one's products.
+// What helps is workgroups on a CU: 16 rows leave registers for more of them.  32 tokens on 1025
+// to 32701 keys, 16 heads on 4 of 128, e4m3: 120 us with 32 rows, 115 with 16, 110 with three
+// workgroups a CU, 5.9 TB/s, where plain reads of this kind reach 7.1 and the card's copy 4.9;
+// 16 such on 8 heads of 64 84, 64, and 62 with K's next rows sent for before V's are stored.  Two
+// steps ahead are slower: 116 for 115, and 77 for 64.
+// One token on 6144 keys, 8 heads of 64, f16: 6.6 us.
 constexpr int FEW_WAVES = 4;
 
+// workgroups a CU
+constexpr int few_at_once(int bm, int hd, bool e4m3) { return hd == 64 ? (bm == 16 ? 4 : 3) : bm == 16 && e4m3 ? 3 : 2; }
+
 template <typename T, int HD, int KV, typename R>
-__global__ __launch_bounds__(64 * FEW_WAVES, 2) void attend_few_kernel(const AttendParams p) {
+__global__ __launch_bounds__(64 * FEW_WAVES, few_at_once(R::BM, HD, KV == KV_E4M3)) void attend_few_kernel(const AttendParams p) {
   constexpr int BM = R::BM, KEYS = 32, TILE = KEYS * HD, NW = FEW_WAVES;
-  __shared__ __attribute__((aligned(1024))) T lds[NW][2 * TILE];   // at the end: O f32 [NW][32][HD]
+  // 1: V takes K's place in LDS, so that three workgroups of 128 features fit a CU
+  constexpr int PARTS = HD == 128 && few_at_once(BM, HD, KV == KV_E4M3) == 3 ? 1 : 2;
+  __shared__ __attribute__((aligned(1024))) T lds[NW][PARTS * TILE];   // at the end: O f32 [NW][BM][HD]
   __shared__ float2_t ml[NW][BM];
   __shared__ int bad[NW][3][HD];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -989,7 +1003,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attend_few_kernel(const Att
   Stage<T, HD, KV, KEYS, 64, false, true> ks;
   Stage<T, HD, KV, KEYS, 64, true, true> vs;
   T* const kt = lds[wave];
-  T* const vt = kt + TILE;
+  T* const vt = kt + (PARTS - 1) * TILE;
   int key0 = kbeg + wave * KEYS;
   if (key0 < kend) {
     ks.begin(p, it, hk, key0, NW * KEYS, lane, 0, false);
@@ -997,18 +1011,26 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attend_few_kernel(const Att
   }
   unsigned va[R::VA];
   r.values_at(va, vt, lane);
-  auto load = [&](int key) {
-    ks.load(p, it, hk, key, lane, 0);
-    vs.load(p, it, hk, key, lane, 0);
-  };
-  if (key0 < kend) load(key0);
+  if (key0 < kend) {
+    ks.load(p, it, hk, key0, lane, 0);
+    vs.load(p, it, hk, key0, lane, 0);
+  }
   for (; key0 < kend; key0 += NW * KEYS) {
     const bool part = key0 + KEYS > klo;
     wave_order();
+    typename R::scores_t s;
+    const bool more = key0 + NW * KEYS < kend;
     ks.store(kt, lane);
+    if (more) ks.load(p, it, hk, key0 + NW * KEYS, lane, 0);
+    if constexpr (PARTS == 1) {
+      wave_order();
+      r.look(s, kt, part, key0, lane);
+      wave_order();
+    }
     vs.store(vt, lane);
-    if (key0 + NW * KEYS < kend) load(key0 + NW * KEYS);
+    if (more) vs.load(p, it, hk, key0 + NW * KEYS, lane, 0);
     wave_order();
+    if constexpr (PARTS == 2) r.look(s, kt, part, key0, lane);
     const bool fix = part && __any(any_odd<T, TILE, 64>(vt, lane));
     if (fix) {
       for (int i = lane; i < 3 * HD; i += 64) (&bad[wave][0][0])[i] = 0x7FFFFFFF;
@@ -1016,7 +1038,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 2) void attend_few_kernel(const Att
       take_out_odd<T, HD, KEYS, 64>(vt, bad[wave], key0, lane);
       wave_order();
     }
-    r.step(kt, va, part, key0, p.scale_log2e, lane);
+    r.take(s, va, p.scale_log2e, lane);
     if (fix) r.add_odd(bad[wave], lane);
   }
 
@@ -1144,12 +1166,13 @@ struct Plan {
   int bm, target, min_blocks;
   long tiles, items;   // at most
 };
-// keys: the most that the sequences can have, all together
-Plan plan_of(int B, int Tq, long keys, int n_heads, int n_kv) {
+// keys: the most that the sequences can have, all together; few3: three workgroups of few rows
+// run on a CU.  (The workspace is asked for without that: the larger of the two counts.)
+Plan plan_of(int B, int Tq, long keys, int n_heads, int n_kv, bool few3 = false) {
   Plan pl{};
   const int G = n_heads / n_kv;
   const long rows = (long)Tq * G;
-  // 32 rows where a sequence has that many on average: bound by the keys, not by the rows.
+  // 16 or 32 rows where a sequence has that many on average: bound by the keys, not by the rows.
   // 256 rows where they fill the 256 CUs at least twice without splitting keys (prompt of 16384
   // tokens, 441 us against 508 with 128); with fewer, tiles of 256 with their keys split take
   // 80 us against 82 (512 tokens on 12800 keys) and 81 against 77 (eight mixed chunks).
@@ -1157,8 +1180,10 @@ Plan plan_of(int B, int Tq, long keys, int n_heads, int n_kv) {
   pl.tiles = rows / pl.bm + B;       // sum of ceil(rows_b / bm) is at most this
   // items to aim at: workgroups that run at once, one a CU or two (tiles of 128, three, four, six
   // a CU in place of two: 512 tokens on 12800 keys 99, 104, 119 for 86 us); of few rows twice as
-  // many, as their chunks come out uneven (32 ragged histories 127 -> 122 us; three times 125)
-  const long slots = pl.bm == 256 ? 256 : pl.bm == 128 ? 512 : 1024;
+  // many, as their chunks come out uneven (32 ragged histories 127 -> 122 us; three times 125),
+  // or as many where three run on a CU (768 items 110 us, 1024 136, 1536 113; where two do, 16 of
+  // the histories, 768 110 and 1024 104)
+  const long slots = pl.bm == 256 ? 256 : pl.bm == 128 ? 512 : pl.bm == 16 && few3 ? 768 : 1024;
   pl.min_blocks = pl.bm <= 32 ? 2 : 4;
   // keys stay whole where the tiles fill the card twice, or the sequences have too few to pay for
   // the second launch (prompts of 548, 652 and less, 128 features, split 31 us, whole 20; one of
@@ -1217,7 +1242,7 @@ void launch_attend(const char* what, AttendParams& p, const AttendQuery& a, int 
   p.G = a.n_heads / p.Hkv;
   p.causal = a.causal;
   p.scale_log2e = a.scale * AT_LOG2E;
-  const Plan pl = plan_of(a.B, a.T, keys, a.n_heads, p.Hkv);
+  const Plan pl = plan_of(a.B, a.T, keys, a.n_heads, p.Hkv, a.head_dim == 128 && kv == KV_E4M3);
   // (a launch has under 2^32 threads)
   CK_REQUIRE(pl.items * p.Hkv < (1L << 32) / std::max(256, 2 * pl.bm), w + ": too many sequences and rows for one launch");
   if (pl.target) {

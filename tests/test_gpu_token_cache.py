@@ -369,6 +369,40 @@ def test_nan_codes_that_a_row_does_not_see_do_not_reach_it(gpu, dt, n, m):
     assert not torch.isfinite(out[clean:]).all(-1).any()
 
 
+@pytest.mark.parametrize('G', [1, 6, 15, 16, 17, 31, 32, 33])
+@pytest.mark.parametrize('hd', [64, 128])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('cache', ['rows', 'pages', 'e4m3'])
+def test_few_rows(gpu, G, hd, dt, cache):
+    """Single tokens of every group size around the tiles' heights, two tokens at once among them;
+    the last key of that sequence holds what its first token must not see."""
+    from chestnut import kernels as K
+    qlens, klens, kv, page = [2, 0, 1, 1], [777, 9, 64, 5], 2, 16
+    q = rows(1, 4, G * kv, hd, dt)
+    if cache == 'rows':
+        k, v = rows(2, sum(klens), kv, hd, dt), rows(3, sum(klens), kv, hd, dt)
+        v[776, 0, 3], v[776, 1, 5] = float('inf'), float('nan')
+        out = K.attention_varlen(q, k, v, cu(qlens), cu(klens))
+        ks, vs = ([x[sum(klens[:b]):sum(klens[:b + 1])] for b in range(4)] for x in (k, v))
+    else:
+        table, n = tables(klens, page, 5)
+        kp, vp, sk, sv = filled(n, kv, page, hd, dt, 'e4m3' if cache == 'e4m3' else dt, 6)
+        at = (int(table[0][776 // page]), 1, 776 % page, 5)
+        vp.view(torch.uint8 if cache == 'e4m3' else torch.int16)[at] = 0x7F if cache == 'e4m3' else 0x7FC1
+        out = K.attention_paged(q, kp, vp, i32(table), cu(qlens), i32(klens), k_scale=sk, v_scale=sv)
+        ks, vs = ([torch.from_numpy(gathered(p, s, table[b], m, page)).cuda() for b, m in enumerate(klens)]
+                  for p, s in ((kp, sk), (vp, sv)))
+    assert torch.isnan(out[1, G:, 5]).all() and (cache != 'rows' or (out[1, :G, 3] == float('inf')).all())
+    assert torch.isfinite(out[0]).all() and torch.isfinite(out[2:]).all()
+    vs[0] = torch.where(torch.isfinite(vs[0]), vs[0], torch.zeros_like(vs[0]))
+    out[1, :, 3], out[1, :, 5] = 0, 0
+    for a, b, n in ((0, 0, 2), (2, 2, 1), (3, 3, 1)):
+        ref, mag, most = attention_on_gpu(q[a:a + n], ks[b], vs[b], True)
+        if n == 2:
+            ref[1, :, 3], ref[1, :, 5] = 0, 0
+        near(out[a:a + n], ref, mag, most, klens[b], hd, dt, f'sequence {b}')
+
+
 @pytest.mark.parametrize('dt', ['f16', 'bf16'])
 def test_infinite_values_of_v_reach_the_rows_that_see_them(gpu, dt):
     from chestnut import kernels as K
