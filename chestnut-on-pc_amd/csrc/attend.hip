@@ -7,7 +7,7 @@
 //
 // Rows.  The queries of the G heads that share a K/V head are the rows of one product:
 // row r of a sequence is query r / G of head g = r % G, so that K and V pass once for all
-// of them.  A wave owns 32 rows:
+// of them.  A wave owns 32 rows (or 16: Rows16):
 //   S^T = K Q^T (v_mfma 32x32x16, A = 32 keys, B = 32 rows): lane l holds row l % 32 and
 //     the keys 8 (i / 4) + 4 (l / 32) + i % 4, i < 16, of a block of 32;
 //   the softmax needs the other half of the wave for its maximum and sum only;
@@ -200,7 +200,7 @@ __device__ __forceinline__ int keys_of(const AttendParams& p, const Seq& s, int 
 
 // ---- LDS tiles --------------------------------------------------------------------------
 // Element offsets of 16-byte chunk c of a row: K's fragments are one chunk of 16 consecutive
-// rows, V's four chunks of 4 consecutive rows; both hit every bank once this way.
+// rows, V's four chunks of 4 consecutive rows (Rows16: two of 8); all hit every bank once this way.
 template <int HD>
 __device__ __forceinline__ int k_at(int key, int c) {
   return HD == 128 ? key * HD + ((c ^ (key & 15)) << 3) : key * HD + ((c ^ ((key >> 1) & 7)) << 3);
@@ -817,7 +817,7 @@ __device__ __forceinline__ float2_t* part_ml(const AttendParams& p, long row) {
 // leaves: what bounds it is those two side by side.  Slower were the compiler's own order (sched
 // groups 517-535 against 508), rings of four tiles (467 against 455) and f16 tiles by way of
 // registers (466).  128 rows with the keys split: 512 tokens on 12800 keys, 16 heads of 128,
-// f16, 71 us and 8 to join them, 690 TFLOP/s in all; from an e4m3 cache, eight sequences of 1 to
+// f16, 70 us and 8 to join them, 690 TFLOP/s in all; from an e4m3 cache, eight sequences of 1 to
 // 511 tokens, 75 us = 545.  Short prompts (40 of 1 to 239 tokens, 8 heads of 64) 12.3 us.
 template <typename T, int HD, int KV, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendParams p) {
@@ -974,7 +974,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
 // workgroups a CU, 5.9 TB/s, where plain reads of this kind reach 7.1 and the card's copy 4.9;
 // 16 such on 8 heads of 64 84, 64, and 62 with K's next rows sent for before V's are stored.  Two
 // steps ahead are slower: 116 for 115, and 77 for 64.
-// One token on 6144 keys, 8 heads of 64, f16: 6.6 us.
+// One token on 6144 keys, 8 heads of 64, f16: 6.1 us.
 constexpr int FEW_WAVES = 4;
 
 // workgroups a CU
