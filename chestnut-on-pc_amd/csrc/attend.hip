@@ -1064,7 +1064,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, few_at_once(R::BM, HD, KV == KV_E4M
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
       const float2_t x = ml[w][q];
-      if (x[0] == -INFINITY) continue;   // saw no key
+      if (x[1] == 0.f) continue;   // saw no key; a maximum of -inf alone may stand for scores of NaN, and so does its sum
       const float f = __builtin_amdgcn_exp2f(x[0] - M);
       sum += f * x[1];
       a += f * *reinterpret_cast<const float4_t*>(ob + (w * BM + q) * HD + ((c ^ (q & 7)) << 2));
@@ -1119,7 +1119,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const AttendParams p) 
       float m = M;
 #pragma unroll
       for (int i = 0; i < AT; ++i) {
-        if (n0 + i * CG >= it.nch) x[i][0] = -INFINITY;
+        if (n0 + i * CG >= it.nch) x[i] = float2_t{-INFINITY, 0.f};
         m = fmaxf(m, x[i][0]);
       }
       const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - m);
@@ -1128,7 +1128,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const AttendParams p) 
       a *= f;
 #pragma unroll
       for (int i = 0; i < AT; ++i) {
-        if (x[i][0] == -INFINITY) continue;   // saw no key, has no O
+        if (x[i][1] == 0.f) continue;   // saw no key, has no O
         const float h = __builtin_amdgcn_exp2f(x[i][0] - m);
         sum += x[i][1] * h;
         a += y[i] * h;
@@ -1146,7 +1146,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const AttendParams p) 
     a = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < CG; ++w) {
-      if (sm[w][0] == -INFINITY) continue;
+      if (sm[w][1] == 0.f) continue;
       const float f = __builtin_amdgcn_exp2f(sm[w][0] - M);
       sum += f * sm[w][1];
       a += f * so[w][c];

@@ -628,3 +628,70 @@ def test_on_another_stream(gpu):
         got = K.attention_varlen(q, k, v, c)
     s.synchronize()
     assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------- NaN that a row sees --
+def cached(cache, m, kv, hd, dt, page=16):
+    """m keys of a sequence as rows, pages or quantised pages: (k, v) f64 and put(which, a, b): NaN
+    into feature 5 of keys a .. b of K/V head 0, and attend(q, causal)."""
+    from chestnut import kernels as K
+    if cache == 'rows':
+        kv_ = [rows(2, m, kv, hd, dt), rows(3, m, kv, hd, dt)]
+
+        def put(which, a, b):
+            kv_[which][a:b, 0, 5] = float('nan')
+        return f64(kv_[0]), f64(kv_[1]), put, lambda q, causal: K.attention_varlen(q, *kv_, cu([q.shape[0]]), cu([m]), causal=causal)
+    table, n = tables([m], page, 3)
+    kp, vp, ks, vs = filled(n, kv, page, hd, dt, 'e4m3' if cache == 'e4m3' else dt, 4)
+
+    def put(which, a, b):
+        p = (kp, vp)[which]
+        j = np.arange(a, b)
+        at = (i32(table[0][j // page]).long(), 0, i32(j % page).long(), 5)
+        if cache == 'e4m3':
+            p.view(torch.uint8)[at] = 0x7F
+        else:
+            p[at] = float('nan')
+    k, v = (gathered(p, s, table[0], m, page) for p, s in ((kp, ks), (vp, vs)))
+    return k, v, put, lambda q, causal: K.attention_paged(q, kp, vp, i32(table), cu([q.shape[0]]), i32([m]), k_scale=ks, v_scale=vs,
+                                                          causal=causal)
+
+
+# n queries over m keys of which a .. b are NaN.  Of one or 12 queries the keys are taken in blocks of 32
+# over four waves, and in chunks of 128 where they pass 256; of 70 in chunks of 256 where they pass 512:
+# the NaN fill a wave's share, a chunk, all the keys, or stand beside finite keys.
+NAN_KEYS = [(1, 33, 32, 33), (1, 190, 64, 96), (1, 512, 128, 256), (1, 700, 0, 700), (1, 700, 3, 4), (12, 44, 32, 44), (12, 512, 128, 256),
+            (70, 300, 290, 291), (70, 1024, 256, 512), (70, 1024, 0, 1024)]
+
+
+@pytest.mark.parametrize('n,m,a,b', NAN_KEYS)
+@pytest.mark.parametrize('hd', [64, 128])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('cache', ['rows', 'pages', 'e4m3'])
+@pytest.mark.parametrize('causal', [True, False])
+def test_nan_keys_reach_every_row_that_sees_them(gpu, n, m, a, b, hd, dt, cache, causal):
+    k, v, put, attend = cached(cache, m, 2, hd, dt)
+    put(0, a, b)
+    q = rows(1, n, 4, hd, dt)
+    out = attend(q, causal)
+    clean = min(max(0, a - (m - n)), n) if causal else 0        # queries before the first that sees key a
+    assert torch.isnan(out[clean:, :2]).all()
+    near(out[:, 2:], *O.attention(f64(q[:, 2:]), k[:, 1:], v[:, 1:], causal), m, hd, dt, 'the other K/V head')
+    if clean:
+        near(out[:clean, :2], *O.attention(f64(q[:clean, :2]), k[:m - n + clean, :1], v[:m - n + clean, :1], True), m, hd, dt, 'before')
+
+
+@pytest.mark.parametrize('n,m', [(1, 1), (1, 33), (1, 700), (12, 44), (12, 700), (70, 100), (70, 1024)])
+@pytest.mark.parametrize('hd', [64, 128])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('cache', ['rows', 'pages', 'e4m3'])
+@pytest.mark.parametrize('causal', [True, False])
+def test_a_nan_query_gives_a_nan_row(gpu, n, m, hd, dt, cache, causal):
+    k, v, _, attend = cached(cache, m, 2, hd, dt)
+    q = rows(1, n, 4, hd, dt)
+    ref, mag, most = O.attention(f64(q), k, v, causal)
+    q[n // 2, 1, 7] = float('nan')
+    out = attend(q, causal)
+    assert torch.isnan(out[n // 2, 1]).all()
+    out[n // 2, 1] = torch.from_numpy(ref[n // 2, 1]).to(out)
+    near(out, ref, mag, most, m, hd, dt)

@@ -226,3 +226,14 @@ def test_attention_workspace():
     for bad in ((1, 1, 64, 8, 3, 64), (-1, 1, 64, 8, 8, 64), (1, 1, -64, 8, 8, 64)):
         with pytest.raises(RuntimeError, match='bad sizes'):
             K.attention_workspace(*bad)
+
+
+def test_oracle_attention_of_nan_scores_is_nan():
+    r = np.random.default_rng(3)
+    q, k, v = r.standard_normal((3, 4, 8)), r.standard_normal((5, 2, 8)), r.standard_normal((5, 2, 8))
+    want = O.attention(q, k, v)[0]
+    q[1, 2, 0], k[4, 0, 3] = np.nan, np.nan              # one query row; one key, which the last query alone sees
+    out = O.attention(q, k, v)[0]
+    nan = np.zeros((3, 4), bool)
+    nan[1, 2], nan[2, :2] = True, True
+    assert np.isnan(out[nan]).all() and np.array_equal(out[~nan], want[~nan])
