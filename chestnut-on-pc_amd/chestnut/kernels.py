@@ -525,14 +525,21 @@ def _queries(q, cu_q, kv, hd, out, scale):
     return T, H, cu_q.shape[0] - 1, qs, os, scale
 
 
-@functools.lru_cache(maxsize=256)
-def attention_workspace(B, Tq, keys, n_heads, n_kv, head_dim):
-    """Bytes of workspace (0: none) of attention_varlen (keys = Tk) and
-    attention_paged (keys = B * table width * page) for B sequences of Tq
-    queries in all."""
+def _attention_bytes(B, Tq, keys, n_heads, n_kv, head_dim):
     nb = ctypes.c_size_t()
     check(lib().ck_attention_workspace(B, Tq, keys, n_heads, n_kv, head_dim, ctypes.byref(nb)))
     return nb.value
+
+
+_cached_attention_bytes = functools.lru_cache(maxsize=256)(_attention_bytes)
+
+
+def attention_workspace(B, Tq, keys, n_heads, n_kv, head_dim):
+    """Bytes of workspace (0: none) of attention_varlen (keys = Tk) and
+    attention_paged (keys = B * table width * page) for B sequences of Tq
+    queries in all.  Remembered for plain integers only, as gemm_workspace."""
+    ints = type(B) is type(Tq) is type(keys) is type(n_heads) is type(n_kv) is type(head_dim) is int
+    return (_cached_attention_bytes if ints else _attention_bytes)(B, Tq, keys, n_heads, n_kv, head_dim)
 
 
 def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None, workspace=None):
@@ -562,7 +569,7 @@ def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None
         _is(cu_k, torch.int32, 'cu_k', (B + 1,))
     dev = _on_device('q k v cu_q cu_k out', q, k, v, cu_q, cu_k, out)
     o = out if out is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    nb = attention_workspace(B, T, Tk, H, kv, hd)
+    nb = _cached_attention_bytes(B, T, Tk, H, kv, hd)
     ws = _workspace(workspace, nb, q.device)
     check(lib().ck_attention_varlen(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu_q.data_ptr(),
                                     cu_k.data_ptr(), B, T, Tk, H, kv, hd, qt, qh, kt, kh, vt, vh, ot, oh,
@@ -592,7 +599,7 @@ def attention_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, k_scale=Non
     dev = _on_device('q k_pages v_pages block_table cu_q kv_lens k_scale v_scale out', q, k_pages, v_pages, block_table,
                      cu_q, kv_lens, k_scale, v_scale, out)
     o = out if out is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    nb = attention_workspace(B, T, B * width * page, H, kv, hd)
+    nb = _cached_attention_bytes(B, T, B * width * page, H, kv, hd)
     ws = _workspace(workspace, nb, q.device)
     check(lib().ck_attention_paged(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale),
                                    o.data_ptr(), block_table.data_ptr(), width, cu_q.data_ptr(), kv_lens.data_ptr(), B,

@@ -237,3 +237,16 @@ def test_oracle_attention_of_nan_scores_is_nan():
     nan = np.zeros((3, 4), bool)
     nan[1, 2], nan[2, :2] = True, True
     assert np.isnan(out[nan]).all() and np.array_equal(out[~nan], want[~nan])
+
+
+def test_attention_workspace_remembers_plain_integers_only():
+    t = torch.tensor(1)
+    assert K.attention_workspace(t, 200, 6400, 8, 8, 64) == K.attention_workspace(1, 200, 6400, 8, 8, 64) > 0
+    t.fill_(200)
+    assert K.attention_workspace(t, 200, 6400, 8, 8, 64) == K.attention_workspace(200, 200, 6400, 8, 8, 64) == 0
+    for at in range(6):
+        args = [3, 200, 6400, 8, 8, 64]
+        K.attention_workspace(*args)
+        args[at] = float(args[at])
+        with pytest.raises(ctypes.ArgumentError):
+            K.attention_workspace(*args)
