@@ -132,11 +132,14 @@ __device__ __forceinline__ bool find_item(const AttendParams& p, int index, Item
   int c = 1 << 30;
   if (p.target) {
     float work = readlane_f32(lanes_scan((float)tiles * (float)blocks), 63);
-    int all = lane63(lanes_scan(tiles));
+    // (offsets that do not ascend may name 2^26 tiles of few rows or 2^30 of 128 in 64 sequences, and more
+    // than an int holds in all; past 2^29 the number itself does not count)
+    constexpr int MOST = 1 << 29;
+    int all = min(lane63(lanes_scan(tiles)), MOST);
     for (int b0 = 64; b0 < p.B; b0 += 64) {
       get(b0);
       work += readlane_f32(lanes_scan((float)tiles * (float)blocks), 63);
-      all += lane63(lanes_scan(tiles));
+      all = min(all + lane63(lanes_scan(tiles)), MOST);
     }
     // each tile adds up to one item that is not full
     const int full = max(p.target - all, (p.target + 1) >> 1);

@@ -695,3 +695,20 @@ def test_a_nan_query_gives_a_nan_row(gpu, n, m, hd, dt, cache, causal):
     assert torch.isnan(out[n // 2, 1]).all()
     out[n // 2, 1] = torch.from_numpy(ref[n // 2, 1]).to(out)
     near(out, ref, mag, most, m, hd, dt)
+
+
+def test_offsets_that_name_more_tiles_than_32_bits_hold(gpu):
+    """66000 sequences of which every other is all of the queries, 66000 tiles of 16 rows: over 2^31 in all.  All
+    compute the same rows, so that the output is that of one.  (k and v are one row repeated, of which 640 are used,
+    so that the keys seem many enough to be split.)"""
+    from chestnut import kernels as K
+    B = T = 66000
+    q = rows(1, T, 16, 64, 'f16')
+    k, v = (rows(s, 1, 1, 64, 'f16').expand(300 * B, 1, 64) for s in (2, 3))
+    assert K.attention_workspace(B, T, 300 * B, 16, 1, 64) > 0
+    ends = np.arange(B + 1) % 2
+    out = torch.full((T + 2, 16, 64), 9.0, dtype=torch.float16, device='cuda')
+    K.attention_varlen(q, k, v, i32(ends * T), i32(ends * 640), causal=False, out=out[1:T + 1])
+    want = v[:1].double()
+    assert ((out[1:T + 1].double() - want).abs() <= 2 * u('f16') * want.abs()).all()   # equal weights: one rounding
+    assert (out[0] == 9.0).all() and (out[T + 1] == 9.0).all()
