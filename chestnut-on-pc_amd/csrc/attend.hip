@@ -130,7 +130,7 @@ __device__ __forceinline__ bool find_item(const AttendParams& p, int index, Item
   };
   get(0);
   int c = 1 << 30;
-  if (p.target) {
+  if (BM <= 128 && p.target) {   // tiles of 256 keep their keys whole
     float work = readlane_f32(lanes_scan((float)tiles * (float)blocks), 63);
     // (offsets that do not ascend may name 2^26 tiles of few rows or 2^30 of 128 in 64 sequences, and more
     // than an int holds in all; past 2^29 the number itself does not count)
@@ -825,6 +825,7 @@ __device__ __forceinline__ float2_t* part_ml(const AttendParams& p, long row) {
 template <typename T, int HD, int KV, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendParams p) {
   constexpr int BM = 32 * NW, TILE = AT_KEYS * HD, NT = 64 * NW;
+  constexpr bool SPLIT = NW == 4;   // a tile's keys may be split over workgroups
   constexpr bool DMA = KV != KV_E4M3;
   // one array: with several, the compiler holds every read of one back until all loads to the
   // others have landed
@@ -841,8 +842,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
   // the keys of the tile's first and last rows, and of this chunk
   const int klo = keys_of(p, it.s, tile * BM / p.G);
   const int khi = keys_of(p, it.s, min(it.s.nq - 1, (tile * BM + BM - 1) / p.G));
-  const int kbeg = it.nch > 1 ? it.chunk * it.c * AT_KEYS : 0;
-  const int kend = it.nch > 1 ? min(khi, kbeg + it.c * AT_KEYS) : khi;
+  const int kbeg = SPLIT && it.nch > 1 ? it.chunk * it.c * AT_KEYS : 0;
+  const int kend = SPLIT && it.nch > 1 ? min(khi, kbeg + it.c * AT_KEYS) : khi;
 
   Stage<T, HD, KV, AT_KEYS, NT, false> ks;
   Stage<T, HD, KV, AT_KEYS, NT, true> vs;
@@ -951,7 +952,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
   }
   wait_vm_lgkm0<0>();   // the loads past the last tile land before this workgroup's LDS is another's
 
-  if (it.nch == 1) {
+  if (!SPLIT || it.nch == 1) {
     r.finish(p, it, hk, lane);
     return;
   }
@@ -1181,17 +1182,17 @@ Plan plan_of(int B, int Tq, long keys, int n_heads, int n_kv, bool few3 = false)
   // 80 us against 82 (512 tokens on 12800 keys) and 81 against 77 (eight mixed chunks).
   pl.bm = rows <= 16L * B ? 16 : rows <= 32L * B ? 32 : (rows / 256 + B) * n_kv >= 512 ? 256 : 128;
   pl.tiles = rows / pl.bm + B;       // sum of ceil(rows_b / bm) is at most this
-  // items to aim at: workgroups that run at once, one a CU or two (tiles of 128, three, four, six
+  // items to aim at: workgroups that run at once, two a CU (tiles of 128, three, four, six
   // a CU in place of two: 512 tokens on 12800 keys 99, 104, 119 for 86 us); of few rows twice as
   // many, as their chunks come out uneven (32 ragged histories 127 -> 122 us; three times 125),
   // or as many where three run on a CU (768 items 110 us, 1024 136, 1536 113; where two do, 16 of
   // the histories, 768 110 and 1024 104)
-  const long slots = pl.bm == 256 ? 256 : pl.bm == 128 ? 512 : pl.bm == 16 && few3 ? 768 : 1024;
+  const long slots = pl.bm == 128 ? 512 : pl.bm == 16 && few3 ? 768 : 1024;
   pl.min_blocks = pl.bm <= 32 ? 2 : 4;
   // keys stay whole where the tiles fill the card twice, or the sequences have too few to pay for
   // the second launch (prompts of 548, 652 and less, 128 features, split 31 us, whole 20; one of
   // 1031 with two short ones 20 and 26, but the host knows the average only)
-  const bool many = pl.bm > 32 && pl.tiles * n_kv >= 2 * slots;
+  const bool many = pl.bm == 256 || (pl.bm == 128 && pl.tiles * n_kv >= 2 * slots);
   if (!many && keys / B > 2 * pl.min_blocks * AT_KEYS) pl.target = (int)std::max(1L, slots / n_kv);
   pl.items = pl.tiles + pl.target;
   return pl;
@@ -1208,8 +1209,7 @@ void launch_kv(const AttendParams& p, const Plan& pl, hipStream_t s) {
   const unsigned tiles = (unsigned)(pl.tiles * p.Hkv);
   if (pl.bm == 16) CK_LAUNCH((attend_join_kernel<T, HD, KV, 16>), dim3(tiles, 16), dim3(256), 0, s, p);
   else if (pl.bm == 32) CK_LAUNCH((attend_join_kernel<T, HD, KV, 32>), dim3(tiles, 32), dim3(256), 0, s, p);
-  else if (pl.bm == 128) CK_LAUNCH((attend_join_kernel<T, HD, KV, 128>), dim3(tiles, 128 / (1024 / HD)), dim3(256), 0, s, p);
-  else CK_LAUNCH((attend_join_kernel<T, HD, KV, 256>), dim3(tiles, 256 / (1024 / HD)), dim3(256), 0, s, p);
+  else CK_LAUNCH((attend_join_kernel<T, HD, KV, 128>), dim3(tiles, 128 / (1024 / HD)), dim3(256), 0, s, p);
 }
 template <typename T, int HD>
 void launch_hd(const AttendParams& p, int kv, const Plan& pl, hipStream_t s) {

@@ -712,3 +712,24 @@ def test_offsets_that_name_more_tiles_than_32_bits_hold(gpu):
     want = v[:1].double()
     assert ((out[1:T + 1].double() - want).abs() <= 2 * u('f16') * want.abs()).all()   # equal weights: one rounding
     assert (out[0] == 9.0).all() and (out[T + 1] == 9.0).all()
+
+
+# ------------------------------------------------------------------ forms by size --
+@pytest.mark.parametrize('hd', [64, 128])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('quant', [False, True])
+@pytest.mark.parametrize('causal', [True, False])
+def test_long_chunks_over_pages(gpu, hd, dt, quant, causal):
+    """Enough rows for tiles of 256 over pages: (4101 * 4 / 256 + 2) * 8 of them."""
+    from chestnut import kernels as K
+    qlens, klens, H, kv, page = [3001, 1100], [3078, 2001], 32, 8, 32
+    assert K.attention_workspace(2, sum(qlens), 2 * 99 * page, H, kv, hd) == 0
+    table, n = tables(klens, page, 5)
+    kp, vp, ks, vs = filled(n, kv, page, hd, dt, 'e4m3' if quant else dt, 6)
+    q = rows(8, sum(qlens), H, hd, dt)
+    out = K.attention_paged(q, kp, vp, i32(table), cu(qlens), i32(klens), k_scale=ks, v_scale=vs, causal=causal)
+    a = 0
+    for b, (x, m) in enumerate(zip(qlens, klens)):
+        k, v = (torch.from_numpy(gathered(p, s, table[b], m, page)).cuda() for p, s in ((kp, ks), (vp, vs)))
+        near(out[a:a + x], *attention_on_gpu(q[a:a + x], k, v, causal), m, hd, dt, f'{x} over {m}')
+        a += x

@@ -250,3 +250,12 @@ def test_attention_workspace_remembers_plain_integers_only():
         args[at] = float(args[at])
         with pytest.raises(ctypes.ArgumentError):
             K.attention_workspace(*args)
+
+
+def test_tiles_of_256_rows_keep_their_keys_whole():
+    for B in (1, 2, 7, 40):
+        for T in (1000, 4101, 8192, 100000):
+            for H, kv in ((32, 8), (16, 16), (64, 1)):
+                if T * H // kv > 32 * B and (T * (H // kv) // 256 + B) * kv >= 512:
+                    assert K.attention_workspace(B, T, 1 << 24, H, kv, 128) == 0
+    assert K.attention_workspace(2, 1000, 1 << 24, 32, 8, 128) > 0
