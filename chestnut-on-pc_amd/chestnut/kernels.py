@@ -286,7 +286,8 @@ def warp_nv12(frame, big_frame, tfm, big_tfm, cam_w, cam_h, stride, y_height, mo
 # ------------------------------------------------------------ the token cache --
 # K and V rows of past tokens in pages k_pages, v_pages [n_pages, n_kv, page, head_dim] (page a
 # power of two, 16 to 1024): f16, bf16, or float8_e4m3fn with k_scale, v_scale [n_pages, n_kv, page]
-# of float8_e8m0fnu, a power of two a row (cache_write leaves 2^-126 to 2^120; 2^-127 reads as 0).
+# of float8_e8m0fnu, a power of two a row (cache_write leaves 2^-126 to 2^120; a row whose scale is
+# that type's NaN is NaN).
 # A slot is page index * page + place.
 #
 # Index tensors are int32 on the device; their values are not checked here (that would wait for

@@ -160,7 +160,9 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const ReadParams p) {
         y = *reinterpret_cast<const v8*>(static_cast<const T*>(isv ? p.vp : p.kp) + row * p.hd + c * 8);
       } else {
         const u32x2_t w = *reinterpret_cast<const u32x2_t*>(static_cast<const uint8_t*>(isv ? p.vp : p.kp) + row * p.hd + c * 8);
-        const float s = __builtin_bit_cast(float, (unsigned)(isv ? p.vs : p.ks)[row] << 23);
+        // 2^(byte - 127); of the type's ends, 0 is the f32 subnormal 2^-127 and 255 is NaN
+        const unsigned byte = (isv ? p.vs : p.ks)[row];
+        const float s = __builtin_bit_cast(float, byte << 23 | (((byte + 1) & 255) < 2 ? 0x400000u : 0u));
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int u = w[j];

@@ -328,8 +328,8 @@ int ck_rope(const void* x, void* out, const int32_t* positions, const double* in
 /* A cache: k_pages, v_pages [n_pages][n_kv][page][head_dim], 16-byte
  * aligned; page a power of two from 16 to 1024, head_dim a multiple of 8 up
  * to 256, n_pages * page < 2^31.  cache_dtype e4m3: k_scale, v_scale
- * [n_pages][n_kv][page] hold each row's scale 2^(byte - 127), byte 1 to 254;
- * a value is code * scale.  Other cache types: the scales are NULL.
+ * [n_pages][n_kv][page] hold each row's scale 2^(byte - 127), byte 0 to 254
+ * (cache_write leaves 1 to 247; 255 makes the row NaN); a value is code * scale.  Other cache types: the scales are NULL.
  *
  * ck_cache_write: row t of k and v to slot slots[t] = page index * page +
  * place; negative slots are not written, slots must differ.  e4m3: the scale

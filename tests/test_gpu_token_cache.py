@@ -733,3 +733,25 @@ def test_long_chunks_over_pages(gpu, hd, dt, quant, causal):
         k, v = (torch.from_numpy(gathered(p, s, table[b], m, page)).cuda() for p, s in ((kp, ks), (vp, vs)))
         near(out[a:a + x], *attention_on_gpu(q[a:a + x], k, v, causal), m, hd, dt, f'{x} over {m}')
         a += x
+
+
+@pytest.mark.parametrize('byte', [0, 1, 127, 247, 254, 255])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('n', [1, 70])
+def test_scales_at_the_ends_of_their_type(gpu, byte, dt, n):
+    """A code times its scale as the two types have them (255 is NaN), read back and, being the only key's V, attended."""
+    from chestnut import kernels as K
+    codes = torch.arange(256, dtype=torch.uint8, device='cuda').view(4, 64)[None, :, None].expand(1, 4, 16, 64).contiguous()
+    kp, vp = torch.zeros_like(codes).view(torch.float8_e4m3fn), codes.view(torch.float8_e4m3fn)
+    ks, vs = (torch.full((1, 4, 16), b, dtype=torch.uint8, device='cuda').view(torch.float8_e8m0fnu) for b in (127, byte))
+    with np.errstate(invalid='ignore', over='ignore'):
+        want = torch.from_numpy(O.e4m3_values() * (np.nan if byte == 255 else 2.0 ** (byte - 127))).to(DT[dt]).view(4, 64)
+    _, v = K.cache_read(kp, vp, i32([[0]]), cu([1]), 1, k_scale=ks, v_scale=vs, dtype=DT[dt])
+    out = K.attention_paged(rows(1, n, 4, 64, dt), kp, vp, i32([[0]]), cu([n]), i32([1]), k_scale=ks, v_scale=vs, causal=False)
+    # below the smallest normal number of bf16 a value may be a subnormal or zero
+    small = 2.0 ** -126 if dt == 'bf16' else 0.0
+    for got in [v[0]] + list(out):
+        got = got.cpu()
+        nan = torch.isnan(want)
+        assert torch.equal(torch.isnan(got), nan)
+        assert torch.equal(got[~nan], want[~nan]) if not small else ((got == want) | nan | (want.abs() < small) & (got.abs() < small)).all()
