@@ -295,6 +295,7 @@ def warp_nv12(frame, big_frame, tfm, big_tfm, cam_w, cam_h, stride, y_height, mo
 
 _F16, _BF16, _E4M3, _E8M0 = torch.float16, torch.bfloat16, torch.float8_e4m3fn, torch.float8_e8m0fnu
 _DTYPE = {_F16: 1, _BF16: 4, _E4M3: 5}   # the codes of include/chestnut.h
+_INT = 2 ** 31 - 1   # counts reach the library as C ints, to which ctypes would cut larger ones
 
 
 def _rows(t, dtype, name, shape, unit=8, write=False):
@@ -308,6 +309,8 @@ def _rows(t, dtype, name, shape, unit=8, write=False):
     T, H, hd = shape
     if t.shape != shape:
         raise ValueError(f'{name} must have shape {(T, H, hd)}, got {tuple(t.shape)}')
+    if T > _INT:
+        raise ValueError(f'{name} must have under 2^31 rows, got {T}')
     s0, s1, s2 = t.stride()
     if s2 != 1 and hd > 1:
         raise ValueError(f'{name} must be contiguous in its last dimension')
@@ -486,10 +489,12 @@ def cache_read(k_pages, v_pages, block_table, cu_seqlens, tokens, k_scale=None, 
         dtype = k_out.dtype if k_out is not None else k_pages.dtype
     if dtype not in (_F16, _BF16) or k_pages.dtype not in (dtype, _E4M3):
         raise ValueError(f'dtype must be float16 or bfloat16, and that of the cache ({k_pages.dtype}) unless it is e4m3')
-    if not isinstance(tokens, int) or tokens < 0:
-        raise ValueError('tokens must be the number of rows')
+    if not isinstance(tokens, int) or not 0 <= tokens <= _INT:
+        raise ValueError('tokens must be the number of rows, under 2^31')
     _check(block_table, torch.int32, 'block_table', (None, None))
     B, width = block_table.shape
+    if B > _INT or width > _INT:
+        raise ValueError(f'block_table must have under 2^31 rows and columns, got {(B, width)}')
     _is(cu_seqlens, torch.int32, 'cu_seqlens', (B + 1,))
     for t, name in ((k_out, 'k_out'), (v_out, 'v_out')):
         if t is not None:
@@ -516,8 +521,8 @@ def _queries(q, cu_q, kv, hd, out, scale):
         raise ValueError(f'the query heads ({H}, up to 1024) must be a multiple of the K/V heads ({kv})')
     if type(cu_q) is not torch.Tensor or cu_q.dtype is not torch.int32 or cu_q.dim() != 1 or not cu_q.is_contiguous():
         _check(cu_q, torch.int32, 'cu_q', (None,))
-    if cu_q.shape[0] < 1:
-        raise ValueError('cu_q must hold B + 1 offsets')
+    if not 1 <= cu_q.shape[0] <= _INT:
+        raise ValueError('cu_q must hold B + 1 offsets, under 2^31')
     qs = _rows(q, q.dtype, 'q', q.shape)
     os = (H * d, d) if out is None else _rows(out, q.dtype, 'out', q.shape, 4, True)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
@@ -540,6 +545,8 @@ def attention_workspace(B, Tq, keys, n_heads, n_kv, head_dim):
     attention_paged (keys = B * table width * page) for B sequences of Tq
     queries in all.  Remembered for plain integers only, as gemm_workspace."""
     ints = type(B) is type(Tq) is type(keys) is type(n_heads) is type(n_kv) is type(head_dim) is int
+    if any(abs(n) > _INT for n in (B, Tq, n_heads, n_kv, head_dim)) or abs(keys) >= 2 ** 63:
+        raise ValueError('counts must be under 2^31, and keys under 2^63')
     return (_cached_attention_bytes if ints else _attention_bytes)(B, Tq, keys, n_heads, n_kv, head_dim)
 
 

@@ -259,3 +259,34 @@ def test_tiles_of_256_rows_keep_their_keys_whole():
                 if T * H // kv > 32 * B and (T * (H // kv) // 256 + B) * kv >= 512:
                     assert K.attention_workspace(B, T, 1 << 24, H, kv, 128) == 0
     assert K.attention_workspace(2, 1000, 1 << 24, 32, 8, 128) > 0
+
+
+def many(n, *shape, dtype=f16):
+    """n rows that take no memory."""
+    return torch.empty(1, *shape, dtype=dtype, device='meta').expand(n, *shape)
+
+
+def ints(*shape):
+    return torch.empty(*shape, dtype=i32, device='meta')
+
+
+N = 2 ** 32 + 4                       # 4 if it is cut to 32 bits
+PAST_32_BITS = [
+    ('rope tokens', lambda: K.rope(many(N, 2, 64), ints(N), F)),
+    ('write tokens', lambda: K.cache_write(many(N, 2, 64), many(N, 2, 64), *cache(), ints(N))),
+    ('read tokens', lambda: K.cache_read(*cache(), z(2, 3, dtype=i32), z(3, dtype=i32), N)),
+    ('read table width', lambda: K.cache_read(*cache(), ints(2, N), z(3, dtype=i32), 4)),
+    ('read sequences', lambda: K.cache_read(*cache(), ints(N, 3), ints(N + 1), 4)),
+    ('varlen queries', lambda: varlen(many(N, 4, 64), many(N, 2, 64), many(N, 2, 64))),
+    ('varlen keys', lambda: varlen(k=many(N, 2, 64), v=many(N, 2, 64), cu_k=z(3, dtype=i32))),
+    ('varlen sequences', lambda: varlen(cu=ints(N + 1))),
+    ('paged sequences', lambda: paged(table=ints(N, 3), cu=ints(N + 1), lens=ints(N))),
+    ('workspace', lambda: K.attention_workspace(N, N, 64, 8, 8, 64)),
+    ('workspace keys', lambda: K.attention_workspace(1, 1, 2 ** 64 + 1, 8, 8, 64)),
+]
+
+
+@pytest.mark.parametrize('name,fn', PAST_32_BITS, ids=[r[0] for r in PAST_32_BITS])
+def test_counts_past_32_bits_are_refused(name, fn):
+    with pytest.raises(ValueError, match='under 2\\^31'):
+        fn()
