@@ -526,8 +526,8 @@ def _queries(q, cu_q, kv, hd, out, scale):
     qs = _rows(q, q.dtype, 'q', q.shape)
     os = (H * d, d) if out is None else _rows(out, q.dtype, 'out', q.shape, 4, True)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError('scale must be positive and finite')
+    if not 2.0 ** -149 <= scale < 2e38:   # of an f32, and log2(e) times it too
+        raise ValueError(f'scale must be positive and finite, from 2^-149 to 2e38, got {scale}')
     return T, H, cu_q.shape[0] - 1, qs, os, scale
 
 

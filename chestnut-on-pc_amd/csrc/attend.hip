@@ -1225,7 +1225,8 @@ void launch_attend(const char* what, AttendParams& p, const AttendQuery& a, int 
   CK_REQUIRE(a.n_heads > 0 && p.Hkv > 0 && a.n_heads % p.Hkv == 0 && a.n_heads <= 1024,
              w + ": query heads (up to 1024) must be a multiple of the K/V heads");
   CK_REQUIRE(a.T >= 0 && a.B >= 0 && (long)a.T * a.n_heads < (1L << 31) && a.B < (1 << 20), w + ": bad sizes");
-  CK_REQUIRE(a.scale > 0.f && a.scale < INFINITY, w + ": scale must be positive and finite");
+  // (the exponents are of 2: past 2.3e38 their factor is infinite)
+  CK_REQUIRE(a.scale > 0.f && a.scale * AT_LOG2E < INFINITY, w + ": scale must be positive and finite, and under 2e38");
   if (a.T == 0 || a.B == 0) return;
   CK_REQUIRE(a.q && a.out && a.cu_q && p.kv, w + ": null pointer");
   // a lane's bytes from its wave's first row are counted in 32 bits

@@ -359,7 +359,7 @@ int ck_attention_workspace(int B, int Tq, long keys, int n_heads, int n_kv, int 
  * causal: query i of n over m keys sees keys j <= i + m - n, else all.  A
  * query that sees none gets zeros; what a query does not see (infinities and
  * NaN included) does not reach it.  Query head h reads K/V head
- * h / (n_heads / n_kv).  head_dim 64 or 128, scale > 0, f16 or bf16;
+ * h / (n_heads / n_kv).  head_dim 64 or 128, 0 < scale < 2e38, f16 or bf16;
  * q, k, v rows 16-byte aligned, out rows 8-byte aligned and apart from k and v; k_st, v_st < 2^24,
  * at most 2^30 keys a sequence, B < 2^20, Tq * n_heads < 2^31 and fewer than
  * 2^24 workgroups (B * n_kv at least).  The workspace belongs to the call until it has run:

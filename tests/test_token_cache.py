@@ -290,3 +290,11 @@ PAST_32_BITS = [
 def test_counts_past_32_bits_are_refused(name, fn):
     with pytest.raises(ValueError, match='under 2\\^31'):
         fn()
+
+
+@pytest.mark.parametrize('scale', [1e-50, 2.5e38, 1e39, math.inf])
+def test_scales_that_f32_does_not_hold_are_refused(scale):
+    with pytest.raises(ValueError, match='scale must be positive and finite'):
+        varlen(scale=scale)
+    with pytest.raises(RuntimeError, match='positive and finite'):
+        _lib.call(*attn(scale=scale))
