@@ -483,7 +483,8 @@ def cache_read(k_pages, v_pages, block_table, cu_seqlens, tokens, k_scale=None, 
     """(k, v) [tokens, n_kv, head_dim]: the first cu_seqlens[b+1] - cu_seqlens[b]
     places of every sequence b, whose pages are block_table[b] (int32 [B,
     width]), at rows cu_seqlens[b]...  dtype: float16 or bfloat16 for an e4m3
-    cache, else the cache's own.  Rows behind the last sequence are not written."""
+    cache (whose values above 65504, of rows that were bfloat16, are infinite in
+    float16), else the cache's own.  Rows behind the last sequence are not written."""
     n, kv, page, hd = _cache(k_pages, v_pages, k_scale, v_scale)
     if dtype is None:
         dtype = k_out.dtype if k_out is not None else k_pages.dtype
@@ -592,7 +593,8 @@ def attention_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, k_scale=Non
     cu_q[b+1] (int32 [B+1]), its kv_lens[b] keys (int32 [B]) at places 0.. of the
     pages block_table[b] (int32 [B, width]); the queries are the last of them
     (causal: query i of n sees the keys j <= i + kv_lens[b] - n; else all).  The
-    cache has q's type or is e4m3.  Otherwise as attention_varlen."""
+    cache has q's type or is e4m3, whose values are rounded to q's type as cache_read
+    rounds them (past float16's range: infinite).  Otherwise as attention_varlen."""
     n, kv, page, hd = _cache(k_pages, v_pages, k_scale, v_scale)
     T, H, B, (qt, qh), (ot, oh), scale = _queries(q, cu_q, kv, hd, out, scale)
     if k_pages.dtype not in (q.dtype, _E4M3):

@@ -344,7 +344,8 @@ int ck_cache_write(const void* k, const void* v, void* k_pages, void* v_pages, v
 /* The first cu[b+1] - cu[b] places of each sequence (pages block_table[b][..],
  * int32 [B][table_width]) to rows cu[b].. of k and v [tokens][n_kv][head_dim]
  * (contiguous, dtype f16 or bf16; the cache's own type unless that is e4m3),
- * tokens < 2^28. */
+ * tokens < 2^28.  e4m3: a value is rounded once to dtype, so that above 65504
+ * in f16 (the rows were bf16, or the scales are the caller's) it is infinite. */
 int ck_cache_read(const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale,
                   const int32_t* block_table, int table_width, const int32_t* cu_seqlens, int B, int tokens,
                   int n_pages, int n_kv, int page, int head_dim, void* k, void* v, int dtype, int cache_dtype,
@@ -370,7 +371,8 @@ int ck_attention_varlen(const void* q, const void* k, const void* v, void* out, 
                         int causal, float scale, void* workspace, size_t ws_bytes, void* stream);
 
 /* The same over a paged cache: sequence b has kv_lens[b] keys, at places
- * 0 .. of its pages block_table[b][..]; its queries are the last of them. */
+ * 0 .. of its pages block_table[b][..]; its queries are the last of them.
+ * e4m3: the values are rounded to dtype first, as ck_cache_read does. */
 int ck_attention_paged(const void* q, const void* k_pages, const void* v_pages, const void* k_scale,
                        const void* v_scale, void* out, const int32_t* block_table, int table_width,
                        const int32_t* cu_q, const int32_t* kv_lens, int B, int Tq, int n_heads, int n_pages, int n_kv,

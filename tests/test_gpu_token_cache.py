@@ -755,3 +755,19 @@ def test_scales_at_the_ends_of_their_type(gpu, byte, dt, n):
         nan = torch.isnan(want)
         assert torch.equal(torch.isnan(got), nan)
         assert torch.equal(got[~nan], want[~nan]) if not small else ((got == want) | nan | (want.abs() < small) & (got.abs() < small)).all()
+
+
+@pytest.mark.parametrize('n', [1, 70])
+def test_rows_of_bf16_past_the_range_of_f16(gpu, n):
+    """Cached as e4m3 they read and attend as they are in bf16, as infinities in f16."""
+    from chestnut import kernels as K
+    x = rows(1, 16, 2, 64, 'bf16').clamp(-3, 3)
+    x[:, :, ::2] = 2.0 ** 20
+    kp, vp, ks, vs = pages_of(1, 2, 16, 64, 'bf16', 'e4m3')
+    K.cache_write(torch.zeros_like(x), x, kp, vp, i32(np.arange(16)), k_scale=ks, v_scale=vs)
+    for dt in ('bf16', 'f16'):
+        _, v = K.cache_read(kp, vp, i32([[0]]), cu([16]), 16, k_scale=ks, v_scale=vs, dtype=DT[dt])
+        out = K.attention_paged(rows(2, n, 2, 64, dt), kp, vp, i32([[0]]), cu([n]), i32([16]), k_scale=ks, v_scale=vs, causal=False)
+        want = 2.0 ** 20 if dt == 'bf16' else float('inf')
+        assert (v[..., ::2] == want).all() and (out[..., ::2] == want).all()
+        assert torch.isfinite(v[..., 1::2]).all() and torch.isfinite(out[..., 1::2]).all()
