@@ -558,7 +558,8 @@ def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None
     cu_k None: the same).  causal: query i of n over m keys sees the keys
     j <= i + m - n; else all.  heads a multiple of n_kv, head_dim 64 or 128,
     scale 1/sqrt(head_dim) unless given.  A query without a key gets zeros; rows
-    behind the last sequence are not written.  out must not overlap k or v.
+    behind the last sequence are not written.  out may be q itself, and must not
+    overlap q, k or v otherwise.
     workspace: a buffer to keep, of at least attention_workspace bytes (else a new
     one is made); one for each call that may run beside another, and for each
     captured graph."""

@@ -361,7 +361,8 @@ int ck_attention_workspace(int B, int Tq, long keys, int n_heads, int n_kv, int 
  * query that sees none gets zeros; what a query does not see (infinities and
  * NaN included) does not reach it.  Query head h reads K/V head
  * h / (n_heads / n_kv).  head_dim 64 or 128, 0 < scale < 2e38, f16 or bf16;
- * q, k, v rows 16-byte aligned, out rows 8-byte aligned and apart from k and v; k_st, v_st < 2^24,
+ * q, k, v rows 16-byte aligned, out rows 8-byte aligned; out may be q (with its strides) and is
+ * else apart from q, k and v; k_st, v_st < 2^24,
  * at most 2^30 keys a sequence, B < 2^20, Tq * n_heads < 2^31 and fewer than
  * 2^24 workgroups (B * n_kv at least).  The workspace belongs to the call until it has run:
  * calls that may overlap, and graphs that may, need one each. */

@@ -771,3 +771,94 @@ def test_rows_of_bf16_past_the_range_of_f16(gpu, n):
         want = 2.0 ** 20 if dt == 'bf16' else float('inf')
         assert (v[..., ::2] == want).all() and (out[..., ::2] == want).all()
         assert torch.isfinite(v[..., 1::2]).all() and torch.isfinite(out[..., 1::2]).all()
+
+
+@pytest.mark.parametrize('inter', [False, True])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+def test_rope_of_an_output_that_the_caches_do_not_hold(gpu, inter, dt):
+    from chestnut import kernels as K
+    T, H, hd, rot = 6401, 21, 128, 64
+    assert T * H * hd * 2 > 32 << 20
+    x = rows(1, T, H, hd, dt)
+    pos = np.random.default_rng(1).integers(0, 1 << 20, T)
+    f, _ = K.rope_frequencies(rot, base=5e5)
+    out = K.rope(x, i32(pos), f, interleaved=inter)
+    ref = O.rope(f64(x), pos, f64(f), inter)
+    mag = np.abs(f64(x)).max() * 2
+    assert np.all(np.abs(f64(out) - ref) <= u(dt) * np.abs(ref) * (1 + 2.0 ** -6) + 2.0 ** -20 * mag + 2.0 ** -25)
+    assert torch.equal(out[..., rot:], x[..., rot:])
+    assert K.rope(x, i32(pos), f, interleaved=inter, out=x) is x and torch.equal(x, out)
+
+
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('quant', [False, True])
+def test_cache_read_of_an_output_that_the_caches_do_not_hold(gpu, dt, quant):
+    from chestnut import kernels as K
+    lens, kv, hd, page = [5001, 0, 3299], 16, 128, 64
+    assert sum(lens) * kv * hd * 2 > 32 << 20
+    table, n = tables(lens, page, 7)
+    kp, vp, ks, vs = filled(n, kv, page, hd, dt, 'e4m3' if quant else dt, 9)
+    T = sum(lens) + 3
+    ko, vo = (torch.full((T, kv, hd), 5.0, dtype=DT[dt], device='cuda') for _ in 'kv')
+    K.cache_read(kp, vp, i32(table), cu(lens), T, k_scale=ks, v_scale=vs, k_out=ko, v_out=vo)
+    for got, p, s in ((ko, kp, ks), (vo, vp, vs)):
+        want = np.concatenate([gathered(p, s, table[b], m, page) for b, m in enumerate(lens)])
+        assert torch.equal(got[:T - 3].cpu(), torch.from_numpy(want).to(DT[dt])) and (got[T - 3:] == 5.0).all()
+
+
+@pytest.mark.parametrize('qlens,klens,H,kv,hd,page', [([1], [1], 4, 4, 64, 16), ([1, 1, 1, 1], [63, 64, 1025, 0], 8, 2, 128, 32),
+                                                      ([9, 0, 5], [70, 20, 333], 4, 2, 64, 256), ([130, 1, 31], [700, 900, 17], 7, 1, 128, 16),
+                                                      ([200, 100], [4000, 2501], 4, 2, 64, 16), ([200, 100], [4000, 2501], 4, 2, 128, 256),
+                                                      ([3001, 1100], [3001, 1999], 32, 8, 64, 64)])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('quant', [False, True])
+@pytest.mark.parametrize('causal', [True, False])
+def test_places_behind_the_last_key_do_not_count(gpu, qlens, klens, H, kv, hd, page, dt, quant, causal):
+    """NaN (and scale bytes of 255) in every place that holds no key, the pages that no sequence names among them."""
+    from chestnut import kernels as K
+    table, n = tables(klens, page, 5)
+    kp, vp, ks, vs = filled(n, kv, page, hd, dt, 'e4m3' if quant else dt, 6)
+    q = rows(8, sum(qlens), H, hd, dt)
+
+    def attend():
+        return K.attention_paged(q, kp, vp, i32(table), cu(qlens), i32(klens), k_scale=ks, v_scale=vs, causal=causal)
+    want = attend()
+    none = np.ones((n, page), bool)
+    for b, m in enumerate(klens):
+        j = np.arange(m)
+        none[table[b][j // page], j % page] = False
+    none = torch.from_numpy(none).cuda()[:, None].expand(n, kv, page)
+    for p, s in ((kp, ks), (vp, vs)):
+        if quant:
+            p.view(torch.uint8)[none] = 0x7F
+            s.view(torch.uint8)[none] = 255
+        else:
+            p[none] = float('nan')
+    assert torch.isfinite(want).all() and torch.equal(attend(), want)
+
+
+@pytest.mark.parametrize('n,m', [(1, 90), (12, 90), (70, 300)])
+@pytest.mark.parametrize('hd', [64, 128])
+def test_e4m3_rows_below_the_normal_numbers_of_f16(gpu, n, m, hd):
+    """V of about 2^-17, whose values in f16 are subnormal: each is rounded to a multiple of 2^-24 (half a
+    step: 2^-25), and so is the output."""
+    from chestnut import kernels as K
+    table, pages = tables([m], 16, 3)
+    kp, vp, ks, vs = filled(pages, 2, 16, hd, 'f16', 'e4m3', 4)
+    vs.view(torch.uint8).sub_(17)
+    q = rows(1, n, 4, hd, 'f16')
+    out = f64(K.attention_paged(q, kp, vp, i32(table), cu([n]), i32([m]), k_scale=ks, v_scale=vs))
+    k, v = (gathered(p, s, table[0], m, 16) for p, s in ((kp, ks), (vp, vs)))
+    assert np.abs(v).max() < 2.0 ** -14 and np.abs(v).mean() > 2.0 ** -19
+    ref, mag, most = O.attention(f64(q), k, v)
+    tol = u('f16') * mag * (1 + 2.0 ** -6) + (2 * (hd + 4) * 2.0 ** -24 * most + 2.0 ** -17) * mag + 2 * 2.0 ** -25 * (1 + 2.0 ** -6)
+    assert np.all(np.abs(out - ref) <= tol) and np.abs(ref).max() > 2.0 ** -20
+
+
+def test_out_may_be_q(gpu):
+    """Whole keys and split ones, few rows and many."""
+    from chestnut import kernels as K
+    for n, m in ((1, 40), (1, 3000), (12, 2000), (70, 300), (70, 3000), (300, 300)):
+        q, k, v = rows(1, n, 4, 64, 'f16'), rows(2, m, 2, 64, 'f16'), rows(3, m, 2, 64, 'f16')
+        want = K.attention_varlen(q, k, v, cu([n]), cu([m]))
+        assert K.attention_varlen(q, k, v, cu([n]), cu([m]), out=q) is q and torch.equal(q, want)
