@@ -18,7 +18,8 @@
 //
 // Three kernels (their figures stand at each):
 //   attend_tile_kernel  128 or 256 rows, tiles of 64 keys in LDS: prompts and chunks of one;
-//                       bound by the matrix cores beside the vector unit's exponentials;
+//                       bound by the matrix cores, the vector unit's exponentials and the
+//                       tiles' loads, which run side by side in part only;
 //   attend_few_kernel   16 or 32 rows, the keys over four waves: tokens one by one; bound by memory;
 //   attend_join_kernel  joins the parts of rows whose keys were split over workgroups.
 #include <algorithm>
@@ -814,14 +815,17 @@ __device__ __forceinline__ float2_t* part_ml(const AttendParams& p, long row) {
 // and K(j+2) (f16, bf16: straight to LDS; e4m3: through registers, where it is turned into
 // values).
 // 256 rows (two waves a SIMD, one workgroup a CU): prompts of 9001, 5120 and 2263 tokens, 16
-// heads on 4 of 128, bf16, 441 us = 1.04 PFLOP/s, where a product of 8192^3 reaches 1.55; 128
-// rows 508.  Without its loads it takes 392 (less than 471 at the time), without barrier and LDS
-// reads too 369, without the softmax as well 316 = the matrix cores at the clock their power
-// leaves: what bounds it is those two side by side.  Slower were the compiler's own order (sched
-// groups 517-535 against 508), rings of four tiles (467 against 455) and f16 tiles by way of
-// registers (466).  128 rows with the keys split: 512 tokens on 12800 keys, 16 heads of 128,
-// f16, 70 us and 8 to join them, 690 TFLOP/s in all; from an e4m3 cache, eight sequences of 1 to
-// 511 tokens, 75 us = 545.  Short prompts (40 of 1 to 239 tokens, 8 heads of 64) 12.3 us.
+// heads on 4 of 128, bf16, 447 us a call (443 the kernel) = 1.03 PFLOP/s, where a product of
+// 8192^3 reaches 1.55; 128 rows 460.  At 471 us it took 392 without its loads, 369 without
+// barrier and LDS reads as well, 316 without the softmax too = the matrix cores at the clock
+// their power leaves: of the 155 us over those, half are the loads and a third the softmax.
+// Slower were the compiler's own order (sched groups 517-535 against 508 then), rings of four
+// tiles (467 against 455) and f16 tiles by way of registers (466).
+// 128 rows with the keys split: 512 tokens on 12800 keys, 16 heads of 128, f16, 69 us and 8 to
+// join them, 680 TFLOP/s by the call; from an e4m3 cache, eight sequences of 1 to 511 tokens, 65
+// and 10 us, 545 by the call, though with 128 features that kernel spills 43 registers (tiles
+// of 256 rows: 19; without codes to turn into values: 1).  Short prompts (40 of 1 to 239 tokens,
+// 8 heads of 64) 12.4 us.
 template <typename T, int HD, int KV, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendParams p) {
   constexpr int BM = 32 * NW, TILE = AT_KEYS * HD, NT = 64 * NW;
@@ -978,7 +982,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
 // workgroups a CU, 5.9 TB/s, where plain reads of this kind reach 7.1 and the card's copy 4.9;
 // 16 such on 8 heads of 64 84, 64, and 62 with K's next rows sent for before V's are stored.  Two
 // steps ahead are slower: 116 for 115, and 77 for 64.
-// One token on 6144 keys, 8 heads of 64, f16: 6.1 us.
+// One token on 6144 keys, 8 heads of 64, f16: 6.1 to 6.4 us.
 constexpr int FEW_WAVES = 4;
 
 // workgroups a CU
@@ -1089,8 +1093,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES, few_at_once(R::BM, HD, KV == KV_E4M
 
 // ---- the chunks of a tile joined ----------------------------------------------------------
 // HD / 4 lanes a row, RP rows and CG groups of chunks a workgroup of 256.  Its work is small (4
-// to 11 us); a launch of its own, as the last workgroup of a tile doing it needs counters that
-// are zero at the start and stay so where a call is cut short or two replays overlap.
+// to 10 us); a launch of its own, as the last workgroup of a tile doing it needs counters that
+// are zero at the start, and the workspace comes with whatever it held.
 template <typename T, int HD, int KV, int BM>
 __global__ __launch_bounds__(256) void attend_join_kernel(const AttendParams p) {
   constexpr int LPR = HD / 4, CG = BM <= 32 ? 256 / LPR : 1, RP = 256 / LPR / CG;
@@ -1177,8 +1181,8 @@ Plan plan_of(int B, int Tq, long keys, int n_heads, int n_kv, bool few3 = false)
   const int G = n_heads / n_kv;
   const long rows = (long)Tq * G;
   // 16 or 32 rows where a sequence has that many on average: bound by the keys, not by the rows.
-  // 256 rows where they fill the 256 CUs at least twice without splitting keys (prompt of 16384
-  // tokens, 441 us against 508 with 128); with fewer, tiles of 256 with their keys split take
+  // 256 rows where they fill the 256 CUs at least twice without splitting keys (prompts of 16384
+  // tokens, 446 us against 460 with 128); with fewer, tiles of 256 with their keys split take
   // 80 us against 82 (512 tokens on 12800 keys) and 81 against 77 (eight mixed chunks).
   pl.bm = rows <= 16L * B ? 16 : rows <= 32L * B ? 32 : (rows / 256 + B) * n_kv >= 512 ? 256 : 128;
   pl.tiles = rows / pl.bm + B;       // sum of ceil(rows_b / bm) is at most this

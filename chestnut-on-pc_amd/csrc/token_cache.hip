@@ -44,8 +44,8 @@ __device__ __forceinline__ float row_max(float v) {
 
 // LPR lanes a row (those behind its end idle), E elements each, K and V of a row together:
 // four 16-byte loads a thread are under way at once.  12288 tokens of 16 x 128, bf16 to e4m3,
-// 151 MB: 32.4 us = 4.7 TB/s, the card's copy rate (K and V apart, 8 elements a lane: 38); 32
-// tokens of 4 x 128: 3.8 us, a launch.
+// 151 MB: 32.4 us = 4.7 TB/s, the card's copy rate (K and V apart, 8 elements a lane: 38); to
+// bf16, 201 MB: 41.1 us = 4.9 TB/s; 32 tokens of 4 x 128: 3.7 us, a launch.
 template <typename T, bool Q, int E, int LPR>
 __global__ __launch_bounds__(256) void cache_write_kernel(const WriteParams p) {
   typedef typename Elem<T>::v8 v8;
@@ -124,7 +124,8 @@ __device__ __forceinline__ int sequence_of(const int* cu, int B, int t) {
 
 // Eight elements a thread and token (16 leave every other 16 bytes to a second store: 203 against
 // 174 us below).  NT: past the caches, for an output that the L2s do not hold (8 x 4 MiB): 71822
-// tokens of 16 x 128 from e4m3, 885 MB in all, 180 -> 174 us = 5.1 TB/s.
+// tokens of 16 x 128 from e4m3, 885 MB in all, 180 -> 174 us = 5.1 TB/s; from f16, 1177 MB,
+// 248 us = 4.8 TB/s.
 template <typename T, bool Q, bool NT>
 __global__ __launch_bounds__(256) void cache_read_kernel(const ReadParams p) {
   __shared__ long base[READ_TOK];   // page * Hkv * page size + place; -1: no such token
