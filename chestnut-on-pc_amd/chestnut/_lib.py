@@ -70,6 +70,13 @@ _SIGS = {
     'ck_attention': (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     'ck_layernorm': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p]),
     'ck_rope': (c_int, [c_void_p] * 4 + [c_int] * 4 + [c_long] * 4 + [c_int, c_int, c_float, c_int, c_void_p]),
+    'ck_rope_axes': (c_int, [c_void_p] * 3 + [c_int, c_void_p, c_void_p] + [c_int] * 4 + [c_long] * 4 +
+                     [c_int, c_int, c_float, c_int, c_void_p]),
+    'ck_norm_rope': (c_int, [c_void_p] * 7 + [c_int, c_void_p, c_void_p] + [c_int] * 5 + [c_long] * 8 +
+                     [c_int, c_int, c_float, c_int, c_float, c_void_p]),
+    'ck_cache_maps_workspace': (c_int, [c_int, c_int, c_int, P(c_size_t)]),
+    'ck_cache_maps': (c_int, [c_void_p] * 3 + [c_int, c_void_p, c_int, c_void_p] + [c_int] * 3 + [c_void_p] * 6 +
+                      [c_size_t, c_void_p]),
     'ck_cache_write': (c_int, [c_void_p] * 7 + [c_int] * 5 + [c_long] * 4 + [c_int, c_int, c_void_p]),
     'ck_cache_read': (c_int, [c_void_p] * 5 + [c_int, c_void_p] + [c_int] * 6 + [c_void_p, c_void_p, c_int, c_int,
                                                                                  c_void_p]),

@@ -428,34 +428,207 @@ def rope_frequencies(rot, base=10000.0, method='none', factor=1.0, context=None,
     return f.to(device), scale
 
 
-def rope(x, positions, inv_freq, interleaved=False, scale=1.0, inverse=False, out=None):
+def rope_axes(sections, turns=False, device='cuda'):
+    """int32 [sum(sections)] for `rope` and `norm_rope`: every pair's axis, of which
+    axis a has sections[a] pairs -- the axes' sections one after the other, or
+    (turns) an axis after the other while it has pairs left.  With inv_freq =
+    rope_frequencies(2 * sum(sections)) the axes share one ladder of
+    frequencies; torch.cat of one rope_frequencies(2 * n) a section gives each its own."""
+    left = list(sections)
+    if not left or any(not isinstance(n, int) or n < 0 for n in left) or not any(left):
+        raise ValueError('sections must be whole numbers of pairs, one for each axis')
+    out = [] if turns else [a for a, n in enumerate(left) for _ in range(n)]
+    while turns and any(left):
+        for a, n in enumerate(left):
+            if n:
+                out.append(a)
+                left[a] -= 1
+    return torch.tensor(out, dtype=torch.int32, device=device)
+
+
+def _angles(what, positions, inv_freq, axes, T, hd):
+    """The checks of positions, frequencies and axes: (rot, number of axes)."""
+    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dim() != 1:
+        raise ValueError('inv_freq must be float64 [rot/2]')
+    half = inv_freq.shape[0]
+    _check(inv_freq, torch.float64, 'inv_freq')
+    if half < 1 or 2 * half > hd:
+        raise ValueError(f'inv_freq must have 1 to head_dim / 2 = {hd // 2} entries, got {half}')
+    if axes is None:
+        _is(positions, torch.int32, 'positions', (T,))
+        return 2 * half, 1
+    _is(axes, torch.int32, 'axes', (half,))
+    if not isinstance(positions, torch.Tensor) or positions.dim() != 2 or not 1 <= positions.shape[0] <= _INT:
+        raise ValueError(f'positions must be int32 [axes, T] where {what} gets axes')
+    n = positions.shape[0]
+    _is(positions, torch.int32, 'positions', (n, T))
+    return 2 * half, n
+
+
+def rope(x, positions, inv_freq, interleaved=False, scale=1.0, inverse=False, out=None, axes=None):
     """Rotary positions: the first 2 * len(inv_freq) elements of every head of x
     [T, heads, head_dim] (f16 or bf16; token and head strides are free) turned
     by positions[t] * inv_freq[i], pairs (i, i + rot/2) or, interleaved, (2i,
     2i+1), times scale; the rest is copied.  positions int32 [T], inv_freq f64.
-    out: x itself (in place) or rows that do not overlap it."""
+    out: x itself (in place) or rows that do not overlap it.
+    axes (int32 [rot/2], `rope_axes`): positions are int32 [n, T], one row for
+    each of n axes (time, row, column, ...), and pair i goes by positions[axes[i], t];
+    an axis outside 0 .. n - 1 is held to it."""
     if not isinstance(x, torch.Tensor) or x.dim() != 3 or x.dtype not in (_F16, _BF16):
         raise ValueError('x must be float16 or bfloat16 [T, heads, head_dim]')
     T, H, hd = x.shape
-    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dim() != 1:
-        raise ValueError('inv_freq must be float64 [rot/2]')
-    rot = 2 * inv_freq.shape[0]
-    _check(inv_freq, torch.float64, 'inv_freq')
-    if rot < 2 or rot > hd:
-        raise ValueError(f'inv_freq must have 1 to head_dim / 2 = {hd // 2} entries, got {rot // 2}')
+    rot, n = _angles('rope', positions, inv_freq, axes, T, hd)
     if H < 1 or hd > 512 or H > 1024 or H * hd > 65536:
         raise ValueError('rope takes head_dim up to 512, heads up to 1024 and 65536 elements a token')
-    _is(positions, torch.int32, 'positions', (T,))
     st, sh = _rows(x, x.dtype, 'x', x.shape, 1, out is x)
     if out is None:
         ot, oh = H * hd, hd
     else:
         ot, oh = (st, sh) if out is x else _rows(out, x.dtype, 'out', x.shape, 1, True)
-    dev = _on_device('x positions inv_freq out', x, positions, inv_freq, out)
+    dev = _on_device('x positions inv_freq out axes', x, positions, inv_freq, out, axes)
     y = out if out is not None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    check(lib().ck_rope(x.data_ptr(), y.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), T, H, hd, rot, st, sh,
-                        ot, oh, _DTYPE[x.dtype], 1 if interleaved else 0, scale, 1 if inverse else 0, _raw_stream(dev)))
+    check(lib().ck_rope_axes(x.data_ptr(), y.data_ptr(), positions.data_ptr(), n, _ptr(axes), inv_freq.data_ptr(), T, H, hd,
+                             rot, st, sh, ot, oh, _DTYPE[x.dtype], 1 if interleaved else 0, scale, 1 if inverse else 0,
+                             _raw_stream(dev)))
     return y
+
+
+_WEIGHT = {torch.float32: 0, _F16: 1, _BF16: 4}
+
+
+def norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, axes=None, interleaved=False, scale=1.0,
+              q_out=None, k_out=None):
+    """Every head of q [T, heads, head_dim] and k [T, n_kv, head_dim] (f16 or bf16
+    alike; token and head strides are free) divided by sqrt(mean of its squares
+    + eps), times q_weight or k_weight [head_dim] (both float32 or of q's type;
+    None: ones), then turned as `rope` turns it, in one pass and with one rounding:
+    (q_out, k_out).  k None: q alone (and k_out None).  q_out may be q and
+    k_out k (in place); outputs overlap nothing else."""
+    if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in (_F16, _BF16):
+        raise ValueError('q must be float16 or bfloat16 [T, heads, head_dim]')
+    T, H, hd = q.shape
+    if k is None:
+        if k_weight is not None or k_out is not None:
+            raise ValueError('k_weight and k_out belong to k')
+        kv = 0
+    else:
+        if not isinstance(k, torch.Tensor) or k.dim() != 3:
+            raise ValueError('k must be [T, n_kv, head_dim]')
+        kv = k.shape[1]
+    rot, n = _angles('norm_rope', positions, inv_freq, axes, T, hd)
+    if H < 1 or hd > 512 or H > 1024 or kv > 1024 or (H + kv) * hd > 65536 or (k is not None and kv < 1):
+        raise ValueError('norm_rope takes head_dim up to 512, heads up to 1024 and 65536 elements a token')
+    eps = float(eps)
+    if not 2.0 ** -126 <= eps < 3e38:
+        raise ValueError(f'eps must be positive and finite, from 2^-126, got {eps}')
+    wt = q.dtype
+    for w, name in ((q_weight, 'q_weight'), (k_weight, 'k_weight')):
+        if w is not None:
+            wt = w.dtype if isinstance(w, torch.Tensor) and w.dtype is torch.float32 else q.dtype
+            _is(w, wt, name, (hd,))
+    if q_weight is not None and k_weight is not None and q_weight.dtype is not k_weight.dtype:
+        raise ValueError('q_weight and k_weight must have one type')
+    strides, outs = [], []
+    for x, out, name in ((q, q_out, 'q'), (k, k_out, 'k')):
+        if x is None:
+            strides.append((0, 0, 0, 0))
+            outs.append(None)
+            continue
+        shape = (T, x.shape[1], hd)
+        st, sh = _rows(x, q.dtype, name, shape, 1, out is x)
+        ot, oh = (shape[1] * hd, hd) if out is None else (st, sh) if out is x else _rows(out, q.dtype, name + '_out', shape, 1, True)
+        strides.append((st, sh, ot, oh))
+        outs.append(out)
+    dev = _on_device('q k q_weight k_weight positions inv_freq axes q_out k_out', q, k, q_weight, k_weight, positions, inv_freq,
+                     axes, q_out, k_out)
+    y, z = (o if o is not None or x is None else torch.empty(x.shape, dtype=q.dtype, device=q.device) for x, o in ((q, outs[0]), (k, outs[1])))
+    (qt, qh, qot, qoh), (kt, kh, kot, koh) = strides
+    check(lib().ck_norm_rope(q.data_ptr(), _ptr(k), y.data_ptr(), _ptr(z), _ptr(q_weight), _ptr(k_weight), positions.data_ptr(), n,
+                             _ptr(axes), inv_freq.data_ptr(), T, H, kv, hd, rot, qt, qh, kt, kh, qot, qoh, kot, koh,
+                             _DTYPE[q.dtype], _WEIGHT[wt], eps, 1 if interleaved else 0, scale, _raw_stream(dev)))
+    return y, z
+
+
+def cache_maps_workspace(B, tokens, in_place):
+    """Bytes of workspace (0: none) of cache_maps for B requests and `tokens` rows;
+    in_place: kv_out is kv_lens or taken_out is taken."""
+    if any(abs(n) > _INT for n in (B, tokens)):
+        raise ValueError('counts must be under 2^31')
+    nb = ctypes.c_size_t()
+    check(lib().ck_cache_maps_workspace(B, tokens, 1 if in_place else 0, ctypes.byref(nb)))
+    return nb.value
+
+
+def cache_maps(new_lens, kv_lens, block_table, page, tokens, free_pages=None, taken=None, kv_out=None, taken_out=None,
+               workspace=None):
+    """The index tensors of a step, built on the device from the lengths of its
+    requests: new_lens [B] new tokens behind the kv_lens [B] places that each has
+    (int32, as are all).  (cu_q [B+1], kv_out [B] = kv_lens + new_lens, positions
+    [tokens], slots [tokens]): row cu_q[b] + i is place kv_lens[b] + i of request
+    b, at slot block_table[b, place // page] * page + place % page -- what `rope`,
+    `cache_write` and `attention_paged` take.  Rows behind the last request have
+    position 0 and slot -1, which cache_write leaves out; tokens must hold the
+    sum of new_lens (what passes it gets no row).
+
+    free_pages [n] and taken [1]: new pages come from this list, request by request
+    from entry taken on, and are entered in block_table; taken is advanced (in
+    taken_out, if given, else in place) by all that were asked for.  Past the list's
+    end entries and slots are -1, and taken above n says so.  Without them
+    block_table names the new pages already.  A place without a page (a negative entry, or past the
+    table) has slot -1.
+    kv_out: kv_lens itself (a captured step then advances by itself), another
+    tensor, or None: a new one."""
+    if not isinstance(tokens, int) or not 0 <= tokens < 1 << 30:
+        raise ValueError('tokens must be the number of rows, under 2^30')
+    if not isinstance(page, int) or page < 16 or page > 1024 or page & (page - 1):
+        raise ValueError(f'the page size must be a power of two from 16 to 1024, got {page}')
+    if type(new_lens) is not torch.Tensor or new_lens.dim() != 1:
+        raise ValueError('new_lens must be int32 [B]')
+    B = new_lens.shape[0]
+    if B >= 1 << 20:
+        raise ValueError(f'new_lens must have under 2^20 requests, got {B}')
+    i32 = torch.int32
+    _is(new_lens, i32, 'new_lens', (B,))
+    _is(kv_lens, i32, 'kv_lens', (B,))
+    if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
+        raise ValueError('block_table must be int32 [B, width]')
+    width = block_table.shape[1]
+    if width * page > 1 << 30:
+        raise ValueError('block_table must name at most 2^30 places of a request')
+    _is(block_table, i32, 'block_table', (B, width))
+    if (free_pages is None) != (taken is None) or (taken is None and taken_out is not None):
+        raise ValueError('free_pages, taken and taken_out belong together')
+    n_free = 0
+    if free_pages is not None:
+        _check(free_pages, i32, 'free_pages', (None,))
+        n_free = free_pages.shape[0]
+        if n_free > _INT:
+            raise ValueError(f'free_pages must have under 2^31 entries, got {n_free}')
+        _is(taken, i32, 'taken', (1,))
+        if taken_out is None:
+            taken_out = taken
+        else:
+            _is(taken_out, i32, 'taken_out', (1,))
+    if kv_out is not None:
+        _is(kv_out, i32, 'kv_out', (B,))
+    dev = _on_device('new_lens kv_lens block_table free_pages taken kv_out taken_out', new_lens, kv_lens, block_table, free_pages,
+                     taken, kv_out, taken_out)
+    # one allocation, cut up on 16-byte borders (an allocation costs about 1 us)
+    b4, t4 = (B + 4) & -4, (tokens + 3) & -4
+    buf = torch.empty(b4 + 2 * t4 + (B if kv_out is None else 0), dtype=i32, device=new_lens.device)
+    cu, positions, slots = buf[:B + 1], buf[b4:b4 + tokens], buf[b4 + t4:b4 + t4 + tokens]
+    if kv_out is None:
+        kv_out = buf[b4 + 2 * t4:]
+    nb = 0
+    if tokens > 1024:
+        nb = cache_maps_workspace(B, tokens, kv_out.data_ptr() == kv_lens.data_ptr() or (taken is not None and
+                                                                                          taken_out.data_ptr() == taken.data_ptr()))
+    ws = _workspace(workspace, nb, new_lens.device)
+    check(lib().ck_cache_maps(new_lens.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), width,
+                              (free_pages.data_ptr() or taken.data_ptr()) if free_pages is not None else None, n_free, _ptr(taken), B, page, tokens,
+                              cu.data_ptr(), kv_out.data_ptr(), positions.data_ptr(), slots.data_ptr(), _ptr(taken_out), _ptr(ws),
+                              nb, _raw_stream(dev)))
+    return cu, kv_out, positions, slots
 
 
 def cache_write(k, v, k_pages, v_pages, slots, k_scale=None, v_scale=None):

@@ -431,8 +431,79 @@ int ck_rope(const void* x, void* out, const int32_t* positions, const double* in
             int head_dim, int rot, long x_st, long x_sh, long o_st, long o_sh, int dtype, int interleaved, float scale,
             int inverse, void* stream) {
   CK_API_BEGIN
-  launch_rope(x, out, positions, inv_freq, T, n_heads, head_dim, rot, x_st, x_sh, o_st, o_sh, dtype, interleaved != 0,
-              scale, inverse != 0, as_stream(stream));
+  launch_rope(x, out, positions, 1, nullptr, inv_freq, T, n_heads, head_dim, rot, x_st, x_sh, o_st, o_sh, dtype,
+              interleaved != 0, scale, inverse != 0, as_stream(stream));
+  CK_API_END
+}
+
+int ck_rope_axes(const void* x, void* out, const int32_t* positions, int n_axes, const int32_t* axes,
+                 const double* inv_freq, int T, int n_heads, int head_dim, int rot, long x_st, long x_sh, long o_st,
+                 long o_sh, int dtype, int interleaved, float scale, int inverse, void* stream) {
+  CK_API_BEGIN
+  launch_rope(x, out, positions, n_axes, axes, inv_freq, T, n_heads, head_dim, rot, x_st, x_sh, o_st, o_sh, dtype,
+              interleaved != 0, scale, inverse != 0, as_stream(stream));
+  CK_API_END
+}
+
+int ck_norm_rope(const void* q, const void* k, void* q_out, void* k_out, const void* q_weight, const void* k_weight,
+                 const int32_t* positions, int n_axes, const int32_t* axes, const double* inv_freq, int T, int n_heads,
+                 int n_kv, int head_dim, int rot, long q_st, long q_sh, long k_st, long k_sh, long qo_st, long qo_sh,
+                 long ko_st, long ko_sh, int dtype, int weight_dtype, float eps, int interleaved, float scale,
+                 void* stream) {
+  CK_API_BEGIN
+  NormRopeHeads a, b;
+  a.x = q;
+  a.out = q_out;
+  a.weight = q_weight;
+  a.heads = n_heads;
+  a.x_st = q_st;
+  a.x_sh = q_sh;
+  a.o_st = qo_st;
+  a.o_sh = qo_sh;
+  b.x = k;
+  b.out = k_out;
+  b.weight = k_weight;
+  b.heads = n_kv;
+  b.x_st = k_st;
+  b.x_sh = k_sh;
+  b.o_st = ko_st;
+  b.o_sh = ko_sh;
+  launch_norm_rope(a, b, positions, n_axes, axes, inv_freq, T, head_dim, rot, dtype, weight_dtype, eps, interleaved != 0,
+                   scale, as_stream(stream));
+  CK_API_END
+}
+
+int ck_cache_maps_workspace(int B, int tokens, int in_place, size_t* ws_bytes) {
+  CK_API_BEGIN
+  CK_REQUIRE(ws_bytes, "ck_cache_maps_workspace: null argument");
+  *ws_bytes = cache_maps_workspace(B, tokens, in_place != 0);
+  CK_API_END
+}
+
+int ck_cache_maps(const int32_t* new_lens, const int32_t* kv_lens, int32_t* block_table, int table_width,
+                  const int32_t* free_pages, int n_free, const int32_t* taken, int B, int page, int tokens,
+                  int32_t* cu_q, int32_t* kv_out, int32_t* positions, int32_t* slots, int32_t* taken_out,
+                  void* workspace, size_t ws_bytes, void* stream) {
+  CK_API_BEGIN
+  CacheMaps m;
+  m.new_lens = new_lens;
+  m.kv = kv_lens;
+  m.table = block_table;
+  m.width = table_width;
+  m.free_pages = free_pages;
+  m.n_free = n_free;
+  m.taken = taken;
+  m.B = B;
+  m.page = page;
+  m.tokens = tokens;
+  m.cu = cu_q;
+  m.kv_out = kv_out;
+  m.positions = positions;
+  m.slots = slots;
+  m.taken_out = taken_out;
+  m.ws = static_cast<int*>(workspace);
+  m.ws_bytes = ws_bytes;
+  launch_cache_maps(m, as_stream(stream));
   CK_API_END
 }
 

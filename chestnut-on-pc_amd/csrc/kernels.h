@@ -117,9 +117,37 @@ void launch_attention_oproj(const half_t* qk, const half_t* vt, const half_t* wo
 // see: whatever they hold, no kernel reads or writes outside the tensors it is given.
 //
 // out = x with the first rot elements of every head turned (rope.hip); strides in elements.
-void launch_rope(const void* x, void* out, const int* positions, const double* inv_freq, int T, int H, int hd, int rot,
-                 long xst, long xsh, long ost, long osh, int dtype, bool interleaved, float scale, bool inverse,
-                 hipStream_t s);
+// axes (or null: n_axes 1): every pair's row of positions [n_axes][T].
+void launch_rope(const void* x, void* out, const int* positions, int n_axes, const int* axes, const double* inv_freq,
+                 int T, int H, int hd, int rot, long xst, long xsh, long ost, long osh, int dtype, bool interleaved,
+                 float scale, bool inverse, hipStream_t s);
+struct RopeAngles;   // rope_angles.h
+RopeAngles rope_angles_of(const char* what, const int* positions, int n_axes, const int* axes, const double* inv_freq,
+                          int T, int rot, float scale, bool inverse);
+// The heads of q and k divided by their root mean square, times a weight each, then turned (norm_rope.hip).
+struct NormRopeHeads {
+  const void* x = nullptr;
+  void* out = nullptr;
+  const void* weight = nullptr;   // [head_dim] or null: ones
+  int heads = 0;
+  long x_st = 0, x_sh = 0, o_st = 0, o_sh = 0;
+};
+void launch_norm_rope(const NormRopeHeads& q, const NormRopeHeads& k, const int* positions, int n_axes, const int* axes,
+                      const double* inv_freq, int T, int hd, int rot, int dtype, int weight_dtype, float eps,
+                      bool interleaved, float scale, hipStream_t s);
+// Offsets, lengths, positions, slots and new pages of a step (cache_maps.hip).
+struct CacheMaps {
+  const int *new_lens = nullptr, *kv = nullptr;            // [B]
+  int* table = nullptr;                                    // [B][width]
+  const int *free_pages = nullptr, *taken = nullptr;       // [n_free], [1]; both or neither
+  int *cu = nullptr, *kv_out = nullptr, *positions = nullptr, *slots = nullptr, *taken_out = nullptr;
+  int B = 0, width = 0, page = 0, tokens = 0, n_free = 0;
+  int* ws = nullptr;
+  size_t ws_bytes = 0;
+};
+// Bytes (0: none needed); in_place: kv_out is kv or taken_out is taken.
+size_t cache_maps_workspace(int B, int tokens, bool in_place);
+void launch_cache_maps(const CacheMaps& m, hipStream_t s);
 // K and V pages [n_pages][n_kv][page][head_dim]; e4m3: scales [n_pages][n_kv][page], a
 // row's power of two as its biased exponent.
 struct PagedCache {

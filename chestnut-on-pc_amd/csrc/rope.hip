@@ -2,8 +2,8 @@
 // a = position * inv_freq[i]:
 //   y0 = s (x0 cos a - x1 sin a),  y1 = s (x1 cos a + x0 sin a),
 // pairs (i, i + rot/2), or (2i, 2i + 1) where interleaved; the elements behind `rot`
-// are copied.  A position of 10^6 makes a 10^6 rad, of which 32 bits hold no more than
-// 0.06 rad: a is a product of 64 bits, taken modulo one turn before it is rounded.
+// are copied.  With axes (time, row, column, ...) there is a position for each, and a pair's
+// angle goes by the one that axes[i] names.
 //
 // Bound by memory: every element is read and written once.  The angles belong to a
 // token, not to its heads, so a workgroup computes those of its tokens once into LDS
@@ -11,6 +11,7 @@
 #include "common.h"
 #include "elem16.h"
 #include "kernels.h"
+#include "rope_angles.h"
 
 namespace ck {
 namespace {
@@ -20,14 +21,12 @@ constexpr int ROPE_LDS = 1024;   // pairs of a workgroup's tokens: cos and sin i
 struct RopeParams {
   const void* x;
   void* out;
-  const int* pos;
-  const double* inv_freq;
+  RopeAngles a;
   long xst, xsh, ost, osh;   // element strides of tokens and heads
   int T, H, hd, rot, tpw;    // tpw: tokens per workgroup
   unsigned per_tok, m_tok;   // items (2V elements) per token and its div_magic
   unsigned per_head, m_head; // items per head and its div_magic
   int interleaved, copy;     // copy: the elements behind rot are to be copied (out is not x)
-  float scale, sign;
 };
 
 // V: pairs per item.  8 where rows and strides are whole 16-byte chunks and rot a multiple of 16, else 1.
@@ -38,14 +37,7 @@ template <typename T, int V, bool NT>
 __global__ __launch_bounds__(256) void rope_kernel(const RopeParams p) {
   __shared__ float2_t cs[ROPE_LDS];
   const int t0 = blockIdx.x * p.tpw, nt = min(p.tpw, p.T - t0), half = p.rot >> 1;
-  for (int i = threadIdx.x; i < nt * half; i += 256) {
-    const int t = i / half;
-    double turns = (double)p.pos[t0 + t] * p.inv_freq[i - t * half] * 0.15915494309189533577;
-    turns -= rint(turns);
-    float s, c;
-    sincospif(2.0f * (float)turns, &s, &c);
-    cs[i] = float2_t{p.scale * c, p.sign * p.scale * s};
-  }
+  rope_angles<256>(p.a, t0, nt, cs, threadIdx.x);
   __syncthreads();
   const T* x = static_cast<const T*>(p.x);
   T* out = static_cast<T*>(p.out);
@@ -101,9 +93,24 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeParams p) {
 
 }  // namespace
 
-void launch_rope(const void* x, void* out, const int* positions, const double* inv_freq, int T, int H, int hd, int rot,
-                 long xst, long xsh, long ost, long osh, int dtype, bool interleaved, float scale, bool inverse,
-                 hipStream_t s) {
+RopeAngles rope_angles_of(const char* what, const int* positions, int n_axes, const int* axes, const double* inv_freq,
+                          int T, int rot, float scale, bool inverse) {
+  CK_REQUIRE(n_axes >= 1 && (axes || n_axes == 1), std::string(what) + ": positions of several axes need every pair's axis");
+  RopeAngles a{};
+  a.pos = positions;
+  a.inv_freq = inv_freq;
+  a.axes = axes;
+  a.n_axes = n_axes;
+  a.T = T;
+  a.half = rot / 2;
+  a.scale = scale;
+  a.sign = inverse ? -1.0f : 1.0f;
+  return a;
+}
+
+void launch_rope(const void* x, void* out, const int* positions, int n_axes, const int* axes, const double* inv_freq,
+                 int T, int H, int hd, int rot, long xst, long xsh, long ost, long osh, int dtype, bool interleaved,
+                 float scale, bool inverse, hipStream_t s) {
   CK_REQUIRE(T >= 0 && H > 0 && hd > 0, "rope: sizes must be positive");
   CK_REQUIRE(rot > 0 && rot % 2 == 0 && rot <= hd, "rope: 2 * len(inv_freq) must be even and at most head_dim");
   CK_REQUIRE(dtype == DT_F16 || dtype == DT_BF16, "rope: f16 or bf16");
@@ -114,8 +121,7 @@ void launch_rope(const void* x, void* out, const int* positions, const double* i
   RopeParams p{};
   p.x = x;
   p.out = out;
-  p.pos = positions;
-  p.inv_freq = inv_freq;
+  p.a = rope_angles_of("rope", positions, n_axes, axes, inv_freq, T, rot, scale, inverse);
   p.xst = xst;
   p.xsh = xsh;
   p.ost = ost;
@@ -126,8 +132,6 @@ void launch_rope(const void* x, void* out, const int* positions, const double* i
   p.rot = rot;
   p.interleaved = interleaved;
   p.copy = rot < hd && x != out;
-  p.scale = scale;
-  p.sign = inverse ? -1.0f : 1.0f;
   const bool wide = rot % 16 == 0 && hd % 16 == 0 && ((xst | xsh | ost | osh) & 7) == 0 &&
                     ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
   p.per_head = wide ? hd / 16 : (hd + 1) / 2;

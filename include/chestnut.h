@@ -325,6 +325,53 @@ int ck_rope(const void* x, void* out, const int32_t* positions, const double* in
             int head_dim, int rot, long x_st, long x_sh, long o_st, long o_sh, int dtype, int interleaved, float scale,
             int inverse, void* stream);
 
+/* The same with a position for each of n_axes axes (time, row, column, ...):
+ * positions [n_axes][T], pair i's angle by the row axes[i] (int32 [rot / 2],
+ * held to 0 .. n_axes - 1).  axes NULL and n_axes 1: ck_rope. */
+int ck_rope_axes(const void* x, void* out, const int32_t* positions, int n_axes, const int32_t* axes,
+                 const double* inv_freq, int T, int n_heads, int head_dim, int rot, long x_st, long x_sh, long o_st,
+                 long o_sh, int dtype, int interleaved, float scale, int inverse, void* stream);
+
+/* Query and key heads normed and turned in one pass: y = w x /
+ * sqrt(mean(x^2) + eps) over a head's elements, then as ck_rope_axes; f32
+ * throughout, one rounding.  q [T][n_heads][head_dim], k [T][n_kv][head_dim];
+ * either may have no heads.  Weights [head_dim] of weight_dtype (0 = f32, 1,
+ * 4), NULL: ones.  q_out may be q, k_out may be k (same strides); outputs are
+ * else apart from inputs and from each other.  eps a normal positive number; head_dim <=
+ * 512, n_heads, n_kv <= 1024, (n_heads + n_kv) * head_dim <= 65536.  The
+ * squares are summed in f32: values of 2^59 and more (bf16) make zeros. */
+int ck_norm_rope(const void* q, const void* k, void* q_out, void* k_out, const void* q_weight, const void* k_weight,
+                 const int32_t* positions, int n_axes, const int32_t* axes, const double* inv_freq, int T, int n_heads,
+                 int n_kv, int head_dim, int rot, long q_st, long q_sh, long k_st, long k_sh, long qo_st, long qo_sh,
+                 long ko_st, long ko_sh, int dtype, int weight_dtype, float eps, int interleaved, float scale,
+                 void* stream);
+
+/* The index arrays of a step, from the lengths of its B requests (int32, all
+ * on the device): new_lens[b] new tokens behind the kv_lens[b] places that
+ * request b has (negative ones count as 0; sums are held at 2^31 - 1).
+ *   cu_q [B + 1]: offsets of the new tokens; kv_out [B]: kv_lens + new_lens;
+ *   positions, slots [tokens]: row cu_q[b] + i is place kv_lens[b] + i, at slot
+ *   block_table[b][place / page] * page + place % page.
+ * With free_pages [n_free] and taken [1] a request's new pages come from the
+ * list, in the order of the requests, from entry *taken on, and are written
+ * to the table; taken_out [1] = taken + all that were asked for.  Past the
+ * list's end there is no page: entry -1 (taken_out > n_free says so).
+ * Without them (all three NULL) the table names the new pages already.  A
+ * place without a page (a negative entry, a column past table_width, a slot
+ * past 2^31) has slot -1.  Rows behind the last request: position 0, slot -1.
+ * tokens: the rows there are; what new_lens asks for beyond them gets no row
+ * and enters no page in the table.  kv_out may be kv_lens and taken_out may
+ * be taken; else the outputs are apart from the inputs.  page a power of two
+ * from 16 to 1024, B < 2^20, tokens < 2^30, table_width * page <= 2^30.
+ * Workspace: as many bytes as ck_cache_maps_workspace says (0: none), one for
+ * each call that may run beside another; in_place: kv_out is kv_lens or
+ * taken_out is taken. */
+int ck_cache_maps_workspace(int B, int tokens, int in_place, size_t* ws_bytes);
+int ck_cache_maps(const int32_t* new_lens, const int32_t* kv_lens, int32_t* block_table, int table_width,
+                  const int32_t* free_pages, int n_free, const int32_t* taken, int B, int page, int tokens,
+                  int32_t* cu_q, int32_t* kv_out, int32_t* positions, int32_t* slots, int32_t* taken_out,
+                  void* workspace, size_t ws_bytes, void* stream);
+
 /* A cache: k_pages, v_pages [n_pages][n_kv][page][head_dim], 16-byte
  * aligned; page a power of two from 16 to 1024, head_dim a multiple of 8 up
  * to 256, n_pages * page < 2^31.  cache_dtype e4m3: k_scale, v_scale

@@ -5,11 +5,15 @@ import math
 import numpy as np
 
 
-def rope(x, positions, inv_freq, interleaved=False, scale=1.0, inverse=False):
-    """x f64 [T, H, hd]; the first 2 * len(inv_freq) elements of every head turned."""
+def rope(x, positions, inv_freq, interleaved=False, scale=1.0, inverse=False, axes=None):
+    """x f64 [T, H, hd]; the first 2 * len(inv_freq) elements of every head turned.  axes: the
+    row of positions [n, T] that each pair goes by."""
     y = np.array(x, np.float64)
     half = len(inv_freq)
-    a = np.outer(np.asarray(positions, np.float64), np.asarray(inv_freq, np.float64))
+    if axes is None:
+        a = np.outer(np.asarray(positions, np.float64), np.asarray(inv_freq, np.float64))
+    else:
+        a = np.stack([np.asarray(positions[min(max(n, 0), len(positions) - 1)], np.float64) * f for n, f in zip(axes, inv_freq)], -1)
     if inverse:
         a = -a
     c, s = np.cos(a)[:, None] * scale, np.sin(a)[:, None] * scale
@@ -17,6 +21,36 @@ def rope(x, positions, inv_freq, interleaved=False, scale=1.0, inverse=False):
     x0, x1 = y[..., i0].copy(), y[..., i1].copy()
     y[..., i0], y[..., i1] = x0 * c - x1 * s, x1 * c + x0 * s
     return y
+
+
+def rms_norm(x, weight=None, eps=1e-6):
+    """x f64 [..., hd] over the root of the mean of its squares (and eps), times weight."""
+    y = x / np.sqrt((x * x).mean(-1, keepdims=True) + eps)
+    return y if weight is None else y * weight
+
+
+def cache_maps(new, kv, table, page, tokens, free=None, taken=0):
+    """Request by request: (cu, kv + new, positions, slots, table, taken) as lists of whole numbers."""
+    table = [list(map(int, row)) for row in table]
+    cu, kv_out, positions, slots = [0], [], [], []
+    for b, (n, m) in enumerate(zip(new, kv)):
+        n, m = max(int(n), 0), max(int(m), 0)
+        have = -(-m // page)
+        for at in range(m, m + n):
+            col = at // page
+            if free is not None and col >= have and at % page == 0:   # the first place of a page that it has not
+                got = int(free[taken]) if taken < len(free) else -1
+                taken += 1
+                if col < len(table[b]) and len(positions) < tokens:
+                    table[b][col] = got
+            row = table[b][col] if col < len(table[b]) else -1
+            positions.append(at)
+            slots.append(row * page + at % page if row >= 0 and row * page + at % page < 2 ** 31 else -1)
+        cu.append(cu[-1] + n)
+        kv_out.append(m + n)
+    positions, slots = positions[:tokens], slots[:tokens]
+    rest = tokens - len(positions)
+    return cu, kv_out, positions + [0] * rest, slots + [-1] * rest, table, taken
 
 
 def e4m3_values():
