@@ -85,6 +85,13 @@ _SIGS = {
                                                                                   c_size_t, c_void_p]),
     'ck_attention_paged': (c_int, [c_void_p] * 7 + [c_int, c_void_p, c_void_p] + [c_int] * 7 + [c_long] * 4 +
                            [c_int, c_int, c_int, c_float, c_void_p, c_size_t, c_void_p]),
+    'ck_attention_range_workspace': (c_int, [c_int, c_int, c_long] + [c_int] * 6 + [P(c_size_t)]),
+    'ck_attention_varlen_window': (c_int, [c_void_p] * 6 + [c_int] * 6 + [c_long] * 8 + [c_int, c_int, c_int, c_float,
+                                                                                         c_void_p, c_size_t, c_void_p]),
+    'ck_attention_paged_window': (c_int, [c_void_p] * 7 + [c_int, c_void_p, c_void_p] + [c_int] * 7 + [c_long] * 4 +
+                                  [c_int] * 4 + [c_float, c_void_p, c_size_t, c_void_p]),
+    'ck_attention_paged_shared': (c_int, [c_void_p] * 7 + [c_int] + [c_void_p] * 4 + [c_int] * 8 + [c_long] * 4 +
+                                  [c_int] * 3 + [c_float, c_void_p, c_size_t, c_void_p]),
 }
 
 

@@ -711,20 +711,49 @@ def _attention_bytes(B, Tq, keys, n_heads, n_kv, head_dim):
     return nb.value
 
 
+def _range_bytes(B, Tq, keys, n_heads, n_kv, head_dim, window, sinks, groups):
+    nb = ctypes.c_size_t()
+    check(lib().ck_attention_range_workspace(B, Tq, keys, n_heads, n_kv, head_dim, window, sinks, groups, ctypes.byref(nb)))
+    return nb.value
+
+
 _cached_attention_bytes = functools.lru_cache(maxsize=256)(_attention_bytes)
+_cached_range_bytes = functools.lru_cache(maxsize=256)(_range_bytes)
 
 
-def attention_workspace(B, Tq, keys, n_heads, n_kv, head_dim):
+def attention_workspace(B, Tq, keys, n_heads, n_kv, head_dim, window=None, sinks=0, groups=0):
     """Bytes of workspace (0: none) of attention_varlen (keys = Tk) and
     attention_paged (keys = B * table width * page) for B sequences of Tq
-    queries in all.  Remembered for plain integers only, as gemm_workspace."""
+    queries in all, through a window or with this many groups of shared pages.
+    Remembered for plain integers only, as gemm_workspace."""
     ints = type(B) is type(Tq) is type(keys) is type(n_heads) is type(n_kv) is type(head_dim) is int
     if any(abs(n) > _INT for n in (B, Tq, n_heads, n_kv, head_dim)) or abs(keys) >= 2 ** 63:
         raise ValueError('counts must be under 2^31, and keys under 2^63')
-    return (_cached_attention_bytes if ints else _attention_bytes)(B, Tq, keys, n_heads, n_kv, head_dim)
+    if window is None and not groups:
+        _window(None, sinks, True)
+        return (_cached_attention_bytes if ints else _attention_bytes)(B, Tq, keys, n_heads, n_kv, head_dim)
+    window, sinks = _window(window, sinks, True)
+    if not isinstance(groups, int) or not 0 <= groups < 1 << 20 or (groups and window):
+        raise ValueError('groups must be a number under 2^20, and 0 with a window')
+    return (_cached_range_bytes if ints else _range_bytes)(B, Tq, keys, n_heads, n_kv, head_dim, window, sinks, groups)
 
 
-def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None, workspace=None):
+def _window(window, sinks, causal):
+    """The checks of a window: (window or 0, sinks), held to 2^30."""
+    if type(sinks) is not int or sinks < 0:
+        raise ValueError('sinks must be a number of keys, 0 or more')
+    if window is None:
+        if sinks:
+            raise ValueError('sinks belong to a window')
+        return 0, 0
+    if type(window) is not int or window < 1:
+        raise ValueError('window must be a number of keys, 1 or more')
+    if not causal:
+        raise ValueError('a window belongs to causal attention')
+    return min(window, 1 << 30), min(sinks, 1 << 30)
+
+
+def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None, workspace=None, window=None, sinks=0):
     """Attention of packed sequences: q [Tq, heads, head_dim] over k, v [Tk, n_kv,
     head_dim] (f16 or bf16; token and head strides are free), sequence b at rows
     cu_q[b] .. cu_q[b+1] of q and cu_k[b] .. cu_k[b+1] of k and v (int32 [B+1];
@@ -735,11 +764,16 @@ def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None
     overlap q, k or v otherwise.
     workspace: a buffer to keep, of at least attention_workspace bytes (else a new
     one is made); one for each call that may run beside another, and for each
-    captured graph."""
+    captured graph.
+    window (causal only): of the keys above, query i sees the last `window` -- its own
+    place and those before it -- and the first `sinks` of its sequence."""
     if not isinstance(k, torch.Tensor) or k.dim() != 3:
         raise ValueError('k must be [Tk, n_kv, head_dim]')
     Tk, kv, hd = k.shape
     T, H, B, (qt, qh), (ot, oh), scale = _queries(q, cu_q, kv, hd, out, scale)
+    ranged = window is not None or sinks != 0
+    if ranged:
+        window, sinks = _window(window, sinks, causal)
     kt, kh = _rows(k, q.dtype, 'k', k.shape)
     vt, vh = _rows(v, q.dtype, 'v', k.shape)
     if kt >= 1 << 24 or vt >= 1 << 24:
@@ -752,6 +786,13 @@ def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None
         _is(cu_k, torch.int32, 'cu_k', (B + 1,))
     dev = _on_device('q k v cu_q cu_k out', q, k, v, cu_q, cu_k, out)
     o = out if out is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if ranged:
+        nb = _cached_range_bytes(B, T, Tk, H, kv, hd, window, sinks, 0)
+        ws = _workspace(workspace, nb, q.device)
+        check(lib().ck_attention_varlen_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu_q.data_ptr(),
+                                               cu_k.data_ptr(), B, T, Tk, H, kv, hd, qt, qh, kt, kh, vt, vh, ot, oh,
+                                               _DTYPE[q.dtype], window, sinks, scale, _ptr(ws), nb, _raw_stream(dev)))
+        return o
     nb = _cached_attention_bytes(B, T, Tk, H, kv, hd)
     ws = _workspace(workspace, nb, q.device)
     check(lib().ck_attention_varlen(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu_q.data_ptr(),
@@ -761,18 +802,36 @@ def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None
 
 
 def attention_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, k_scale=None, v_scale=None, causal=True,
-                    scale=None, out=None, workspace=None):
+                    scale=None, out=None, workspace=None, window=None, sinks=0, shared=None):
     """Attention of new tokens over a paged cache that holds their own K and V
     rows already: q [Tq, heads, head_dim], sequence b at rows cu_q[b] ..
     cu_q[b+1] (int32 [B+1]), its kv_lens[b] keys (int32 [B]) at places 0.. of the
     pages block_table[b] (int32 [B, width]); the queries are the last of them
     (causal: query i of n sees the keys j <= i + kv_lens[b] - n; else all).  The
     cache has q's type or is e4m3, whose values are rounded to q's type as cache_read
-    rounds them (past float16's range: infinite).  Otherwise as attention_varlen."""
+    rounds them (past float16's range: infinite).  Otherwise as attention_varlen.
+    shared: (cu_shared int32 [N+1], shared_lens int32 [N]) on the device -- the tables of the
+    sequences cu_shared[g] .. cu_shared[g+1] begin with the same pages, which hold their first
+    shared_lens[g] keys (as far as these fill whole pages).  The shared keys are then read
+    once for all queries of the group, from the table of its first sequence; the result
+    is the same up to rounding.  Sequences may be in no group; not with a window."""
     n, kv, page, hd = _cache(k_pages, v_pages, k_scale, v_scale)
     T, H, B, (qt, qh), (ot, oh), scale = _queries(q, cu_q, kv, hd, out, scale)
     if k_pages.dtype not in (q.dtype, _E4M3):
         raise ValueError(f'the cache must be {q.dtype} or float8_e4m3fn, got {k_pages.dtype}')
+    ranged, groups, cu_s, s_lens = window is not None or sinks != 0, 0, None, None
+    if ranged:
+        window, sinks = _window(window, sinks, causal)
+    if shared is not None:
+        if ranged:
+            raise ValueError('a window and shared pages exclude each other')
+        if not isinstance(shared, (tuple, list)) or len(shared) != 2 or not isinstance(shared[1], torch.Tensor) or \
+                shared[1].dim() != 1 or not 1 <= shared[1].shape[0] < 1 << 20:
+            raise ValueError('shared must be (cu_shared int32 [N + 1], shared_lens int32 [N]) of 1 to 2^20 - 1 groups')
+        cu_s, s_lens = shared
+        groups = s_lens.shape[0]
+        _is(s_lens, torch.int32, 'shared_lens', (groups,))
+        _is(cu_s, torch.int32, 'cu_shared', (groups + 1,))
     _is(kv_lens, torch.int32, 'kv_lens', (B,))
     if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
         raise ValueError('block_table must be int32 [B, width]')
@@ -780,9 +839,21 @@ def attention_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, k_scale=Non
     if width * page > 1 << 30:
         raise ValueError('block_table must name at most 2^30 places of a sequence')
     _is(block_table, torch.int32, 'block_table', (B, width))
-    dev = _on_device('q k_pages v_pages block_table cu_q kv_lens k_scale v_scale out', q, k_pages, v_pages, block_table,
-                     cu_q, kv_lens, k_scale, v_scale, out)
+    dev = _on_device('q k_pages v_pages block_table cu_q kv_lens k_scale v_scale out cu_shared shared_lens', q, k_pages,
+                     v_pages, block_table, cu_q, kv_lens, k_scale, v_scale, out, cu_s, s_lens)
     o = out if out is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if ranged or groups:
+        nb = _cached_range_bytes(B, T, B * width * page, H, kv, hd, window if ranged else 0, sinks, groups)
+        ws = _workspace(workspace, nb, q.device)
+        head = (q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), o.data_ptr(),
+                block_table.data_ptr(), width, cu_q.data_ptr(), kv_lens.data_ptr())
+        sizes = (B, T, H, n, kv, page, hd, qt, qh, ot, oh, _DTYPE[q.dtype], _DTYPE[k_pages.dtype])
+        if ranged:
+            check(lib().ck_attention_paged_window(*head, *sizes, window, sinks, scale, _ptr(ws), nb, _raw_stream(dev)))
+        else:
+            check(lib().ck_attention_paged_shared(*head, cu_s.data_ptr(), s_lens.data_ptr(), groups, *sizes, 1 if causal else 0,
+                                                  scale, _ptr(ws), nb, _raw_stream(dev)))
+        return o
     nb = _cached_attention_bytes(B, T, B * width * page, H, kv, hd)
     ws = _workspace(workspace, nb, q.device)
     check(lib().ck_attention_paged(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale),

@@ -1,0 +1,54 @@
+// Attention through a sliding window, and of sequences that share their first pages (attend.h).
+#include "attend.h"
+
+namespace ck {
+namespace {
+
+constexpr int MOST_KEYS = 1 << 30;   // of a sequence: a window of as many is none
+
+// As plan_of (attend.hip) where window and groups are 0.
+Plan range_plan(int B, int Tq, long keys, int n_heads, int n_kv, int window, int sinks, int groups, bool few3 = false) {
+  Plan pl{};
+  const int G = n_heads / n_kv;
+  const long rows = (long)Tq * G;
+  // the rows that share keys: a sequence's, or a group's
+  const long units = groups ? groups : B;
+  pl.bm = rows <= 16 * units ? 16 : rows <= 32 * units ? 32 : 128;
+  pl.tiles = groups ? 2 * (rows / pl.bm) + B + groups : rows / pl.bm + B;
+  const long slots = pl.bm == 128 ? 512 : pl.bm == 16 && few3 ? 768 : 1024;
+  pl.min_blocks = pl.bm <= 32 ? 2 : 4;
+  const bool many = pl.bm == 128 && pl.tiles * n_kv >= 2 * slots;
+  long each = keys / B;
+  if (window) each = std::min(each, (long)window + sinks + pl.bm / G);
+  if (!many && each > 2 * pl.min_blocks * AT_KEYS) pl.target = (int)std::max(1L, slots / n_kv);
+  pl.items = pl.tiles + pl.target;
+  return pl;
+}
+
+}  // namespace
+
+size_t attend_range_floats(int B, int Tq, long keys, int n_heads, int n_kv, int head_dim, int window, int sinks, int groups) {
+  const Plan pl = range_plan(B, Tq, keys, n_heads, n_kv, window, sinks, groups);
+  return pl.target || groups ? (size_t)pl.items * n_kv * pl.bm * (head_dim + 2) : 0;
+}
+
+void launch_attend_range(const char* what, AttendParams& p, const AttendQuery& a, int kv, long keys, hipStream_t s) {
+  const std::string w(what);
+  CK_REQUIRE(a.window >= 0 && a.sinks >= 0 && a.groups >= 0 && a.groups < (1 << 20), w + ": window, sinks and groups (under 2^20) must not be negative");
+  CK_REQUIRE(!a.window || a.causal, w + ": a window belongs to causal attention");
+  CK_REQUIRE(a.window || !a.sinks, w + ": sinks belong to a window");
+  CK_REQUIRE(!a.window || !a.groups, w + ": a window and shared pages exclude each other");
+  CK_REQUIRE(!a.groups || kv != KV_ROWS, w + ": shared pages belong to a cache");
+  if (!attend_begin(w, p, a)) return;
+  CK_REQUIRE(!a.groups || (a.cu_shared && a.shared_lens), w + ": null pointer");
+  p.window = std::min(a.window, MOST_KEYS);
+  p.sinks = std::min(a.sinks, MOST_KEYS);
+  p.N = a.groups;
+  p.cu_s = a.cu_shared;
+  p.s_lens = a.shared_lens;
+  const Plan pl = range_plan(a.B, a.T, keys, a.n_heads, p.Hkv, a.window, a.sinks, a.groups, a.head_dim == 128 && kv == KV_E4M3);
+  const size_t need = pl.target || a.groups ? attend_range_floats(a.B, a.T, keys, a.n_heads, p.Hkv, a.head_dim, a.window, a.sinks, a.groups) : 0;
+  attend_launch<RANGE>(w, p, a, kv, pl, need, s);
+}
+
+}  // namespace ck

@@ -571,6 +571,65 @@ int ck_attention_workspace(int B, int Tq, long keys, int n_heads, int n_kv, int 
   CK_API_END
 }
 
+int ck_attention_range_workspace(int B, int Tq, long keys, int n_heads, int n_kv, int head_dim, int window, int sinks,
+                                 int groups, size_t* ws_bytes) {
+  CK_API_BEGIN
+  CK_REQUIRE(ws_bytes, "ck_attention_range_workspace: null argument");
+  *ws_bytes = attention_workspace(B, Tq, keys, n_heads, n_kv, head_dim, window, sinks, groups) * sizeof(float);
+  CK_API_END
+}
+
+int ck_attention_varlen_window(const void* q, const void* k, const void* v, void* out, const int32_t* cu_q,
+                               const int32_t* cu_k, int B, int Tq, int Tk, int n_heads, int n_kv, int head_dim,
+                               long q_st, long q_sh, long k_st, long k_sh, long v_st, long v_sh, long o_st, long o_sh,
+                               int dtype, int window, int sinks, float scale, void* workspace, size_t ws_bytes,
+                               void* stream) {
+  CK_API_BEGIN
+  AttendQuery a = attend_query(q, out, cu_q, B, Tq, n_heads, head_dim, q_st, q_sh, o_st, o_sh, dtype, 1, scale, workspace,
+                               ws_bytes);
+  CK_REQUIRE(window > 0, "attention_varlen: a window must have a key");
+  a.window = window;
+  a.sinks = sinks;
+  launch_attention_varlen(a, k, v, k_st, k_sh, v_st, v_sh, cu_k, Tk, n_kv, as_stream(stream));
+  CK_API_END
+}
+
+int ck_attention_paged_window(const void* q, const void* k_pages, const void* v_pages, const void* k_scale,
+                              const void* v_scale, void* out, const int32_t* block_table, int table_width,
+                              const int32_t* cu_q, const int32_t* kv_lens, int B, int Tq, int n_heads, int n_pages,
+                              int n_kv, int page, int head_dim, long q_st, long q_sh, long o_st, long o_sh, int dtype,
+                              int cache_dtype, int window, int sinks, float scale, void* workspace, size_t ws_bytes,
+                              void* stream) {
+  CK_API_BEGIN
+  AttendQuery a = attend_query(q, out, cu_q, B, Tq, n_heads, head_dim, q_st, q_sh, o_st, o_sh, dtype, 1, scale, workspace,
+                               ws_bytes);
+  CK_REQUIRE(window > 0, "attention_paged: a window must have a key");
+  a.window = window;
+  a.sinks = sinks;
+  launch_attention_paged(a, paged_cache(k_pages, v_pages, k_scale, v_scale, n_pages, n_kv, page, head_dim, cache_dtype),
+                         block_table, table_width, kv_lens, as_stream(stream));
+  CK_API_END
+}
+
+int ck_attention_paged_shared(const void* q, const void* k_pages, const void* v_pages, const void* k_scale,
+                              const void* v_scale, void* out, const int32_t* block_table, int table_width,
+                              const int32_t* cu_q, const int32_t* kv_lens, const int32_t* cu_shared,
+                              const int32_t* shared_lens, int groups, int B, int Tq, int n_heads, int n_pages,
+                              int n_kv, int page, int head_dim, long q_st, long q_sh, long o_st, long o_sh, int dtype,
+                              int cache_dtype, int causal, float scale, void* workspace, size_t ws_bytes,
+                              void* stream) {
+  CK_API_BEGIN
+  AttendQuery a = attend_query(q, out, cu_q, B, Tq, n_heads, head_dim, q_st, q_sh, o_st, o_sh, dtype, causal, scale,
+                               workspace, ws_bytes);
+  CK_REQUIRE(groups > 0, "attention_paged: shared pages need a group");
+  a.groups = groups;
+  a.cu_shared = cu_shared;
+  a.shared_lens = shared_lens;
+  launch_attention_paged(a, paged_cache(k_pages, v_pages, k_scale, v_scale, n_pages, n_kv, page, head_dim, cache_dtype),
+                         block_table, table_width, kv_lens, as_stream(stream));
+  CK_API_END
+}
+
 int ck_attention_varlen(const void* q, const void* k, const void* v, void* out, const int32_t* cu_q,
                         const int32_t* cu_k, int B, int Tq, int Tk, int n_heads, int n_kv, int head_dim, long q_st,
                         long q_sh, long k_st, long k_sh, long v_st, long v_sh, long o_st, long o_sh, int dtype,

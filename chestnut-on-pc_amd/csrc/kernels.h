@@ -177,9 +177,14 @@ struct AttendQuery {
   float scale = 0.f;
   float* ws = nullptr;         // attention_workspace floats
   size_t ws_floats = 0;
+  int window = 0, sinks = 0;   // window > 0: only its last `window` keys and the first `sinks` (causal)
+  // groups > 0: the sequences cu_shared[g] .. cu_shared[g + 1] have their first shared_lens[g] keys in the same pages
+  int groups = 0;
+  const int *cu_shared = nullptr, *shared_lens = nullptr;
 };
 // Workspace of a call, in floats (0: none needed); keys: the most that its sequences can have, all together.
-size_t attention_workspace(int B, int Tq, long keys, int n_heads, int n_kv, int head_dim);
+size_t attention_workspace(int B, int Tq, long keys, int n_heads, int n_kv, int head_dim, int window = 0, int sinks = 0,
+                           int groups = 0);
 // K/V rows contiguous, sequence b's at rows cu_k[b] .. cu_k[b+1] of k and v [Tk][n_kv][head_dim].
 void launch_attention_varlen(const AttendQuery& a, const void* k, const void* v, long kst, long ksh, long vst, long vsh,
                              const int* cu_k, int Tk, int n_kv, hipStream_t s);

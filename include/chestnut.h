@@ -427,6 +427,43 @@ int ck_attention_paged(const void* q, const void* k_pages, const void* v_pages, 
                        int page, int head_dim, long q_st, long q_sh, long o_st, long o_sh, int dtype, int cache_dtype,
                        int causal, float scale, void* workspace, size_t ws_bytes, void* stream);
 
+/* Causal attention through a sliding window: of the keys that ck_attention_varlen
+ * and ck_attention_paged (causal) let query i of n see, j <= i' = i + m - n, it
+ * sees those with j > i' - window (its own place and the window - 1 before it)
+ * or j < sinks.  window >= 1, sinks >= 0 (past 2^30 they are held at that).
+ * Keys that no query sees are not read. */
+int ck_attention_varlen_window(const void* q, const void* k, const void* v, void* out, const int32_t* cu_q,
+                               const int32_t* cu_k, int B, int Tq, int Tk, int n_heads, int n_kv, int head_dim,
+                               long q_st, long q_sh, long k_st, long k_sh, long v_st, long v_sh, long o_st, long o_sh,
+                               int dtype, int window, int sinks, float scale, void* workspace, size_t ws_bytes,
+                               void* stream);
+int ck_attention_paged_window(const void* q, const void* k_pages, const void* v_pages, const void* k_scale,
+                              const void* v_scale, void* out, const int32_t* block_table, int table_width,
+                              const int32_t* cu_q, const int32_t* kv_lens, int B, int Tq, int n_heads, int n_pages,
+                              int n_kv, int page, int head_dim, long q_st, long q_sh, long o_st, long o_sh, int dtype,
+                              int cache_dtype, int window, int sinks, float scale, void* workspace, size_t ws_bytes,
+                              void* stream);
+
+/* ck_attention_paged for sequences that share their first pages: those of group
+ * g are cu_shared[g] .. cu_shared[g+1] (int32 [groups + 1], ascending; a sequence may be
+ * in none), and the tables of all of them begin with the same pages, which
+ * hold their first shared_lens[g] keys (int32 [groups], counted down to whole
+ * pages; only the table of the group's first sequence is read for them).  The
+ * result is that of ck_attention_paged up to rounding; the shared keys are
+ * read once for the group.  groups under 2^20. */
+int ck_attention_paged_shared(const void* q, const void* k_pages, const void* v_pages, const void* k_scale,
+                              const void* v_scale, void* out, const int32_t* block_table, int table_width,
+                              const int32_t* cu_q, const int32_t* kv_lens, const int32_t* cu_shared,
+                              const int32_t* shared_lens, int groups, int B, int Tq, int n_heads, int n_pages,
+                              int n_kv, int page, int head_dim, long q_st, long q_sh, long o_st, long o_sh, int dtype,
+                              int cache_dtype, int causal, float scale, void* workspace, size_t ws_bytes,
+                              void* stream);
+
+/* The workspace of these calls, as ck_attention_workspace: window and sinks of
+ * the one kind (groups 0), or the groups of the other (window 0). */
+int ck_attention_range_workspace(int B, int Tq, long keys, int n_heads, int n_kv, int head_dim, int window, int sinks,
+                                 int groups, size_t* ws_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -89,10 +89,11 @@ def values(codes, byte):
     return e4m3_values()[codes] * 2.0 ** (byte.astype(np.float64) - 127)[..., None]
 
 
-def attention(q, k, v, causal=True, scale=None):
+def attention(q, k, v, causal=True, scale=None, window=None, sinks=0):
     """One sequence, f64: q [n, H, hd], k, v [m, Hkv, hd] -> (out [n, H, hd], the same with
     |v| for v, the largest sum of |products| of a score).  Rows that see no key are zero;
-    what a row does not see does not reach it."""
+    what a row does not see does not reach it.  window: the last that many of the keys that a
+    row sees, and the first `sinks` of all."""
     n, H, hd = q.shape
     m, Hkv = k.shape[:2]
     scale = 1.0 / math.sqrt(hd) if scale is None else scale
@@ -102,6 +103,9 @@ def attention(q, k, v, causal=True, scale=None):
         with np.errstate(invalid='ignore'):
             s = q[:, h] @ k[:, g].T * scale
         see = np.arange(m)[None] <= np.arange(n)[:, None] + (m - n if causal else m)
+        if window is not None:
+            place = np.arange(n)[:, None] + (m - n)
+            see &= (np.arange(m)[None] > place - window) | (np.arange(m)[None] < sinks)
         s = np.where(see, s, -np.inf)
         if m:
             b = (np.abs(q[:, h]) @ np.abs(k[:, g]).T * scale)[see]

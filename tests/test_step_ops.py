@@ -1,5 +1,5 @@
-"""What stands around a step over the token cache, without a GPU: what the entry points refuse, and the
-64-bit oracle against torch and against itself."""
+"""What stands around a step over the token cache, and attention through a window and over shared pages, without a
+GPU: what the entry points refuse, and the 64-bit oracle against torch and against itself."""
 import ctypes
 import math
 
@@ -30,6 +30,18 @@ def norm(q=None, k=None, wq=None, wk=None, pos=None, f=F, **kw):
 def maps(new=None, kv=None, table=None, page=16, tokens=8, **kw):
     return K.cache_maps(z(3, dtype=i32) if new is None else new, z(3, dtype=i32) if kv is None else kv,
                         z(3, 5, dtype=i32) if table is None else table, page, tokens, **kw)
+
+
+def varlen(**kw):
+    return K.attention_varlen(z(4, 4, 64), z(4, 2, 64), z(4, 2, 64), z(3, dtype=i32), **kw)
+
+
+def paged(**kw):
+    return K.attention_paged(z(4, 4, 64), z(3, 2, 16, 64), z(3, 2, 16, 64), z(2, 3, dtype=i32), z(3, dtype=i32), z(2, dtype=i32), **kw)
+
+
+def groups(n=1, cu=None, lens=None):
+    return (z(n + 1, dtype=i32) if cu is None else cu, z(n, dtype=i32) if lens is None else lens)
 
 
 FREE = dict(free_pages=z(9, dtype=i32), taken=z(1, dtype=i32))
@@ -96,6 +108,30 @@ REFUSED = [
     ('maps taken_out', lambda: maps(taken_out=z(1, dtype=torch.int64), **FREE), 'taken_out must be torch.int32'),
     ('maps kv_out', lambda: maps(kv_out=z(2, dtype=i32)), 'kv_out must have shape'),
     ('maps cpu tensors', lambda: maps(**FREE), 'must be a CUDA tensor'),
+    ('varlen window of none', lambda: varlen(window=0), 'window must be'),
+    ('varlen window negative', lambda: varlen(window=-1), 'window must be'),
+    ('varlen window fraction', lambda: varlen(window=2.0), 'window must be'),
+    ('varlen window true', lambda: varlen(window=True), 'window must be'),
+    ('varlen window, not causal', lambda: varlen(window=4, causal=False), 'belongs to causal'),
+    ('varlen sinks negative', lambda: varlen(window=4, sinks=-1), 'sinks must be'),
+    ('varlen sinks fraction', lambda: varlen(window=4, sinks=1.0), 'sinks must be'),
+    ('varlen sinks without a window', lambda: varlen(sinks=3), 'sinks belong to a window'),
+    ('varlen window cpu tensors', lambda: varlen(window=4), 'must be a CUDA tensor'),
+    ('paged window, not causal', lambda: paged(window=4, causal=False), 'belongs to causal'),
+    ('paged sinks without a window', lambda: paged(sinks=3), 'sinks belong to a window'),
+    ('paged window and shared', lambda: paged(window=4, shared=groups()), 'exclude each other'),
+    ('paged shared alone', lambda: paged(shared=z(2, dtype=i32)), 'shared must be'),
+    ('paged shared of no group', lambda: paged(shared=groups(0)), 'shared must be'),
+    ('paged shared lens type', lambda: paged(shared=groups(lens=z(1, dtype=torch.int64))), 'shared_lens must be torch.int32'),
+    ('paged shared cu type', lambda: paged(shared=groups(cu=z(2, dtype=torch.int64))), 'cu_shared must be torch.int32'),
+    ('paged shared cu length', lambda: paged(shared=groups(2, cu=z(2, dtype=i32))), 'cu_shared must have shape'),
+    ('paged shared strided', lambda: paged(shared=groups(2, lens=z(4, dtype=i32)[::2])), 'shared_lens must be contiguous'),
+    ('paged shared groups', lambda: paged(shared=groups(lens=torch.empty(1 << 20, dtype=i32, device='meta'))), 'shared must be'),
+    ('paged shared on the CPU', lambda: paged(shared=groups()), 'must be a CUDA tensor'),
+    ('workspace window', lambda: K.attention_workspace(1, 1, 64, 8, 8, 64, window=0), 'window must be'),
+    ('workspace sinks', lambda: K.attention_workspace(1, 1, 64, 8, 8, 64, sinks=2), 'sinks belong to a window'),
+    ('workspace groups', lambda: K.attention_workspace(1, 1, 64, 8, 8, 64, groups=-1), 'groups must be'),
+    ('workspace window and groups', lambda: K.attention_workspace(1, 1, 64, 8, 8, 64, window=4, groups=1), 'groups must be'),
 ]
 
 
@@ -116,7 +152,29 @@ def native_maps(B=3, width=5, n_free=9, page=16, tokens=8, free=X, taken=X, out=
     return ('ck_cache_maps', X, X, table, width, free, n_free, taken, B, page, tokens, cu, X, X, X, out, ws, 0, None)
 
 
+def native_window(window=8, sinks=0, scale=0.1, paged=True):
+    return ('ck_attention_paged_window', X, X, X, None, None, X, X, 3, X, X, 2, 4, 4, 3, 2, 16, 64, 256, 64, 256, 64, 1, 1, window, sinks, scale,
+            None, 0, None) if paged else ('ck_attention_varlen_window', X, X, X, X, X, X, 2, 4, 4, 4, 2, 64, 256, 64, 128, 64, 128, 64, 256, 64, 1,
+                                          window, sinks, scale, None, 0, None)
+
+
+def native_shared(n=1, cu=X, lens=X, hd=64):
+    return ('ck_attention_paged_shared', X, X, X, None, None, X, X, 3, X, X, cu, lens, n, 2, 4, 4, 3, 2, 16, hd, 256, hd, 256, hd, 1, 1, 1, 0.1,
+            None, 0, None)
+
+
 NATIVE = [
+    ('paged window', native_window(0), 'must have a key'),
+    ('varlen window', native_window(-4, paged=False), 'must have a key'),
+    ('paged sinks', native_window(8, -1), 'must not be negative'),
+    ('varlen scale', native_window(scale=-1.0, paged=False), 'positive and finite'),
+    ('shared groups', native_shared(0), 'need a group'),
+    ('shared too many groups', native_shared(1 << 20), 'under 2\\^20'),
+    ('shared null', native_shared(cu=None), 'null pointer'),
+    ('shared head_dim', native_shared(hd=96), 'head_dim must be 64 or 128'),
+    ('shared workspace', native_shared(), 'workspace too small'),
+    ('range workspace', ('ck_attention_range_workspace', 1, 1, 64, 8, 8, 64, 0, 0, 1, None), 'null argument'),
+    ('range workspace sizes', ('ck_attention_range_workspace', 1, 1, 64, 8, 8, 64, -1, 0, 0, ctypes.byref(ctypes.c_size_t())), 'bad sizes'),
     ('rope axes', ('ck_rope_axes', X, X, X, 3, None, X, 4, 2, 64, 64, 128, 64, 128, 64, 1, 0, 1.0, 0, None), "every pair's axis"),
     ('rope no axis', ('ck_rope_axes', X, X, X, 0, X, X, 4, 2, 64, 64, 128, 64, 128, 64, 1, 0, 1.0, 0, None), "every pair's axis"),
     ('norm rot', native_norm(rot=7), 'must be even'),
@@ -205,3 +263,28 @@ def test_oracle_maps():
     used = [x for row in got for x in row if x >= 0]
     assert len(set(used)) == len(used) and taken == 4 + sum(-(-int(m) // page) for m in out) - sum(have)
     assert sorted(used) == sorted([int(x) for x in free[4:taken]] + [int(x) for x in table[table >= 0]])
+
+
+@pytest.mark.parametrize('n,m,window,sinks', [(5, 5, 2, 0), (3, 9, 4, 2), (6, 2, 1, 1), (4, 7, 100, 0), (2, 0, 3, 3), (4, 12, 3, 20)])
+def test_oracle_window(n, m, window, sinks):
+    r = np.random.default_rng(n + m)
+    q, k, v = r.standard_normal((n, 4, 8)), r.standard_normal((m, 2, 8)), r.standard_normal((m, 2, 8))
+    out, _, _ = O.attention(q, k, v, window=window, sinks=sinks)
+    for i in range(n):
+        place = i + m - n
+        js = [j for j in range(m) if j <= place and (place - j < window or j < sinks)]
+        for h in range(4):
+            w = np.array([math.exp(q[i, h] @ k[j, h // 2] / math.sqrt(8)) for j in js])
+            want = sum((x * v[j, h // 2] for x, j in zip(w / w.sum(), js)), np.zeros(8)) if js else np.zeros(8)
+            assert np.allclose(out[i, h], want, atol=1e-12)
+
+
+def test_range_workspace():
+    whole = K.attention_workspace(1, 1, 6144, 8, 8, 64)
+    assert K.attention_workspace(1, 1, 6144, 8, 8, 64, window=6144) == whole > 0
+    assert K.attention_workspace(1, 1, 6144, 8, 8, 64, window=1 << 40, sinks=1 << 40) == whole
+    assert K.attention_workspace(1, 1, 6144, 8, 8, 64, window=64) == 0          # few keys: not split
+    assert K.attention_workspace(40, 4000, 4000, 8, 8, 64, groups=3) > 0         # what is shared is always joined
+    assert K.attention_workspace(0, 0, 0, 8, 8, 64, groups=3) == 0
+    t = torch.tensor(1)
+    assert K.attention_workspace(t, 1, 6144, 8, 8, 64, window=6144) == whole
