@@ -57,6 +57,7 @@ struct AttendParams {
   int window, sinks;
   int N;
   const int *cu_s, *s_lens;
+  int front_items, own_items;       // N > 0: of each kind at most, by the rows that the workspace holds
 };
 
 namespace {
@@ -148,6 +149,7 @@ struct Item {
   // RANGE (Piece); whole: every row of a front sees all its keys
   int v, first, s1;
   bool front, whole;
+  int fronts, rank;                 // items of all fronts; the tile's number among the sequences' own ones
 };
 
 template <int KV, int BM>
@@ -183,8 +185,8 @@ __device__ __forceinline__ N lanes_scan(N v) {
 }
 __device__ __forceinline__ int lane63(int v) { return __builtin_amdgcn_readlane(v, 63); }
 
-// index counts items, or tiles where TILES.  False: there are not so many.
-template <int KV, int BM, bool TILES, int FORM>
+// index counts items, or tiles where TILES.  False: there are not so many.  BMF: rows of a front's tiles.
+template <int KV, int BM, bool TILES, int FORM, int BMF = BM>
 __device__ __forceinline__ bool find_item(const AttendParams& p, int index, Item& it) {
   const int lane = threadIdx.x & 63;
   const int count = FORM == RANGE ? p.B + p.N : p.B;
@@ -205,7 +207,7 @@ __device__ __forceinline__ bool find_item(const AttendParams& p, int index, Item
         s = sequence<KV>(p, b0 + lane);
         blocks = blocks_of(s.nk);
       }
-      tiles = tiles_of<KV, BM>(s, p.G);
+      tiles = FORM == RANGE && BMF != BM && b0 + lane < p.N ? tiles_of<KV, BMF>(s, p.G) : tiles_of<KV, BM>(s, p.G);
     }
   };
   get(0);
@@ -221,12 +223,13 @@ __device__ __forceinline__ bool find_item(const AttendParams& p, int index, Item
       work += readlane_f32(lanes_scan((float)tiles * (float)blocks), 63);
       all = min(all + lane63(lanes_scan(tiles)), MOST);
     }
-    // each tile adds up to one item that is not full
-    const int full = max(p.target - all, (p.target + 1) >> 1);
+    // each tile adds up to one item that is not full (shared pages: most tiles are a sequence's own few keys, and
+    // the fronts' items as long as their share of the card)
+    const int full = FORM == RANGE && p.N ? p.target : max(p.target - all, (p.target + 1) >> 1);
     if (work < 16777216.f) {   // a whole number
       const int w = (int)work;
       c = max(p.min_blocks, (w + full - 1) / full);
-      if (count <= 16) {
+      if (count <= 16 && !(FORM == RANGE && p.N)) {
         // few sequences: lane i counts the items that chunks of c0 + i blocks make, and the shortest
         // chunk that does not make too many is taken (eight chunks and tokens, 80 -> 76 us)
         const int c0 = max(p.min_blocks, (w + p.target - 1) / p.target), ci = c0 + lane;
@@ -246,12 +249,18 @@ __device__ __forceinline__ bool find_item(const AttendParams& p, int index, Item
     c = __builtin_amdgcn_readfirstlane(c);
     if (count > 64) get(0);
   }
-  int base = 0;
+  int base = 0, fronts = 0, rank = 0;
   for (int b0 = 0; b0 < count; b0 += 64) {
     if (b0) get(b0);
     const int nch = max(1, (blocks + c - 1) / c), items = tiles * nch;
     const int si = lanes_scan(items), su = TILES ? lanes_scan(tiles) : si;
     const unsigned long long m = __ballot(su > index);
+    int so = 0;   // own tiles up to the lane's
+    if constexpr (FORM == RANGE)
+      if (p.N) {
+        so = lanes_scan(b0 + lane < p.N ? 0 : tiles);
+        if (b0 < p.N) fronts += lane63(lanes_scan(b0 + lane < p.N ? items : 0));
+      }
     if (m) {
       const int w = __ffsll(m) - 1;
       const int local = __builtin_amdgcn_readlane(index - (su - (TILES ? tiles : items)), w);
@@ -275,11 +284,14 @@ __device__ __forceinline__ bool find_item(const AttendParams& p, int index, Item
         it.first = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_readlane(x.first, w));
         it.s1 = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_readlane(x.s1, w));
         it.whole = false;
+        it.fronts = fronts;
+        it.rank = rank + __builtin_amdgcn_readlane(so - (b0 + lane < p.N ? 0 : tiles), w) + it.tile;
       }
       return true;
     }
     index -= lane63(su);
     base += lane63(si);
+    if (FORM == RANGE) rank += lane63(so);
   }
   return false;
 }
@@ -352,6 +364,8 @@ __device__ __forceinline__ Blocks blocks(const AttendParams& p, const Item& it, 
   x.fs = min(min(p.sinks, lim_lo) / AT_KEYS, x.sn);
   x.fa = max(blocks_of(lo_hi), x.w0) - x.w0 + x.sn;
   x.fb = lim_lo / AT_KEYS - x.w0 + x.sn;
+  // (the compiler does not see that these are the same for all lanes)
+  for (int* i : {&x.sn, &x.w0, &x.nb, &x.fs, &x.fa, &x.fb, &x.lim}) *i = __builtin_amdgcn_readfirstlane(*i);
   return x;
 }
 
@@ -1038,6 +1052,103 @@ __device__ __forceinline__ float2_t* part_ml(const AttendParams& p, long row) {
   return reinterpret_cast<float2_t*>(p.ws + p.part_rows * HD) + row;
 }
 
+// Where the row q of an item's partial sums is, or -1 (offsets that do not ascend may name more rows than
+// there are).  Shared pages: the fronts' items, of BMF rows each, then the sequences' own.
+template <int BM, int BMF, int FORM>
+__device__ __forceinline__ long part_row(const AttendParams& p, const Item& it, int hk, int q) {
+  const int item = it.base + it.chunk;
+  if constexpr (FORM == RANGE)
+    if (p.N) {
+      if (it.front) return item < 0 || item >= p.front_items ? -1 : ((long)item * p.Hkv + hk) * BMF + q;
+      const int own = item - it.fronts;
+      if (it.fronts < 0 || it.fronts > p.front_items || own < 0 || own >= p.own_items) return -1;
+      return (long)it.fronts * p.Hkv * BMF + ((long)own * p.Hkv + hk) * BM + q;
+    }
+  return ((long)item * p.Hkv + hk) * BM + q;
+}
+// Shared pages: what the joining launch has to know of a sequence's own tile, so that it need not look for it.
+struct Parts {
+  int q0, row0, rows;          // the sequence's first query; the tile's first row, its rows
+  int own, nch;                // its first item among the own ones, items (0: none)
+  int front, fnch, frow0;      // the group's first item, items a tile (0: no group), the group's row that is row0
+  int frows, pad[3];           // the group's rows
+};
+// The workspace behind the sums: how many own tiles there are and how many items of fronts, then Parts for each tile.
+template <int HD>
+__device__ __forceinline__ int* parts_head(const AttendParams& p) { return reinterpret_cast<int*>(p.ws + p.part_rows * (HD + 2)); }
+template <int HD>
+__device__ __forceinline__ Parts* parts_at(const AttendParams& p) { return reinterpret_cast<Parts*>(parts_head<HD>(p) + 4); }
+
+// Where the parts of a sequence's group are: its first item, items a tile, rows; nch 0: no group.
+struct Front {
+  int base, nch, q0;
+  long rows;
+};
+template <int KV, int BMF>
+__device__ __forceinline__ Front front_of(const AttendParams& p, const Item& it) {
+  Front f{};
+  const int g = group_of(p, it.v - p.N), lane = threadIdx.x & 63;
+  if (g < 0) return f;
+  for (int g0 = 0; g0 <= g; g0 += 64) {
+    Piece x{};
+    int nch = 0, items = 0;
+    if (g0 + lane <= g) {
+      x = piece<KV>(p, g0 + lane);
+      nch = max(1, (blocks_of<BMF>(p, x) + it.c - 1) / it.c);
+      items = tiles_of<KV, BMF>(x.s, p.G) * nch;
+    }
+    const int all = lane63(lanes_scan(items));
+    if (g < g0 + 64) {
+      const int w = g - g0;
+      f.base += all - __builtin_amdgcn_readlane(items, w);
+      f.nch = __builtin_amdgcn_readlane(nch, w);
+      f.q0 = __builtin_amdgcn_readlane(x.s.q0, w);
+      f.rows = (long)__builtin_amdgcn_readlane(x.s.nq, w) * p.G;
+      if (__builtin_amdgcn_readlane(x.s.nk, w) <= 0 || f.base < 0) f.nch = 0;
+    } else {
+      f.base += all;
+    }
+  }
+  return f;
+}
+
+// By one wave: the Parts of an own tile's first item.
+template <int HD, int KV, int BM, int BMF>
+__device__ __forceinline__ void leave_parts(const AttendParams& p, const Item& it, int hk, int tile, int lane) {
+  if (it.front || it.chunk || hk || it.rank < 0 || it.rank >= p.own_items) return;
+  const Front f = front_of<KV, BMF>(p, it);
+  Parts x{};
+  x.q0 = it.s.q0;
+  x.row0 = tile * BM;
+  x.rows = (int)min((long)BM, (long)it.s.nq * p.G - (long)tile * BM);
+  x.own = it.base - it.fronts;
+  x.nch = it.fronts < 0 || it.fronts > p.front_items || x.own < 0 || x.own + it.nch > p.own_items ? 0 : it.nch;
+  x.front = f.base;
+  x.fnch = f.nch;
+  x.frows = (int)min(f.rows, 0x7FFFFFFFl);
+  x.frow0 = (int)max(((long)it.s.q0 - f.q0) * p.G + (long)tile * BM, -1l);
+  if (lane == 0) parts_at<HD>(p)[it.rank] = x;
+}
+// By the first workgroup: how many own tiles and items of fronts there are.
+template <int HD, int KV, int BM, int BMF>
+__device__ __forceinline__ void leave_head(const AttendParams& p, int c, int lane) {
+  int tiles = 0, fronts = 0;
+  for (int b0 = 0; b0 < p.N + p.B; b0 += 64) {
+    int t = 0, f = 0;
+    if (b0 + lane < p.N + p.B) {
+      const Piece x = piece<KV>(p, b0 + lane);
+      if (b0 + lane < p.N) f = tiles_of<KV, BMF>(x.s, p.G) * max(1, (blocks_of<BMF>(p, x) + c - 1) / c);
+      else t = tiles_of<KV, BM>(x.s, p.G);
+    }
+    tiles = min(tiles + lane63(lanes_scan(t)), 1 << 29);
+    fronts = min(fronts + lane63(lanes_scan(f)), 1 << 29);
+  }
+  if (lane == 0) {
+    parts_head<HD>(p)[0] = tiles < 0 ? 0 : min(tiles, p.own_items);
+    parts_head<HD>(p)[1] = fronts;
+  }
+}
+
 // ---- many rows: NW waves of 32 rows over the same keys -----------------------------------
 // Tiles of 64 keys.  A wave computes the scores of one tile while it turns those of the tile
 // before into weights, so that the matrix cores and the vector unit work at the same time:
@@ -1058,25 +1169,25 @@ __device__ __forceinline__ float2_t* part_ml(const AttendParams& p, long row) {
 // and 10 us, 545 by the call, though with 128 features that kernel spills 43 registers (tiles
 // of 256 rows: 19; without codes to turn into values: 1).  Short prompts (40 of 1 to 239 tokens,
 // 8 heads of 64) 12.4 us.
-template <typename T, int HD, int KV, int NW, int FORM>
-__global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendParams p) {
+template <typename T, int HD, int FORM>
+struct TileLds {
+  // (bad: WHOLE, the first key of a kind and feature; RANGE, a bit for each key of the tile)
+  typedef std::conditional_t<FORM == RANGE, unsigned long long, int> bad_t;
+  static constexpr int TILE = AT_KEYS * HD, BAD = 3 * HD * sizeof(bad_t), BYTES = 4 * TILE * 2 + BAD + 16;
+};
+// BMO: rows of the tiles of sequences' own keys, where this is a front's
+template <typename T, int HD, int KV, int NW, int FORM, int BMO = 32 * NW>
+__device__ __forceinline__ void tile_item(const AttendParams& p, Item& it, const int hk, char* const lds) {
   constexpr int BM = 32 * NW, TILE = AT_KEYS * HD, NT = 64 * NW;
   constexpr bool SPLIT = NW == 4;   // a tile's keys may be split over workgroups
   constexpr bool DMA = KV != KV_E4M3;
-  // one array: with several, the compiler holds every read of one back until all loads to the
-  // others have landed
-  // (bad: WHOLE, the first key of a kind and feature; RANGE, a bit for each key of the tile)
-  typedef std::conditional_t<FORM == RANGE, unsigned long long, int> bad_t;
-  constexpr int BAD = 3 * HD * sizeof(bad_t);
-  __shared__ __attribute__((aligned(1024))) char lds[4 * TILE * 2 + BAD + 16];
+  typedef typename TileLds<T, HD, FORM>::bad_t bad_t;
+  constexpr int BAD = TileLds<T, HD, FORM>::BAD;
   auto kt = [&](int buf) { return reinterpret_cast<T*>(lds) + buf * TILE; };
   auto vt = [&](int buf) { return reinterpret_cast<T*>(lds) + (2 + buf) * TILE; };
   bad_t (*const bad)[HD] = reinterpret_cast<bad_t (*)[HD]>(lds + 4 * TILE * 2);
   int& odd = *reinterpret_cast<int*>(lds + 4 * TILE * 2 + BAD);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hk = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv;
-  Item it;
-  if (!find_item<KV, BM, false, FORM>(p, index, it)) return;
   const int tile = tiles_of<KV, BM>(it.s, p.G) - 1 - it.tile;   // the longest first
   const int tok0 = tile * BM / p.G, tok1 = min(it.s.nq - 1, (tile * BM + BM - 1) / p.G);
   // WHOLE: the keys of the tile's first and last rows, and of this chunk
@@ -1086,6 +1197,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
   int vbeg = 0, vend = 0;
   if constexpr (FORM == RANGE) {
     it.whole = it.front && front_is_whole<KV>(p, it, lane);
+    if (KV != KV_ROWS && p.N && wave == 0) leave_parts<HD, KV, BMO, BM>(p, it, hk, tile, lane);
     bl = blocks<KV>(p, it, tok0, tok1);
     vbeg = SPLIT && it.nch > 1 ? it.chunk * it.c : 0;
     vend = SPLIT && it.nch > 1 ? min(bl.nb, vbeg + it.c) : bl.nb;
@@ -1149,17 +1261,20 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
   // A tile whose scores are in sa by itself; part: some row does not see all of it, and an infinity
   // or NaN of V must not reach that row.
   auto alone = [&](bool part, bool more) {
+    int lane_ = lane, tid_ = tid;
+    if constexpr (FORM == RANGE)   // or the addresses of this rarer path stay in registers through the other one
+      asm volatile("" : "+v"(lane_), "+v"(tid_));
     bool fix = false;
     if (part) {
-      r.template mask<2>(sa, key0, lane);
-      if (any_odd<T, TILE, NT>(vt(cur), tid)) odd = 1;
+      r.template mask<2>(sa, key0, lane_);
+      if (any_odd<T, TILE, NT>(vt(cur), tid_)) odd = 1;
       __syncthreads();
       fix = odd;
       if (fix) {
-        for (int i = tid; i < 3 * HD; i += NT) (&bad[0][0])[i] = FORM == RANGE ? 0 : 0x7FFFFFFF;
+        for (int i = tid_; i < 3 * HD; i += NT) (&bad[0][0])[i] = FORM == RANGE ? 0 : 0x7FFFFFFF;
         __syncthreads();
-        if constexpr (FORM == RANGE) take_out_odd<T, HD, AT_KEYS, NT>(vt(cur), bad, tid);
-        else take_out_odd<T, HD, AT_KEYS, NT>(vt(cur), bad, key0, tid);
+        if constexpr (FORM == RANGE) take_out_odd<T, HD, AT_KEYS, NT>(vt(cur), bad, tid_);
+        else take_out_odd<T, HD, AT_KEYS, NT>(vt(cur), bad, key0, tid_);
         __syncthreads();
       }
     }
@@ -1171,12 +1286,12 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
     for (int ct = 0; ct < Rows<T, HD>::CT; ++ct) vc[ct] = va[ct] + cur * TILE * 2;
     r.template values<2, 0>(vc, pf);
     if (fix) {
-      r.add_odd(bad, key0, lane);
+      r.add_odd(bad, key0, lane_);
       __syncthreads();
-      if (tid == 0) odd = 0;
+      if (tid_ == 0) odd = 0;
     }
     if (more) {
-      r.template scores<2>(sa, kt(cur ^ 1), lane);
+      r.template scores<2>(sa, kt(cur ^ 1), lane_);
       keep(cur);
     }
   };
@@ -1248,13 +1363,14 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
   wait_vm_lgkm0<0>();   // the loads past the last tile land before this workgroup's LDS is another's
 
   // (the parts of shared pages are always joined)
-  if ((!SPLIT || it.nch == 1) && (FORM != RANGE || !p.N)) {
+  if ((!SPLIT || it.nch == 1) && (FORM != RANGE || KV == KV_ROWS || !p.N)) {
     r.finish(p, it, hk, lane);
     return;
   }
   const float t = r.sum();
   if (r.tok < 0) return;
-  const long row = ((long)(it.base + it.chunk) * p.Hkv + hk) * BM + wave * 32 + (lane & 31);
+  const long row = part_row<BMO, BM, FORM>(p, it, hk, wave * 32 + (lane & 31));
+  if (FORM == RANGE && row < 0) return;
   if (lane < 32) *part_ml<HD>(p, row) = float2_t{r.m * p.scale_log2e, t};
   if (kbeg >= kend) return;
   float* o = part_o<HD>(p, row) + 4 * (lane >> 5);
@@ -1263,6 +1379,20 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
 #pragma unroll
     for (int i = 0; i < 16; i += 4)
       *reinterpret_cast<float4_t*>(o + ct * 32 + 2 * i) = float4_t{r.o[ct][i], r.o[ct][i + 1], r.o[ct][i + 2], r.o[ct][i + 3]};
+}
+
+template <typename T, int HD, int KV, int NW, int FORM>
+__global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendParams p) {
+  // one array: with several, the compiler holds every read of one back until all loads to the
+  // others have landed
+  __shared__ __attribute__((aligned(1024))) char lds[TileLds<T, HD, FORM>::BYTES];
+  const int hk = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv;
+  Item it;
+  const bool some = find_item<KV, 32 * NW, false, FORM>(p, index, it);
+  if constexpr (FORM == RANGE)
+    if (KV != KV_ROWS && p.N && blockIdx.x == 0 && threadIdx.x < 64) leave_head<HD, KV, 32 * NW, 32 * NW>(p, some ? it.c : 1, threadIdx.x);
+  if (!some) return;
+  tile_item<T, HD, KV, NW, FORM>(p, it, hk, lds);
 }
 
 // ---- few rows: 16 or 32 of them, the keys over the waves -----------------------------------
@@ -1280,19 +1410,30 @@ constexpr int FEW_WAVES = 4;
 // workgroups a CU
 constexpr int few_at_once(int bm, int hd, bool e4m3) { return hd == 64 ? (bm == 16 ? 4 : 3) : bm == 16 && e4m3 ? 3 : 2; }
 
-template <typename T, int HD, int KV, typename R, int FORM>
-__global__ __launch_bounds__(64 * FEW_WAVES, few_at_once(R::BM, HD, KV == KV_E4M3)) void attend_few_kernel(const AttendParams p) {
-  constexpr int BM = R::BM, KEYS = 32, TILE = KEYS * HD, NW = FEW_WAVES;
+// MIXED (shared pages, single tokens): the groups' fronts by tiles of 128 rows, the sequences' own keys by few rows.
+template <typename T, int HD, int KV, typename R, int FORM, bool MIXED = false>
+__global__ __launch_bounds__(64 * FEW_WAVES, MIXED ? 2 : few_at_once(R::BM, HD, KV == KV_E4M3)) void attend_few_kernel(const AttendParams p) {
+  constexpr int BM = R::BM, KEYS = 32, TILE = KEYS * HD, NW = FEW_WAVES, BMF = MIXED ? 128 : BM;
   // 1: V takes K's place in LDS, so that three workgroups of 128 features fit a CU
   constexpr int PARTS = HD == 128 && few_at_once(BM, HD, KV == KV_E4M3) == 3 ? 1 : 2;
-  __shared__ __attribute__((aligned(1024))) T lds[NW][PARTS * TILE];   // at the end: O f32 [NW][BM][HD]
+  constexpr int FRONT = MIXED ? (TileLds<T, HD, RANGE>::BYTES / 2 / NW + 511) / 512 * 512 : 0;   // of each wave's part; rows stay aligned
+  static_assert(!MIXED || FRONT * NW * 2 >= TileLds<T, HD, RANGE>::BYTES, "a tile's LDS");
+  __shared__ __attribute__((aligned(1024))) T lds[NW][PARTS * TILE > FRONT ? PARTS * TILE : FRONT];   // at the end: O f32 [NW][BM][HD]
   __shared__ float2_t ml[NW][BM];
-  typedef std::conditional_t<FORM == RANGE, unsigned, int> bad_t;   // as in attend_tile_kernel
+  typedef std::conditional_t<FORM == RANGE, unsigned, int> bad_t;   // as TileLds
   __shared__ bad_t bad[NW][3][HD];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hk = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv;
   Item it;
-  if (!find_item<KV, BM, false, FORM>(p, index, it)) return;
+  const bool some = find_item<KV, BM, false, FORM, BMF>(p, index, it);
+  if constexpr (FORM == RANGE)
+    if (KV != KV_ROWS && p.N && blockIdx.x == 0 && wave == 0) leave_head<HD, KV, BM, BMF>(p, some ? it.c : 1, lane);
+  if (!some) return;
+  if constexpr (MIXED)
+    if (it.front) {
+      tile_item<T, HD, KV, 4, RANGE, BM>(p, it, hk, reinterpret_cast<char*>(&lds));
+      return;
+    }
   if constexpr (FORM == RANGE) it.whole = it.front && front_is_whole<KV>(p, it, lane);
   R r;
   r.template begin<KV>(p, it, hk, it.tile * BM + lane % BM, lane);
@@ -1398,58 +1539,60 @@ __global__ __launch_bounds__(64 * FEW_WAVES, few_at_once(R::BM, HD, KV == KV_E4M
       sum += f * x[1];
       a += f * *reinterpret_cast<const float4_t*>(ob + (w * BM + q) * HD + ((c ^ (q & 7)) << 2));
     }
-    if (it.nch == 1 && (FORM != RANGE || !p.N)) {
+    if (it.nch == 1 && (FORM != RANGE || KV == KV_ROWS || !p.N)) {
       const float rs = sum == 0.f ? 0.f : 1.0f / sum;
       const int row = it.tile * BM + q, tok = row / p.G;
       T* out = static_cast<T*>(p.out) + (long)(it.s.q0 + tok) * p.o_st + (long)(hk * p.G + row - tok * p.G) * p.o_sh + c * 4;
       const auto x = pack2<T>(a[0] * rs, a[1] * rs), y = pack2<T>(a[2] * rs, a[3] * rs);
       *reinterpret_cast<typename Elem<T>::v4*>(out) = typename Elem<T>::v4{x[0], x[1], y[0], y[1]};
     } else {
-      const long row = ((long)(it.base + it.chunk) * p.Hkv + hk) * BM + q;
+      const long row = part_row<BM, BMF, FORM>(p, it, hk, q);
+      if (FORM == RANGE && row < 0) continue;
       *reinterpret_cast<float4_t*>(part_o<HD>(p, row) + c * 4) = a;
       if (c == 0) *part_ml<HD>(p, row) = float2_t{M, sum};
     }
-  }
+  }  if constexpr (FORM == RANGE)
+    if (KV != KV_ROWS && p.N && wave == 0) leave_parts<HD, KV, BM, BMF>(p, it, hk, it.tile, lane);
 }
 
-// Where the parts of a sequence's group are: its first item, items a tile, rows; nch 0: no group.
-struct Front {
-  int base, nch, q0;
-  long rows;
-};
-template <int KV, int BM>
-__device__ __forceinline__ Front front_of(const AttendParams& p, const Item& it) {
-  Front f{};
-  const int g = group_of(p, it.v - p.N), lane = threadIdx.x & 63;
-  if (g < 0) return f;
-  for (int g0 = 0; g0 <= g; g0 += 64) {
-    Piece x{};
-    int nch = 0, items = 0;
-    if (g0 + lane <= g) {
-      x = piece<KV>(p, g0 + lane);
-      nch = max(1, (blocks_of<BM>(p, x) + it.c - 1) / it.c);
-      items = tiles_of<KV, BM>(x.s, p.G) * nch;
+// One group's (cg of CG) share of nch parts of a row, the first at `row`, added to a (chunk c), its sum and maximum.
+template <int HD, int CG>
+__device__ __forceinline__ void add_parts(const AttendParams& p, long row, long pitch, int nch, int cg, int c, float& M, float& sum, float4_t& a) {
+  // four at a time, their loads together
+  constexpr int AT = 4;
+  for (int n0 = cg; n0 < nch; n0 += AT * CG) {
+    float2_t x[AT];
+    float4_t y[AT];
+#pragma unroll
+    for (int i = 0; i < AT; ++i) {
+      const long at = row + (long)min(n0 + i * CG, nch - 1) * pitch;
+      x[i] = *part_ml<HD>(p, at);
+      y[i] = *reinterpret_cast<const float4_t*>(part_o<HD>(p, at) + c * 4);
     }
-    const int all = lane63(lanes_scan(items));
-    if (g < g0 + 64) {
-      const int w = g - g0;
-      f.base += all - __builtin_amdgcn_readlane(items, w);
-      f.nch = __builtin_amdgcn_readlane(nch, w);
-      f.q0 = __builtin_amdgcn_readlane(x.s.q0, w);
-      f.rows = (long)__builtin_amdgcn_readlane(x.s.nq, w) * p.G;
-      if (__builtin_amdgcn_readlane(x.s.nk, w) <= 0 || f.base < 0) f.nch = 0;
-    } else {
-      f.base += all;
+    float m = M;
+#pragma unroll
+    for (int i = 0; i < AT; ++i) {
+      if (n0 + i * CG >= nch) x[i] = float2_t{-INFINITY, 0.f};
+      m = fmaxf(m, x[i][0]);
+    }
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - m);
+    M = m;
+    sum *= f;
+    a *= f;
+#pragma unroll
+    for (int i = 0; i < AT; ++i) {
+      if (x[i][1] == 0.f) continue;   // saw no key, has no O
+      const float h = __builtin_amdgcn_exp2f(x[i][0] - m);
+      sum += x[i][1] * h;
+      a += y[i] * h;
     }
   }
-  return f;
 }
 
 // ---- the chunks of a tile joined ----------------------------------------------------------
 // HD / 4 lanes a row, RP rows and CG groups of chunks a workgroup of 256.  Its work is small (4
 // to 10 us); a launch of its own, as the last workgroup of a tile doing it needs counters that
 // are zero at the start, and the workspace comes with whatever it held.
-// RANGE, shared pages: a sequence's own chunks, then those of its group's front.
 template <typename T, int HD, int KV, int BM, int FORM>
 __global__ __launch_bounds__(256) void attend_join_kernel(const AttendParams p) {
   constexpr int LPR = HD / 4, CG = BM <= 32 ? 256 / LPR : 1, RP = 256 / LPR / CG;
@@ -1458,11 +1601,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const AttendParams p) 
   const int hk = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv;
   Item it;
   // (offsets that do not ascend may name more rows than there are: what has no item has no sums)
-  if (!find_item<KV, BM, true, FORM>(p, index, it) || it.base < 0 || it.base + it.nch > p.items) return;
-  const bool shared = FORM == RANGE && p.N;
-  if (shared ? it.front : it.nch == 1) return;
-  Front fr{};
-  if (shared) fr = front_of<KV, BM>(p, it);
+  if (!find_item<KV, BM, true, FORM>(p, index, it) || it.nch == 1 || it.base < 0 || it.base + it.nch > p.items) return;
   const int c = threadIdx.x % LPR, cg = CG > 1 ? threadIdx.x / LPR : 0;
   const int q = blockIdx.y * RP + (CG > 1 ? 0 : threadIdx.x / LPR);
   const int tile = BM <= 32 ? it.tile : tiles_of<KV, BM>(it.s, p.G) - 1 - it.tile;
@@ -1470,49 +1609,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const AttendParams p) 
   if (CG > 1 && !in) return;
   float M = -INFINITY, sum = 0.f;
   float4_t a = {0.f, 0.f, 0.f, 0.f};
-  auto add = [&](const long row, const int nch) {
-    // four at a time, their loads together
-    constexpr int AT = 4;
-    for (int n0 = cg; n0 < nch; n0 += AT * CG) {
-      float2_t x[AT];
-      float4_t y[AT];
-#pragma unroll
-      for (int i = 0; i < AT; ++i) {
-        const long at = row + (long)min(n0 + i * CG, nch - 1) * p.Hkv * BM;
-        x[i] = *part_ml<HD>(p, at);
-        y[i] = *reinterpret_cast<const float4_t*>(part_o<HD>(p, at) + c * 4);
-      }
-      float m = M;
-#pragma unroll
-      for (int i = 0; i < AT; ++i) {
-        if (n0 + i * CG >= nch) x[i] = float2_t{-INFINITY, 0.f};
-        m = fmaxf(m, x[i][0]);
-      }
-      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - m);
-      M = m;
-      sum *= f;
-      a *= f;
-#pragma unroll
-      for (int i = 0; i < AT; ++i) {
-        if (x[i][1] == 0.f) continue;   // saw no key, has no O
-        const float h = __builtin_amdgcn_exp2f(x[i][0] - m);
-        sum += x[i][1] * h;
-        a += y[i] * h;
-      }
-    }
-  };
-  if (in) {
-    add(((long)it.base * p.Hkv + hk) * BM + q, it.nch);
-    if (shared && fr.nch) {
-      // the same row among the group's
-      const long of = ((long)it.s.q0 - fr.q0) * p.G + (long)tile * BM + q;
-      if (of >= 0 && of < fr.rows) {
-        const int ft = (int)(of / BM), item = BM <= 32 ? ft : (int)((fr.rows + BM - 1) / BM) - 1 - ft;
-        const long base = (long)fr.base + (long)item * fr.nch;
-        if (base + fr.nch <= p.items) add((base * p.Hkv + hk) * BM + of % BM, fr.nch);
-      }
-    }
-  }
+  if (in) add_parts<HD, CG>(p, ((long)it.base * p.Hkv + hk) * BM + q, (long)p.Hkv * BM, it.nch, cg, c, M, sum, a);
   if constexpr (CG > 1) {
     so[cg][c] = a;
     if (c == 0) sm[cg] = float2_t{M, sum};
@@ -1538,20 +1635,96 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const AttendParams p) 
   *reinterpret_cast<typename Elem<T>::v4*>(out) = typename Elem<T>::v4{x[0], x[1], y[0], y[1]};
 }
 
+// Shared pages: a sequence's own parts and those of its group's front, by the Parts that the launch before left.
+template <typename T, int HD, int BM, int BMF>
+__global__ __launch_bounds__(256) void attend_join_shared_kernel(const AttendParams p) {
+  constexpr int LPR = HD / 4, CG = BM <= 32 ? 256 / LPR : 1, RP = 256 / LPR / CG;
+  __shared__ float4_t so[CG][LPR];
+  __shared__ float2_t sm[CG];
+  const int hk = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv;
+  const int tiles = parts_head<HD>(p)[0], fronts = parts_head<HD>(p)[1];
+  const Parts x = parts_at<HD>(p)[index];
+  const int c = threadIdx.x % LPR, cg = CG > 1 ? threadIdx.x / LPR : 0;
+  const int q = blockIdx.y * RP + (CG > 1 ? 0 : threadIdx.x / LPR);
+  // (offsets that do not ascend may name more rows than there are; a tile without an item then has no Parts, and what
+  // stands there is held to the tensors)
+  const bool sound = index < tiles && fronts >= 0 && fronts <= p.front_items && x.nch > 0 && x.own >= 0 && x.own <= p.own_items - x.nch &&
+                     x.rows <= BM && x.row0 >= 0 && x.q0 >= 0 && (long)x.q0 * p.G + x.row0 + x.rows <= (long)p.Tq * p.G;
+  const bool in = sound && q < x.rows;
+  if (CG > 1 && !in) return;
+  float M = -INFINITY, sum = 0.f;
+  float4_t a = {0.f, 0.f, 0.f, 0.f};
+  if (in) {
+    add_parts<HD, CG>(p, (long)fronts * p.Hkv * BMF + ((long)x.own * p.Hkv + hk) * BM + q, (long)p.Hkv * BM, x.nch, cg, c, M, sum, a);
+    const int of = x.frow0 + q;
+    if (x.fnch > 0 && x.frow0 >= 0 && of < x.frows) {
+      // its tile of the group's rows; those of 128 are in order of falling length
+      const int ft = of / BMF, item = x.front + (BMF <= 32 ? ft : (x.frows + BMF - 1) / BMF - 1 - ft) * x.fnch;
+      if (item >= 0 && item <= fronts - x.fnch)
+        add_parts<HD, CG>(p, ((long)item * p.Hkv + hk) * BMF + of % BMF, (long)p.Hkv * BMF, x.fnch, cg, c, M, sum, a);
+    }
+  }
+  if constexpr (CG > 1) {
+    so[cg][c] = a;
+    if (c == 0) sm[cg] = float2_t{M, sum};
+    __syncthreads();
+    if (cg) return;
+#pragma unroll
+    for (int w = 1; w < CG; ++w) M = fmaxf(M, sm[w][0]);
+    sum = 0.f;
+    a = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < CG; ++w) {
+      if (sm[w][1] == 0.f) continue;
+      const float f = __builtin_amdgcn_exp2f(sm[w][0] - M);
+      sum += f * sm[w][1];
+      a += f * so[w][c];
+    }
+  }
+  if (!in) return;
+  const float rs = sum == 0.f ? 0.f : 1.0f / sum;
+  const int row = x.row0 + q, tok = row / p.G;
+  T* out = static_cast<T*>(p.out) + (long)(x.q0 + tok) * p.o_st + (long)(hk * p.G + row - tok * p.G) * p.o_sh + c * 4;
+  const auto u = pack2<T>(a[0] * rs, a[1] * rs), v = pack2<T>(a[2] * rs, a[3] * rs);
+  *reinterpret_cast<typename Elem<T>::v4*>(out) = typename Elem<T>::v4{u[0], u[1], v[0], v[1]};
+}
+
 // ---- host ---------------------------------------------------------------------------------
 // The form of a call: rows per tile, items per K/V head to aim at (0: keys are not split).
 struct Plan {
   int bm, target, min_blocks;
+  int bmf;             // shared pages: rows of the fronts' tiles
+  long front_items, own_items;
   long tiles, items;   // at most
 };
+template <typename T, int HD, int KV>
+void launch_shared(const AttendParams& p, const Plan& pl, hipStream_t s) {
+  const dim3 grid((unsigned)(pl.items * p.Hkv));
+  const unsigned tiles = (unsigned)(pl.tiles * p.Hkv);
+  if (pl.bmf == 16) {
+    CK_LAUNCH((attend_few_kernel<T, HD, KV, Rows16<T, HD, RANGE>, RANGE>), grid, dim3(256), 0, s, p);
+    CK_LAUNCH((attend_join_shared_kernel<T, HD, 16, 16>), dim3(tiles, 16), dim3(256), 0, s, p);
+  } else if (pl.bmf == 32) {
+    CK_LAUNCH((attend_few_kernel<T, HD, KV, Rows<T, HD, RANGE>, RANGE>), grid, dim3(256), 0, s, p);
+    CK_LAUNCH((attend_join_shared_kernel<T, HD, 32, 32>), dim3(tiles, 32), dim3(256), 0, s, p);
+  } else if (pl.bm == 16) {
+    CK_LAUNCH((attend_few_kernel<T, HD, KV, Rows16<T, HD, RANGE>, RANGE, true>), grid, dim3(256), 0, s, p);
+    CK_LAUNCH((attend_join_shared_kernel<T, HD, 16, 128>), dim3(tiles, 16), dim3(256), 0, s, p);
+  } else {
+    CK_LAUNCH((attend_tile_kernel<T, HD, KV, 4, RANGE>), grid, dim3(256), 0, s, p);
+    CK_LAUNCH((attend_join_shared_kernel<T, HD, 128, 128>), dim3(tiles, 128 / (1024 / HD)), dim3(256), 0, s, p);
+  }
+}
 template <typename T, int HD, int KV, int FORM>
 void launch_kv(const AttendParams& p, const Plan& pl, hipStream_t s) {
+  if constexpr (FORM == RANGE && KV != KV_ROWS)
+    if (p.N) return launch_shared<T, HD, KV>(p, pl, s);
   const dim3 grid((unsigned)(pl.items * p.Hkv));
   if (pl.bm == 16) CK_LAUNCH((attend_few_kernel<T, HD, KV, Rows16<T, HD, FORM>, FORM>), grid, dim3(64 * FEW_WAVES), 0, s, p);
   else if (pl.bm == 32) CK_LAUNCH((attend_few_kernel<T, HD, KV, Rows<T, HD, FORM>, FORM>), grid, dim3(64 * FEW_WAVES), 0, s, p);
   else if (pl.bm == 128) CK_LAUNCH((attend_tile_kernel<T, HD, KV, 4, FORM>), grid, dim3(256), 0, s, p);
   else if constexpr (FORM == WHOLE) CK_LAUNCH((attend_tile_kernel<T, HD, KV, 8, FORM>), grid, dim3(512), 0, s, p);
-  if (!pl.target && !p.N) return;
+  if (!pl.target) return;
   const unsigned tiles = (unsigned)(pl.tiles * p.Hkv);
   if (pl.bm == 16) CK_LAUNCH((attend_join_kernel<T, HD, KV, 16, FORM>), dim3(tiles, 16), dim3(256), 0, s, p);
   else if (pl.bm == 32) CK_LAUNCH((attend_join_kernel<T, HD, KV, 32, FORM>), dim3(tiles, 32), dim3(256), 0, s, p);
@@ -1607,7 +1780,9 @@ void attend_launch(const std::string& w, AttendParams& p, const AttendQuery& a, 
   p.min_blocks = pl.min_blocks;
   p.ws = a.ws;
   p.items = (int)pl.items;
-  p.part_rows = pl.items * p.Hkv * pl.bm;
+  p.part_rows = p.N ? (pl.front_items * pl.bmf + pl.own_items * pl.bm) * p.Hkv : pl.items * p.Hkv * pl.bm;
+  p.front_items = (int)pl.front_items;
+  p.own_items = (int)pl.own_items;
   if (a.dtype == DT_F16) {
     if (a.head_dim == 64) launch_hd<half_t, 64, FORM>(p, kv, pl, s);
     else launch_hd<half_t, 128, FORM>(p, kv, pl, s);

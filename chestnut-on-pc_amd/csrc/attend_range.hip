@@ -11,15 +11,26 @@ Plan range_plan(int B, int Tq, long keys, int n_heads, int n_kv, int window, int
   Plan pl{};
   const int G = n_heads / n_kv;
   const long rows = (long)Tq * G;
-  // the rows that share keys: a sequence's, or a group's
-  const long units = groups ? groups : B;
-  pl.bm = rows <= 16 * units ? 16 : rows <= 32 * units ? 32 : 128;
-  pl.tiles = groups ? 2 * (rows / pl.bm) + B + groups : rows / pl.bm + B;
+  if (groups) {
+    // the rows that share keys are a group's
+    pl.bmf = rows <= 16L * groups ? 16 : rows <= 32L * groups ? 32 : 128;
+    pl.bm = pl.bmf < 128 ? pl.bmf : rows <= 16L * B ? 16 : 128;
+    pl.tiles = rows / pl.bm + B;                // the sequences' own
+    const long fronts = rows / pl.bmf + groups, slots = pl.bmf == 128 ? 512 : pl.bmf == 16 && few3 ? 768 : 1024;
+    pl.min_blocks = pl.bmf <= 32 ? 2 : 4;
+    const bool many = pl.bmf == 128 && (fronts + pl.tiles) * n_kv >= 2 * slots;
+    if (!many && keys / B > 2 * pl.min_blocks * AT_KEYS) pl.target = (int)std::max(1L, slots / n_kv);
+    pl.front_items = fronts + pl.target;
+    pl.own_items = pl.tiles + pl.target;
+    pl.items = fronts + pl.tiles + pl.target;
+    return pl;
+  }
+  pl.bm = rows <= 16L * B ? 16 : rows <= 32L * B ? 32 : 128;
+  pl.tiles = rows / pl.bm + B;
   const long slots = pl.bm == 128 ? 512 : pl.bm == 16 && few3 ? 768 : 1024;
   pl.min_blocks = pl.bm <= 32 ? 2 : 4;
   const bool many = pl.bm == 128 && pl.tiles * n_kv >= 2 * slots;
-  long each = keys / B;
-  if (window) each = std::min(each, (long)window + sinks + pl.bm / G);
+  const long each = std::min(keys / B, (long)window + sinks + pl.bm / G);
   if (!many && each > 2 * pl.min_blocks * AT_KEYS) pl.target = (int)std::max(1L, slots / n_kv);
   pl.items = pl.tiles + pl.target;
   return pl;
@@ -29,7 +40,9 @@ Plan range_plan(int B, int Tq, long keys, int n_heads, int n_kv, int window, int
 
 size_t attend_range_floats(int B, int Tq, long keys, int n_heads, int n_kv, int head_dim, int window, int sinks, int groups) {
   const Plan pl = range_plan(B, Tq, keys, n_heads, n_kv, window, sinks, groups);
-  return pl.target || groups ? (size_t)pl.items * n_kv * pl.bm * (head_dim + 2) : 0;
+  if (groups)
+    return (size_t)(pl.front_items * pl.bmf + pl.own_items * pl.bm) * n_kv * (head_dim + 2) + 4 + (size_t)pl.own_items * (sizeof(Parts) / 4);
+  return pl.target ? (size_t)pl.items * n_kv * pl.bm * (head_dim + 2) : 0;
 }
 
 void launch_attend_range(const char* what, AttendParams& p, const AttendQuery& a, int kv, long keys, hipStream_t s) {
