@@ -102,35 +102,6 @@ __device__ __forceinline__ int group_of(const AttendParams& p, int b) {
   }
   return p.cu_s[lo] <= b && b < p.cu_s[lo + 1] ? lo : -1;
 }
-// A piece of work: sequence b, or what group g shares (front).  row: of the table; first: the keys
-// below are another piece's; s1: front: its sequences are row .. s1.
-struct Piece {
-  Seq s;
-  int row, first, s1;
-};
-// pieces: the groups' fronts, then the sequences
-template <int KV>
-__device__ __forceinline__ Piece piece(const AttendParams& p, int v) {
-  Piece x{};
-  if (v >= p.N) {
-    const int b = v - p.N;
-    x.s = sequence<KV>(p, b);
-    x.row = b;
-    if (p.N) {
-      const int g = group_of(p, b);
-      if (g >= 0) x.first = shared_keys(p, g);
-    }
-    return x;
-  }
-  const int s0 = min(max(p.cu_s[v], 0), p.B);
-  x.s1 = min(max(p.cu_s[v + 1], s0), p.B);
-  x.s.q0 = min(max(p.cu_q[s0], 0), p.Tq);
-  x.s.nq = min(max(p.cu_q[x.s1], x.s.q0), p.Tq) - x.s.q0;
-  x.s.nk = shared_keys(p, v);
-  x.row = min(s0, p.B - 1);
-  return x;
-}
-
 // ---- which part of the work a workgroup does -------------------------------------------
 // A sequence's rows make tiles of BM; a tile's keys make chunks of `c` blocks of 64, so that
 // about `target` items of equal length per K/V head fill the card whatever the lengths are:
@@ -143,13 +114,20 @@ __device__ __forceinline__ Piece piece(const AttendParams& p, int v) {
 // chunks 78 -> 83.  Dividing all blocks of keys exactly, with several pieces a workgroup,
 // measured no faster for single tokens and 80 -> 115 us for mixed chunks (the loop over pieces
 // costs the tile loop its registers).
+// Where the parts of a sequence's group are: its first item, chunks, first query, rows; nch 0: no group.
+struct Front {
+  int base, nch, q0;
+  long rows;
+};
 struct Item {
   int b, tile, chunk, nch, c, base;   // base: the tile's first item; b: the row of the table
   Seq s;
-  // RANGE (Piece); whole: every row of a front sees all its keys
-  int v, first, s1;
+  // shared pages: front: the keys that the sequences b .. s1 share (s: their queries); whole: every row sees
+  // all of them.  Else first: the keys below are the front's, of which f says where its parts are; rank: the
+  // tile's number among the sequences' own ones; fronts: items of all fronts
   bool front, whole;
-  int fronts, rank;                 // items of all fronts; the tile's number among the sequences' own ones
+  int s1, first, rank, fronts;
+  Front f;
 };
 
 template <int KV, int BM>
@@ -157,14 +135,12 @@ __device__ __forceinline__ int tiles_of(const Seq& s, int G) {
   return (int)(((long)s.nq * G + BM - 1) / BM);
 }
 __device__ __forceinline__ int blocks_of(int keys) { return (keys + AT_KEYS - 1) / AT_KEYS; }
-// RANGE: the most blocks that a tile of BM rows of a piece has
+// through a window: the most blocks that a tile of BM rows of a sequence has
 template <int BM>
-__device__ __forceinline__ int blocks_of(const AttendParams& p, const Piece& x) {
-  const int all = max(0, blocks_of(x.s.nk) - x.first / AT_KEYS);
-  if (p.N) return all;
+__device__ __forceinline__ int window_blocks(const AttendParams& p, const Seq& s) {
   // its rows are of (BM - 1) / G + 2 neighbouring tokens at most, and see this many keys together, from any place on
-  const int tokens = min(x.s.nq, (BM - 1) / p.G + 2);
-  return min(all, blocks_of(min(p.sinks, x.s.nk)) + (p.window + tokens + 2 * AT_KEYS - 3) / AT_KEYS);
+  const int tokens = min(s.nq, (BM - 1) / p.G + 2);
+  return min(blocks_of(s.nk), blocks_of(min(p.sinks, s.nk)) + (p.window + tokens + 2 * AT_KEYS - 3) / AT_KEYS);
 }
 
 // Sum over lanes 0..l, in lane l (DPP: six steps without LDS).
@@ -185,29 +161,20 @@ __device__ __forceinline__ N lanes_scan(N v) {
 }
 __device__ __forceinline__ int lane63(int v) { return __builtin_amdgcn_readlane(v, 63); }
 
-// index counts items, or tiles where TILES.  False: there are not so many.  BMF: rows of a front's tiles.
-template <int KV, int BM, bool TILES, int FORM, int BMF = BM>
+// index counts items, or tiles where TILES.  False: there are not so many.
+template <int KV, int BM, bool TILES, int FORM>
 __device__ __forceinline__ bool find_item(const AttendParams& p, int index, Item& it) {
   const int lane = threadIdx.x & 63;
-  const int count = FORM == RANGE ? p.B + p.N : p.B;
   // the first 64 sequences, one a lane
   Seq s{};
-  Piece x{};
   int tiles = 0, blocks = 0;
   auto get = [&](int b0) {
     s = Seq{};
-    x = Piece{};
     tiles = blocks = 0;
-    if (b0 + lane < count) {
-      if constexpr (FORM == RANGE) {
-        x = piece<KV>(p, b0 + lane);
-        s = x.s;
-        blocks = blocks_of<BM>(p, x);
-      } else {
-        s = sequence<KV>(p, b0 + lane);
-        blocks = blocks_of(s.nk);
-      }
-      tiles = FORM == RANGE && BMF != BM && b0 + lane < p.N ? tiles_of<KV, BMF>(s, p.G) : tiles_of<KV, BM>(s, p.G);
+    if (b0 + lane < p.B) {
+      s = sequence<KV>(p, b0 + lane);
+      tiles = tiles_of<KV, BM>(s, p.G);
+      blocks = FORM == RANGE ? window_blocks<BM>(p, s) : blocks_of(s.nk);
     }
   };
   get(0);
@@ -218,24 +185,23 @@ __device__ __forceinline__ bool find_item(const AttendParams& p, int index, Item
     // than an int holds in all; past 2^29 the number itself does not count)
     constexpr int MOST = 1 << 29;
     int all = min(lane63(lanes_scan(tiles)), MOST);
-    for (int b0 = 64; b0 < count; b0 += 64) {
+    for (int b0 = 64; b0 < p.B; b0 += 64) {
       get(b0);
       work += readlane_f32(lanes_scan((float)tiles * (float)blocks), 63);
       all = min(all + lane63(lanes_scan(tiles)), MOST);
     }
-    // each tile adds up to one item that is not full (shared pages: most tiles are a sequence's own few keys, and
-    // the fronts' items as long as their share of the card)
-    const int full = FORM == RANGE && p.N ? p.target : max(p.target - all, (p.target + 1) >> 1);
+    // each tile adds up to one item that is not full
+    const int full = max(p.target - all, (p.target + 1) >> 1);
     if (work < 16777216.f) {   // a whole number
       const int w = (int)work;
       c = max(p.min_blocks, (w + full - 1) / full);
-      if (count <= 16 && !(FORM == RANGE && p.N)) {
+      if (p.B <= 16) {
         // few sequences: lane i counts the items that chunks of c0 + i blocks make, and the shortest
         // chunk that does not make too many is taken (eight chunks and tokens, 80 -> 76 us)
         const int c0 = max(p.min_blocks, (w + p.target - 1) / p.target), ci = c0 + lane;
         const float inv = __builtin_amdgcn_rcpf((float)ci);
         int items = 0;
-        for (int b = 0; b < count; ++b) {
+        for (int b = 0; b < p.B; ++b) {
           const int nb = __builtin_amdgcn_readlane(blocks, b), nt = __builtin_amdgcn_readlane(tiles, b);
           const int q = (int)((float)nb * inv + 0.5f);   // nb / ci to the nearest: the ceiling is it or the next
           items += nt * max(1, q + (q * ci < nb ? 1 : 0));
@@ -247,20 +213,14 @@ __device__ __forceinline__ bool find_item(const AttendParams& p, int index, Item
       c = max(p.min_blocks, (int)fminf(work / (float)full * 1.0001f, 1e9f) + 1);
     }
     c = __builtin_amdgcn_readfirstlane(c);
-    if (count > 64) get(0);
+    if (p.B > 64) get(0);
   }
-  int base = 0, fronts = 0, rank = 0;
-  for (int b0 = 0; b0 < count; b0 += 64) {
+  int base = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
     if (b0) get(b0);
     const int nch = max(1, (blocks + c - 1) / c), items = tiles * nch;
     const int si = lanes_scan(items), su = TILES ? lanes_scan(tiles) : si;
     const unsigned long long m = __ballot(su > index);
-    int so = 0;   // own tiles up to the lane's
-    if constexpr (FORM == RANGE)
-      if (p.N) {
-        so = lanes_scan(b0 + lane < p.N ? 0 : tiles);
-        if (b0 < p.N) fronts += lane63(lanes_scan(b0 + lane < p.N ? items : 0));
-      }
     if (m) {
       const int w = __ffsll(m) - 1;
       const int local = __builtin_amdgcn_readlane(index - (su - (TILES ? tiles : items)), w);
@@ -275,23 +235,13 @@ __device__ __forceinline__ bool find_item(const AttendParams& p, int index, Item
       it.s.k0 = __builtin_amdgcn_readlane(s.k0, w);
       it.s.nk = __builtin_amdgcn_readlane(s.nk, w);
       // the compiler does not see that these are the same for all lanes
-      for (int* i : {&it.b, &it.tile, &it.chunk, &it.nch, &it.c, &it.base, &it.s.q0, &it.s.nq, &it.s.k0, &it.s.nk})
-        *i = __builtin_amdgcn_readfirstlane(*i);
-      if constexpr (FORM == RANGE) {
-        it.v = it.b;
-        it.front = it.b < p.N;
-        it.b = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_readlane(x.row, w));
-        it.first = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_readlane(x.first, w));
-        it.s1 = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_readlane(x.s1, w));
-        it.whole = false;
-        it.fronts = fronts;
-        it.rank = rank + __builtin_amdgcn_readlane(so - (b0 + lane < p.N ? 0 : tiles), w) + it.tile;
-      }
+      for (int* x : {&it.b, &it.tile, &it.chunk, &it.nch, &it.c, &it.base, &it.s.q0, &it.s.nq, &it.s.k0, &it.s.nk})
+        *x = __builtin_amdgcn_readfirstlane(*x);
+      if (FORM == RANGE) it.front = it.whole = false;
       return true;
     }
     index -= lane63(su);
     base += lane63(si);
-    if (FORM == RANGE) rank += lane63(so);
   }
   return false;
 }
@@ -299,6 +249,196 @@ __device__ __forceinline__ bool find_item(const AttendParams& p, int index, Item
 // keys that query tok of a sequence sees: all below this
 __device__ __forceinline__ int keys_of(const AttendParams& p, const Seq& s, int tok) {
   return p.causal ? min(s.nk, max(0, tok + 1 + s.nk - s.nq)) : s.nk;
+}
+
+// Shared pages: the pieces are what the groups share (fronts, tiles of BMF rows) and the keys behind
+// that of every sequence (tiles of BM), the fronts' items first.  All loads of the first 64 groups and 64 sequences are
+// sent for together, and their answers stay in registers: what a workgroup does before its first key counts
+// for as much as several blocks of keys (64 streams on two groups' pages 52.4 us where the lengths were read again and
+// again, 47.3 so).  tiles_all: own tiles of all.
+template <int KV, int BM, int BMF>
+__device__ __forceinline__ bool find_shared(const AttendParams& p, int index, Item& it, int& tiles_all) {
+  const int lane = threadIdx.x & 63;
+  constexpr int MOST = 1 << 29;   // as in find_item
+  it = Item{};
+  // a group a lane
+  int c0 = 0, c1 = 0, share = 0, s0 = 0, s1 = 0, ftiles = 0;
+  Seq fs{};
+  auto get_fronts = [&](int g0) {
+    c0 = c1 = share = s0 = s1 = ftiles = 0;
+    fs = Seq{};
+    if (g0 + lane < p.N) {
+      c0 = p.cu_s[g0 + lane];
+      c1 = p.cu_s[g0 + lane + 1];
+      share = shared_keys(p, g0 + lane);
+    }
+  };
+  auto get_fronts_queries = [&](int g0) {
+    if (g0 + lane < p.N) {
+      s0 = min(max(c0, 0), p.B);
+      s1 = min(max(c1, s0), p.B);
+      fs.q0 = min(max(p.cu_q[s0], 0), p.Tq);
+      fs.nq = min(max(p.cu_q[s1], fs.q0), p.Tq) - fs.q0;
+      fs.nk = share;
+      ftiles = tiles_of<KV, BMF>(fs, p.G);
+    }
+  };
+  // a sequence a lane
+  Seq s{};
+  int g = -1, first = 0, tiles = 0, blocks = 0;
+  auto get_own = [&](int b0) {
+    s = Seq{};
+    if (b0 + lane < p.B) s = sequence<KV>(p, b0 + lane);
+  };
+  auto group_own = [&](int b0) {
+    g = -1;
+    first = tiles = blocks = 0;
+    if (p.N <= 64) {
+      for (int j = 0; j < p.N; ++j)
+        if (b0 + lane >= __builtin_amdgcn_readlane(c0, j) && b0 + lane < __builtin_amdgcn_readlane(c1, j)) {
+          g = j;
+          first = __builtin_amdgcn_readlane(share, j);
+        }
+    } else if (b0 + lane < p.B) {
+      g = group_of(p, b0 + lane);
+      if (g >= 0) first = shared_keys(p, g);
+    }
+    if (b0 + lane < p.B) {
+      tiles = tiles_of<KV, BM>(s, p.G);
+      blocks = max(0, blocks_of(s.nk) - first / AT_KEYS);
+    }
+  };
+  get_fronts(0);
+  get_own(0);
+  get_fronts_queries(0);
+  group_own(0);
+  // how long a chunk is, whether every query of a group sees all that it shares, and how many own tiles there are
+  float work = readlane_f32(lanes_scan((float)ftiles * (float)blocks_of(fs.nk)), 63);
+  for (int g0 = 64; g0 < p.N; g0 += 64) {
+    get_fronts(g0);
+    get_fronts_queries(g0);
+    work += readlane_f32(lanes_scan((float)ftiles * (float)blocks_of(fs.nk)), 63);
+  }
+  bool whole = true;
+  tiles_all = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    if (b0) {
+      get_own(b0);
+      group_own(b0);
+    }
+    work += readlane_f32(lanes_scan((float)tiles * (float)blocks), 63);
+    tiles_all = min(tiles_all + lane63(lanes_scan(tiles)), MOST);
+    whole = whole && __all(g < 0 || s.nq <= 0 || keys_of(p, s, 0) >= first);
+  }
+  int c = 1 << 30;
+  if (p.target)
+    c = max(p.min_blocks, work < 16777216.f ? ((int)work + p.target - 1) / p.target : (int)fminf(work / (float)p.target * 1.0001f, 1e9f) + 1);
+  auto chunks = [&](int blocks) { return max(1, (blocks + c - 1) / c); };
+  // up to half as long again where no more items than run at once come of it (a second round begins anew: 32 tokens on
+  // 37376 shared keys 36.0 -> 34.4 us, 64 on two groups' 47.4 -> 44; twice as long, with many tiny tiles, 37 -> 41)
+  if (p.target && p.N <= 64 && p.B <= 64) {
+    const int least = c;
+#pragma unroll 1
+    for (int i = 4; i <= 6; ++i) {
+      c = max(least * i / 4, least + (i > 4));
+      if (lane63(lanes_scan(ftiles * chunks(blocks_of(fs.nk)) + tiles * chunks(blocks))) <= p.target) break;
+      if (i == 6) {
+        c = least;
+        break;
+      }
+    }
+  }
+  c = __builtin_amdgcn_readfirstlane(c);
+  // the fronts
+  it.c = c;
+  it.whole = __builtin_amdgcn_readfirstlane(whole ? 1 : 0);
+  bool found = false;
+  int base = 0, fbase = 0, fnch = 0;
+  for (int g0 = 0; g0 < p.N; g0 += 64) {
+    if (p.N > 64) {
+      get_fronts(g0);
+      get_fronts_queries(g0);
+    }
+    fnch = chunks(blocks_of(fs.nk));
+    const int items = ftiles * fnch, si = lanes_scan(items);
+    fbase = base + si - items;
+    const unsigned long long m = __ballot(base + si > index);
+    if (m && !found) {
+      const int w = __ffsll(m) - 1, local = index - __builtin_amdgcn_readlane(fbase, w);
+      found = true;
+      it.front = true;
+      it.nch = __builtin_amdgcn_readlane(fnch, w);
+      // all tiles' first chunks, then their second ones ...: the last ones are short
+      it.chunk = local / __builtin_amdgcn_readlane(ftiles, w);
+      it.tile = local - it.chunk * __builtin_amdgcn_readlane(ftiles, w);
+      it.base = index - it.chunk;
+      it.b = min(__builtin_amdgcn_readlane(s0, w), p.B - 1);
+      it.s1 = __builtin_amdgcn_readlane(s1, w);
+      it.s.q0 = __builtin_amdgcn_readlane(fs.q0, w);
+      it.s.nq = __builtin_amdgcn_readlane(fs.nq, w);
+      it.s.k0 = 0;
+      it.s.nk = __builtin_amdgcn_readlane(fs.nk, w);
+      it.first = it.rank = 0;
+    }
+    base += lane63(si);
+  }
+  it.fronts = base;
+  // the sequences' own keys
+  int rank = 0;
+  for (int b0 = 0; b0 < p.B && !found; b0 += 64) {
+    if (p.B > 64) {
+      get_own(b0);
+      group_own(b0);
+    }
+    const int nch = chunks(blocks), items = tiles * nch, si = lanes_scan(items), so = lanes_scan(tiles);
+    const unsigned long long m = __ballot(base + si > index);
+    if (m) {
+      const int w = __ffsll(m) - 1, before = base + __builtin_amdgcn_readlane(si - items, w), local = index - before;
+      found = true;
+      it.front = false;
+      it.nch = __builtin_amdgcn_readlane(nch, w);
+      it.tile = local / it.nch;
+      it.chunk = local - it.tile * it.nch;
+      it.base = before + it.tile * it.nch;
+      it.b = b0 + w;
+      it.s1 = 0;
+      it.s.q0 = __builtin_amdgcn_readlane(s.q0, w);
+      it.s.nq = __builtin_amdgcn_readlane(s.nq, w);
+      it.s.k0 = 0;
+      it.s.nk = __builtin_amdgcn_readlane(s.nk, w);
+      it.first = __builtin_amdgcn_readlane(first, w);
+      it.rank = rank + __builtin_amdgcn_readlane(so - tiles, w) + it.tile;
+      it.f = Front{};
+      int of = __builtin_amdgcn_readlane(g, w);
+      if (of >= 0 && it.first > 0) {
+        if (p.N > 64) {   // the group's items, from the first one's on
+          int at = 0;
+          for (int g0 = 0; g0 <= of; g0 += 64) {
+            get_fronts(g0);
+            get_fronts_queries(g0);
+            fnch = chunks(blocks_of(fs.nk));
+            const int n = ftiles * fnch, sn = lanes_scan(n);
+            fbase = at + sn - n;
+            at += lane63(sn);
+          }
+          of &= 63;
+        }
+        it.f.base = __builtin_amdgcn_readlane(fbase, of);
+        it.f.nch = __builtin_amdgcn_readlane(fnch, of);
+        it.f.q0 = __builtin_amdgcn_readlane(fs.q0, of);
+        it.f.rows = (long)__builtin_amdgcn_readlane(fs.nq, of) * p.G;
+        if (it.f.base < 0) it.f.nch = 0;
+      }
+    }
+    base += lane63(si);
+    rank += lane63(so);
+  }
+  // the compiler does not see that these are the same for all lanes
+  for (int* x : {&it.b, &it.tile, &it.chunk, &it.nch, &it.base, &it.s.q0, &it.s.nq, &it.s.nk, &it.s1, &it.first, &it.rank, &it.fronts,
+                 &it.f.base, &it.f.nch, &it.f.q0})
+    *x = __builtin_amdgcn_readfirstlane(*x);
+  it.front = __builtin_amdgcn_readfirstlane(it.front ? 1 : 0);
+  return found;
 }
 
 // RANGE: the keys that a row sees: those below lim that are from lo on, or below the sinks.
@@ -323,22 +463,6 @@ __device__ __forceinline__ Sees sees(const AttendParams& p, const Item& it, int 
   const int at = t - s.q0;
   return Sees{at < 0 || at >= s.nq ? 0 : min(it.s.nk, keys_of(p, s, at)), 0};
 }
-// Whether every query of a front sees all its keys, as it does unless a sequence's own queries
-// reach into them (the rows then look for their sequences one by one).
-template <int KV>
-__device__ __forceinline__ bool front_is_whole(const AttendParams& p, const Item& it, int lane) {
-  bool all = true;
-  for (int b0 = it.b; b0 < it.s1; b0 += 64) {
-    bool ok = true;
-    if (b0 + lane < it.s1) {
-      const Seq s = sequence<KV>(p, b0 + lane);
-      ok = s.nq <= 0 || keys_of(p, s, 0) >= it.s.nk;
-    }
-    all = all && __all(ok);
-  }
-  return all;
-}
-
 // RANGE: the blocks of 64 keys that a tile's rows see together: the first sn, then those from
 // block w0 on, nb in all.  Of these its rows all see all keys of the blocks below fs and of fa .. fb.
 struct Blocks {
@@ -1070,7 +1194,7 @@ __device__ __forceinline__ long part_row(const AttendParams& p, const Item& it, 
 struct Parts {
   int q0, row0, rows;          // the sequence's first query; the tile's first row, its rows
   int own, nch;                // its first item among the own ones, items (0: none)
-  int front, fnch, frow0;      // the group's first item, items a tile (0: no group), the group's row that is row0
+  int front, fnch, frow0;      // the group's first item, chunks (0: no group), the group's row that is row0
   int frows, pad[3];           // the group's rows
 };
 // The workspace behind the sums: how many own tiles there are and how many items of fronts, then Parts for each tile.
@@ -1079,74 +1203,27 @@ __device__ __forceinline__ int* parts_head(const AttendParams& p) { return reint
 template <int HD>
 __device__ __forceinline__ Parts* parts_at(const AttendParams& p) { return reinterpret_cast<Parts*>(parts_head<HD>(p) + 4); }
 
-// Where the parts of a sequence's group are: its first item, items a tile, rows; nch 0: no group.
-struct Front {
-  int base, nch, q0;
-  long rows;
-};
-template <int KV, int BMF>
-__device__ __forceinline__ Front front_of(const AttendParams& p, const Item& it) {
-  Front f{};
-  const int g = group_of(p, it.v - p.N), lane = threadIdx.x & 63;
-  if (g < 0) return f;
-  for (int g0 = 0; g0 <= g; g0 += 64) {
-    Piece x{};
-    int nch = 0, items = 0;
-    if (g0 + lane <= g) {
-      x = piece<KV>(p, g0 + lane);
-      nch = max(1, (blocks_of<BMF>(p, x) + it.c - 1) / it.c);
-      items = tiles_of<KV, BMF>(x.s, p.G) * nch;
-    }
-    const int all = lane63(lanes_scan(items));
-    if (g < g0 + 64) {
-      const int w = g - g0;
-      f.base += all - __builtin_amdgcn_readlane(items, w);
-      f.nch = __builtin_amdgcn_readlane(nch, w);
-      f.q0 = __builtin_amdgcn_readlane(x.s.q0, w);
-      f.rows = (long)__builtin_amdgcn_readlane(x.s.nq, w) * p.G;
-      if (__builtin_amdgcn_readlane(x.s.nk, w) <= 0 || f.base < 0) f.nch = 0;
-    } else {
-      f.base += all;
-    }
-  }
-  return f;
-}
-
-// By one wave: the Parts of an own tile's first item.
-template <int HD, int KV, int BM, int BMF>
-__device__ __forceinline__ void leave_parts(const AttendParams& p, const Item& it, int hk, int tile, int lane) {
+// By one lane: the Parts of an own tile's first item.
+template <int HD, int BM>
+__device__ __forceinline__ void leave_parts(const AttendParams& p, const Item& it, int hk, int tile) {
   if (it.front || it.chunk || hk || it.rank < 0 || it.rank >= p.own_items) return;
-  const Front f = front_of<KV, BMF>(p, it);
   Parts x{};
   x.q0 = it.s.q0;
   x.row0 = tile * BM;
   x.rows = (int)min((long)BM, (long)it.s.nq * p.G - (long)tile * BM);
   x.own = it.base - it.fronts;
-  x.nch = it.fronts < 0 || it.fronts > p.front_items || x.own < 0 || x.own + it.nch > p.own_items ? 0 : it.nch;
-  x.front = f.base;
-  x.fnch = f.nch;
-  x.frows = (int)min(f.rows, 0x7FFFFFFFl);
-  x.frow0 = (int)max(((long)it.s.q0 - f.q0) * p.G + (long)tile * BM, -1l);
-  if (lane == 0) parts_at<HD>(p)[it.rank] = x;
+  x.nch = it.nch;
+  x.front = it.f.base;
+  x.fnch = it.f.nch;
+  x.frows = (int)min(it.f.rows, 0x7FFFFFFFl);
+  x.frow0 = (int)max(((long)it.s.q0 - it.f.q0) * p.G + (long)tile * BM, -1l);
+  parts_at<HD>(p)[it.rank] = x;
 }
-// By the first workgroup: how many own tiles and items of fronts there are.
-template <int HD, int KV, int BM, int BMF>
-__device__ __forceinline__ void leave_head(const AttendParams& p, int c, int lane) {
-  int tiles = 0, fronts = 0;
-  for (int b0 = 0; b0 < p.N + p.B; b0 += 64) {
-    int t = 0, f = 0;
-    if (b0 + lane < p.N + p.B) {
-      const Piece x = piece<KV>(p, b0 + lane);
-      if (b0 + lane < p.N) f = tiles_of<KV, BMF>(x.s, p.G) * max(1, (blocks_of<BMF>(p, x) + c - 1) / c);
-      else t = tiles_of<KV, BM>(x.s, p.G);
-    }
-    tiles = min(tiles + lane63(lanes_scan(t)), 1 << 29);
-    fronts = min(fronts + lane63(lanes_scan(f)), 1 << 29);
-  }
-  if (lane == 0) {
-    parts_head<HD>(p)[0] = tiles < 0 ? 0 : min(tiles, p.own_items);
-    parts_head<HD>(p)[1] = fronts;
-  }
+// By one lane of the first workgroup: how many own tiles and items of fronts there are.
+template <int HD>
+__device__ __forceinline__ void leave_head(const AttendParams& p, const Item& it, int tiles) {
+  parts_head<HD>(p)[0] = min(tiles, p.own_items);
+  parts_head<HD>(p)[1] = it.fronts;
 }
 
 // ---- many rows: NW waves of 32 rows over the same keys -----------------------------------
@@ -1196,8 +1273,7 @@ __device__ __forceinline__ void tile_item(const AttendParams& p, Item& it, const
   Blocks bl;
   int vbeg = 0, vend = 0;
   if constexpr (FORM == RANGE) {
-    it.whole = it.front && front_is_whole<KV>(p, it, lane);
-    if (KV != KV_ROWS && p.N && wave == 0) leave_parts<HD, KV, BMO, BM>(p, it, hk, tile, lane);
+    if (KV != KV_ROWS && p.N && tid == 0) leave_parts<HD, BMO>(p, it, hk, tile);
     bl = blocks<KV>(p, it, tok0, tok1);
     vbeg = SPLIT && it.nch > 1 ? it.chunk * it.c : 0;
     vend = SPLIT && it.nch > 1 ? min(bl.nb, vbeg + it.c) : bl.nb;
@@ -1258,6 +1334,20 @@ __device__ __forceinline__ void tile_item(const AttendParams& p, Item& it, const
     }
   };
   int key0 = kbeg, cur = 0;
+  // The infinities and NaN of this tile's V taken out, if there are any.
+  auto take_out = [&](int tid_) {
+    if (any_odd<T, TILE, NT>(vt(cur), tid_)) odd = 1;
+    __syncthreads();
+    const bool fix = odd;
+    if (fix) {
+      for (int i = tid_; i < 3 * HD; i += NT) (&bad[0][0])[i] = FORM == RANGE ? 0 : 0x7FFFFFFF;
+      __syncthreads();
+      if constexpr (FORM == RANGE) take_out_odd<T, HD, AT_KEYS, NT>(vt(cur), bad, tid_);
+      else take_out_odd<T, HD, AT_KEYS, NT>(vt(cur), bad, key0, tid_);
+      __syncthreads();
+    }
+    return fix;
+  };
   // A tile whose scores are in sa by itself; part: some row does not see all of it, and an infinity
   // or NaN of V must not reach that row.
   auto alone = [&](bool part, bool more) {
@@ -1267,16 +1357,7 @@ __device__ __forceinline__ void tile_item(const AttendParams& p, Item& it, const
     bool fix = false;
     if (part) {
       r.template mask<2>(sa, key0, lane_);
-      if (any_odd<T, TILE, NT>(vt(cur), tid_)) odd = 1;
-      __syncthreads();
-      fix = odd;
-      if (fix) {
-        for (int i = tid_; i < 3 * HD; i += NT) (&bad[0][0])[i] = FORM == RANGE ? 0 : 0x7FFFFFFF;
-        __syncthreads();
-        if constexpr (FORM == RANGE) take_out_odd<T, HD, AT_KEYS, NT>(vt(cur), bad, tid_);
-        else take_out_odd<T, HD, AT_KEYS, NT>(vt(cur), bad, key0, tid_);
-        __syncthreads();
-      }
+      fix = take_out(tid_);
     }
     r.raise(r.template top<2>(sa), c);
     typename Elem<T>::v8 pf[4];
@@ -1296,6 +1377,17 @@ __device__ __forceinline__ void tile_item(const AttendParams& p, Item& it, const
     }
   };
   if constexpr (FORM == RANGE) {
+    auto whole = [&](int v) { return v < bl.fs || (v >= bl.fa && v < bl.fb); };
+    if ((long)tile * BM + wave * 32 >= (long)it.s.nq * p.G) {
+      // a wave without a row only brings tiles, and leaves the CU's units to the others
+      for (int v = vbeg; v < vend; ++v, cur ^= 1) {
+        next(bl.key(v + 1), bl.key(v + 2), cur);
+        if (!whole(v) && take_out(tid)) __syncthreads();   // (as below, behind add_odd)
+        if (v + 1 < vend) keep(cur);
+      }
+      wait_vm_lgkm0<0>();
+      return;
+    }
     for (int v = vbeg; v < vend; ++v, cur ^= 1) {
       // runs of tiles of which every row sees all
       const int run = min(v < bl.fs ? bl.fs : v >= bl.fa ? bl.fb : v, vend);
@@ -1328,7 +1420,7 @@ __device__ __forceinline__ void tile_item(const AttendParams& p, Item& it, const
       }
       key0 = bl.key(v);
       next(bl.key(v + 1), bl.key(v + 2), cur);
-      alone(!(v < bl.fs || (v >= bl.fa && v < bl.fb)), v + 1 < vend);
+      alone(!whole(v), v + 1 < vend);
     }
   } else {
     // while every row sees all of this tile and of the next one
@@ -1388,10 +1480,14 @@ __global__ __launch_bounds__(64 * NW, 2) void attend_tile_kernel(const AttendPar
   __shared__ __attribute__((aligned(1024))) char lds[TileLds<T, HD, FORM>::BYTES];
   const int hk = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv;
   Item it;
-  const bool some = find_item<KV, 32 * NW, false, FORM>(p, index, it);
-  if constexpr (FORM == RANGE)
-    if (KV != KV_ROWS && p.N && blockIdx.x == 0 && threadIdx.x < 64) leave_head<HD, KV, 32 * NW, 32 * NW>(p, some ? it.c : 1, threadIdx.x);
-  if (!some) return;
+  if (FORM == RANGE && KV != KV_ROWS && p.N) {
+    int tiles;
+    const bool some = find_shared<KV, 32 * NW, 32 * NW>(p, index, it, tiles);
+    if (blockIdx.x == 0 && threadIdx.x == 0) leave_head<HD>(p, it, tiles);
+    if (!some) return;
+  } else if (!find_item<KV, 32 * NW, false, FORM>(p, index, it)) {
+    return;
+  }
   tile_item<T, HD, KV, NW, FORM>(p, it, hk, lds);
 }
 
@@ -1425,16 +1521,19 @@ __global__ __launch_bounds__(64 * FEW_WAVES, MIXED ? 2 : few_at_once(R::BM, HD, 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hk = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv;
   Item it;
-  const bool some = find_item<KV, BM, false, FORM, BMF>(p, index, it);
-  if constexpr (FORM == RANGE)
-    if (KV != KV_ROWS && p.N && blockIdx.x == 0 && wave == 0) leave_head<HD, KV, BM, BMF>(p, some ? it.c : 1, lane);
-  if (!some) return;
+  if (FORM == RANGE && KV != KV_ROWS && (MIXED || p.N)) {
+    int tiles;
+    const bool some = find_shared<KV, BM, BMF>(p, index, it, tiles);
+    if (blockIdx.x == 0 && tid == 0) leave_head<HD>(p, it, tiles);
+    if (!some) return;
+  } else if (!find_item<KV, BM, false, FORM>(p, index, it)) {
+    return;
+  }
   if constexpr (MIXED)
     if (it.front) {
       tile_item<T, HD, KV, 4, RANGE, BM>(p, it, hk, reinterpret_cast<char*>(&lds));
       return;
     }
-  if constexpr (FORM == RANGE) it.whole = it.front && front_is_whole<KV>(p, it, lane);
   R r;
   r.template begin<KV>(p, it, hk, it.tile * BM + lane % BM, lane);
   const int tok0 = it.tile * BM / p.G, tok1 = min(it.s.nq - 1, (it.tile * BM + BM - 1) / p.G);
@@ -1551,8 +1650,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, MIXED ? 2 : few_at_once(R::BM, HD, 
       *reinterpret_cast<float4_t*>(part_o<HD>(p, row) + c * 4) = a;
       if (c == 0) *part_ml<HD>(p, row) = float2_t{M, sum};
     }
-  }  if constexpr (FORM == RANGE)
-    if (KV != KV_ROWS && p.N && wave == 0) leave_parts<HD, KV, BM, BMF>(p, it, hk, it.tile, lane);
+  }  if (FORM == RANGE && KV != KV_ROWS && p.N && tid == 0) leave_parts<HD, BM>(p, it, hk, it.tile);
 }
 
 // One group's (cg of CG) share of nch parts of a row, the first at `row`, added to a (chunk c), its sum and maximum.
@@ -1658,10 +1756,10 @@ __global__ __launch_bounds__(256) void attend_join_shared_kernel(const AttendPar
     add_parts<HD, CG>(p, (long)fronts * p.Hkv * BMF + ((long)x.own * p.Hkv + hk) * BM + q, (long)p.Hkv * BM, x.nch, cg, c, M, sum, a);
     const int of = x.frow0 + q;
     if (x.fnch > 0 && x.frow0 >= 0 && of < x.frows) {
-      // its tile of the group's rows; those of 128 are in order of falling length
-      const int ft = of / BMF, item = x.front + (BMF <= 32 ? ft : (x.frows + BMF - 1) / BMF - 1 - ft) * x.fnch;
-      if (item >= 0 && item <= fronts - x.fnch)
-        add_parts<HD, CG>(p, ((long)item * p.Hkv + hk) * BMF + of % BMF, (long)p.Hkv * BMF, x.fnch, cg, c, M, sum, a);
+      // its tile of the group's rows (those of 128 come last first), chunk by chunk
+      const int ftiles = (x.frows + BMF - 1) / BMF, ft = of / BMF, item = x.front + (BMF <= 32 ? ft : ftiles - 1 - ft);
+      if (item >= 0 && item + (long)(x.fnch - 1) * ftiles < fronts)
+        add_parts<HD, CG>(p, ((long)item * p.Hkv + hk) * BMF + of % BMF, (long)ftiles * p.Hkv * BMF, x.fnch, cg, c, M, sum, a);
     }
   }
   if constexpr (CG > 1) {
