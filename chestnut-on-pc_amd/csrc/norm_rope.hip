@@ -8,7 +8,9 @@
 // hold 16 elements each, both halves of eight pairs, so that the sum takes shuffles within a
 // few lanes and the rotation none; a lane holds the same pairs of every head that it comes
 // across, and their weights in registers.  The angles belong to a token: a workgroup computes
-// those of its tokens once into LDS.
+// those of its tokens once into LDS.  A lane's heads are sent for together, before the angles: 12288
+// tokens of 32 heads of 128, half of each turned, 201 MB, 59 us with one head under way, 41.6 with
+// four, 38.9 with six = 5.2 TB/s, 39 with eight, 67 with twelve.
 #include "common.h"
 #include "elem16.h"
 #include "kernels.h"
@@ -18,13 +20,14 @@ namespace ck {
 namespace {
 
 constexpr int NR_LDS = 1024;   // pairs of a workgroup's tokens: cos and sin in 8 KB
+constexpr int NR_HEADS = 6;      // of a lane, that are under way together
 
 struct NormRopeParams {
   NormRopeHeads q, k;
   RopeAngles a;
   int T, H, hd, tpw;           // H: heads of q and k together; tpw: tokens per workgroup
   unsigned m_H;                // div_magic of H
-  int interleaved, wtype;
+  int interleaved, wtype, w_aligned;
   float eps, inv_hd;
 };
 
@@ -45,74 +48,122 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
+// Eight weights from element i on (a multiple of 8).
+__device__ __forceinline__ void weights_at(float (&f)[8], const void* w, int type, int i, bool aligned) {
+  if (!w || !aligned) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = weight_at(w, type, i + j);
+  } else if (type == DT_F16) {
+    const half8_t v = *reinterpret_cast<const half8_t*>(static_cast<const half_t*>(w) + i);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (float)v[j];
+  } else if (type == DT_BF16) {
+    const bf16x8_t v = *reinterpret_cast<const bf16x8_t*>(static_cast<const bf16_t*>(w) + i);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (float)v[j];
+  } else {
+    const float4_t *v = reinterpret_cast<const float4_t*>(static_cast<const float*>(w) + i), x = v[0], y = v[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f[j] = x[j];
+      f[4 + j] = y[j];
+    }
+  }
+}
+
 template <typename T, int LPR, bool NT>
 __global__ __launch_bounds__(256) void norm_rope_kernel(const NormRopeParams p) {
   typedef typename Elem<T>::v8 v8;
+  constexpr int U = NR_HEADS, STEP = 256 / LPR;   // STEP: heads side by side
   __shared__ float2_t cs[NR_LDS];
   const int t0 = blockIdx.x * p.tpw, nt = min(p.tpw, p.T - t0), half = p.a.half;
-  rope_angles<256>(p.a, t0, nt, cs, threadIdx.x);
+  const unsigned n = nt * p.H;
   const int e = (int)(threadIdx.x % LPR) * 8;   // the lane's first pair
   const bool turn = e < half;
-  // its two runs of eight elements
-  const int a = turn && !p.interleaved ? e : 2 * e, b = turn && !p.interleaved ? e + half : 2 * e + 8;
-  float wq[16], wk[16];
+  // its two runs of eight elements: both halves of eight pairs, else two that lie apart, so that neighbouring lanes
+  // have neighbouring runs; where interleaved, each is turned by itself
+  const int from = p.interleaved ? 0 : 2 * half, a = turn && !p.interleaved ? e : from + e - (p.interleaved ? 0 : half);
+  const int b = turn && !p.interleaved ? e + half : a + (p.hd - from) / 2;
+  v8 v0[U], v1[U];
+  auto load = [&](unsigned r0) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    wq[j] = weight_at(p.q.weight, p.wtype, a + j);
-    wq[8 + j] = weight_at(p.q.weight, p.wtype, b + j);
-    wk[j] = weight_at(p.k.weight, p.wtype, a + j);
-    wk[8 + j] = weight_at(p.k.weight, p.wtype, b + j);
-  }
+    for (int i = 0; i < U; ++i) {
+      const unsigned r = min(r0 + i * STEP, n - 1), t = div_by(r, p.m_H), h = r - t * p.H;
+      const bool isk = (int)h >= p.q.heads;
+      const long g = isk ? (int)h - p.q.heads : (int)h;
+      const T* x = static_cast<const T*>(isk ? p.k.x : p.q.x) + (t0 + t) * (isk ? p.k.x_st : p.q.x_st) + g * (isk ? p.k.x_sh : p.q.x_sh);
+      v0[i] = *reinterpret_cast<const v8*>(x + a);
+      v1[i] = *reinterpret_cast<const v8*>(x + b);
+    }
+  };
+  unsigned r0 = threadIdx.x / LPR;
+  load(r0);
+  float wq[2][8], wk[2][8];
+  weights_at(wq[0], p.q.weight, p.wtype, a, p.w_aligned);
+  weights_at(wq[1], p.q.weight, p.wtype, b, p.w_aligned);
+  weights_at(wk[0], p.k.weight, p.wtype, a, p.w_aligned);
+  weights_at(wk[1], p.k.weight, p.wtype, b, p.w_aligned);
+  rope_angles<256>(p.a, t0, nt, cs, threadIdx.x);
   __syncthreads();
   auto put = [](T* to, v8 v) {
     if (NT) __builtin_nontemporal_store(v, reinterpret_cast<v8*>(to));
     else *reinterpret_cast<v8*>(to) = v;
   };
-  for (unsigned r = threadIdx.x / LPR; r < (unsigned)(nt * p.H); r += 256 / LPR) {
-    const unsigned t = div_by(r, p.m_H), h = r - t * p.H;
-    const bool isk = (int)h >= p.q.heads;
-    const long g = isk ? (int)h - p.q.heads : (int)h;
-    const T* x = static_cast<const T*>(isk ? p.k.x : p.q.x) + (t0 + t) * (isk ? p.k.x_st : p.q.x_st) + g * (isk ? p.k.x_sh : p.q.x_sh);
-    T* y = static_cast<T*>(isk ? p.k.out : p.q.out) + (t0 + t) * (isk ? p.k.o_st : p.q.o_st) + g * (isk ? p.k.o_sh : p.q.o_sh);
-    const v8 v0 = *reinterpret_cast<const v8*>(x + a), v1 = *reinterpret_cast<const v8*>(x + b);
-    float f[16], sum = 0.f;
+  for (; r0 < n; r0 += U * STEP) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      f[j] = (float)v0[j];
-      f[8 + j] = (float)v1[j];
-      sum = __builtin_fmaf(f[j], f[j], sum);
-      sum = __builtin_fmaf(f[8 + j], f[8 + j], sum);
-    }
-    const float inv = 1.0f / sqrtf(__builtin_fmaf(lanes_sum<LPR>(sum), p.inv_hd, p.eps));
+    for (int i = 0; i < U; ++i) {
+      const unsigned r = r0 + i * STEP;
+      if (r >= n) break;
+      const unsigned t = div_by(r, p.m_H), h = r - t * p.H;
+      const bool isk = (int)h >= p.q.heads;
+      const long g = isk ? (int)h - p.q.heads : (int)h;
+      T* y = static_cast<T*>(isk ? p.k.out : p.q.out) + (t0 + t) * (isk ? p.k.o_st : p.q.o_st) + g * (isk ? p.k.o_sh : p.q.o_sh);
+      float f[16], sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) f[j] *= inv * (isk ? wk[j] : wq[j]);
-    v8 y0, y1;
-    const float2_t* c = cs + t * half + e;
-    if (!turn) {
+      for (int j = 0; j < 8; ++j) {
+        f[j] = (float)v0[i][j];
+        f[8 + j] = (float)v1[i][j];
+        sum = __builtin_fmaf(f[j], f[j], sum);
+        sum = __builtin_fmaf(f[8 + j], f[8 + j], sum);
+      }
+      const float inv = 1.0f / sqrtf(__builtin_fmaf(lanes_sum<LPR>(sum), p.inv_hd, p.eps));
+#pragma unroll
+      for (int j = 0; j < 16; ++j) f[j] *= inv * (isk ? wk[j / 8][j % 8] : wq[j / 8][j % 8]);
+      if (p.interleaved) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int at = k ? b : a;
+          if (at < 2 * half) {
+            const float2_t* c = cs + t * half + at / 2;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2_t u = c[j];
+              const float x0 = f[8 * k + 2 * j], x1 = f[8 * k + 2 * j + 1];
+              f[8 * k + 2 * j] = x0 * u[0] - x1 * u[1];
+              f[8 * k + 2 * j + 1] = x1 * u[0] + x0 * u[1];
+            }
+          }
+        }
+      } else if (turn) {
+        const float2_t* c = cs + t * half + e;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float2_t u = c[j];
+          const float x0 = f[j], x1 = f[8 + j];
+          f[j] = x0 * u[0] - x1 * u[1];
+          f[8 + j] = x1 * u[0] + x0 * u[1];
+        }
+      }
+      v8 y0, y1;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         y0[j] = (T)f[j];
         y1[j] = (T)f[8 + j];
       }
-    } else if (p.interleaved) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2_t u = c[j], w = c[4 + j];
-        y0[2 * j] = (T)(f[2 * j] * u[0] - f[2 * j + 1] * u[1]);
-        y0[2 * j + 1] = (T)(f[2 * j + 1] * u[0] + f[2 * j] * u[1]);
-        y1[2 * j] = (T)(f[8 + 2 * j] * w[0] - f[9 + 2 * j] * w[1]);
-        y1[2 * j + 1] = (T)(f[9 + 2 * j] * w[0] + f[8 + 2 * j] * w[1]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float2_t u = c[j];
-        y0[j] = (T)(f[j] * u[0] - f[8 + j] * u[1]);
-        y1[j] = (T)(f[8 + j] * u[0] + f[j] * u[1]);
-      }
+      put(y + a, y0);
+      put(y + b, y1);
     }
-    put(y + a, y0);
-    put(y + b, y1);
+    if (r0 + U * STEP < n) load(r0 + U * STEP);
   }
 }
 
@@ -200,8 +251,9 @@ void launch_norm_rope(const NormRopeHeads& q, const NormRopeHeads& k, const int*
       ends |= reinterpret_cast<uintptr_t>(x->x) | reinterpret_cast<uintptr_t>(x->out);
     }
   const bool wide = rot % 16 == 0 && hd >= 64 && (hd & (hd - 1)) == 0 && (strides & 7) == 0 && (ends & 15) == 0;
-  // four heads a lane, but enough workgroups to fill the CUs twice first
-  int tpw = std::max(1, std::min<int>(4 * (wide ? 4096 / hd : 4) / p.H, ceil_div(T, 512)));
+  p.w_aligned = ((reinterpret_cast<uintptr_t>(q.weight) | reinterpret_cast<uintptr_t>(k.weight)) & 15) == 0;
+  // a lane's heads loaded at once, but enough workgroups to fill the CUs twice first
+  int tpw = std::max(1, std::min<int>(NR_HEADS * (wide ? 4096 / hd : 4) / p.H, ceil_div(T, 512)));
   tpw = std::max(1, std::min(tpw, NR_LDS / (rot / 2)));
   p.tpw = tpw;
   const dim3 grid(ceil_div(T, tpw)), block(256);
