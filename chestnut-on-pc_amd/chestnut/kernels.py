@@ -549,14 +549,21 @@ def norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, axes=None
     return y, z
 
 
+def _maps_bytes(B, tokens, in_place):
+    nb = ctypes.c_size_t()
+    check(lib().ck_cache_maps_workspace(B, tokens, 1 if in_place else 0, ctypes.byref(nb)))
+    return nb.value
+
+
+_cached_maps_bytes = functools.lru_cache(maxsize=256)(_maps_bytes)
+
+
 def cache_maps_workspace(B, tokens, in_place):
     """Bytes of workspace (0: none) of cache_maps for B requests and `tokens` rows;
     in_place: kv_out is kv_lens or taken_out is taken."""
     if any(abs(n) > _INT for n in (B, tokens)):
         raise ValueError('counts must be under 2^31')
-    nb = ctypes.c_size_t()
-    check(lib().ck_cache_maps_workspace(B, tokens, 1 if in_place else 0, ctypes.byref(nb)))
-    return nb.value
+    return _maps_bytes(B, tokens, in_place)
 
 
 def cache_maps(new_lens, kv_lens, block_table, page, tokens, free_pages=None, taken=None, kv_out=None, taken_out=None,
@@ -578,6 +585,58 @@ def cache_maps(new_lens, kv_lens, block_table, page, tokens, free_pages=None, ta
     table) has slot -1.
     kv_out: kv_lens itself (a captured step then advances by itself), another
     tensor, or None: a new one."""
+    B, width, n_free, dev = _maps(new_lens, kv_lens, block_table, page, tokens, free_pages, taken, kv_out, taken_out)
+    # one allocation for all outputs (an allocation costs about 1 us, as does a view)
+    sizes = [B + 1, tokens, tokens]
+    if kv_out is None:
+        cu, positions, slots, kv_out = torch.empty(2 * (B + tokens) + 1, dtype=torch.int32, device=new_lens.device).split(sizes + [B])
+    else:
+        cu, positions, slots = torch.empty(B + 1 + 2 * tokens, dtype=torch.int32, device=new_lens.device).split(sizes)
+    if taken is not None and taken_out is None:
+        taken_out = taken
+    nb = 0
+    if tokens > 1024:   # (fewer need none)
+        nb = _cached_maps_bytes(B, tokens, kv_out.data_ptr() == kv_lens.data_ptr() or
+                                (taken is not None and taken_out.data_ptr() == taken.data_ptr()))
+    ws = _workspace(workspace, nb, new_lens.device) if nb else None
+    check(lib().ck_cache_maps(new_lens.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), width,
+                              (free_pages.data_ptr() or taken.data_ptr()) if free_pages is not None else None, n_free, _ptr(taken),
+                              B, page, tokens, cu.data_ptr(), kv_out.data_ptr(), positions.data_ptr(), slots.data_ptr(),
+                              _ptr(taken_out), _ptr(ws), nb, _raw_stream(dev)))
+    return cu, kv_out, positions, slots
+
+
+def _maps(new_lens, kv_lens, block_table, page, tokens, free_pages, taken, kv_out, taken_out):
+    """The checks of cache_maps: (B, table width, pages in the list, device)."""
+    T, i32 = torch.Tensor, torch.int32
+    if type(new_lens) is T and type(block_table) is T and type(tokens) is type(page) is int and \
+            (free_pages is None) == (taken is None) and (taken is not None or taken_out is None):
+        # all in one pass where all is well
+        shape, dev = block_table.shape, new_lens.get_device()
+        if len(shape) == 2 and shape[0] < 1 << 20 and 0 <= tokens < 1 << 30 and 16 <= page <= 1024 and not page & (page - 1) and \
+                shape[1] * page <= 1 << 30 and dev >= 0 and dev == _device():
+            B = shape[:1]
+            each = [(new_lens, B), (kv_lens, B), (block_table, shape)]
+            if kv_out is not None:
+                each.append((kv_out, B))
+            n_free = 0
+            if taken is not None:
+                if type(free_pages) is T and free_pages.dim() == 1:
+                    n_free = free_pages.shape[0]
+                each += [(free_pages, (n_free,)), (taken, (1,))]
+                if taken_out is not None:
+                    each.append((taken_out, (1,)))
+            for t, want in each:
+                if type(t) is not T or t.dtype is not i32 or t.shape != want or t.get_device() != dev or not t.is_contiguous():
+                    break
+            else:
+                if n_free <= _INT:
+                    return shape[0], shape[1], n_free, dev
+    return _maps_each(new_lens, kv_lens, block_table, page, tokens, free_pages, taken, kv_out, taken_out)
+
+
+def _maps_each(new_lens, kv_lens, block_table, page, tokens, free_pages, taken, kv_out, taken_out):
+    """The checks of _maps one by one, with the message of the first that fails."""
     if not isinstance(tokens, int) or not 0 <= tokens < 1 << 30:
         raise ValueError('tokens must be the number of rows, under 2^30')
     if not isinstance(page, int) or page < 16 or page > 1024 or page & (page - 1):
@@ -605,30 +664,12 @@ def cache_maps(new_lens, kv_lens, block_table, page, tokens, free_pages=None, ta
         if n_free > _INT:
             raise ValueError(f'free_pages must have under 2^31 entries, got {n_free}')
         _is(taken, i32, 'taken', (1,))
-        if taken_out is None:
-            taken_out = taken
-        else:
+        if taken_out is not None:
             _is(taken_out, i32, 'taken_out', (1,))
     if kv_out is not None:
         _is(kv_out, i32, 'kv_out', (B,))
-    dev = _on_device('new_lens kv_lens block_table free_pages taken kv_out taken_out', new_lens, kv_lens, block_table, free_pages,
-                     taken, kv_out, taken_out)
-    # one allocation, cut up on 16-byte borders (an allocation costs about 1 us)
-    b4, t4 = (B + 4) & -4, (tokens + 3) & -4
-    buf = torch.empty(b4 + 2 * t4 + (B if kv_out is None else 0), dtype=i32, device=new_lens.device)
-    cu, positions, slots = buf[:B + 1], buf[b4:b4 + tokens], buf[b4 + t4:b4 + t4 + tokens]
-    if kv_out is None:
-        kv_out = buf[b4 + 2 * t4:]
-    nb = 0
-    if tokens > 1024:
-        nb = cache_maps_workspace(B, tokens, kv_out.data_ptr() == kv_lens.data_ptr() or (taken is not None and
-                                                                                          taken_out.data_ptr() == taken.data_ptr()))
-    ws = _workspace(workspace, nb, new_lens.device)
-    check(lib().ck_cache_maps(new_lens.data_ptr(), kv_lens.data_ptr(), block_table.data_ptr(), width,
-                              (free_pages.data_ptr() or taken.data_ptr()) if free_pages is not None else None, n_free, _ptr(taken), B, page, tokens,
-                              cu.data_ptr(), kv_out.data_ptr(), positions.data_ptr(), slots.data_ptr(), _ptr(taken_out), _ptr(ws),
-                              nb, _raw_stream(dev)))
-    return cu, kv_out, positions, slots
+    return B, width, n_free, _on_device('new_lens kv_lens block_table free_pages taken kv_out taken_out', new_lens, kv_lens,
+                                        block_table, free_pages, taken, kv_out, taken_out)
 
 
 def cache_write(k, v, k_pages, v_pages, slots, k_scale=None, v_scale=None):

@@ -36,6 +36,7 @@
 #include "common.h"
 #include "elem16.h"
 #include "kernels.h"
+#include "lanes_scan.h"
 
 namespace ck {
 
@@ -142,24 +143,6 @@ __device__ __forceinline__ int window_blocks(const AttendParams& p, const Seq& s
   const int tokens = min(s.nq, (BM - 1) / p.G + 2);
   return min(blocks_of(s.nk), blocks_of(min(p.sinks, s.nk)) + (p.window + tokens + 2 * AT_KEYS - 3) / AT_KEYS);
 }
-
-// Sum over lanes 0..l, in lane l (DPP: six steps without LDS).
-template <typename N>
-__device__ __forceinline__ N lanes_scan(N v) {
-  auto shifted = [](N x, auto CTRL, auto ROWS) {
-    return __builtin_bit_cast(N, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(CTRL)::value,
-                                                             decltype(ROWS)::value, 0xF, false));
-  };
-  using std::integral_constant;
-  v += shifted(v, integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{});   // row_shr:1, 2, 4, 8
-  v += shifted(v, integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{});
-  v += shifted(v, integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{});
-  v += shifted(v, integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{});
-  v += shifted(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});   // row_bcast:15, 31
-  v += shifted(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});
-  return v;
-}
-__device__ __forceinline__ int lane63(int v) { return __builtin_amdgcn_readlane(v, 63); }
 
 // index counts items, or tiles where TILES.  False: there are not so many.
 template <int KV, int BM, bool TILES, int FORM>

@@ -15,6 +15,7 @@
 #include "common.h"
 #include "elem16.h"
 #include "kernels.h"
+#include "lanes_scan.h"
 
 namespace ck {
 namespace {
@@ -34,7 +35,10 @@ struct MapsParams {
 struct Scan {
   long rows, pages;
 };
-__device__ __forceinline__ Scan wave_scan(Scan v, int lane) {
+// Sums over lanes 0..l, in lane l: by DPP where 32 bits hold them, as they do but for lengths that make no sense.
+__device__ __forceinline__ Scan wave_scan(int rows, int pages, int lane) {
+  if (!__any(rows >= 1 << 24 || pages >= 1 << 24)) return Scan{lanes_scan(rows), lanes_scan(pages)};
+  Scan v{rows, pages};
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
     const long r = __shfl_up(v.rows, d), g = __shfl_up(v.pages, d);
@@ -84,7 +88,7 @@ __global__ __launch_bounds__(CM_ROWS) void cache_maps_kernel(const MapsParams p)
         old = max(p.kv[b], 0);
       }
       const int need = pages_of((long)old + n, p.shift) - pages_of(old, p.shift);
-      const Scan s = wave_scan(Scan{n, need}, lane);
+      const Scan s = wave_scan(n, need, lane);
       if (b0) __syncthreads();   // part of the requests before has been read
       if (lane == 63) part[wave] = s;
       __syncthreads();
