@@ -1737,12 +1737,12 @@ __global__ __launch_bounds__(256) void attend_join_shared_kernel(const AttendPar
   float4_t a = {0.f, 0.f, 0.f, 0.f};
   if (in) {
     add_parts<HD, CG>(p, (long)fronts * p.Hkv * BMF + ((long)x.own * p.Hkv + hk) * BM + q, (long)p.Hkv * BM, x.nch, cg, c, M, sum, a);
-    const int of = x.frow0 + q;
-    if (x.fnch > 0 && x.frow0 >= 0 && of < x.frows) {
+    const long of = (long)x.frow0 + q;
+    if (x.fnch > 0 && x.frow0 >= 0 && of < x.frows && x.frows <= (long)p.Tq * p.G) {
       // its tile of the group's rows (those of 128 come last first), chunk by chunk
-      const int ftiles = (x.frows + BMF - 1) / BMF, ft = of / BMF, item = x.front + (BMF <= 32 ? ft : ftiles - 1 - ft);
-      if (item >= 0 && item + (long)(x.fnch - 1) * ftiles < fronts)
-        add_parts<HD, CG>(p, ((long)item * p.Hkv + hk) * BMF + of % BMF, (long)ftiles * p.Hkv * BMF, x.fnch, cg, c, M, sum, a);
+      const long ftiles = ((long)x.frows + BMF - 1) / BMF, ft = of / BMF, item = x.front + (BMF <= 32 ? ft : ftiles - 1 - ft);
+      if (item >= 0 && item + (x.fnch - 1) * ftiles < fronts)
+        add_parts<HD, CG>(p, (item * p.Hkv + hk) * BMF + of % BMF, ftiles * p.Hkv * BMF, x.fnch, cg, c, M, sum, a);
     }
   }
   if constexpr (CG > 1) {

@@ -294,3 +294,333 @@ def test_sequences_that_end_within_the_shared_pages(gpu, H, kv, hd, dt, causal, 
         k, v = gathered(vals, table[b], m, page)
         near(out[a:a + x], *O.attention(f64(q[a:a + x]), k, v, causal), max(1, m), hd, dt, f'sequence {b}: {x} over {m}')
         a += x
+
+
+@pytest.mark.parametrize('sizes', [[1] * 70, [3] * 70 + [0] * 5 + [40], [100, 31]], ids=['70 of one', '76', '2 of many'])
+@pytest.mark.parametrize('q', [1, 9])
+@pytest.mark.parametrize('H,kv,hd', [(4, 4, 64), (16, 2, 128)])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+def test_many_groups_and_sequences(gpu, sizes, q, H, kv, hd, dt):
+    """More groups and sequences than a wave has lanes; the last sequences in no group."""
+    from chestnut import kernels as K
+    page = 16
+    r = np.random.default_rng(7)
+    common = [int(x) * page for x in r.integers(0, 9, len(sizes))]
+    n = sum(sizes)
+    qlens = list(r.integers(0, q + 1, n + 4)) if q > 1 else [1] * (n + 4)
+    own = [int(x + y) for x, y in zip(qlens, r.integers(0, 100, n + 4))]
+    table, pages, lens = shared_batch(sizes + [1] * 4, common + [0] * 4, qlens, own, page, 1)
+    (kp, vp, _, _), vals = pages_of(2, pages, kv, page, hd, dt, dt)
+    x = rows(3, int(sum(qlens)), H, hd, dt)
+    out = K.attention_paged(x, kp, vp, i32(table), cu(qlens), i32(lens), shared=(cu(sizes), i32(common)))
+    a = 0
+    for b, (m, l) in enumerate(zip(qlens, lens)):
+        k, v = gathered(vals, table[b], l, page)
+        near(out[a:a + m], *expect(x[a:a + m], k, v), max(1, l), hd, dt, f'sequence {b}')
+        a += m
+
+
+@pytest.mark.parametrize('quant', [False, True])
+def test_many_rows_over_shared_pages(gpu, quant):
+    """So many tiles that no keys are split: the two parts of every row are joined all the same."""
+    from chestnut import kernels as K
+    H, kv, hd, page, dt = 32, 8, 64, 64, 'bf16'
+    groups, common, qlens, own = [2, 1], [640, 128], [1500, 1001, 1800], [1500, 1300, 1800]
+    table, n, lens = shared_batch(groups, common, qlens, own, page, 1)
+    (kp, vp, ks, vs), vals = pages_of(2, n, kv, page, hd, dt, 'e4m3' if quant else dt)
+    q = rows(3, sum(qlens), H, hd, dt)
+    out = K.attention_paged(q, kp, vp, i32(table), cu(qlens), i32(lens), k_scale=ks, v_scale=vs, shared=(cu(groups), i32(common)))
+    a = 0
+    for b, (x, m) in enumerate(zip(qlens, lens)):
+        k, v = gathered(vals, table[b], m, page)
+        near(out[a:a + x], *expect(q[a:a + x], k, v), m, hd, dt, f'sequence {b}')
+        a += x
+
+
+@pytest.mark.parametrize('n', [1, 12, 70])
+@pytest.mark.parametrize('hd', [64, 128])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+def test_infinities_and_nan_over_shared_pages(gpu, n, hd, dt):
+    """In V, in keys that some rows see and others do not, within the shared pages and behind them; NaN in a shared key's K;
+    NaN in every place that holds no key."""
+    from chestnut import kernels as K
+    H, kv, page, common = 4, 2, 16, 128
+    lens, qlens = [100 + n, 190, 128 + n, 700], [n] * 4              # the first one's queries end within the shared keys
+    B, width = 4, 48
+    table = np.array([list(range(8)) + list(range(8 + 40 * b, 8 + 40 * b + 40)) for b in range(B)])
+    pages = 8 + 40 * B
+    r = np.random.default_rng(4)
+    k, v = (torch.full((pages, kv, page, hd), float('nan'), dtype=DT[dt], device='cuda') for _ in 'kv')
+    kx, vx = (torch.from_numpy(r.standard_normal((B, width * page, kv, hd))).to(DT[dt]).cuda() for _ in 'kv')
+    kx[1:, :common], vx[1:, :common] = kx[:1, :common], vx[:1, :common]
+    for x in (float('inf'), float('-inf'), float('nan')):
+        for j in r.integers(0, common, 3):
+            vx[:, j, r.integers(kv), r.integers(hd)] = x
+        for b in range(B):
+            vx[b, r.integers(common, max(common + 1, lens[b])), r.integers(kv), r.integers(hd)] = x
+    vx[:, 100 + n - 1, 1, 3] = float('inf')                          # the first sequence's last key
+    kx[:, 100 + n - 1, 0, 0] = float('nan')
+    for b in range(B):
+        j = np.arange(max(lens[b], common))
+        K.cache_write(kx[b, j], vx[b, j], k, v, i32(table[b][j // page] * page + j % page))
+    q = rows(1, sum(qlens), H, hd, dt)
+    out = f64(K.attention_paged(q, k, v, i32(table), cu(qlens), i32(lens), shared=(i32([0, B]), i32([common]))))
+    for b in range(B):
+        a = b * n
+        ref, mag, most = O.attention(f64(q[a:a + n]), f64(kx[b, :lens[b]]), f64(vx[b, :lens[b]]))
+        got, odd = out[a:a + n], ~np.isfinite(ref)
+        assert np.array_equal(np.isnan(got), np.isnan(ref)), b
+        assert np.array_equal(got[odd & ~np.isnan(ref)], ref[odd & ~np.isnan(ref)])
+        ref[odd], mag[odd] = 0, 0
+        near(torch.from_numpy(np.where(odd, 0, got)), ref, np.nan_to_num(mag), most, lens[b], hd, dt, f'sequence {b}')
+
+
+# --------------------------------------------------------- what users do with them --
+def test_index_values_outside_the_tensors_stay_inside(gpu):
+    """Whatever the index tensors hold, rows outside `out` and the workspace stay as they were, and the call returns."""
+    from chestnut import kernels as K
+    r = np.random.default_rng(11)
+    B, H, kv, hd, page, n, width, T = 50, 8, 2, 64, 16, 40, 6, 90
+    (kp, vp, _, _), _ = pages_of(2, n, kv, page, hd, 'f16', 'f16')
+    q = rows(3, T, H, hd, 'f16')
+    wild = lambda *s: i32(np.where(r.random(s) < 0.5, r.integers(-2 ** 31, 2 ** 31, s), r.integers(-3, 100, s)))
+    for trial in range(12):
+        N = [1, 3, 70][trial % 3]
+        out = torch.full((T + 2, H, hd), 7.0, dtype=torch.float16, device='cuda')
+        nb = K.attention_workspace(B, T, B * width * page, H, kv, hd, groups=N)
+        ws = torch.full((nb // 4 + 64,), float(trial), device='cuda')
+        ws[:nb // 4].view(torch.int32).copy_(wild(nb // 4))              # what stands in a workspace says nothing
+        table, lens, offs = wild(B, width), wild(B), wild(B + 1)
+        if trial % 2:
+            offs = i32(np.sort(r.integers(0, T + 1, B + 1)))
+        K.attention_paged(q, kp, vp, table, offs, lens, out=out[1:T + 1], workspace=ws[:nb // 4], shared=(wild(N + 1), wild(N)))
+        K.attention_paged(q, kp, vp, table, offs, lens, out=out[1:T + 1], window=int(r.integers(1, 60)), sinks=int(r.integers(0, 9)))
+        K.attention_varlen(q, rows(4, 200, kv, hd, 'f16'), rows(5, 200, kv, hd, 'f16'), offs, wild(B + 1), out=out[1:T + 1], window=17, sinks=3)
+        torch.cuda.synchronize()
+        assert (out[0] == 7.0).all() and (out[T + 1] == 7.0).all() and (ws[nb // 4:] == float(trial)).all()
+
+
+def test_what_stands_in_a_workspace_does_not_count(gpu):
+    from chestnut import kernels as K
+    for qlens, own, H, kv, hd in (([1] * 30, [40 * i + 1 for i in range(30)], 8, 2, 128), ([1] * 5, [9, 800, 30, 1, 64], 8, 8, 64),
+                                  ([50, 1, 90, 7], [60, 1000, 90, 7], 8, 2, 64)):
+        B, page = len(qlens), 32
+        table, n, lens = shared_batch([B], [1600], qlens, own, page, 1)
+        (kp, vp, ks, vs), _ = pages_of(2, n, kv, page, hd, 'bf16', 'e4m3')
+        q = rows(3, sum(qlens), H, hd, 'bf16')
+        call = lambda ws, **kw: K.attention_paged(q, kp, vp, i32(table), cu(qlens), i32(lens), k_scale=ks, v_scale=vs, workspace=ws, **kw)
+        for kw, nb in ((dict(shared=(i32([0, B]), i32([1600]))), K.attention_workspace(B, sum(qlens), table.size * page, H, kv, hd, groups=1)),
+                       (dict(window=1500, sinks=4), K.attention_workspace(B, sum(qlens), table.size * page, H, kv, hd, window=1500, sinks=4))):
+            want = call(None, **kw)
+            for fill in (float('nan'), 0.0, 1e30):
+                assert torch.equal(call(torch.full((nb // 4 + 1,), fill, device='cuda'), **kw), want)
+            assert torch.equal(call(torch.full((nb // 4 + 1,), -1, dtype=torch.int32, device='cuda').view(torch.float32), **kw), want)
+
+
+def test_two_streams_at_once(gpu):
+    from chestnut import kernels as K
+    H, kv, hd, page = 8, 2, 128, 32
+    sets = []
+    for i in range(2):
+        qlens, own = [1] * 20, [13 * j + i + 1 for j in range(20)]
+        table, n, lens = shared_batch([12, 8], [3200, 640], qlens, own, page, i)
+        c, _ = pages_of(i, n, kv, page, hd, 'f16', 'e4m3')
+        sets.append((rows(i, 20, H, hd, 'f16'), c, i32(table), cu(qlens), i32(lens), (i32([0, 12, 20]), i32([3200, 640]))))
+
+    def run(s, ws, window):
+        kw = dict(window=1000, sinks=4) if window else dict(shared=s[5])
+        return K.attention_paged(s[0], s[1][0], s[1][1], s[2], s[3], s[4], k_scale=s[1][2], v_scale=s[1][3], workspace=ws, **kw)
+    want = [[run(s, None, w) for w in (False, True)] for s in sets]
+    kept = [torch.full((1 << 24,), float('nan'), device='cuda') for _ in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], [[], []]
+    for j in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(run(sets[i], kept[i], j % 2))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i][j % 2]) for j, g in enumerate(got[i]))
+
+
+def test_out_may_be_q(gpu):
+    from chestnut import kernels as K
+    for qlens, own in (([1] * 6, [40] * 6), ([1] * 40, [500] * 40), ([70, 3, 200], [70, 300, 900])):
+        B, page, H, kv, hd = len(qlens), 16, 8, 2, 64
+        table, n, lens = shared_batch([B], [1024], qlens, own, page, 1)
+        (kp, vp, _, _), _ = pages_of(2, n, kv, page, hd, 'f16', 'f16')
+        for kw in (dict(shared=(i32([0, B]), i32([1024]))), dict(window=700, sinks=5)):
+            q = rows(3, sum(qlens), H, hd, 'f16')
+            want = K.attention_paged(q, kp, vp, i32(table), cu(qlens), i32(lens), **kw)
+            assert K.attention_paged(q, kp, vp, i32(table), cu(qlens), i32(lens), out=q, **kw) is q and torch.equal(q, want)
+
+
+def test_strided_queries_and_outputs(gpu):
+    from chestnut import kernels as K
+    H, kv, hd, page, qlens, own = 6, 3, 64, 16, [1, 5, 33], [20, 5, 400]
+    table, n, lens = shared_batch([3], [160], qlens, own, page, 1)
+    (kp, vp, _, _), _ = pages_of(2, n, kv, page, hd, 'bf16', 'bf16')
+    wide = rows(3, sum(qlens), H + 4, hd + 8, 'bf16')
+    q = wide[:, 2:2 + H, :hd]
+    for kw in (dict(shared=(i32([0, 3]), i32([160]))), dict(window=100, sinks=5)):
+        want = K.attention_paged(q.contiguous(), kp, vp, i32(table), cu(qlens), i32(lens), **kw)
+        buf = torch.full((sum(qlens), H + 2, hd + 4), 5.0, dtype=torch.bfloat16, device='cuda')
+        K.attention_paged(q, kp, vp, i32(table), cu(qlens), i32(lens), out=buf[:, 1:1 + H, :hd], **kw)
+        assert torch.equal(buf[:, 1:1 + H, :hd], want)
+        buf[:, 1:1 + H, :hd] = 5.0
+        assert (buf == 5.0).all()
+
+
+def test_empty_calls(gpu):
+    from chestnut import kernels as K
+    (kp, vp, _, _), _ = pages_of(2, 3, 2, 16, 64, 'f16', 'f16')
+    none = torch.zeros(0, 4, 64, dtype=torch.float16, device='cuda')
+    for kw in (dict(shared=(i32([0, 2]), i32([16]))), dict(window=5)):
+        assert K.attention_paged(none, kp, vp, i32([[0], [0]]), i32([0, 0, 0]), i32([16, 16]), **kw).shape == (0, 4, 64)
+        q = rows(1, 3, 4, 64, 'f16')
+        assert (K.attention_paged(q, kp, vp, i32(np.zeros((2, 0))), i32([0, 1, 3]), i32([5, 5]), **kw) == 0).all()     # no pages: no keys
+        out = torch.full_like(q, 3.0)
+        K.attention_paged(q, kp, vp, i32([[0], [0]]), i32([0, 0, 0]), i32([16, 16]), out=out, **kw)                    # no sequence has a row
+        assert (out == 3.0).all()
+    assert K.attention_varlen(none, none, none, i32([0]), window=3).shape == (0, 4, 64)
+
+
+def test_long_cache_offsets_pass_32_bits(gpu):
+    """A cache of over 2^32 elements: shared pages and a window on its last pages."""
+    from chestnut import kernels as K
+    kv, hd, page, n = 8, 128, 1024, 4200
+    kp, vp = (torch.zeros(n, kv, page, hd, dtype=torch.uint8, device='cuda').view(torch.float8_e4m3fn) for _ in 'kv')
+    ks, vs = (torch.full((n, kv, page), 127, dtype=torch.uint8, device='cuda').view(torch.float8_e8m0fnu) for _ in 'kv')
+    table = np.array([[n - 1, n - 3], [n - 1, n - 2]])
+    lens = [1500, 1324]
+    k, v = rows(1, 2048 + 1024, kv, hd, 'f16'), rows(2, 2048 + 1024, kv, hd, 'f16')
+    j = np.arange(1024)
+    K.cache_write(k, v, kp, vp, i32(np.concatenate([(n - 1) * page + j, (n - 3) * page + j, (n - 2) * page + j])), k_scale=ks, v_scale=vs)
+    gk, gv = (O.values(*O.quantise(f64(x), 61440.0)) for x in (k, v))
+    for m in (1, 60):
+        q = rows(3, 2 * m, kv, hd, 'f16')
+        for kw in (dict(shared=(i32([0, 2]), i32([1024]))), dict(window=700, sinks=70)):
+            out = K.attention_paged(q, kp, vp, i32(table), cu([m, m]), i32(lens), k_scale=ks, v_scale=vs, **kw)
+            for b in range(2):
+                at = np.concatenate([j, (1 + b) * 1024 + j])[:lens[b]]
+                ref = O.attention(f64(q[b * m:b * m + m]), gk[at], gv[at], window=kw.get('window'), sinks=kw.get('sinks', 0))
+                near(out[b * m:b * m + m], *ref, lens[b], hd, 'f16', str(kw.keys()))
+
+
+# ------------------------------------------------------------------ a run of them --
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('quant', [False, True])
+@pytest.mark.parametrize('kind', ['window', 'shared'])
+def test_a_run_of_steps(gpu, dt, quant, kind):
+    """Prompts, then single tokens, a step each of cache_maps, norm_rope, cache_write and attention_paged, whose results follow
+    from the whole sequence: its rows normed, turned by three axes, cached (e4m3: as cache_read reads them) and attended in
+    64 bits.  The last steps are replays of a captured one, beside the same steps run eagerly on state of their own."""
+    from chestnut import kernels as K
+    H, kv, hd, page, B, steps = 8, 2, 64, 16, 5, 9
+    r = np.random.default_rng(12)
+    lens, pre = np.array([3, 40, 17, 1, 64]), (48 if kind == 'shared' else 0)
+    total = lens + steps
+    qkv = [rows(30 + b, int(total[b]), H + 2 * kv, hd, dt) for b in range(B)]
+    first = rows(29, pre, H + 2 * kv, hd, dt)                                         # what all share
+    f, s = K.rope_frequencies(48, base=1e4)
+    axes = K.rope_axes([8, 8, 8], turns=True)
+    wq, wk = (torch.rand(hd, device='cuda').to(DT[dt]) + 0.5 for _ in 'qk')
+    width = -(-int(pre + total.max()) // page) + 1
+    n_pages = B * width + 3
+    free = i32(r.permutation(n_pages))
+
+    def state():
+        if quant:
+            c = [torch.zeros(n_pages, kv, page, hd, dtype=torch.uint8, device='cuda').view(torch.float8_e4m3fn) for _ in 'kv'] + \
+                [torch.zeros(n_pages, kv, page, dtype=torch.uint8, device='cuda').view(torch.float8_e8m0fnu) for _ in 'kv']
+        else:
+            c = [torch.zeros(n_pages, kv, page, hd, dtype=DT[dt], device='cuda') for _ in 'kv'] + [None, None]
+        return dict(cache=c, table=torch.full((B, width), -1, dtype=torch.int32, device='cuda'), kv=torch.zeros(B, dtype=torch.int32, device='cuda'),
+                    taken=i32([0]))
+
+    def step(st, new, x, out=None):
+        cu_q, kv_lens, pos, slots = K.cache_maps(new, st['kv'], st['table'], page, x.shape[0], free_pages=free, taken=st['taken'], kv_out=st['kv'])
+        at = torch.stack([pos, pos // 7, pos % 7])                                     # time, row and column of a place
+        q, k = x[:, :H], x[:, H:H + kv]
+        K.norm_rope(q, k, wq, wk, at, f, axes=axes, scale=s, q_out=q, k_out=k)
+        kp, vp, ks, vs = st['cache']
+        K.cache_write(k, x[:, H + kv:], kp, vp, slots, k_scale=ks, v_scale=vs)
+        kw = dict(window=21, sinks=2) if kind == 'window' else dict(shared=(i32_dev[0], i32_dev[1]))
+        return K.attention_paged(q, kp, vp, st['table'], cu_q, kv_lens, k_scale=ks, v_scale=vs, out=out, **kw)
+    i32_dev = (i32([0, B]), i32([pre]))
+
+    def begin(st):
+        """The shared rows in pages that all tables begin with."""
+        if not pre:
+            return
+        K.cache_maps(i32([pre]), i32([0]), st['table'][:1], page, pre, free_pages=free, taken=st['taken'])
+        st['table'][1:] = st['table'][:1]
+        j = np.arange(pre)
+        slots = (st['table'][0][i32(j // page).long()] * page + i32(j % page)).int()
+        x = first.clone()
+        pos = i32(j)
+        K.norm_rope(x[:, :H], x[:, H:H + kv], wq, wk, torch.stack([pos, pos // 7, pos % 7]), f, axes=axes, scale=s, q_out=x[:, :H],
+                    k_out=x[:, H:H + kv])
+        K.cache_write(x[:, H:H + kv], x[:, H + kv:], st['cache'][0], st['cache'][1], slots, k_scale=st['cache'][2], v_scale=st['cache'][3])
+        st['kv'].fill_(pre)
+
+    # the whole sequences in 64 bits
+    want = []
+    for b in range(B):
+        x = f64(torch.cat([first, qkv[b]]))
+        j = np.arange(x.shape[0])
+        at = np.stack([j, j // 7, j % 7])
+        y = [O.rope(O.rms_norm(x[:, a:c], f64(w)), at, f64(f), False, s, axes=axes.tolist()) for a, c, w in ((0, H, wq), (H, H + kv, wk))]
+        q, k = (f64(torch.from_numpy(t).to(DT[dt])) for t in y)
+        v = x[:, H + kv:]
+        if quant:
+            k, v = (O.values(*O.quantise(t, 61440.0 if dt == 'f16' else 1.875 * 2.0 ** 127)) for t in (k, v))
+        ref, mag, most = O.attention(q, k, v, window=21 if kind == 'window' else None, sinks=2 if kind == 'window' else 0)
+        want.append((ref[pre:], mag[pre:], most))
+
+    def close(out, b, i, what):
+        """q, k (and their codes) differ from the oracle's by a step here and there: a rounding of the norm's result that falls
+        the other way, u of its size each, moves a score by 2 u sum |q k| (e4m3: a code by 2^-3 of its size), and the
+        weights and the output by as much of A."""
+        ref, mag, most = want[b]
+        move = 2 * u(dt) * most + (2.0 ** -3 * most if quant else 0)
+        tol = (u(dt) * 3 + 2 * move + 2.0 ** -10) * mag[i]
+        assert np.all(np.abs(f64(out) - ref[i]) <= tol + u(dt) * np.abs(ref[i])), f'{what}: request {b}, row {i}'
+
+    a, e = state(), state()                  # one stepped by replays at last, one eagerly
+    outs = []
+    for st in (a, e):
+        begin(st)
+        x = torch.cat([qkv[b][:lens[b]] for b in range(B)] + [torch.zeros(2, H + 2 * kv, hd, dtype=DT[dt], device='cuda')])     # and padded rows
+        outs.append(step(st, i32(lens), x)[:int(lens.sum())])
+    assert torch.equal(*outs)
+    at = 0
+    for b in range(B):
+        for i in range(lens[b]):
+            close(outs[0][at + i], b, i, 'prompt')
+        at += lens[b]
+    ones, x = i32([1] * B), torch.zeros(B, H + 2 * kv, hd, dtype=DT[dt], device='cuda')
+    token = lambda t: torch.stack([qkv[b][lens[b] + t] for b in range(B)])
+    out = torch.zeros(B, H, hd, dtype=DT[dt], device='cuda')
+    x.copy_(token(0))
+    step(a, ones, x, out)
+    wanted = step(e, ones, token(0))
+    assert torch.equal(out, wanted)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=side):
+            step(a, ones, x, out)
+    torch.cuda.synchronize()
+    for t in range(1, steps):
+        x.copy_(token(t))
+        g.replay()
+        wanted = step(e, ones, token(t))
+        torch.cuda.synchronize()
+        assert torch.equal(out, wanted) and torch.equal(a['kv'], e['kv']) and torch.equal(a['table'], e['table']), t
+        assert torch.equal(a['cache'][0].view(torch.uint8), e['cache'][0].view(torch.uint8)) and torch.equal(a['taken'], e['taken'])
+        for b in range(B):
+            close(out[b], b, lens[b] + t, f'step {t}')
+    assert np.array_equal(a['kv'].cpu().numpy(), pre + total)
