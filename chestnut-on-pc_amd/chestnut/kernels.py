@@ -311,6 +311,11 @@ def _rows(t, dtype, name, shape, unit=8, write=False):
         raise ValueError(f'{name} must have shape {(T, H, hd)}, got {tuple(t.shape)}')
     if T > _INT:
         raise ValueError(f'{name} must have under 2^31 rows, got {T}')
+    if t.is_contiguous():   # rows side by side
+        s0, s1 = H * hd if T > 1 else 0, hd if H > 1 else 0
+        if (s0 | s1) % unit or t.data_ptr() % (2 * unit):
+            raise ValueError(f'{name} must have rows that start at multiples of {2 * unit} bytes')
+        return s0, s1
     s0, s1, s2 = t.stride()
     if s2 != 1 and hd > 1:
         raise ValueError(f'{name} must be contiguous in its last dimension')
@@ -586,12 +591,11 @@ def cache_maps(new_lens, kv_lens, block_table, page, tokens, free_pages=None, ta
     kv_out: kv_lens itself (a captured step then advances by itself), another
     tensor, or None: a new one."""
     B, width, n_free, dev = _maps(new_lens, kv_lens, block_table, page, tokens, free_pages, taken, kv_out, taken_out)
-    # one allocation for all outputs (an allocation costs about 1 us, as does a view)
-    sizes = [B + 1, tokens, tokens]
+    # one allocation for all outputs, cut up in one call
     if kv_out is None:
-        cu, positions, slots, kv_out = torch.empty(2 * (B + tokens) + 1, dtype=torch.int32, device=new_lens.device).split(sizes + [B])
+        cu, positions, slots, kv_out = torch.split_with_sizes(new_lens.new_empty(2 * (B + tokens) + 1), (B + 1, tokens, tokens, B))
     else:
-        cu, positions, slots = torch.empty(B + 1 + 2 * tokens, dtype=torch.int32, device=new_lens.device).split(sizes)
+        cu, positions, slots = torch.split_with_sizes(new_lens.new_empty(B + 1 + 2 * tokens), (B + 1, tokens, tokens))
     if taken is not None and taken_out is None:
         taken_out = taken
     nb = 0
@@ -609,27 +613,23 @@ def cache_maps(new_lens, kv_lens, block_table, page, tokens, free_pages=None, ta
 def _maps(new_lens, kv_lens, block_table, page, tokens, free_pages, taken, kv_out, taken_out):
     """The checks of cache_maps: (B, table width, pages in the list, device)."""
     T, i32 = torch.Tensor, torch.int32
-    if type(new_lens) is T and type(block_table) is T and type(tokens) is type(page) is int and \
-            (free_pages is None) == (taken is None) and (taken is not None or taken_out is None):
+    if type(new_lens) is type(kv_lens) is type(block_table) is T and type(tokens) is type(page) is int and \
+            new_lens.dtype is kv_lens.dtype is block_table.dtype is i32:
         # all in one pass where all is well
-        shape, dev = block_table.shape, new_lens.get_device()
-        if len(shape) == 2 and shape[0] < 1 << 20 and 0 <= tokens < 1 << 30 and 16 <= page <= 1024 and not page & (page - 1) and \
-                shape[1] * page <= 1 << 30 and dev >= 0 and dev == _device():
-            B = shape[:1]
-            each = [(new_lens, B), (kv_lens, B), (block_table, shape)]
-            if kv_out is not None:
-                each.append((kv_out, B))
-            n_free = 0
-            if taken is not None:
-                if type(free_pages) is T and free_pages.dim() == 1:
-                    n_free = free_pages.shape[0]
-                each += [(free_pages, (n_free,)), (taken, (1,))]
-                if taken_out is not None:
-                    each.append((taken_out, (1,)))
-            for t, want in each:
-                if type(t) is not T or t.dtype is not i32 or t.shape != want or t.get_device() != dev or not t.is_contiguous():
-                    break
-            else:
+        shape, at, dev = block_table.shape, new_lens.shape, new_lens.get_device()
+        if len(shape) == 2 and at == shape[:1] == kv_lens.shape and shape[0] < 1 << 20 and 0 <= tokens < 1 << 30 and \
+                16 <= page <= 1024 and not page & (page - 1) and shape[1] * page <= 1 << 30 and dev >= 0 and \
+                kv_lens.get_device() == block_table.get_device() == dev == _device() and new_lens.is_contiguous() and \
+                kv_lens.is_contiguous() and block_table.is_contiguous():
+            ok = kv_out is None or (type(kv_out) is T and kv_out.dtype is i32 and kv_out.shape == at and
+                                    kv_out.get_device() == dev and kv_out.is_contiguous())
+            if ok and free_pages is None and taken is None and taken_out is None:
+                return shape[0], shape[1], 0, dev
+            if ok and type(free_pages) is type(taken) is T and free_pages.dtype is taken.dtype is i32 and free_pages.dim() == 1 and \
+                    taken.shape == (1,) and free_pages.get_device() == taken.get_device() == dev and free_pages.is_contiguous() and \
+                    (taken_out is None or (type(taken_out) is T and taken_out.dtype is i32 and taken_out.shape == (1,) and
+                                           taken_out.get_device() == dev)):
+                n_free = free_pages.shape[0]
                 if n_free <= _INT:
                     return shape[0], shape[1], n_free, dev
     return _maps_each(new_lens, kv_lens, block_table, page, tokens, free_pages, taken, kv_out, taken_out)
@@ -886,14 +886,17 @@ def attention_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, k_scale=Non
     if ranged or groups:
         nb = _cached_range_bytes(B, T, B * width * page, H, kv, hd, window if ranged else 0, sinks, groups)
         ws = _workspace(workspace, nb, q.device)
-        head = (q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale), o.data_ptr(),
-                block_table.data_ptr(), width, cu_q.data_ptr(), kv_lens.data_ptr())
-        sizes = (B, T, H, n, kv, page, hd, qt, qh, ot, oh, _DTYPE[q.dtype], _DTYPE[k_pages.dtype])
         if ranged:
-            check(lib().ck_attention_paged_window(*head, *sizes, window, sinks, scale, _ptr(ws), nb, _raw_stream(dev)))
+            check(lib().ck_attention_paged_window(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale),
+                                                  o.data_ptr(), block_table.data_ptr(), width, cu_q.data_ptr(), kv_lens.data_ptr(), B,
+                                                  T, H, n, kv, page, hd, qt, qh, ot, oh, _DTYPE[q.dtype], _DTYPE[k_pages.dtype],
+                                                  window, sinks, scale, _ptr(ws), nb, _raw_stream(dev)))
         else:
-            check(lib().ck_attention_paged_shared(*head, cu_s.data_ptr(), s_lens.data_ptr(), groups, *sizes, 1 if causal else 0,
-                                                  scale, _ptr(ws), nb, _raw_stream(dev)))
+            check(lib().ck_attention_paged_shared(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale),
+                                                  o.data_ptr(), block_table.data_ptr(), width, cu_q.data_ptr(), kv_lens.data_ptr(),
+                                                  cu_s.data_ptr(), s_lens.data_ptr(), groups, B, T, H, n, kv, page, hd, qt, qh, ot,
+                                                  oh, _DTYPE[q.dtype], _DTYPE[k_pages.dtype], 1 if causal else 0, scale, _ptr(ws),
+                                                  nb, _raw_stream(dev)))
         return o
     nb = _cached_attention_bytes(B, T, B * width * page, H, kv, hd)
     ws = _workspace(workspace, nb, q.device)
