@@ -508,7 +508,8 @@ def norm_rope(q, k, q_weight, k_weight, positions, inv_freq, eps=1e-6, axes=None
     + eps), times q_weight or k_weight [head_dim] (both float32 or of q's type;
     None: ones), then turned as `rope` turns it, in one pass and with one rounding:
     (q_out, k_out).  k None: q alone (and k_out None).  q_out may be q and
-    k_out k (in place); outputs overlap nothing else."""
+    k_out k (in place); outputs overlap nothing else.  The squares are summed in
+    32 bits: heads with values of 2^59 and more (bfloat16) become zeros."""
     if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in (_F16, _BF16):
         raise ValueError('q must be float16 or bfloat16 [T, heads, head_dim]')
     T, H, hd = q.shape
@@ -589,8 +590,12 @@ def cache_maps(new_lens, kv_lens, block_table, page, tokens, free_pages=None, ta
     block_table names the new pages already.  A place without a page (a negative entry, or past the
     table) has slot -1.
     kv_out: kv_lens itself (a captured step then advances by itself), another
-    tensor, or None: a new one."""
+    tensor that overlaps no input, or None: a new one.
+    workspace: a float32 buffer to keep, of at least cache_maps_workspace bytes (else
+    a new one is made), one for each call that may run beside another."""
     B, width, n_free, dev = _maps(new_lens, kv_lens, block_table, page, tokens, free_pages, taken, kv_out, taken_out)
+    if kv_out is not None and B and kv_out.data_ptr() == new_lens.data_ptr():
+        raise ValueError('kv_out must not be new_lens')
     # one allocation for all outputs, cut up in one call
     if kv_out is None:
         cu, positions, slots, kv_out = torch.split_with_sizes(new_lens.new_empty(2 * (B + tokens) + 1), (B + 1, tokens, tokens, B))
@@ -829,7 +834,7 @@ def attention_varlen(q, k, v, cu_q, cu_k=None, causal=True, scale=None, out=None
     o = out if out is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if ranged:
         nb = _cached_range_bytes(B, T, Tk, H, kv, hd, window, sinks, 0)
-        ws = _workspace(workspace, nb, q.device)
+        ws = _workspace(workspace, nb, q.device) if workspace is not None else q.new_empty(nb >> 1) if nb else None
         check(lib().ck_attention_varlen_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu_q.data_ptr(),
                                                cu_k.data_ptr(), B, T, Tk, H, kv, hd, qt, qh, kt, kh, vt, vh, ot, oh,
                                                _DTYPE[q.dtype], window, sinks, scale, _ptr(ws), nb, _raw_stream(dev)))
@@ -852,10 +857,11 @@ def attention_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, k_scale=Non
     cache has q's type or is e4m3, whose values are rounded to q's type as cache_read
     rounds them (past float16's range: infinite).  Otherwise as attention_varlen.
     shared: (cu_shared int32 [N+1], shared_lens int32 [N]) on the device -- the tables of the
-    sequences cu_shared[g] .. cu_shared[g+1] begin with the same pages, which hold their first
-    shared_lens[g] keys (as far as these fill whole pages).  The shared keys are then read
-    once for all queries of the group, from the table of its first sequence; the result
-    is the same up to rounding.  Sequences may be in no group; not with a window."""
+    sequences cu_shared[g] .. cu_shared[g+1] (ascending) begin with the same pages, which hold
+    their first shared_lens[g] keys (as far as these fill whole pages).  The shared keys are then
+    read once for all queries of the group, from the table of its first sequence; the result
+    is the same up to rounding.  Sequences may be in no group; not with a window.  Its
+    workspace: attention_workspace with groups=N."""
     n, kv, page, hd = _cache(k_pages, v_pages, k_scale, v_scale)
     T, H, B, (qt, qh), (ot, oh), scale = _queries(q, cu_q, kv, hd, out, scale)
     if k_pages.dtype not in (q.dtype, _E4M3):
@@ -885,7 +891,7 @@ def attention_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, k_scale=Non
     o = out if out is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if ranged or groups:
         nb = _cached_range_bytes(B, T, B * width * page, H, kv, hd, window if ranged else 0, sinks, groups)
-        ws = _workspace(workspace, nb, q.device)
+        ws = _workspace(workspace, nb, q.device) if workspace is not None else q.new_empty(nb >> 1) if nb else None
         if ranged:
             check(lib().ck_attention_paged_window(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scale), _ptr(v_scale),
                                                   o.data_ptr(), block_table.data_ptr(), width, cu_q.data_ptr(), kv_lens.data_ptr(), B,

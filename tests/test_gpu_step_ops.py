@@ -283,6 +283,48 @@ def test_lengths_that_make_no_sense_stay_inside(gpu, in_place):
     assert (slots < 200 * 16).all() and (positions >= 0).all()
 
 
+def test_kv_out_may_not_be_new_lens(gpu):
+    from chestnut import kernels as K
+    n = i32([1, 2])
+    with pytest.raises(ValueError, match='kv_out must not be new_lens'):
+        K.cache_maps(n, i32([0, 0]), i32([[0], [1]]), 16, 3, kv_out=n)
+
+
+def test_maps_norms_and_axes_replay(gpu):
+    """Captured with padded rows; lengths, positions and rows change between the replays, beside eager calls."""
+    from chestnut import kernels as K
+    B, T, H, kv, hd, page = 6, 1500, 4, 2, 64, 16                     # (over 1024 rows and in place: two launches)
+    r = np.random.default_rng(9)
+    f, axes = K.rope_frequencies(64)[0], K.rope_axes([16, 8, 8])
+    free = i32(r.permutation(2000))
+    new, kvl, x = i32([1] * B), i32([0] * B), rows(1, T, H + 2 * kv, hd, 'bf16')
+    table, taken = torch.full((B, 200), -1, dtype=torch.int32, device='cuda'), i32([0])
+    y = torch.empty(T, H + kv, hd, dtype=torch.bfloat16, device='cuda')
+
+    def step(kvl, table, taken):
+        cu, k, pos, slots = K.cache_maps(new, kvl, table, page, T, free_pages=free, taken=taken, kv_out=kvl)
+        at = torch.stack([pos, pos // 5, pos % 5])
+        a, b = K.norm_rope(x[:, :H], x[:, H:H + kv], None, None, at, f, axes=axes)
+        return cu, pos, slots, a, b, K.rope(x[:, :H + kv], at, f, interleaved=True, axes=axes, out=y)
+    mine = [t.clone() for t in (kvl, table, taken)]
+    side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=side):
+            got = step(kvl, table, taken)
+    torch.cuda.synchronize()
+    for lens in ([1] * 6, [250] * 6, [0, 0, 900, 1, 0, 3], [3, 1, 4, 1, 5, 9], [0] * 6):
+        new.copy_(i32(lens))
+        x.copy_(rows(sum(lens) + 3, T, H + 2 * kv, hd, 'bf16'))
+        g.replay()
+        out = [t.clone() for t in got]
+        want = step(*mine)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want)), lens
+        assert torch.equal(kvl, mine[0]) and torch.equal(table, mine[1]) and torch.equal(taken, mine[2])
+
+
 def test_cache_maps_on_two_streams_with_workspaces_of_their_own(gpu):
     from chestnut import kernels as K
     sets, want = [], []
