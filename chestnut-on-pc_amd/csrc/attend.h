@@ -1,5 +1,6 @@
-// Attention of packed sequences of queries over their K/V rows, contiguous or in a paged
-// cache; causal or full; query heads in groups that share a K/V head.
+// The kernels of attention of packed sequences of queries over their K/V rows, contiguous or in a
+// paged cache; causal or full, through a sliding window, or with first pages that sequences share;
+// query heads in groups that share a K/V head.
 //
 //   s_ij = scale * q_i . k_j,   o_i = sum_j softmax(s_i)_j v_j
 // over the keys j < kv_len that query i may see (causal: j <= i + kv_len - q_len, the queries
@@ -22,12 +23,15 @@
 //   shared pages:    the sequences of a group hold their first keys in the same pages.  These keys
 //                    and all the group's queries are one piece of work (the front), the keys behind
 //                    them one for each sequence; a row's sums of both are joined.
-// Three kernels (their figures stand at each):
+// RANGE walks a list of blocks of 64 keys that need not follow one another, with one more limit a row, and
+// keeps a bit a key, not the first key alone, of the infinities and NaN of V that it takes out of a tile.
+// The kernels (their figures stand at each):
 //   attend_tile_kernel  128 or 256 rows, tiles of 64 keys in LDS: prompts and chunks of one;
 //                       bound by the matrix cores, the vector unit's exponentials and the
 //                       tiles' loads, which run side by side in part only;
 //   attend_few_kernel   16 or 32 rows, the keys over four waves: tokens one by one; bound by memory;
-//   attend_join_kernel  joins the parts of rows whose keys were split over workgroups.
+//   attend_join_kernel  joins the parts of rows whose keys were split over workgroups;
+//   attend_join_shared_kernel  the same for the parts of shared pages and of a sequence's own keys.
 #pragma once
 
 #include <algorithm>
@@ -1229,6 +1233,10 @@ __device__ __forceinline__ void leave_head(const AttendParams& p, const Item& it
 // and 10 us, 545 by the call, though with 128 features that kernel spills 43 registers (tiles
 // of 256 rows: 19; without codes to turn into values: 1).  Short prompts (40 of 1 to 239 tokens,
 // 8 heads of 64) 12.4 us.
+// RANGE, 128 rows: prompts of 9001, 5120 and 2263 through 2048 keys and 4 first ones, 16 heads on 4 of 128, bf16, 268 us:
+// 224 GFLOP seen, 240 issued, 0.90 PFLOP/s of these (through all keys 467, where WHOLE takes 460 with 128 rows).  256 rows:
+// 288.  Six chunks of 1 to 512 tokens on 12800 shared keys, f16, 224 us and 11.5 to join them, 178 GFLOP, 0.79 PFLOP/s.
+// Masked tiles in the pipeline with the others: prompts 272 -> 270, but e4m3 spills in the loop (46 -> 70 below).
 template <typename T, int HD, int FORM>
 struct TileLds {
   // (bad: WHOLE, the first key of a kind and feature; RANGE, a bit for each key of the tile)
@@ -1489,7 +1497,14 @@ constexpr int FEW_WAVES = 4;
 // workgroups a CU
 constexpr int few_at_once(int bm, int hd, bool e4m3) { return hd == 64 ? (bm == 16 ? 4 : 3) : bm == 16 && e4m3 ? 3 : 2; }
 
+// RANGE: one token of 32 streams through 4096 keys and 16 first ones, 16 heads on 4 of 128, e4m3, 133 MB: 29.9 us = 4.4
+// TB/s, of which about 8 are a workgroup's beginning (lengths, then the table, then keys, each a wait for memory), and 4.7 to
+// join them; one token through 512 keys, 8 heads of 64, whole: 10.0 us.
 // MIXED (shared pages, single tokens): the groups' fronts by tiles of 128 rows, the sequences' own keys by few rows.
+// 64 streams on 24576 and 12800 shared keys and 1 to 1500 of their own, 16 heads on 4 of 128, e4m3, 87 MB: 40.7 us and 5.2 to
+// join them (all by tiles 62 and 5.5).  Bound by the waits for memory: a step of e4m3 tiles takes 1.6 us where the next
+// tile's keys come from HBM, and two workgroups a CU are all that registers allow.  Own keys two steps ahead: 46.6 us a
+// call for 45.7; in chunks twice as long 46.0, four times 63.
 template <typename T, int HD, int KV, typename R, int FORM, bool MIXED = false>
 __global__ __launch_bounds__(64 * FEW_WAVES, MIXED ? 2 : few_at_once(R::BM, HD, KV == KV_E4M3)) void attend_few_kernel(const AttendParams p) {
   constexpr int BM = R::BM, KEYS = 32, TILE = KEYS * HD, NW = FEW_WAVES, BMF = MIXED ? 128 : BM;
@@ -1504,7 +1519,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, MIXED ? 2 : few_at_once(R::BM, HD, 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hk = blockIdx.x % p.Hkv, index = blockIdx.x / p.Hkv;
   Item it;
-  if (FORM == RANGE && KV != KV_ROWS && (MIXED || p.N)) {
+  if (FORM == RANGE && KV != KV_ROWS && BM == 16 && (MIXED || p.N)) {
     int tiles;
     const bool some = find_shared<KV, BM, BMF>(p, index, it, tiles);
     if (blockIdx.x == 0 && tid == 0) leave_head<HD>(p, it, tiles);
@@ -1785,9 +1800,6 @@ void launch_shared(const AttendParams& p, const Plan& pl, hipStream_t s) {
   if (pl.bmf == 16) {
     CK_LAUNCH((attend_few_kernel<T, HD, KV, Rows16<T, HD, RANGE>, RANGE>), grid, dim3(256), 0, s, p);
     CK_LAUNCH((attend_join_shared_kernel<T, HD, 16, 16>), dim3(tiles, 16), dim3(256), 0, s, p);
-  } else if (pl.bmf == 32) {
-    CK_LAUNCH((attend_few_kernel<T, HD, KV, Rows<T, HD, RANGE>, RANGE>), grid, dim3(256), 0, s, p);
-    CK_LAUNCH((attend_join_shared_kernel<T, HD, 32, 32>), dim3(tiles, 32), dim3(256), 0, s, p);
   } else if (pl.bm == 16) {
     CK_LAUNCH((attend_few_kernel<T, HD, KV, Rows16<T, HD, RANGE>, RANGE, true>), grid, dim3(256), 0, s, p);
     CK_LAUNCH((attend_join_shared_kernel<T, HD, 16, 128>), dim3(tiles, 16), dim3(256), 0, s, p);

@@ -12,12 +12,14 @@ Plan range_plan(int B, int Tq, long keys, int n_heads, int n_kv, int window, int
   const int G = n_heads / n_kv;
   const long rows = (long)Tq * G;
   if (groups) {
-    // the rows that share keys are a group's
-    pl.bmf = rows <= 16L * groups ? 16 : rows <= 32L * groups ? 32 : 128;
-    pl.bm = pl.bmf < 128 ? pl.bmf : rows <= 16L * B ? 16 : 128;
+    // the rows that share keys are a group's: tiles where it has more than 16 on average (24 tokens on 12800 shared keys, 8
+    // heads of 64, 22.0 us by 32 few rows, 18.6 by tiles; 12 of 4 heads a K/V head of 128, f16, 32.1 and 20.1; of up to 16
+    // rows, 4 such tokens, 17.8 by few and 18.9 by tiles), and single tokens' own keys by few rows beside them
+    pl.bmf = rows <= 16L * groups ? 16 : 128;
+    pl.bm = rows <= 16L * (pl.bmf == 16 ? groups : B) ? 16 : 128;
     pl.tiles = rows / pl.bm + B;                // the sequences' own
     const long fronts = rows / pl.bmf + groups, slots = pl.bmf == 128 ? 512 : pl.bmf == 16 && few3 ? 768 : 1024;
-    pl.min_blocks = pl.bmf <= 32 ? 2 : 4;
+    pl.min_blocks = pl.bmf == 16 ? 2 : 4;
     const bool many = pl.bmf == 128 && (fronts + pl.tiles) * n_kv >= 2 * slots;
     if (!many && keys / B > 2 * pl.min_blocks * AT_KEYS) pl.target = (int)std::max(1L, slots / n_kv);
     pl.front_items = fronts + pl.target;

