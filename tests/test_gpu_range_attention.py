@@ -455,6 +455,28 @@ def test_out_may_be_q(gpu):
             assert K.attention_paged(q, kp, vp, i32(table), cu(qlens), i32(lens), out=q, **kw) is q and torch.equal(q, want)
 
 
+@pytest.mark.parametrize('H,kv,hd', [(160, 1, 64), (96, 2, 128), (66, 1, 128)])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('qlens', [[1], [1, 1, 1], [2, 0, 3, 40]], ids=str)
+def test_many_heads_on_one_of_the_cache(gpu, H, kv, hd, dt, qlens):
+    """A query's heads fill a tile and more; rows before the first sequence and behind the last stay as they were."""
+    from chestnut import kernels as K
+    B, page, front, own = len(qlens), 16, 5, [1 + 90 * b + x for b, x in enumerate(qlens)]
+    table, n, lens = shared_batch([B], [448], qlens, own, page, 1)
+    (kp, vp, _, _), vals = pages_of(2, n, kv, page, hd, dt, dt)
+    q = rows(3, front + sum(qlens) + 2, H, hd, dt)
+    starts = cu(qlens) + front
+    for kw in (dict(shared=(i32([0, B]), i32([448]))), dict(window=200, sinks=5)):
+        out = torch.full_like(q, 9.0)
+        K.attention_paged(q, kp, vp, i32(table), starts.int(), i32(lens), out=out, **kw)
+        assert (out[:front] == 9.0).all() and (out[front + sum(qlens):] == 9.0).all()
+        a = front
+        for b, (x, m) in enumerate(zip(qlens, lens)):
+            k, v = gathered(vals, table[b], m, page)
+            near(out[a:a + x], *expect(q[a:a + x], k, v, kw.get('window'), kw.get('sinks', 0)), m, hd, dt, f'sequence {b}: {x} over {m}')
+            a += x
+
+
 def test_strided_queries_and_outputs(gpu):
     from chestnut import kernels as K
     H, kv, hd, page, qlens, own = 6, 3, 64, 16, [1, 5, 33], [20, 5, 400]
