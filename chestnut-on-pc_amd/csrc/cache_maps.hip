@@ -29,7 +29,7 @@ struct MapsParams {
   int* table;
   const int *free_pages, *taken;
   int *cu, *kv_out, *positions, *slots, *taken_out;
-  int* first;             // two launches: each request's first page in the list, [B]
+  int *old, *first;       // two launches: each request's places before (kv may be overwritten) and first page in the list, [B]
   int B, width, shift, T, n_free;
 };
 
@@ -103,7 +103,10 @@ __global__ __launch_bounds__(CM_ROWS) void cache_maps_kernel(const MapsParams p)
       if (writes && b < p.B) {
         p.cu[b + 1] = held(start + n);
         p.kv_out[b] = held((long)old + n);
-        if (MODE == MAPS_SCAN) p.first[b] = held(first);
+        if (MODE == MAPS_SCAN) {
+          p.old[b] = old;
+          p.first[b] = held(first);
+        }
       }
     }
     rows = sum.rows;
@@ -127,8 +130,8 @@ __global__ __launch_bounds__(CM_ROWS) void cache_maps_kernel(const MapsParams p)
     for (int b = lo + tid; b < p.B; b += CM_ROWS) {
       const long start = p.cu[b];
       if (start >= t0 + CM_ROWS) break;
-      const int n = p.cu[b + 1] - (int)start;
-      leave(b, start, n, p.kv_out[b] - n, p.first[b]);
+      // (n and old not from cu's and kv_out's differences: these are held at 2^31 - 1)
+      leave(b, start, max(p.new_lens[b], 0), p.old[b], p.first[b]);
     }
   }
   if (MODE == MAPS_SCAN) return;
@@ -177,7 +180,7 @@ bool in_two(int B, int tokens, bool in_place) { return B > 0 && tokens > CM_ROWS
 
 size_t cache_maps_workspace(int B, int tokens, bool in_place) {
   CK_REQUIRE(B >= 0 && tokens >= 0, "cache_maps: bad sizes");
-  return in_two(B, tokens, in_place) ? sizeof(int) * (size_t)B : 0;
+  return in_two(B, tokens, in_place) ? 2 * sizeof(int) * (size_t)B : 0;
 }
 
 void launch_cache_maps(const CacheMaps& m, hipStream_t s) {
@@ -190,7 +193,7 @@ void launch_cache_maps(const CacheMaps& m, hipStream_t s) {
              "cache_maps: null pointer");
   CK_REQUIRE(!m.free_pages == !m.taken && !m.taken == !m.taken_out, "cache_maps: free pages need the number of them that is taken");
   const bool two = in_two(m.B, m.tokens, m.kv_out == m.kv || (m.taken && m.taken_out == m.taken));
-  CK_REQUIRE(!two || (m.ws && m.ws_bytes >= sizeof(int) * (size_t)m.B), "cache_maps: workspace too small (ck_cache_maps_workspace)");
+  CK_REQUIRE(!two || (m.ws && m.ws_bytes >= 2 * sizeof(int) * (size_t)m.B), "cache_maps: workspace too small (ck_cache_maps_workspace)");
   MapsParams p{};
   p.new_lens = m.new_lens;
   p.kv = m.kv;
@@ -202,7 +205,8 @@ void launch_cache_maps(const CacheMaps& m, hipStream_t s) {
   p.positions = m.positions;
   p.slots = m.slots;
   p.taken_out = m.taken_out;
-  p.first = m.ws;
+  p.old = m.ws;
+  p.first = m.ws + m.B;
   p.B = m.B;
   p.width = m.width;
   p.shift = page_shift(m.page);

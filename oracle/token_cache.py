@@ -53,6 +53,37 @@ def cache_maps(new, kv, table, page, tokens, free=None, taken=0):
     return cu, kv_out, positions + [0] * rest, slots + [-1] * rest, table, taken
 
 
+def cache_maps_of_any_lengths(new, kv, table, page, tokens, free=None, taken=0):
+    """cache_maps by rows in place of tokens, for lengths that no memory holds: negative ones count as none,
+    sums and places are held at 2^31 - 1, and what has no row is counted alone."""
+    most = 2 ** 31 - 1
+    new, kv = (np.maximum(np.asarray(x, np.int64), 0) for x in (new, kv))
+    table, taken = np.array(table, np.int64), max(int(taken), 0)
+    have = -(-kv // page)
+    need = -(-(kv + new) // page) - have
+    ends = np.cumsum(new)
+    first = taken + np.cumsum(need) - need
+    t = np.arange(min(tokens, int(ends[-1]) if len(ends) else 0))
+    b = np.searchsorted(ends, t, side='right')
+    place = np.minimum(kv[b] + t - (ends - new)[b], most)
+    col, inside = place // page, place % page
+    held = np.full(len(t), -1, np.int64)
+    known = col < table.shape[1]
+    old = known & ((col < have[b]) | (free is None))
+    held[old] = table[b[old], col[old]]
+    if free is not None:
+        free, at = np.asarray(free, np.int64), first[b] + col - have[b]
+        got = known & ~old & (at < len(free))
+        held[got] = free[at[got]]
+        opens = known & ~old & (inside == 0)
+        table[b[opens], col[opens]] = held[opens]
+    slots = held * page + inside
+    rest = tokens - len(t)
+    hold = lambda x: np.minimum(x, most)
+    return (hold(np.concatenate([[0], ends])), hold(kv + new), np.concatenate([place, np.zeros(rest, np.int64)]),
+            np.concatenate([np.where((held >= 0) & (slots <= most), slots, -1), np.full(rest, -1)]), table, taken if free is None else int(hold(taken + need.sum())))
+
+
 def e4m3_values():
     """The 256 values of the format: 1 sign, 4 exponent (bias 7), 3 fraction bits; no
     infinities, all ones is NaN."""

@@ -346,3 +346,69 @@ def test_cache_maps_on_two_streams_with_workspaces_of_their_own(gpu):
         for j in range(10):
             for g, w in zip(got[i][j] + (dev[i][2][j],), want[i]):
                 assert np.array_equal(g.cpu().numpy().reshape(-1), np.asarray(w).reshape(-1))
+
+
+def held_batches():
+    most = 2 ** 31 - 1
+    r = np.random.default_rng(31)
+    yield 'a sum that is held', [most], [100]
+    yield 'between others', [5, most, 7], [3, 100, 9]
+    yield 'behind a history that is held', [4, 10, 30, most], [most - 4, most, 50, 33]
+    yield 'none and fewer', [-5, 0, 3, -most - 1, 1500, 20], [-1, 40, -most - 1, 9, -7, most - 10]
+    new, kv = r.integers(-3, 4, 4000), r.integers(-3, 60, 4000)
+    at = r.integers(0, 4000, 300)
+    kv[at] = r.integers(-2 ** 31, 2 ** 31, 300)
+    yield 'many', new, kv
+    new = new.copy()
+    new[2000:] = r.integers(-2 ** 31, 2 ** 31, 2000)
+    yield 'many, past what is held', new, kv
+    yield 'more than one launch takes', np.concatenate([new[:2000], new]), np.concatenate([kv[:2000], kv])
+
+
+@pytest.mark.parametrize('what,new,kv', held_batches(), ids=[x[0] for x in held_batches()])
+@pytest.mark.parametrize('listed', [False, True])
+@pytest.mark.parametrize('taken', [-4, 2])
+def test_both_forms_of_cache_maps(gpu, what, new, kv, listed, taken):
+    """One launch and two answer alike, also where a sum or a place is held at 2^31 - 1."""
+    from chestnut import kernels as K
+    B, page, width, T = len(new), 16, 12, 2600
+    r = np.random.default_rng(32)
+    table = r.integers(-1, 1 << 20, (B, width))
+    free = r.integers(-1, 1 << 20, 900) if listed else None
+    want = O.cache_maps_of_any_lengths(new, kv, table, page, T, free, taken)
+    for in_place in (False, True):
+        assert (K.cache_maps_workspace(B, T, in_place) > 0) == (in_place or B > 4096)
+        t, m = i32(table), i32(kv)
+        args = dict(free_pages=i32(free), taken=i32([taken])) if listed else {}
+        if listed and not in_place:
+            args['taken_out'] = i32([77])
+        got = K.cache_maps(i32(new), m, t, page, T, kv_out=m if in_place else None, **args)
+        for x, w, name in zip(got + (t,), want, 'cu kv positions slots table'.split()):
+            x = x.cpu().numpy()
+            assert np.array_equal(x, w), f'{name}, in place {in_place}: first {np.argwhere(x != w)[0]}'
+        if listed:
+            assert args['taken' if in_place else 'taken_out'].item() == want[5]
+
+
+def test_cache_maps_in_a_workspace_that_is_kept(gpu):
+    """Of the bytes asked for and no more, whatever stands in them; two streams, one each."""
+    from chestnut import kernels as K
+    new, kv, table, free = batch(33, 900, 30, 300, 16)
+    want = O.cache_maps(new, kv, table, 16, 30000, free, 0)
+    nb = K.cache_maps_workspace(900, 30000, True)
+    assert nb % 4 == 0 and nb > 0
+    buf = [torch.full((nb // 4 + 2,), f, device='cuda') for f in (float('nan'), 1e30)]
+    dev = [[(i32(new), i32(kv), i32(table), i32(free), i32([0])) for _ in range(5)] for _ in buf]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in buf], [[], []]
+    for j in range(5):
+        for i in range(2):
+            n, k, t, f, a = dev[i][j]
+            with torch.cuda.stream(streams[i]):
+                got[i].append(K.cache_maps(n, k, t, 16, 30000, free_pages=f, taken=a, kv_out=k, workspace=buf[i][1:nb // 4 + 1]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.isnan(buf[i][[0, -1]]).all() if i == 0 else (buf[i][[0, -1]] == 1e30).all()
+        for j in range(5):
+            for g, w in zip(got[i][j] + (dev[i][j][2], dev[i][j][4]), want):
+                assert np.array_equal(g.cpu().numpy().reshape(-1), np.asarray(w).reshape(-1))

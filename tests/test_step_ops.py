@@ -288,3 +288,22 @@ def test_range_workspace():
     assert K.attention_workspace(0, 0, 0, 8, 8, 64, groups=3) == 0
     t = torch.tensor(1)
     assert K.attention_workspace(t, 1, 6144, 8, 8, 64, window=6144) == whole
+
+
+@pytest.mark.parametrize('listed', [False, True])
+def test_oracle_maps_of_any_lengths(listed):
+    """Row by row as token by token, where both can be had; at lengths past 31 bits by what they must be."""
+    r = np.random.default_rng(6)
+    for page, width in ((16, 7), (16, 3), (32, 40)):
+        new, kv = r.integers(-3, 90, 20), r.integers(-9, 150, 20)
+        table = r.permutation(20 * width).reshape(20, width)
+        table[r.random(table.shape) < 0.1] = -1
+        free = list(r.permutation(100) + 20 * width) if listed else None
+        for tokens in (0, 9, 300, 1400):
+            a, b = (f(new, kv, table, page, tokens, free, 3 * listed) for f in (O.cache_maps, O.cache_maps_of_any_lengths))
+            assert all(np.array_equal(x, y) for x, y in zip(a, b))
+    most = 2 ** 31 - 1
+    cu, out, pos, slots, table, taken = O.cache_maps_of_any_lengths([2, most, 5], [most - 1, 100, 7], [[3] * 8] * 3, 16, 40, [9] * 50, 0)
+    assert list(cu) == [0, 2, most, most] and list(out) == [most, most, 12] and taken == 2 ** 27   # ceil((2^31 + 99) / 16) - 7
+    assert list(pos[:4]) == [most - 1, most, 100, 101] and list(slots[:4]) == [-1, -1, 3 * 16 + 4, 3 * 16 + 5]
+    assert (table[1][:7] == 3).all() and table[1][7] == 9 and pos[14] == 112 and slots[14] == 9 * 16
