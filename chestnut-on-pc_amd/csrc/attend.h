@@ -1870,7 +1870,8 @@ void attend_launch(const std::string& w, AttendParams& p, const AttendQuery& a, 
   // (a launch has under 2^32 threads)
   CK_REQUIRE(pl.items * p.Hkv < (1L << 32) / std::max(256, 2 * pl.bm), w + ": too many sequences and rows for one launch");
   if (need) {
-    CK_REQUIRE(a.ws && a.ws_floats >= need, w + ": workspace too small (ck_attention_workspace)");
+    CK_REQUIRE(a.ws && a.ws_floats >= need,
+               w + ": workspace too small (" + (FORM == RANGE ? "ck_attention_range_workspace" : "ck_attention_workspace") + ")");
     CK_REQUIRE((reinterpret_cast<uintptr_t>(a.ws) & 15) == 0, w + ": workspace must be 16-byte aligned");
   }
   p.target = pl.target;

@@ -307,3 +307,15 @@ def test_oracle_maps_of_any_lengths(listed):
     assert list(cu) == [0, 2, most, most] and list(out) == [most, most, 12] and taken == 2 ** 27   # ceil((2^31 + 99) / 16) - 7
     assert list(pos[:4]) == [most - 1, most, 100, 101] and list(slots[:4]) == [-1, -1, 3 * 16 + 4, 3 * 16 + 5]
     assert (table[1][:7] == 3).all() and table[1][7] == 9 and pos[14] == 112 and slots[14] == 9 * 16
+
+
+def test_a_workspace_that_is_missing_is_named_by_its_function():
+    """The one that knows of windows and groups: ck_attention_workspace may answer 0 for these calls."""
+    few = ('ck_attention_paged_window', X, X, X, None, None, X, X, 400, X, X, 2, 4, 4, 3, 2, 16, 64, 256, 64, 256, 64, 1, 1, 4000, 0, 0.1, None, 0, None)
+    rows = ('ck_attention_varlen_window', X, X, X, X, X, X, 2, 4, 9000, 4, 2, 64, 256, 64, 128, 64, 128, 64, 256, 64, 1, 4000, 0, 0.1, None, 0, None)
+    for args in (native_shared(), few, rows):
+        with pytest.raises(RuntimeError, match='workspace too small \\(ck_attention_range_workspace\\)'):
+            _lib.call(*args)
+    whole = ('ck_attention_paged', X, X, X, None, None, X, X, 400, X, X, 2, 4, 4, 3, 2, 16, 64, 256, 64, 256, 64, 1, 1, 1, 0.1, None, 0, None)
+    with pytest.raises(RuntimeError, match='workspace too small \\(ck_attention_workspace\\)'):
+        _lib.call(*whole)
