@@ -646,3 +646,89 @@ def test_a_run_of_steps(gpu, dt, quant, kind):
         for b in range(B):
             close(out[b], b, lens[b] + t, f'step {t}')
     assert np.array_equal(a['kv'].cpu().numpy(), pre + total)
+
+
+# --------------------------------------------- many groups and sequences, keys split --
+def splits(B, T, keys, H, kv, hd, groups):
+    """Whether a call over shared pages splits its keys: the sums of chunks then have room in the workspace."""
+    from chestnut import kernels as K
+    return K.attention_workspace(B, T, keys, H, kv, hd, groups=groups) > K.attention_workspace(B, T, 0, H, kv, hd, groups=groups)
+
+
+def long_batch(sizes, alone, q, page, seed):
+    """Groups of these sizes on up to 1500 shared keys and sequences of up to 2500 of their own, most of them short;
+    `alone` sequences in no group behind them: (table, pages, kv_lens, q_lens, common)."""
+    r = np.random.default_rng(seed)
+    common = [int(x) // page * page for x in r.choice([0, 40, 700, 1100, 1500], len(sizes), p=[0.1, 0.1, 0.3, 0.3, 0.2])]
+    first = [common[g] for g, n in enumerate(sizes) for _ in range(n)] + [0] * alone
+    qlens = [1] * len(first) if q == 1 else [int(x) for x in r.integers(0, q + 1, len(first))]
+    own = [x + int(y) for x, y in zip(qlens, r.choice([0, 3, 90, 600, 2500], len(first), p=[0.2, 0.3, 0.3, 0.15, 0.05]))]
+    own[-1] = 2500
+    lens = [f + o for f, o in zip(first, own)]
+    need = [-(-o // page) for o in own]
+    order = list(r.permutation(sum(c // page for c in common) + sum(need) + 3))
+    table = np.full((len(first), -(-max(lens) // page)), -1)
+    b = 0
+    for g, n in enumerate(list(sizes) + [1] * alone):
+        pre = [order.pop() for _ in range(common[g] // page)] if g < len(sizes) else []
+        for _ in range(n):
+            mine = pre + [order.pop() for _ in range(need[b])]
+            table[b, :len(mine)] = mine
+            b += 1
+    return table, sum(c // page for c in common) + sum(need) + 3, lens, qlens, common
+
+
+@pytest.mark.parametrize('sizes,alone', [([1] * 70, 4), ([3] * 70 + [0] * 5 + [40], 4), ([100, 31], 4), ([2] * 100, 0)],
+                         ids=['70 of one', '76', '2 of many', '100 of two'])
+@pytest.mark.parametrize('q', [1, 9])
+@pytest.mark.parametrize('H,kv,hd', [(4, 4, 64), (16, 2, 128)])
+@pytest.mark.parametrize('dt,quant', [('f16', False), ('bf16', True)])
+def test_many_groups_and_sequences_whose_keys_are_split(gpu, sizes, alone, q, H, kv, hd, dt, quant):
+    """More groups and sequences than a wave has lanes, several chunks of shared and of own keys each: by 16 rows, by tiles
+    beside 16 rows, and by tiles."""
+    from chestnut import kernels as K
+    page = 32
+    table, pages, lens, qlens, common = long_batch(sizes, alone, q, page, 7)
+    B, T = len(lens), sum(qlens)
+    assert splits(B, T, table.size * page, H, kv, hd, len(sizes))
+    (kp, vp, ks, vs), vals = pages_of(2, pages, kv, page, hd, dt, 'e4m3' if quant else dt)
+    x = rows(3, T, H, hd, dt)
+    out = K.attention_paged(x, kp, vp, i32(table), cu(qlens), i32(lens), k_scale=ks, v_scale=vs, shared=(cu(sizes), i32(common)))
+    a = 0
+    for b, (m, l) in enumerate(zip(qlens, lens)):
+        k, v = gathered(vals, table[b], l, page)
+        near(out[a:a + m], *expect(x[a:a + m], k, v), max(1, l), hd, dt, f'sequence {b}: {m} over {l}')
+        a += m
+
+
+@pytest.mark.parametrize('T', [90, 300, 700])
+def test_index_values_outside_the_tensors_stay_inside_where_keys_are_split(gpu, T):
+    """As test_index_values_outside_the_tensors_stay_inside, with tables and windows of so many keys that every form splits
+    them: by few rows and by tiles, and their joining launches."""
+    from chestnut import kernels as K
+    r = np.random.default_rng(13)
+    B, H, kv, hd, page, n, width, Tk = 50, 8, 2, 64, 16, 40, 200, 45000
+    (kp, vp, _, _), _ = pages_of(2, n, kv, page, hd, 'f16', 'f16')
+    q, k, v = rows(3, T, H, hd, 'f16'), rows(4, Tk, kv, hd, 'f16'), rows(5, Tk, kv, hd, 'f16')
+    wild = lambda *s: i32(np.where(r.random(s) < 0.5, r.integers(-2 ** 31, 2 ** 31, s), r.integers(-3, 4000, s)))
+    for trial in range(12):
+        N, window, sinks = [1, 3, 70][trial % 3], int(r.integers(800, 2500)), int(r.integers(0, 90))
+        assert splits(B, T, B * width * page, H, kv, hd, N)
+        table, lens, offs = wild(B, width), wild(B), wild(B + 1)
+        if trial % 2:
+            offs = i32(np.sort(r.integers(0, T + 1, B + 1)))
+        paged = lambda **kw: K.attention_paged(q, kp, vp, table, offs, lens, **kw)
+        calls = [(B * width * page, dict(groups=N), lambda **kw: paged(shared=(wild(N + 1), wild(N)), **kw)),
+                 (B * width * page, dict(groups=N), lambda **kw: paged(shared=(i32(np.sort(r.integers(0, B + 1, N + 1))), wild(N)), causal=False, **kw)),
+                 (B * width * page, dict(window=window, sinks=sinks), lambda **kw: paged(window=window, sinks=sinks, **kw)),
+                 (Tk, dict(window=window, sinks=sinks), lambda **kw: K.attention_varlen(q, k, v, offs, wild(B + 1), window=window, sinks=sinks, **kw))]
+        for keys, form, call in calls:
+            nb = K.attention_workspace(B, T, keys, H, kv, hd, **form)
+            assert nb > 0
+            ws = torch.full((nb // 4 + 64,), float(trial), device='cuda')
+            ws[:nb // 4].view(torch.int32).copy_(wild(nb // 4))
+            out = torch.full((T + 2, H, hd), 7.0, dtype=torch.float16, device='cuda')
+            print(f'trial {trial}: {form}', flush=True)
+            call(out=out[1:T + 1], workspace=ws[:nb // 4])
+            torch.cuda.synchronize()
+            assert (out[0] == 7.0).all() and (out[T + 1] == 7.0).all() and (ws[nb // 4:] == float(trial)).all()
