@@ -860,8 +860,9 @@ def attention_paged(q, k_pages, v_pages, block_table, cu_q, kv_lens, k_scale=Non
     sequences cu_shared[g] .. cu_shared[g+1] (ascending) begin with the same pages, which hold
     their first shared_lens[g] keys (as far as these fill whole pages).  The shared keys are then
     read once for all queries of the group, from the table of its first sequence; the result
-    is the same up to rounding.  Sequences may be in no group; not with a window.  Its
-    workspace: attention_workspace with groups=N."""
+    is the same up to rounding.  Sequences may be in no group, which is the better place for one
+    whose queries end within the shared keys: in a group it slows the shared keys of all of them
+    (to 2 to 3 times).  Not with a window.  Its workspace: attention_workspace with groups=N."""
     n, kv, page, hd = _cache(k_pages, v_pages, k_scale, v_scale)
     T, H, B, (qt, qh), (ot, oh), scale = _queries(q, cu_q, kv, hd, out, scale)
     if k_pages.dtype not in (q.dtype, _E4M3):

@@ -127,8 +127,8 @@ struct Front {
 struct Item {
   int b, tile, chunk, nch, c, base;   // base: the tile's first item; b: the row of the table
   Seq s;
-  // shared pages: front: the keys that the sequences b .. s1 share (s: their queries); whole: every row sees
-  // all of them.  Else first: the keys below are the front's, of which f says where its parts are; rank: the
+  // shared pages: front: the keys that the sequences b .. s1 share (s: their queries); whole: every row of every front sees
+  // all of its keys.  Else first: the keys below are the front's, of which f says where its parts are; rank: the
   // tile's number among the sequences' own ones; fronts: items of all fronts
   bool front, whole;
   int s1, first, rank, fronts;
@@ -299,7 +299,9 @@ __device__ __forceinline__ bool find_shared(const AttendParams& p, int index, It
   get_own(0);
   get_fronts_queries(0);
   group_own(0);
-  // how long a chunk is, whether every query of a group sees all that it shares, and how many own tiles there are
+  // how long a chunk is, whether every query of every group sees all that its group shares, and how many own tiles there are.
+  // (One answer for all groups: a single sequence that ends within the shared keys sends all fronts' tiles through the masked
+  // path; the 64 streams of two groups with one such 104.6 us for 39.2, and 41.2 with that one in no group.)
   float work = readlane_f32(lanes_scan((float)ftiles * (float)blocks_of(fs.nk)), 63);
   for (int g0 = 64; g0 < p.N; g0 += 64) {
     get_fronts(g0);
@@ -1237,9 +1239,10 @@ __device__ __forceinline__ void leave_head(const AttendParams& p, const Item& it
 // and 10 us, 545 by the call, though with 128 features that kernel spills 43 registers (tiles
 // of 256 rows: 19; without codes to turn into values: 1).  Short prompts (40 of 1 to 239 tokens,
 // 8 heads of 64) 12.4 us.
-// RANGE, 128 rows: prompts of 9001, 5120 and 2263 through 2048 keys and 4 first ones, 16 heads on 4 of 128, bf16, 268 us:
-// 224 GFLOP seen, 240 issued, 0.90 PFLOP/s of these (through all keys 467, where WHOLE takes 460 with 128 rows).  256 rows:
-// 288.  Six chunks of 1 to 512 tokens on 12800 shared keys, f16, 224 us and 11.5 to join them, 178 GFLOP, 0.79 PFLOP/s.
+// RANGE, 128 rows: prompts of 9001, 5120 and 2263 through 2048 keys and 4 first ones, 16 heads on 4 of 128, bf16, 268.5 us:
+// 224 GFLOP seen, 236 issued, 0.88 PFLOP/s of these (through all keys 471 us, 465 issued, 0.99; WHOLE takes 460 a call with 128
+// rows).  256 rows: 288.  Six chunks of 1 to 512 tokens on 12800 shared keys, f16, 227 us and 11.5 to join them, 178 GFLOP, 0.78
+// PFLOP/s.
 // Masked tiles in the pipeline with the others: prompts 272 -> 270, but e4m3 spills in the loop (46 -> 70 below).
 template <typename T, int HD, int FORM>
 struct TileLds {
@@ -1505,7 +1508,7 @@ constexpr int few_at_once(int bm, int hd, bool e4m3) { return hd == 64 ? (bm == 
 // TB/s, of which about 8 are a workgroup's beginning (lengths, then the table, then keys, each a wait for memory), and 4.7 to
 // join them; one token through 512 keys, 8 heads of 64, whole: 10.0 us.
 // MIXED (shared pages, single tokens): the groups' fronts by tiles of 128 rows, the sequences' own keys by few rows.
-// 64 streams on 24576 and 12800 shared keys and 1 to 1500 of their own, 16 heads on 4 of 128, e4m3, 87 MB: 40.7 us and 5.2 to
+// 64 streams on 24576 and 12800 shared keys and 1 to 1500 of their own, 16 heads on 4 of 128, e4m3, 87 MB: 39.2 us and 5.3 to
 // join them (all by tiles 62 and 5.5).  Bound by the waits for memory: a step of e4m3 tiles takes 1.6 us where the next
 // tile's keys come from HBM, and two workgroups a CU are all that registers allow.  Own keys two steps ahead: 46.6 us a
 // call for 45.7; in chunks twice as long 46.0, four times 63.
@@ -1652,7 +1655,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES, MIXED ? 2 : few_at_once(R::BM, HD, 
       *reinterpret_cast<float4_t*>(part_o<HD>(p, row) + c * 4) = a;
       if (c == 0) *part_ml<HD>(p, row) = float2_t{M, sum};
     }
-  }  if (FORM == RANGE && KV != KV_ROWS && p.N && tid == 0) leave_parts<HD, BM>(p, it, hk, it.tile);
+  }
+  if (FORM == RANGE && KV != KV_ROWS && p.N && tid == 0) leave_parts<HD, BM>(p, it, hk, it.tile);
 }
 
 // One group's (cg of CG) share of nch parts of a row, the first at `row`, added to a (chunk c), its sum and maximum.

@@ -9,8 +9,9 @@
 // few lanes and the rotation none; a lane holds the same pairs of every head that it comes
 // across, and their weights in registers.  The angles belong to a token: a workgroup computes
 // those of its tokens once into LDS.  A lane's heads are sent for together, before the angles: 12288
-// tokens of 32 heads of 128, half of each turned, 201 MB, 59 us with one head under way, 41.6 with
-// four, 38.9 with six = 5.2 TB/s, 39 with eight, 67 with twelve.
+// tokens of 32 heads of 128, half of each turned, 201 MB, by calls one after another 59 us with one head
+// under way, 41.6 with four, 38.9 with six = 5.2 TB/s, 39 with eight, 67 with twelve (a kernel trace:
+// 40.9, least 38.2).
 #include "common.h"
 #include "elem16.h"
 #include "kernels.h"
@@ -167,7 +168,8 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(const NormRopeParams p) 
   }
 }
 
-// Any head_dim up to 512, any alignment: a wave a head, pair by pair.
+// Any head_dim up to 512, any alignment: a wave a head, pair by pair.  Bound by its loads and stores of 2 bytes a lane: 12288
+// tokens of 32 heads of 96, 24 pairs turned, 151 MB, 135 us = 1.1 TB/s (heads of 64 and of 128 in the form above 28.6 and 39.8).
 template <typename T>
 __global__ __launch_bounds__(256) void norm_rope_any_kernel(const NormRopeParams p) {
   constexpr int PAIRS = 512 / 2 / 64;   // of a lane
