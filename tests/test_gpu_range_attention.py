@@ -732,3 +732,16 @@ def test_index_values_outside_the_tensors_stay_inside_where_keys_are_split(gpu, 
             call(out=out[1:T + 1], workspace=ws[:nb // 4])
             torch.cuda.synchronize()
             assert (out[0] == 7.0).all() and (out[T + 1] == 7.0).all() and (ws[nb // 4:] == float(trial)).all()
+
+
+@pytest.mark.parametrize('n', [1, 70])
+def test_a_window_over_rows_whose_offsets_pass_32_bits(gpu, n):
+    from chestnut import kernels as K
+    H, kv, hd, m, Tk = 4, 1, 64, 2500, 2 ** 26 + 5000
+    k, v = (torch.zeros(Tk, kv, hd, dtype=torch.float16, device='cuda') for _ in 'kv')
+    k[-m:], v[-m:] = rows(2, m, kv, hd, 'f16'), rows(3, m, kv, hd, 'f16')
+    assert k[-m:].storage_offset() > 2 ** 32
+    q = rows(1, n, H, hd, 'f16')
+    for window, sinks in ((1000, 70), (300, 0)):
+        out = K.attention_varlen(q, k, v, i32([0, 0, n]), i32([0, Tk - m, Tk]), window=window, sinks=sinks)
+        near(out, *expect(q, f64(k[-m:]), f64(v[-m:]), window, sinks), m, hd, 'f16', f'{window} and {sinks}')

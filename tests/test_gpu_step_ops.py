@@ -412,3 +412,26 @@ def test_cache_maps_in_a_workspace_that_is_kept(gpu):
         for j in range(5):
             for g, w in zip(got[i][j] + (dev[i][j][2], dev[i][j][4]), want):
                 assert np.array_equal(g.cpu().numpy().reshape(-1), np.asarray(w).reshape(-1))
+
+
+@pytest.mark.parametrize('hd', [128, 96])
+def test_norms_and_axes_where_offsets_pass_32_bits(gpu, hd):
+    """Rows behind the first 2^32 elements: as a call on these rows alone gives them."""
+    from chestnut import kernels as K
+    H, kv = 40, 8
+    T = 2 ** 32 // ((H + kv) * hd) + 300
+    x = torch.zeros(T, H + kv, hd, dtype=torch.bfloat16, device='cuda')
+    assert x[-200:].storage_offset() > 2 ** 32
+    x[-200:] = rows(1, 200, H + kv, hd, 'bf16')
+    last = x[-200:].clone()
+    pos = torch.zeros(3, T, dtype=torch.int32, device='cuda')
+    pos[:, -200:] = i32(np.random.default_rng(2).integers(0, 5000, (3, 200)))
+    f, axes = K.rope_frequencies(48)[0], K.rope_axes([8, 8, 8])
+    w = torch.rand(hd, device='cuda').bfloat16()
+    at = pos[:, -200:].contiguous()
+    want = K.norm_rope(last[:, :H], last[:, H:], w, w, at, f, axes=axes)
+    turned = K.rope(last, at, f, axes=axes)
+    y = K.rope(x, pos, f, axes=axes, out=torch.empty_like(x))
+    assert torch.equal(y[-200:], turned) and not y[:1000].any()
+    q, k = K.norm_rope(x[:, :H], x[:, H:], w, w, pos, f, axes=axes, q_out=y[:, :H], k_out=y[:, H:])
+    assert torch.equal(q[-200:], want[0]) and torch.equal(k[-200:], want[1]) and not y[:1000].any()
